@@ -523,6 +523,86 @@ int prime_argmax(const void *logits, int dtype, int n, int vocab, int64_t stride
                  void *stream);
 
 /*
+ * Gated linear recurrence.  Per sequence and channel, from h_{-1} = state_in (or 0):
+ *   D_t = clamp(softplus(step_t), 1e-4, 50)   (the selective form's step size,
+ *                                              selective.py:368)
+ *   a_t = exp(-D_t / tau)
+ *   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(gate_t) x_t
+ *   y_t = h_t
+ * in fp32, y rounded once to `dtype` (F32 / BF16 / F16).
+ *   x, step, gate, y : [B, L, C] views of one dtype, any batch and token strides,
+ *                      contiguous channels; y overlaps none of the inputs
+ *   tau              : fp32 [C], positive and finite, in tokens
+ *   state_in, state_out : fp32 [B, C] or NULL; state_out may be state_in
+ *   checkpoints      : NULL, or fp32 [B, ceil(L / 16), C] that receives the state
+ *                      before every 16th token, for the backward
+ *   workspace        : prime_gated_scan_workspace_size bytes (0: may be NULL), this
+ *                      call's own until it has run on `stream`
+ * A non-finite x, step or gate leaves its channel non-finite from that token on.
+ *
+ * prime_gated_scan_backward: gradients for dy (view like y) and dstate_out (fp32
+ * [B, C] or NULL), from the forward's inputs and its checkpoints:
+ *   dx, dstep, dgate : [B, L, C] views of `dtype`, each apart from the others and
+ *                      from the inputs (interleaved columns of one buffer are fine)
+ *   dtau             : fp32 [C], summed over sequences and tokens in a fixed order
+ *   dstate_in        : fp32 [B, C] or NULL
+ * Where softplus(step) lies outside the clamp dstep is 0, as torch.clamp's gradient.
+ * L <= 2^30; C up to 2^23.
+ */
+typedef struct prime_seq {
+    void   *data;
+    int64_t stride_b, stride_l;  /* in ELEMENTS */
+} prime_seq_t;
+size_t prime_gated_scan_workspace_size(int B, int L, int C);
+int prime_gated_scan(const prime_seq_t *x, const prime_seq_t *step, const prime_seq_t *gate, int dtype, int B, int L,
+                     int C, const float *tau, const float *state_in, const prime_seq_t *y, float *state_out,
+                     float *checkpoints, void *workspace, size_t workspace_bytes, void *stream);
+size_t prime_gated_scan_backward_workspace_size(int B, int L, int C);
+int prime_gated_scan_backward(const prime_seq_t *x, const prime_seq_t *step, const prime_seq_t *gate, int dtype, int B,
+                              int L, int C, const float *tau, const float *checkpoints, const prime_seq_t *dy,
+                              const float *dstate_out, const prime_seq_t *dx, const prime_seq_t *dstep,
+                              const prime_seq_t *dgate, float *dtau, float *dstate_in, void *workspace,
+                              size_t workspace_bytes, void *stream);
+
+/*
+ * Dropout with the residual add of a block's branch in training:
+ *   out = residual + (keep ? x / (1 - p) : 0)        (residual may be NULL)
+ * in fp32, rounded once to `dtype` (F32 / BF16 / F16).  p is rounded to n / 65536.
+ * Element e = row * cols + col is kept where 16 random bits are at least n: the
+ * bits e % 8 of the block of Philox4x32-10 (Salmon et al. 2011) with counter
+ * (e / 8, rng[1] + call) and key rng[0], each 64 bits, low word first; of its four
+ * words the low halves come first.  The mask depends on rng, call and e alone and is
+ * never stored: the backward is this call on the gradient, without a residual.
+ *   x, residual, out : rows of cols contiguous elements, ld* elements apart; out may
+ *                      be x or residual (the same rows), else it overlaps neither
+ *   rng              : int64 [2] on the device, read when the kernel runs
+ *   rows * cols <= 2^40, 0 <= p <= 1
+ */
+int prime_dropout_add(const void *x, int64_t ldx, const void *residual, int64_t ldr, void *out, int64_t ldo, int dtype,
+                      int64_t rows, int64_t cols, float p, const int64_t *rng, int64_t call, void *stream);
+
+/*
+ * Sampled tokens: one per row of logits, from one uniform number in [0, 1) each.
+ * Tokens are ranked by logit, equal ones by index; exp((logit - largest) / T) is a
+ * token's weight.  In this order: the first top_k tokens are kept (0 or less: all);
+ * of these the shortest prefix whose weight is at least top_p of theirs (1 or more:
+ * all; at least one token); of these the ones with weight at least min_p.  The
+ * answer is the first kept token by index whose running weight exceeds uniform
+ * times the weight of all kept ones.
+ * T <= 0 takes the first of the largest logits.  NaN logits count as -infinity,
+ * which is never chosen; a row with nothing else is sampled as if all its logits
+ * were equal.  Several +infinity share the weight among them.
+ * Weights are held to 2^-42 of the largest; the result does not depend on timing.
+ *   logits : n rows of `vocab` <= 2^20 elements (F32 / BF16 / F16), stride_n apart
+ *   temperature, top_k, top_p, min_p : one value, or, where the pointer behind it is
+ *            not NULL, one per row on the device
+ *   out    : int64 [n]
+ */
+int prime_sample(const void *logits, int dtype, int n, int vocab, int64_t stride_n, const float *uniforms,
+                 float temperature, const float *temperatures, int top_k, const int32_t *top_ks, float top_p,
+                 const float *top_ps, float min_p, const float *min_ps, int64_t *out, void *stream);
+
+/*
  * Hybrid window-PRIME pieces (hybrid.py:98-170 calls them through the JIT
  * extension of prime_cpp_kernel.cpp).  The reference's prime_prefill_cpp
  * (prime_cpp_kernel.cpp:6-46) is prime_chunked_prefill with eps = 1e-3 and a

@@ -1498,3 +1498,244 @@ size_t prime_chunked_prefill_workspace_size(int B, int H, int L, unsigned flags)
 }
 
 }  // extern "C"
+
+namespace {
+
+// Bytes from a [B, L, C] view's first element to behind its last.
+size_t seq_span(const prime_seq_t *t, int B, int L, int C, int es) {
+    return static_cast<size_t>(((B - 1) * t->stride_b + (L - 1) * t->stride_l + C) * es);
+}
+
+// Whether two views share memory.  Views of the same strides whose rows do not reach
+// each other (columns of one buffer) do not.
+bool seq_overlap(const prime_seq_t *p, const prime_seq_t *q, int B, int L, int C, int es) {
+    if (!overlap(p->data, seq_span(p, B, L, C, es), q->data, seq_span(q, B, L, C, es))) return false;
+    if (p->stride_l != q->stride_l || p->stride_b != q->stride_b) return true;
+    const int64_t row = (L > 1 || B == 1 ? p->stride_l : p->stride_b) * es, d = static_cast<char *>(p->data) - static_cast<char *>(q->data);
+    if (row <= 0 || (B > 1 && L > 1 && (p->stride_b * es) % row)) return true;
+    const int64_t m = (d % row + row) % row, w = static_cast<int64_t>(C) * es;
+    return m < w || row - m < w;
+}
+
+int check_seq(const prime_seq_t *t, int es, int B, int L, int C, const char *name) {
+    if (!t || !t->data) return fail(PRIME_ERR_INVALID_ARG, "%s is null", name);
+    if (t->stride_b < 0 || t->stride_l < 0) return fail(PRIME_ERR_INVALID_ARG, "%s has negative strides", name);
+    if (reinterpret_cast<uintptr_t>(t->data) % es) return fail(PRIME_ERR_MISALIGNED, "%s is misaligned", name);
+    return PRIME_OK;
+}
+
+// an output's rows must not share memory with each other
+int check_seq_out(const prime_seq_t *t, int es, int B, int L, int C, const char *name) {
+    int rc = check_seq(t, es, B, L, C, name);
+    if (rc) return rc;
+    if ((L > 1 && t->stride_l < C) || (B > 1 && t->stride_b < C) ||
+        (B > 1 && L > 1 && t->stride_b < t->stride_l * L && t->stride_l < t->stride_b * B))
+        return fail(PRIME_ERR_ALIAS, "%s: rows overlap each other", name);
+    return PRIME_OK;
+}
+
+int check_floats(const float *p, const char *name) {
+    if (reinterpret_cast<uintptr_t>(p) & 3u) return fail(PRIME_ERR_MISALIGNED, "%s is not 4-byte aligned", name);
+    return PRIME_OK;
+}
+
+int gated_sizes(int dtype, int B, int L, int C) {
+    if (B <= 0 || L <= 0 || C <= 0 || L > (1 << 30) || C > (1 << 23))
+        return fail(PRIME_ERR_INVALID_ARG, "bad sizes B=%d L=%d C=%d", B, L, C);
+    if (!valid_dtype(dtype)) return fail(PRIME_ERR_UNSUPPORTED_DTYPE, "unsupported dtype");
+    int seg;
+    if (static_cast<int64_t>(B) * prime::gated_segments(B, L, C, &seg) >= (int64_t(1) << 31))
+        return fail(PRIME_ERR_INVALID_ARG, "B=%d above the grid's limit", B);
+    return PRIME_OK;
+}
+
+// floats of the segments' folds (two arrays), and of one of them
+size_t gated_fold_floats(int B, int L, int C, int *G) {
+    int seg;
+    *G = prime::gated_segments(B, L, C, &seg);
+    return static_cast<size_t>(B) * *G * C;
+}
+
+prime::GatedView seq_view(const prime_seq_t *t) { return {t->data, t->stride_b, t->stride_l}; }
+
+}  // namespace
+
+extern "C" {
+
+size_t prime_gated_scan_workspace_size(int B, int L, int C) {
+    if (B <= 0 || L <= 0 || C <= 0 || L > (1 << 30)) return 0;
+    int G;
+    const size_t n = gated_fold_floats(B, L, C, &G);
+    return G > 1 ? (2 * n + static_cast<size_t>(B) * C) * sizeof(float) : 0;
+}
+
+size_t prime_gated_scan_backward_workspace_size(int B, int L, int C) {
+    if (B <= 0 || L <= 0 || C <= 0 || L > (1 << 30)) return 0;
+    int G;
+    return gated_fold_floats(B, L, C, &G) * 3 * sizeof(float);
+}
+
+int prime_gated_scan(const prime_seq_t *x, const prime_seq_t *step, const prime_seq_t *gate, int dtype, int B, int L,
+                     int C, const float *tau, const float *state_in, const prime_seq_t *y, float *state_out,
+                     float *checkpoints, void *workspace, size_t workspace_bytes, void *stream) {
+    g_err[0] = 0;
+    int rc = gated_sizes(dtype, B, L, C);
+    if (rc) return rc;
+    const int es = elem_size(dtype);
+    if ((rc = check_seq(x, es, B, L, C, "x")) || (rc = check_seq(step, es, B, L, C, "step")) ||
+        (rc = check_seq(gate, es, B, L, C, "gate")) || (rc = check_seq_out(y, es, B, L, C, "y")))
+        return rc;
+    if (!tau) return fail(PRIME_ERR_INVALID_ARG, "tau is null");
+    if ((rc = check_floats(tau, "tau")) || (rc = check_floats(state_in, "state_in")) ||
+        (rc = check_floats(state_out, "state_out")) || (rc = check_floats(checkpoints, "checkpoints")))
+        return rc;
+    for (const prime_seq_t *t : {x, step, gate})
+        if (seq_overlap(y, t, B, L, C, es)) return fail(PRIME_ERR_ALIAS, "y overlaps an input");
+    const size_t nstate = static_cast<size_t>(B) * C * sizeof(float), need = prime_gated_scan_workspace_size(B, L, C);
+    const int tiles = (L + prime::kGatedTile - 1) / prime::kGatedTile;
+    const void *out[4] = {y->data, state_out, checkpoints, need ? workspace : nullptr};
+    const size_t nout[4] = {seq_span(y, B, L, C, es), nstate, nstate * tiles, need};
+    const void *in[5] = {x->data, step->data, gate->data, tau, state_in};
+    const size_t nin[5] = {seq_span(x, B, L, C, es), seq_span(step, B, L, C, es), seq_span(gate, B, L, C, es),
+                           static_cast<size_t>(C) * sizeof(float), nstate};
+    if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
+        return fail(PRIME_ERR_INVALID_ARG, "workspace of %zu bytes needed, 16-byte aligned", need);
+    for (int i = 0; i < 4; ++i) {
+        if (!out[i]) continue;
+        for (int j = 0; j < i; ++j)
+            if (out[j] && overlap(out[i], nout[i], out[j], nout[j]))
+                return fail(PRIME_ERR_ALIAS, "two of y, state_out, checkpoints and workspace overlap");
+        for (int j = i == 0 ? 3 : 0; j < 5; ++j)
+            if (in[j] && overlap(out[i], nout[i], in[j], nin[j]) && !(i == 1 && j == 4 && out[i] == in[j]))
+                return fail(PRIME_ERR_ALIAS, "an output or the workspace overlaps an input");
+    }
+    prime::GatedArgs a{};
+    a.x = seq_view(x); a.step = seq_view(step); a.gate = seq_view(gate); a.y = seq_view(y);
+    a.dt = dtype; a.B = B; a.L = L; a.C = C; a.tau = tau;
+    a.state_in = state_in; a.state_out = state_out; a.ckpt = checkpoints;
+    a.tiles = tiles;
+    a.G = prime::gated_segments(B, L, C, &a.seg_len);
+    const size_t n = static_cast<size_t>(B) * a.G * C;
+    a.ws_z = static_cast<float *>(workspace); a.ws_h = a.ws_z + n; a.ws_h0 = a.ws_h + n;
+    return check_hip(prime::launch_gated_scan(a, false, static_cast<hipStream_t>(stream)), "gated scan launch");
+}
+
+int prime_gated_scan_backward(const prime_seq_t *x, const prime_seq_t *step, const prime_seq_t *gate, int dtype, int B,
+                              int L, int C, const float *tau, const float *checkpoints, const prime_seq_t *dy,
+                              const float *dstate_out, const prime_seq_t *dx, const prime_seq_t *dstep,
+                              const prime_seq_t *dgate, float *dtau, float *dstate_in, void *workspace,
+                              size_t workspace_bytes, void *stream) {
+    g_err[0] = 0;
+    int rc = gated_sizes(dtype, B, L, C);
+    if (rc) return rc;
+    const int es = elem_size(dtype);
+    if ((rc = check_seq(x, es, B, L, C, "x")) || (rc = check_seq(step, es, B, L, C, "step")) ||
+        (rc = check_seq(gate, es, B, L, C, "gate")) || (rc = check_seq(dy, es, B, L, C, "dy")) ||
+        (rc = check_seq_out(dx, es, B, L, C, "dx")) || (rc = check_seq_out(dstep, es, B, L, C, "dstep")) ||
+        (rc = check_seq_out(dgate, es, B, L, C, "dgate")))
+        return rc;
+    if (!tau || !checkpoints || !dtau) return fail(PRIME_ERR_INVALID_ARG, "tau, checkpoints or dtau is null");
+    if ((rc = check_floats(tau, "tau")) || (rc = check_floats(checkpoints, "checkpoints")) ||
+        (rc = check_floats(dstate_out, "dstate_out")) || (rc = check_floats(dtau, "dtau")) ||
+        (rc = check_floats(dstate_in, "dstate_in")))
+        return rc;
+    const prime_seq_t *outs[3] = {dx, dstep, dgate}, *ins[4] = {x, step, gate, dy};
+    for (int i = 0; i < 3; ++i) {
+        for (int j = 0; j < i; ++j)
+            if (seq_overlap(outs[i], outs[j], B, L, C, es)) return fail(PRIME_ERR_ALIAS, "two of dx, dstep, dgate overlap");
+        for (int j = 0; j < 4; ++j)
+            if (seq_overlap(outs[i], ins[j], B, L, C, es)) return fail(PRIME_ERR_ALIAS, "a gradient overlaps an input");
+    }
+    const size_t need = prime_gated_scan_backward_workspace_size(B, L, C);
+    if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u))
+        return fail(PRIME_ERR_INVALID_ARG, "workspace of %zu bytes needed, 16-byte aligned", need);
+    const size_t nstate = static_cast<size_t>(B) * C * sizeof(float), nc = static_cast<size_t>(C) * sizeof(float);
+    const int tiles = (L + prime::kGatedTile - 1) / prime::kGatedTile;
+    // the plain buffers: dtau, dstate_in, workspace written; tau, checkpoints, dstate_out read
+    const void *buf[6] = {dtau, dstate_in, workspace, tau, checkpoints, dstate_out};
+    const size_t nbuf[6] = {nc, nstate, need, nc, nstate * tiles, nstate};
+    for (int i = 0; i < 6; ++i) {
+        if (!buf[i]) continue;
+        for (int j = 0; j < 3; ++j)
+            if (overlap(buf[i], nbuf[i], outs[j]->data, seq_span(outs[j], B, L, C, es)))
+                return fail(PRIME_ERR_ALIAS, "a gradient overlaps another buffer");
+        if (i >= 3) continue;
+        for (int j = 0; j < 6; ++j)
+            if (j != i && buf[j] && overlap(buf[i], nbuf[i], buf[j], nbuf[j]))
+                return fail(PRIME_ERR_ALIAS, "dtau, dstate_in or the workspace overlaps another buffer");
+        for (int j = 0; j < 4; ++j)
+            if (overlap(buf[i], nbuf[i], ins[j]->data, seq_span(ins[j], B, L, C, es)))
+                return fail(PRIME_ERR_ALIAS, "dtau, dstate_in or the workspace overlaps an input");
+    }
+    prime::GatedArgs a{};
+    a.x = seq_view(x); a.step = seq_view(step); a.gate = seq_view(gate); a.dy = seq_view(dy);
+    a.dx = seq_view(dx); a.dstep = seq_view(dstep); a.dgate = seq_view(dgate);
+    a.dt = dtype; a.B = B; a.L = L; a.C = C; a.tau = tau;
+    a.ckpt = const_cast<float *>(checkpoints); a.dstate_out = dstate_out; a.dstate_in = dstate_in; a.dtau = dtau;
+    a.tiles = tiles;
+    a.G = prime::gated_segments(B, L, C, &a.seg_len);
+    const size_t n = static_cast<size_t>(B) * a.G * C;
+    a.ws_z = static_cast<float *>(workspace); a.ws_h = a.ws_z + n; a.dtau_part = a.ws_h + n;
+    return check_hip(prime::launch_gated_scan(a, true, static_cast<hipStream_t>(stream)), "gated scan backward launch");
+}
+
+int prime_dropout_add(const void *x, int64_t ldx, const void *residual, int64_t ldr, void *out, int64_t ldo, int dtype,
+                      int64_t rows, int64_t cols, float p, const int64_t *rng, int64_t call, void *stream) {
+    g_err[0] = 0;
+    if (!x || !out || !rng) return fail(PRIME_ERR_INVALID_ARG, "prime_dropout_add: null argument");
+    if (!valid_dtype(dtype)) return fail(PRIME_ERR_UNSUPPORTED_DTYPE, "unsupported dtype");
+    if (rows <= 0 || cols <= 0 || rows > (int64_t(1) << 40) || cols > (int64_t(1) << 40) / rows)
+        return fail(PRIME_ERR_INVALID_ARG, "bad sizes rows=%lld cols=%lld", static_cast<long long>(rows),
+                    static_cast<long long>(cols));
+    if (ldx < cols || ldo < cols || (residual && ldr < cols))
+        return fail(PRIME_ERR_INVALID_ARG, "rows overlap: a row stride is below cols");
+    if (!(p >= 0.f && p <= 1.f)) return fail(PRIME_ERR_INVALID_ARG, "p=%g outside [0, 1]", static_cast<double>(p));
+    const int es = elem_size(dtype);
+    if (reinterpret_cast<uintptr_t>(x) % es || reinterpret_cast<uintptr_t>(out) % es ||
+        reinterpret_cast<uintptr_t>(residual) % es || (reinterpret_cast<uintptr_t>(rng) & 7u))
+        return fail(PRIME_ERR_MISALIGNED, "x, residual, out or rng misaligned");
+    auto span = [&](int64_t ld) { return static_cast<size_t>(((rows - 1) * ld + cols) * es); };
+    const bool is_x = out == x && ldo == ldx, is_r = residual && out == residual && ldo == ldr;
+    if ((!is_x && overlap(out, span(ldo), x, span(ldx))) ||
+        (residual && !is_r && overlap(out, span(ldo), residual, span(ldr))) || overlap(out, span(ldo), rng, 16))
+        return fail(PRIME_ERR_ALIAS, "out overlaps x, residual or rng without being the same rows");
+    prime::DropoutArgs a{};
+    a.x = x; a.residual = residual; a.out = out;
+    a.rows = rows; a.cols = cols; a.ldx = ldx; a.ldr = ldr; a.ldo = ldo; a.dt = dtype;
+    a.cut = static_cast<uint32_t>(static_cast<double>(p) * 65536.0 + 0.5);
+    a.scale = a.cut >= 65536u ? 0.f : static_cast<float>(65536.0 / (65536.0 - a.cut));
+    a.rng = rng; a.call = call;
+    return check_hip(prime::launch_dropout_add(a, static_cast<hipStream_t>(stream)), "dropout launch");
+}
+
+int prime_sample(const void *logits, int dtype, int n, int vocab, int64_t stride_n, const float *uniforms,
+                 float temperature, const float *temperatures, int top_k, const int32_t *top_ks, float top_p,
+                 const float *top_ps, float min_p, const float *min_ps, int64_t *out, void *stream) {
+    g_err[0] = 0;
+    if (!logits || !uniforms || !out) return fail(PRIME_ERR_INVALID_ARG, "prime_sample: null argument");
+    if (n <= 0 || vocab <= 0 || vocab > prime::kSampleMaxVocab || stride_n < vocab)
+        return fail(PRIME_ERR_INVALID_ARG, "bad sizes n=%d vocab=%d (at most %d) stride=%lld", n, vocab,
+                    prime::kSampleMaxVocab, static_cast<long long>(stride_n));
+    if (!valid_dtype(dtype)) return fail(PRIME_ERR_UNSUPPORTED_DTYPE, "unsupported logits dtype");
+    const int es = elem_size(dtype);
+    if (reinterpret_cast<uintptr_t>(logits) % es || (reinterpret_cast<uintptr_t>(out) & 7u))
+        return fail(PRIME_ERR_MISALIGNED, "logits or out misaligned");
+    int rc;
+    if ((rc = check_floats(uniforms, "uniforms")) || (rc = check_floats(temperatures, "temperatures")) ||
+        (rc = check_floats(top_ps, "top_ps")) || (rc = check_floats(min_ps, "min_ps")) ||
+        (rc = check_floats(reinterpret_cast<const float *>(top_ks), "top_ks")))
+        return rc;
+    const size_t no = static_cast<size_t>(n) * 8;
+    const void *in[5] = {uniforms, temperatures, top_ks, top_ps, min_ps};
+    for (const void *p : in)
+        if (p && overlap(out, no, p, static_cast<size_t>(n) * 4)) return fail(PRIME_ERR_ALIAS, "out overlaps a parameter");
+    if (overlap(out, no, logits, static_cast<size_t>(((n - 1) * stride_n + vocab) * es)))
+        return fail(PRIME_ERR_ALIAS, "out overlaps the logits");
+    prime::SampleArgs a{};
+    a.logits = logits; a.stride_n = stride_n; a.n = n; a.vocab = vocab; a.dt = dtype; a.uniforms = uniforms;
+    a.temperature = temperature; a.temperatures = temperatures; a.top_k = top_k; a.top_ks = top_ks;
+    a.top_p = top_p; a.top_ps = top_ps; a.min_p = min_p; a.min_ps = min_ps; a.out = out;
+    return check_hip(prime::launch_sample(a, static_cast<hipStream_t>(stream)), "sample launch");
+}
+
+}  // extern "C"

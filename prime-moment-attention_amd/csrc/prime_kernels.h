@@ -419,6 +419,59 @@ hipError_t launch_delta_step(const DeltaStepArgs &a, hipStream_t stream);
 void launch_delta_prep_f32(const DeltaArgs &a, hipStream_t s);
 void launch_delta_scan_f32(const DeltaArgs &a, hipStream_t s);
 
+// Gated linear recurrence (gated.hip): [B, L, C] views with contiguous channels.
+struct GatedView {
+    void *data;
+    int64_t sb, sl;  // elements
+};
+struct GatedArgs {
+    GatedView x, step, gate, y;       // y: forward
+    GatedView dy, dx, dstep, dgate;   // backward
+    int dt, B, L, C;
+    const float *tau;                 // [C]
+    const float *state_in;            // [B, C] or null
+    float *state_out;                 // [B, C] or null; may be state_in
+    float *ckpt;                      // [B, tiles, C]: the state before every kGatedTile-th token (forward: or null)
+    const float *dstate_out;          // [B, C] or null
+    float *dstate_in;                 // [B, C] or null
+    float *dtau;                      // [C]
+    int tiles, G, seg_len;            // ceil(L / kGatedTile); segments of seg_len tokens
+    float *ws_z, *ws_h;               // [B, G, C] each: the segments' folds (G > 1)
+    float *ws_h0;                     // [B, C] (G > 1)
+    float *dtau_part;                 // [B, G, C]
+};
+constexpr int kGatedTile = 16, kGatedThreads = 256;
+int gated_segments(int B, int L, int C, int *seg_len);
+hipError_t launch_gated_scan(const GatedArgs &a, bool bwd, hipStream_t stream);
+
+// Dropout with the residual add (dropout.hip).
+struct DropoutArgs {
+    const void *x, *residual;         // residual may be null
+    void *out;
+    int64_t rows, cols, ldx, ldr, ldo;
+    int dt;
+    uint32_t cut;                     // kept where 16 random bits are at least this
+    float scale;                      // 1 / (1 - cut / 65536); 0 for cut = 65536
+    const int64_t *rng;               // device: seed, offset
+    int64_t call;
+};
+hipError_t launch_dropout_add(const DropoutArgs &a, hipStream_t stream);
+
+// Sampled tokens (sample.hip): each parameter one value, or (pointer not null) one per row.
+struct SampleArgs {
+    const void *logits;
+    int64_t stride_n;
+    int n, vocab, dt;
+    const float *uniforms;
+    const float *temperatures, *top_ps, *min_ps;
+    const int32_t *top_ks;
+    float temperature, top_p, min_p;
+    int top_k;
+    int64_t *out;
+};
+constexpr int kSampleMaxVocab = 1 << 20;
+hipError_t launch_sample(const SampleArgs &a, hipStream_t stream);
+
 // Launch timer (the C-ABI prime_timer_* calls).  timer_events(kernel) hands
 // out the event pair for one launch of `kernel` while that kernel is being
 // timed (both null otherwise); the launch passes them to hipExtLaunchKernelGGL,

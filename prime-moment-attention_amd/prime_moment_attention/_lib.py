@@ -35,7 +35,9 @@ EXPORTS = ("prime_abi_version", "prime_last_error", "prime_decode_step", "prime_
            "prime_selective_prefill_backward_workspace_size", "prime_hbm_stream",
            "prime_frag_rows", "prime_pack_frag", "prime_linear_frag_workspace_size", "prime_linear_frag",
            "prime_delta_prefill_backward", "prime_delta_prefill_backward_workspace_size",
-           "prime_delta_decode_step_backward", "prime_delta_gates")
+           "prime_delta_decode_step_backward", "prime_delta_gates",
+           "prime_gated_scan", "prime_gated_scan_workspace_size", "prime_gated_scan_backward",
+           "prime_gated_scan_backward_workspace_size", "prime_dropout_add", "prime_sample")
 
 # bytes of the fixed device scratch behind prime_accumulate_noalloc
 NOALLOC_SCRATCH_BYTES = 32 << 20
@@ -66,6 +68,10 @@ class PrimeQkNorm(ctypes.Structure):
     _fields_ = [("q_weight", ctypes.c_void_p), ("q_bias", ctypes.c_void_p), ("k_weight", ctypes.c_void_p),
                 ("k_bias", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("eps", ctypes.c_float),
                 ("q_scale", ctypes.c_float)]
+
+
+class PrimeSeq(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("stride_b", ctypes.c_int64), ("stride_l", ctypes.c_int64)]
 
 
 class PrimeSelectiveGate(ctypes.Structure):
@@ -195,6 +201,19 @@ def load() -> ctypes.CDLL:
     L.prime_linear_frag.argtypes = [fp] * 4 + [ctypes.c_int] * 3 + [ctypes.c_int64, ctypes.c_int, ctypes.c_uint,
                                                                    ctypes.c_float, fp, fp, fp, ctypes.c_size_t, fp]
     L.prime_linear_frag.restype = ctypes.c_int
+    i32, i64, f32, seq = ctypes.c_int, ctypes.c_int64, ctypes.c_float, P(PrimeSeq)
+    for n in ("prime_gated_scan_workspace_size", "prime_gated_scan_backward_workspace_size"):
+        getattr(L, n).argtypes = [i32] * 3
+        getattr(L, n).restype = ctypes.c_size_t
+    L.prime_gated_scan.argtypes = [seq] * 3 + [i32] * 4 + [fp, fp, seq, fp, fp, fp, ctypes.c_size_t, fp]
+    L.prime_gated_scan.restype = ctypes.c_int
+    L.prime_gated_scan_backward.argtypes = [seq] * 3 + [i32] * 4 + [fp, fp, seq, fp, seq, seq, seq, fp, fp, fp,
+                                                                   ctypes.c_size_t, fp]
+    L.prime_gated_scan_backward.restype = ctypes.c_int
+    L.prime_dropout_add.argtypes = [fp, i64, fp, i64, fp, i64, i32, i64, i64, f32, fp, i64, fp]
+    L.prime_dropout_add.restype = ctypes.c_int
+    L.prime_sample.argtypes = [fp, i32, i32, i32, i64, fp, f32, fp, i32, fp, f32, fp, f32, fp, fp, fp]
+    L.prime_sample.restype = ctypes.c_int
     v = L.prime_abi_version()
     if v != ABI_VERSION:
         raise RuntimeError(f"libprime_mi355x ABI {v} != expected {ABI_VERSION}")
@@ -1068,6 +1087,141 @@ def delta_decode_step_backward(q, k, v, beta, alpha, feat_eps: float, bound: flo
         dk = dk.view(B, Hkv, H // Hkv, D).sum(2)
         dv = dv.view(B, Hkv, H // Hkv, D).sum(2)
     return dq, dk, dv, dbeta, dalpha, dstate
+
+
+# ---------------------------------------------------------------- gated recurrence, dropout, sampling
+GATED_TILE = 16  # tokens between the checkpoints of the gated recurrence's backward
+
+
+def _same_device(first: torch.Tensor, *ts) -> None:
+    _dev_check(first, *ts)
+    for t in ts:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on {first.device} and {t.device}: one device is needed")
+
+
+def _launch(what: str, dev: torch.device, *args) -> None:
+    """The entry point ``what`` on the current stream of the tensors' device, which
+    need not be the current device."""
+    fn = getattr(load(), what)
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        _check(fn(*args, _stream(dev)), what)
+        return
+    with torch.cuda.device(dev):
+        _check(fn(*args, _stream(dev)), what)
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def seq_desc(t: torch.Tensor) -> PrimeSeq:
+    """Descriptor of a [B, L, C] view with contiguous channels."""
+    return PrimeSeq(t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def _check_gated(x, step, gate, tau, state, *states) -> Tuple[int, int, int]:
+    if x.dim() != 3:
+        raise ValueError(f"x has shape {tuple(x.shape)}, expected [B, L, C]")
+    if x.dtype not in _DTYPES:
+        raise RuntimeError(f"unsupported dtype {x.dtype}")
+    B, Lt, C = x.shape
+    for t, n in ((x, "x"), (step, "step"), (gate, "gate")):
+        _shape(t, (B, Lt, C), n)
+        if t.dtype != x.dtype:
+            raise ValueError(f"{n} is {t.dtype}, x is {x.dtype}: one dtype is needed")
+        if t.stride(2) != 1 and C > 1:
+            raise ValueError(f"{n}: channels must be contiguous")
+    if tau.dtype != torch.float32 or tuple(tau.shape) != (C,) or not tau.is_contiguous():
+        raise ValueError(f"tau must be a contiguous fp32 tensor of {C} values")
+    for t, n in zip((state, *states), ("state", "state_out")):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (B, C) or not t.is_contiguous()):
+            raise ValueError(f"{n} must be a contiguous fp32 [{B}, {C}] tensor")
+    _same_device(x, step, gate, tau, state, *states)
+    return B, Lt, C
+
+
+def gated_scan(x, step, gate, tau, state, y, state_out, checkpoints=None) -> None:
+    """prime_gated_scan over [B, L, C] views of one dtype; tau fp32 [C]; states
+    fp32 [B, C] or None (state_out may be state); checkpoints fp32
+    [B, ceil(L / GATED_TILE), C] for gated_scan_backward, or None."""
+    B, Lt, C = _check_gated(x, step, gate, tau, state, state_out)
+    _shape(y, (B, Lt, C), "y")
+    if y.dtype != x.dtype or (y.stride(2) != 1 and C > 1):
+        raise ValueError("y must have x's dtype and contiguous channels")
+    if checkpoints is not None and (checkpoints.dtype != torch.float32 or not checkpoints.is_contiguous()
+                                    or checkpoints.numel() != B * -(-Lt // GATED_TILE) * C):
+        raise ValueError("checkpoints must be a contiguous fp32 [B, ceil(L / 16), C] tensor")
+    _same_device(x, y, checkpoints)
+    n = load().prime_gated_scan_workspace_size(B, Lt, C)
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+    _launch("prime_gated_scan", x.device, seq_desc(x), seq_desc(step), seq_desc(gate), _DTYPES[x.dtype], B, Lt, C,
+            _ptr(tau), _ptr(state), seq_desc(y), _ptr(state_out), _ptr(checkpoints), _ptr(ws), n)
+
+
+def gated_scan_backward(x, step, gate, tau, checkpoints, dy, dstate_out, dx, dstep, dgate, dtau, dstate_in) -> None:
+    """prime_gated_scan_backward: dx, dstep, dgate [B, L, C] views of x's dtype, dtau
+    fp32 [C], dstate_in fp32 [B, C] or None."""
+    B, Lt, C = _check_gated(x, step, gate, tau, dstate_out, dstate_in)
+    for t, n in ((dy, "dy"), (dx, "dx"), (dstep, "dstep"), (dgate, "dgate")):
+        _shape(t, (B, Lt, C), n)
+        if t.dtype != x.dtype or (t.stride(2) != 1 and C > 1):
+            raise ValueError(f"{n} must have x's dtype and contiguous channels")
+    if checkpoints.dtype != torch.float32 or not checkpoints.is_contiguous() or (
+            checkpoints.numel() != B * -(-Lt // GATED_TILE) * C):
+        raise ValueError("checkpoints must be the forward's")
+    if dtau.dtype != torch.float32 or tuple(dtau.shape) != (C,) or not dtau.is_contiguous():
+        raise ValueError(f"dtau must be a contiguous fp32 tensor of {C} values")
+    _same_device(x, dy, dx, dstep, dgate, checkpoints, dtau)
+    n = load().prime_gated_scan_backward_workspace_size(B, Lt, C)
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+    _launch("prime_gated_scan_backward", x.device, seq_desc(x), seq_desc(step), seq_desc(gate), _DTYPES[x.dtype], B,
+            Lt, C, _ptr(tau), _ptr(checkpoints), seq_desc(dy), _ptr(dstate_out), seq_desc(dx), seq_desc(dstep),
+            seq_desc(dgate), _ptr(dtau), _ptr(dstate_in), _ptr(ws), n)
+
+
+def dropout_add(x, residual, out, p: float, rng, call: int) -> None:
+    """prime_dropout_add over 2-D rows with contiguous columns; residual may be None."""
+    for t, n in ((x, "x"), (residual, "residual"), (out, "out")):
+        if t is None:
+            continue
+        _shape(t, x.shape, n)
+        if t.dim() != 2 or t.dtype != x.dtype or (t.stride(1) != 1 and t.shape[1] > 1):
+            raise ValueError(f"{n} must be rows of x's dtype with contiguous columns")
+    if x.dtype not in _DTYPES:
+        raise RuntimeError(f"unsupported dtype {x.dtype}")
+    if rng.dtype != torch.int64 or rng.numel() != 2 or not rng.is_contiguous():
+        raise ValueError("rng must be a contiguous int64 tensor of two values (seed, offset)")
+    _same_device(x, residual, out, rng)
+    rows, cols = x.shape
+    ld = lambda t: 0 if t is None else t.stride(0) if rows > 1 else cols
+    _launch("prime_dropout_add", x.device, _ptr(x), ld(x), _ptr(residual), ld(residual), _ptr(out), ld(out),
+            _DTYPES[x.dtype], rows, cols, float(p), _ptr(rng), int(call))
+
+
+def sample(logits, uniforms, temperature, top_k, top_p, min_p, out) -> None:
+    """prime_sample: logits [n, vocab] with a contiguous vocab dimension, uniforms fp32
+    [n], out int64 [n]; each parameter a number or a tensor of n values (top_k int32,
+    the others fp32)."""
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("logits must be [n, vocab] with a contiguous vocab dimension")
+    if logits.dtype not in _DTYPES:
+        raise RuntimeError(f"unsupported dtype {logits.dtype}")
+    n, vocab = logits.shape
+    args, keep = [], []
+    for v, name, dt in ((uniforms, "uniforms", torch.float32), (temperature, "temperature", torch.float32),
+                        (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
+                        (min_p, "min_p", torch.float32), (out, "out", torch.int64)):
+        if not torch.is_tensor(v):
+            continue
+        if v.dtype != dt or v.numel() != n or not v.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {dt} tensor of {n} values")
+        keep.append(v)
+    _same_device(logits, *keep)
+    for v, cast in ((temperature, float), (top_k, int), (top_p, float), (min_p, float)):
+        args += [cast(0), _ptr(v)] if torch.is_tensor(v) else [cast(v), None]
+    _launch("prime_sample", logits.device, _ptr(logits), _DTYPES[logits.dtype], n, vocab,
+            logits.stride(0) if n > 1 else vocab, _ptr(uniforms), *args, _ptr(out))
 
 
 def timer_enable(*kernels: int) -> None:

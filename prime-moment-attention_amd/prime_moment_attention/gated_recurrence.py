@@ -1,0 +1,173 @@
+"""The gated linear recurrence: a layer with one fp32 state per channel, beside the
+moment attentions.
+
+``gated_recurrence`` is the operator.  Per sequence and channel,
+
+    D_t = clamp(softplus(step_t), 1e-4, 50)      the selective module's step size
+    a_t = exp(-D_t / tau)                        (selective.py:368, 385-386)
+    h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(gate_t) x_t,    y_t = h_t
+
+The factor sqrt(1 - a^2) keeps a state driven by independent inputs at their scale
+whatever the decay.  Prompts, training (with gradients in x, step, gate, tau and the
+state) and single tokens run prime_gated_scan.
+
+``GatedLinearRecurrence`` is the layer, with the interface of the attention modules:
+``forward(hidden_states, state=None, return_state=False) -> (out, next_state)``.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple
+
+import torch
+import torch.nn as nn
+from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .attention import project_out
+from .chunked_ssd import needs_grad
+
+
+def _channels(t: torch.Tensor) -> torch.Tensor:
+    """t with contiguous channels (as it is where they are)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _thirds(proj: torch.Tensor):
+    C = proj.shape[-1] // 3
+    return proj[..., :C], proj[..., C:2 * C], proj[..., 2 * C:]
+
+
+class _GatedScanFn(torch.autograd.Function):
+    """prime_gated_scan with its backward.  x, step and gate, or (step and gate None) x
+    holding all three as thirds of its columns, whose gradient is then one tensor."""
+
+    @staticmethod
+    def forward(ctx, x, step, gate, tau, state):
+        ctx.stacked = step is None
+        parts = _thirds(x) if ctx.stacked else (x, step, gate)
+        B, L, C = parts[0].shape
+        y = torch.empty(B, L, C, device=x.device, dtype=x.dtype)
+        last = torch.empty(B, C, device=x.device, dtype=torch.float32)
+        ckpt = torch.empty(B, -(-L // _lib.GATED_TILE), C, device=x.device, dtype=torch.float32)
+        _lib.gated_scan(*parts, tau, state, y, last, ckpt)
+        ctx.save_for_backward(x, step, gate, tau, ckpt)
+        ctx.has_state = state is not None
+        ctx.set_materialize_grads(False)
+        return y, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dlast):
+        x, step, gate, tau, ckpt = ctx.saved_tensors
+        parts = _thirds(x) if ctx.stacked else (x, step, gate)
+        B, L, C = parts[0].shape
+        dy = torch.zeros_like(parts[0]) if dy is None else _channels(dy.to(x.dtype))
+        dlast = None if dlast is None else dlast.to(torch.float32).contiguous()
+        new = torch.empty(B, L, 3 * C, device=x.device, dtype=x.dtype)
+        if ctx.stacked:
+            grads, out = _thirds(new), (new, None, None)
+        else:
+            grads = out = tuple(new.view(3, B, L, C))
+        dtau = torch.empty(C, device=x.device, dtype=torch.float32)
+        dstate = torch.empty(B, C, device=x.device, dtype=torch.float32) if ctx.has_state else None
+        _lib.gated_scan_backward(*parts, tau, ckpt, dy, dlast, *grads, dtau, dstate)
+        return (*out, dtau, dstate)
+
+
+def _scan(x, step, gate, tau, state, state_out):
+    """(y, last state) of x, step, gate, or of x's thirds where step is None."""
+    parts = (x, step, gate) if step is not None else _thirds(x)
+    B, L, C = _lib._check_gated(*parts, tau, state, state_out)
+    if L == 0 or B == 0 or C == 0:
+        h = parts[0].new_zeros(B, C, dtype=torch.float32) if state is None else state
+        if state_out is not None:
+            h = state_out.copy_(h)
+        return torch.zeros_like(parts[0]) + 0 * (parts[1] + parts[2]), h + 0
+    if needs_grad(x, step, gate, tau, state) or forward_ad._current_level >= 0:
+        if state_out is not None:
+            raise ValueError("state_out cannot be written while autograd records: take the returned state")
+        return _GatedScanFn.apply(x, step, gate, tau, state)
+    y = torch.empty(B, L, C, device=x.device, dtype=x.dtype)
+    if state_out is None:
+        state_out = torch.empty(B, C, device=x.device, dtype=torch.float32)
+    _lib.gated_scan(*parts, tau, state, y, state_out)
+    return y, state_out
+
+
+def gated_recurrence(x: torch.Tensor, step: torch.Tensor, gate: torch.Tensor, tau: torch.Tensor,
+                     state: Optional[torch.Tensor] = None, return_state: bool = False,
+                     state_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """The recurrence over x, step, gate [B, L, C] (fp32, bf16 or fp16 alike; any batch
+    and token strides) with tau fp32 [C], positive and finite, and state fp32 [B, C] or
+    None (zero): (y [B, L, C] of x's dtype, last state fp32 [B, C] or None without
+    return_state).
+
+    Differentiable once in x, step, gate, tau and state.  The given state is left as it
+    is; without autograd, ``state_out`` names the tensor that receives the last state
+    (it may be ``state``: a decode step in place)."""
+    x, step, gate = _channels(x), _channels(step), _channels(gate)
+    y, last = _scan(x, step, gate, tau, state, state_out)
+    return y, (last if return_state else None)
+
+
+class GatedLinearRecurrence(nn.Module):
+    """in_proj (x, step and gate in one product) -> gated recurrence -> o_proj.  The
+    state is fp32 [B, width].  log_tau [width] is learned; tau is held between min_tau
+    and max_tau as the selective module's, and starts spread evenly over their
+    logarithms, with a step size of 1."""
+
+    def __init__(self, hidden_size: int, width: Optional[int] = None, min_tau: float = 2.0,
+                 max_tau: float = 2000.0):
+        super().__init__()
+        self.hidden_size = hidden_size
+        self.width = width or hidden_size
+        self.min_tau = min_tau
+        self.max_tau = max_tau
+        self.inplace_state = False  # True: without autograd the incoming state tensor is updated in place
+        self.in_proj = nn.Linear(hidden_size, 3 * self.width, bias=True)
+        self.o_proj = nn.Linear(self.width, hidden_size, bias=False)
+        self.log_tau = nn.Parameter(torch.zeros(self.width, dtype=torch.float32))
+        self.init_gate_weights()
+
+    def init_gate_weights(self):
+        """Step size 1 and open-half gates at zero input, memories from min_tau to max_tau."""
+        W = self.width
+        with torch.no_grad():
+            self.in_proj.bias.zero_()
+            self.in_proj.bias[W:2 * W].fill_(math.log(math.exp(1.0) - 1.0))
+            self.log_tau.copy_(torch.linspace(math.log(self.min_tau), math.log(self.max_tau), W))
+
+    def get_tau(self, device: torch.device) -> torch.Tensor:
+        return torch.clamp(torch.exp(self.log_tau.to(device).float()), min=self.min_tau, max=self.max_tau)
+
+    def _tau(self, device: torch.device) -> torch.Tensor:
+        """tau for the kernels; without autograd cached until log_tau changes."""
+        p = self.log_tau
+        if torch.is_grad_enabled() and p.requires_grad:
+            return self.get_tau(device)
+        key = (p.data_ptr(), p._version, str(device), self.min_tau, self.max_tau)
+        cached = self.__dict__.get("_tau_cache")
+        if cached is not None and cached[0] is p and cached[1] == key and (
+                not cached[2].is_inference() or torch.is_inference_mode_enabled()):
+            return cached[2]
+        with torch.no_grad():
+            tau = self.get_tau(device).contiguous()
+        self.__dict__["_tau_cache"] = (p, key, tau)
+        return tau
+
+    def mix(self, hidden_states: torch.Tensor, state: Optional[torch.Tensor] = None, return_state: bool = False):
+        """The layer up to its output projection: (y [B, L, width], next state or None)."""
+        proj = _channels(self.in_proj(hidden_states))
+        if state is not None:
+            state = state.to(device=proj.device, dtype=torch.float32)
+        in_place = (self.inplace_state and return_state and state is not None and state.is_contiguous()
+                    and not needs_grad(proj, state, self.log_tau))
+        y, last = _scan(proj, None, None, self._tau(proj.device), state.contiguous() if state is not None else None,
+                        state if in_place else None)
+        return y.to(hidden_states.dtype), (last if return_state else None)
+
+    def forward(self, hidden_states: torch.Tensor, state: Optional[torch.Tensor] = None, return_state: bool = False):
+        y, next_state = self.mix(hidden_states, state, return_state)
+        return project_out(self.o_proj, y), next_state
