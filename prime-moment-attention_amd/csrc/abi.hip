@@ -1543,17 +1543,17 @@ int gated_sizes(int dtype, int B, int L, int C) {
     if (B <= 0 || L <= 0 || C <= 0 || L > (1 << 30) || C > (1 << 23))
         return fail(PRIME_ERR_INVALID_ARG, "bad sizes B=%d L=%d C=%d", B, L, C);
     if (!valid_dtype(dtype)) return fail(PRIME_ERR_UNSUPPORTED_DTYPE, "unsupported dtype");
-    int seg;
-    if (static_cast<int64_t>(B) * prime::gated_segments(B, L, C, &seg) >= (int64_t(1) << 31))
-        return fail(PRIME_ERR_INVALID_ARG, "B=%d above the grid's limit", B);
+    if (static_cast<int64_t>(B) * ((C + 63) / 64) * prime::gated_spans(L) >= (int64_t(1) << 31))
+        return fail(PRIME_ERR_INVALID_ARG, "B=%d L=%d C=%d above the grid's limit", B, L, C);
     return PRIME_OK;
 }
 
-// floats of the segments' folds (two arrays), and of one of them
-size_t gated_fold_floats(int B, int L, int C, int *G) {
-    int seg;
-    *G = prime::gated_segments(B, L, C, &seg);
-    return static_cast<size_t>(B) * *G * C;
+// the chain at the start of a workspace
+void gated_chain(prime::GatedArgs &a, void *workspace) {
+    a.G = prime::gated_spans(a.L);
+    a.tiles = (a.L + prime::kGatedTile - 1) / prime::kGatedTile;
+    a.counter = static_cast<uint32_t *>(workspace);
+    a.words = reinterpret_cast<uint64_t *>(static_cast<char *>(workspace) + 16);
 }
 
 prime::GatedView seq_view(const prime_seq_t *t) { return {t->data, t->stride_b, t->stride_l}; }
@@ -1564,15 +1564,12 @@ extern "C" {
 
 size_t prime_gated_scan_workspace_size(int B, int L, int C) {
     if (B <= 0 || L <= 0 || C <= 0 || L > (1 << 30)) return 0;
-    int G;
-    const size_t n = gated_fold_floats(B, L, C, &G);
-    return G > 1 ? (2 * n + static_cast<size_t>(B) * C) * sizeof(float) : 0;
+    return prime::gated_chain_bytes(B, L, C);
 }
 
 size_t prime_gated_scan_backward_workspace_size(int B, int L, int C) {
     if (B <= 0 || L <= 0 || C <= 0 || L > (1 << 30)) return 0;
-    int G;
-    return gated_fold_floats(B, L, C, &G) * 3 * sizeof(float);
+    return prime::gated_chain_bytes(B, L, C) + static_cast<size_t>(B) * prime::gated_spans(L) * C * sizeof(float);
 }
 
 int prime_gated_scan(const prime_seq_t *x, const prime_seq_t *step, const prime_seq_t *gate, int dtype, int B, int L,
@@ -1613,10 +1610,7 @@ int prime_gated_scan(const prime_seq_t *x, const prime_seq_t *step, const prime_
     a.x = seq_view(x); a.step = seq_view(step); a.gate = seq_view(gate); a.y = seq_view(y);
     a.dt = dtype; a.B = B; a.L = L; a.C = C; a.tau = tau;
     a.state_in = state_in; a.state_out = state_out; a.ckpt = checkpoints;
-    a.tiles = tiles;
-    a.G = prime::gated_segments(B, L, C, &a.seg_len);
-    const size_t n = static_cast<size_t>(B) * a.G * C;
-    a.ws_z = static_cast<float *>(workspace); a.ws_h = a.ws_z + n; a.ws_h0 = a.ws_h + n;
+    gated_chain(a, workspace);
     return check_hip(prime::launch_gated_scan(a, false, static_cast<hipStream_t>(stream)), "gated scan launch");
 }
 
@@ -1672,10 +1666,8 @@ int prime_gated_scan_backward(const prime_seq_t *x, const prime_seq_t *step, con
     a.dx = seq_view(dx); a.dstep = seq_view(dstep); a.dgate = seq_view(dgate);
     a.dt = dtype; a.B = B; a.L = L; a.C = C; a.tau = tau;
     a.ckpt = const_cast<float *>(checkpoints); a.dstate_out = dstate_out; a.dstate_in = dstate_in; a.dtau = dtau;
-    a.tiles = tiles;
-    a.G = prime::gated_segments(B, L, C, &a.seg_len);
-    const size_t n = static_cast<size_t>(B) * a.G * C;
-    a.ws_z = static_cast<float *>(workspace); a.ws_h = a.ws_z + n; a.dtau_part = a.ws_h + n;
+    gated_chain(a, workspace);
+    a.dtau_part = reinterpret_cast<float *>(static_cast<char *>(workspace) + prime::gated_chain_bytes(B, L, C));
     return check_hip(prime::launch_gated_scan(a, true, static_cast<hipStream_t>(stream)), "gated scan backward launch");
 }
 

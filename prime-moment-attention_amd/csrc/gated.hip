@@ -1,13 +1,20 @@
 // Gated linear recurrence: per sequence and channel
 //   D_t = clamp(softplus(step_t), kStepMin, kStepMax),  z_t = D_t / tau,  a_t = exp(-z_t)
 //   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(gate_t) x_t,   y_t = h_t
-// and its gradients.  Elementwise over channels, so a lane owns V neighbouring
-// channels and walks the tokens; the state stays in its registers, fp32.
+// and its gradients.  Elementwise over channels: a lane owns V neighbouring ones.
 //
-// Time is cut into G segments of seg_len tokens (a multiple of kGatedTile)
-// where B * C lanes cannot fill the chip: a first kernel folds every segment
-// into (sum of z, end state from zero), the second starts each segment from
-// the fold of those before it.  The order of every sum is fixed by the sizes.
+// One pass over the data.  A workgroup takes a span of kSpan tokens by 64 V channels,
+// each of its waves kGatedTile of the tokens: the gates go into registers, the wave's
+// tokens fold into (a's product - 1, end state from zero), the folds meet in LDS, and
+// every wave then runs its tokens once more from its true state, with two fused
+// multiply-adds and the rounding's remainder a token instead of the gates.
+// Spans hand their state on through a workspace word per span and channel.  Every
+// kChain-th span publishes its end state, the others their fold, so that a span needs
+// the last published state and at most kChain - 1 folds, which are there as soon as
+// those spans have read their inputs; which of them it takes is fixed by its number,
+// so the result does not depend on timing.  Spans are numbered by a counter in the order
+// in which workgroups start, time first: whatever a workgroup waits for belongs to one
+// that started before it, so every wait ends.
 //
 // a is carried as a - 1 = expm1(-z): next to 1 (long memories) a itself has
 // lost the decay's low bits, and with it the error of h grows by 2^-25 times
@@ -21,57 +28,50 @@ namespace prime {
 
 constexpr float kStepMin = 1e-4f, kStepMax = 50.f;
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kWaves = 8, kThreads = kWaves * kWave, kSpan = kWaves * kGatedTile;
+constexpr int kChain = 16;
 
 // ------------------------------------------------------------------- gates
-// log(1 + e), 0 <= e <= 1, as 2 atanh(w), w = e / (2 + e) <= 1/3: the odd series
-// to w^15 (next term 1.2e-9), no cancellation for small e.
-__device__ __forceinline__ float log1p_unit(float e) {
-    const float w = e * __builtin_amdgcn_rcpf(2.f + e), u = w * w;
-    float p = 1.f / 15.f;
-    p = fmaf(p, u, 1.f / 13.f);
-    p = fmaf(p, u, 1.f / 11.f);
-    p = fmaf(p, u, 1.f / 9.f);
-    p = fmaf(p, u, 1.f / 7.f);
-    p = fmaf(p, u, 1.f / 5.f);
-    p = fmaf(p, u, 1.f / 3.f);
-    p = fmaf(p, u, 1.f);
-    return 2.f * w * p;
-}
-
-// exp(-z) - 1 for z >= 0: the Taylor polynomial below 1/2 (next term 1.1e-8), else exp2.
+// expm1(-z), z >= 0: the Taylor polynomial below 1/16 (next term 1.3e-7 of the value),
+// else exp2 (its rounding is 2^-24 / (1/16) of the value at most).
 __device__ __forceinline__ float expm1_neg(float z) {
-    float p = -1.f / 40320.f;
-    p = fmaf(p, z, 1.f / 5040.f);
-    p = fmaf(p, z, -1.f / 720.f);
-    p = fmaf(p, z, 1.f / 120.f);
-    p = fmaf(p, z, -1.f / 24.f);
-    p = fmaf(p, z, 1.f / 6.f);
-    p = fmaf(p, z, -1.f / 2.f);
+    float p = fmaf(-1.f / 24.f, z, 1.f / 6.f);
+    p = fmaf(p, z, -0.5f);
     p = fmaf(p, z, 1.f);
     const float far = __builtin_amdgcn_exp2f(-z * kLog2e) - 1.f;
-    return z < 0.5f ? -z * p : far;
+    return z < 0.0625f ? -z * p : far;
 }
 
-// softplus, unclamped, and e = exp(-|s|) for its derivative.  (Selects, not fmax: NaN stays.)
+// softplus, unclamped, and e = exp(-|s|) for its derivative: max(s, 0) + log(1 + e), with
+// log(1 + e) / e on [0, 1] its Chebyshev interpolant of degree 8 (3.4e-8 off at most), so
+// that small e loses nothing.  maximum and minimum hand NaN on.
 __device__ __forceinline__ float softplus(float s, float &e) {
     e = __builtin_amdgcn_exp2f(-fabsf(s) * kLog2e);
-    return (s < 0.f ? 0.f : s) + log1p_unit(e);
+    float p = 0.0051261018961668015f;
+    p = fmaf(p, e, -0.029074065387248993f);
+    p = fmaf(p, e, 0.0775160863995552f);
+    p = fmaf(p, e, -0.13602247834205627f);
+    p = fmaf(p, e, 0.19076880812644958f);
+    p = fmaf(p, e, -0.2483539879322052f);
+    p = fmaf(p, e, 0.3331812024116516f);
+    p = fmaf(p, e, -0.4999944567680359f);
+    p = fmaf(p, e, 0.9999999403953552f);
+    return fmaf(p, e, __builtin_elementwise_maximum(s, 0.f));
 }
 
 __device__ __forceinline__ float clamp_step(float d) {
-    d = d < kStepMin ? kStepMin : d;
-    return d > kStepMax ? kStepMax : d;
+    return __builtin_elementwise_minimum(__builtin_elementwise_maximum(d, kStepMin), kStepMax);
 }
 
 __device__ __forceinline__ float sigmoid(float g) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-g * kLog2e));
 }
 
-// z and a - 1 of one token
-__device__ __forceinline__ void decay(float s, float inv_tau, float &z, float &am1) {
+// a - 1 and b = sqrt(1 - a^2) sigmoid(g) x of one token
+__device__ __forceinline__ void gates(float x, float s, float g, float inv_tau, float &am1, float &b) {
     float e;
-    z = clamp_step(softplus(s, e)) * inv_tau;
-    am1 = expm1_neg(z);
+    am1 = expm1_neg(clamp_step(softplus(s, e)) * inv_tau);
+    b = __builtin_amdgcn_sqrtf(-am1 * (2.f + am1)) * sigmoid(g) * x;
 }
 
 // h <- h + (am1 h + b), `lo` keeping what the sum's rounding drops.  Without it a state
@@ -81,6 +81,12 @@ __device__ __forceinline__ void advance(float &h, float &lo, float am1, float b)
     const float d = fmaf(am1, h, b) + lo, next = h + d;
     lo = d - (next - h);
     h = next;
+}
+
+// A fold (A, H): the tokens take a state h to h + (A h + H).  One more token:
+__device__ __forceinline__ void fold_token(float &A, float &H, float am1, float b) {
+    A += fmaf(am1, A, am1);
+    H += fmaf(am1, H, b);
 }
 
 // ------------------------------------------------------------------- access
@@ -119,280 +125,422 @@ __device__ __forceinline__ typename Packed<DT, V>::type pack(const float (&f)[V]
     return p;
 }
 
+// A row of a view: rows are the same for a whole wave, so the address is a scalar and the
+// lane's offset.
 template <int DT, int V>
-__device__ __forceinline__ const typename Packed<DT, V>::type *at(const GatedView &v, int b, int64_t l, int c) {
-    const int64_t e = b * v.sb + l * v.sl + c;
-    return reinterpret_cast<const typename Packed<DT, V>::type *>(
-        static_cast<const char *>(v.data) + e * (DT == PRIME_F32 ? 4 : 2));
+__device__ __forceinline__ const typename Packed<DT, V>::type &at(const GatedView &v, int b, int l, uint32_t c) {
+    constexpr int es = DT == PRIME_F32 ? 4 : 2;
+    const char *row = static_cast<const char *>(v.data) + (b * v.sb + l * v.sl) * es;
+    return *reinterpret_cast<const typename Packed<DT, V>::type *>(row + c * es);
 }
 template <int DT, int V>
-__device__ __forceinline__ typename Packed<DT, V>::type *at_out(const GatedView &v, int b, int64_t l, int c) {
-    return const_cast<typename Packed<DT, V>::type *>(at<DT, V>(v, b, l, c));
+__device__ __forceinline__ typename Packed<DT, V>::type &at_out(const GatedView &v, int b, int l, uint32_t c) {
+    return const_cast<typename Packed<DT, V>::type &>(at<DT, V>(v, b, l, c));
 }
 
-// The lane's place: V channels from c, sequence b, segment g (blockIdx.x = b * G + g);
-// false for lanes past the last channel.
-template <int V>
-__device__ __forceinline__ bool place(const GatedArgs &a, int &c, int &b, int &g) {
-    c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
-    b = blockIdx.x / a.G;
-    g = blockIdx.x % a.G;
-    return c < a.C;
+// -------------------------------------------------------------- spans' chain
+// A workspace word: two floats, of which the first is never the all-ones NaN that the
+// words are filled with before.
+constexpr uint64_t kEmpty = ~0ull;
+
+__device__ __forceinline__ void publish(uint64_t *w, float first, float second) {
+    uint32_t f = __float_as_uint(first);
+    f = f == 0xFFFFFFFFu ? 0x7FC00000u : f;
+    __hip_atomic_store(w, static_cast<uint64_t>(f) << 32 | __float_as_uint(second), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t peek(const uint64_t *w) {
+    return __hip_atomic_load(w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// The fold of the segments before g, from the state before the first.
+// What reaches span g (counted from where the recurrence starts): the published end state
+// of the last chain head before it, then the folds between.  `words` is this channel's
+// word of span 0, `stride` apart; called for g > 0 only.
+__device__ __forceinline__ void chain_in(const uint64_t *words, int64_t stride, int g, float &h, float &lo) {
+    constexpr int U = 5;  // words in flight, three rounds at most
+    static_assert((kChain - 1) % U == 0, "rounds of U folds");
+    const int head = (g - 1) / kChain * kChain, n = g - 1 - head;
+    uint64_t first = peek(words + head * stride);
+    for (int j0 = 0; j0 < n || j0 == 0; j0 += U) {
+        uint64_t w[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+            if (j0 + j < n) w[j] = peek(words + (head + 1 + j0 + j) * stride);
+        if (j0 == 0) {
+            while (first == kEmpty) {
+                __builtin_amdgcn_s_sleep(1);
+                first = peek(words + head * stride);
+            }
+            h = __uint_as_float(static_cast<uint32_t>(first));
+            lo = __uint_as_float(static_cast<uint32_t>(first >> 32));
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            if (j0 + j >= n) continue;
+            while (w[j] == kEmpty) {
+                __builtin_amdgcn_s_sleep(1);
+                w[j] = peek(words + (head + 1 + j0 + j) * stride);
+            }
+            advance(h, lo, __uint_as_float(static_cast<uint32_t>(w[j] >> 32)), __uint_as_float(static_cast<uint32_t>(w[j])));
+        }
+    }
+}
+
 template <int V>
-__device__ __forceinline__ void carry_in(const GatedArgs &a, int b, int g, int c, float (&h)[V], float (&lo)[V]) {
-    const int64_t row = static_cast<int64_t>(b) * a.C + c;
+struct SpanShared {
+    float A[kWaves][kWave * V], H[kWaves][kWave * V];  // the waves' folds
+    float h[kWave * V], lo[kWave * V];                 // what reaches the span
+    int span;
+};
+
+// The workgroup's place.
+struct Place {
+    int g, b, wave;  // span in time order, sequence, wave
+    uint32_t c;      // first channel of the lane
+    bool in;         // the lane has channels
+};
+template <int V>
+__device__ __forceinline__ Place place(const GatedArgs &a, SpanShared<V> &sh) {
+    int id = blockIdx.x;
+    if (a.G > 1) {  // the counter starts at -1
+        if (threadIdx.x == 0) sh.span = static_cast<int>(atomicAdd(a.counter, 1u) + 1u);
+        __syncthreads();
+        id = __builtin_amdgcn_readfirstlane(sh.span);
+    }
+    const int groups = (a.C + kWave * V - 1) / (kWave * V), cols = a.B * groups, col = id % cols;
+    Place p;
+    p.g = id / cols;
+    p.b = col / groups;
+    p.wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t c = (col % groups * kWave + threadIdx.x % kWave) * V;
+    p.in = c < static_cast<uint32_t>(a.C);
+    p.c = p.in ? c : 0;  // lanes past the last channel read the first and write nothing
+    return p;
+}
+
+// Every wave's fold to where its wave starts: h, lo from the span's start over the folds of
+// the waves before it (`order` is the wave's place in time).  Wave 0 also gets what the
+// span needs from the chain and publishes what the chain needs from the span.
+template <int V, bool REVERSE>
+__device__ __forceinline__ void join(const GatedArgs &a, SpanShared<V> &sh, const Place &p, int g, const float *start,
+                                     const float (&A)[V], const float (&H)[V], float (&h)[V], float (&lo)[V]) {
+    const int lane = threadIdx.x % kWave, order = REVERSE ? kWaves - 1 - p.wave : p.wave;
+#pragma unroll
+    for (int i = 0; i < V; ++i) sh.A[order][lane * V + i] = A[i], sh.H[order][lane * V + i] = H[i];
+    __syncthreads();
+    if (p.wave == 0) {
+        const int64_t row = static_cast<int64_t>(p.b) * a.C + p.c;
+        uint64_t *words = a.words + static_cast<int64_t>(p.b) * a.G * a.C + p.c;
+        if (g + 1 < a.G && g % kChain && p.in) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float fa = 0.f, fh = 0.f;
+                for (int w = 0; w < kWaves; ++w) fold_token(fa, fh, sh.A[w][lane * V + i], sh.H[w][lane * V + i]);
+                publish(words + static_cast<int64_t>(g) * a.C + i, fa, fh);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float sh_h = 0.f, sh_lo = 0.f;
+            if (g == 0) {
+                if (start) sh_h = start[row + i];
+            } else if (p.in) {
+                chain_in(words + i, a.C, g, sh_h, sh_lo);
+            }
+            sh.h[lane * V + i] = sh_h;
+            sh.lo[lane * V + i] = sh_lo;
+            if (g + 1 < a.G && g % kChain == 0 && p.in) {
+                for (int w = 0; w < kWaves; ++w) advance(sh_h, sh_lo, sh.A[w][lane * V + i], sh.H[w][lane * V + i]);
+                publish(words + static_cast<int64_t>(g) * a.C + i, sh_lo, sh_h);
+            }
+        }
+    }
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        h[i] = a.G > 1 ? a.ws_h0[row + i] : (a.state_in ? a.state_in[row + i] : 0.f);
-        lo[i] = 0.f;
-    }
-    for (int j = 0; j < g; ++j) {
-        const int64_t o = (static_cast<int64_t>(b) * a.G + j) * a.C + c;
-#pragma unroll
-        for (int i = 0; i < V; ++i) advance(h[i], lo[i], expm1_neg(a.ws_z[o + i]), a.ws_h[o + i]);
+        h[i] = sh.h[lane * V + i];
+        lo[i] = sh.lo[lane * V + i];
+        for (int w = 0; w < order; ++w) advance(h[i], lo[i], sh.A[w][lane * V + i], sh.H[w][lane * V + i]);
     }
 }
 
 // ------------------------------------------------------------------ forward
-// One segment's (sum of z, end state from zero); segment 0 also copies the incoming
-// state, which the last segment of the second kernel may overwrite (in-place states).
 template <int DT, int V>
-__global__ __launch_bounds__(kGatedThreads) void gated_summary_kernel(const GatedArgs a) {
-    int c, b, g;
-    if (!place<V>(a, c, b, g)) return;
-    float inv_tau[V], h[V], lo[V], zs[V];
+__global__ __launch_bounds__(kThreads) void gated_scan_kernel(const GatedArgs a) {
+    __shared__ SpanShared<V> sh;
+    constexpr int T = kGatedTile;
+    const Place p = place<V>(a, sh);
+    const int l0 = p.g * kSpan + p.wave * T, n = min(T, a.L - l0);  // n <= 0: nothing of the wave's is left
+    float am1[T][V], b[T][V], A[V], H[V], inv_tau[V], h[V], lo[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) inv_tau[i] = 1.f / a.tau[c + i], h[i] = 0.f, lo[i] = 0.f, zs[i] = 0.f;
-    const int l0 = g * a.seg_len, l1 = min(l0 + a.seg_len, a.L);
-#pragma unroll 4
-    for (int l = l0; l < l1; ++l) {
-        float x[V], s[V], gt[V];
-        unpack<DT, V>(*at<DT, V>(a.x, b, l, c), x);
-        unpack<DT, V>(*at<DT, V>(a.step, b, l, c), s);
-        unpack<DT, V>(*at<DT, V>(a.gate, b, l, c), gt);
+    for (int i = 0; i < V; ++i) inv_tau[i] = 1.f / a.tau[p.c + i], A[i] = H[i] = 0.f;
+    {
+        typename Packed<DT, V>::type xs[T], ss[T], gs[T];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            float z, am1;
-            decay(s[i], inv_tau[i], z, am1);
-            const float n = __builtin_amdgcn_sqrtf(-am1 * (2.f + am1));
-            advance(h[i], lo[i], am1, n * sigmoid(gt[i]) * x[i]);
-            zs[i] += z;
+        for (int t = 0; t < T; ++t) {
+            const int l = min(l0 + t, a.L - 1);
+            xs[t] = at<DT, V>(a.x, p.b, l, p.c);
+            ss[t] = at<DT, V>(a.step, p.b, l, p.c);
+            gs[t] = at<DT, V>(a.gate, p.b, l, p.c);
+        }
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            float x[V], s[V], g[V];
+            unpack<DT, V>(xs[t], x);
+            unpack<DT, V>(ss[t], s);
+            unpack<DT, V>(gs[t], g);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                gates(x[i], s[i], g[i], inv_tau[i], am1[t][i], b[t][i]);
+                if (t >= n) am1[t][i] = b[t][i] = 0.f;
+                fold_token(A[i], H[i], am1[t][i], b[t][i]);
+            }
         }
     }
-    const int64_t o = (static_cast<int64_t>(b) * a.G + g) * a.C + c, row = static_cast<int64_t>(b) * a.C + c;
+    join<V, false>(a, sh, p, p.g, a.state_in, A, H, h, lo);
+    if (!p.in || n <= 0) return;
+    if (a.ckpt) {
+        float *o = a.ckpt + (static_cast<int64_t>(p.b) * a.tiles + l0 / T) * a.C + p.c;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        a.ws_z[o + i] = zs[i];
-        a.ws_h[o + i] = h[i];
-        if (g == 0) a.ws_h0[row + i] = a.state_in ? a.state_in[row + i] : 0.f;
+        for (int i = 0; i < V; ++i) o[i] = h[i];
+    }
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) advance(h[i], lo[i], am1[t][i], b[t][i]);
+        if (t < n) at_out<DT, V>(a.y, p.b, l0 + t, p.c) = pack<DT, V>(h);
+    }
+    if (a.state_out && l0 + n == a.L) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) a.state_out[static_cast<int64_t>(p.b) * a.C + p.c + i] = h[i];
     }
 }
 
+// Few tokens: a lane walks them.
 template <int DT, int V>
-__global__ __launch_bounds__(kGatedThreads) void gated_scan_kernel(const GatedArgs a) {
-    int c, b, g;
-    if (!place<V>(a, c, b, g)) return;
+__global__ __launch_bounds__(256) void gated_step_kernel(const GatedArgs a) {
+    const int groups = (a.C + blockDim.x * V - 1) / (blockDim.x * V), b = blockIdx.x / groups;
+    const uint32_t c = (blockIdx.x % groups * blockDim.x + threadIdx.x) * V;
+    if (c >= static_cast<uint32_t>(a.C)) return;
+    const int64_t row = static_cast<int64_t>(b) * a.C + c;
     float inv_tau[V], h[V], lo[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) inv_tau[i] = 1.f / a.tau[c + i];
-    carry_in<V>(a, b, g, c, h, lo);
-    const int l0 = g * a.seg_len, l1 = min(l0 + a.seg_len, a.L);
-#pragma unroll 4
-    for (int l = l0; l < l1; ++l) {
-        if (a.ckpt && l % kGatedTile == 0) {
-            float *o = a.ckpt + (static_cast<int64_t>(b) * a.tiles + l / kGatedTile) * a.C + c;
+    for (int i = 0; i < V; ++i) {
+        inv_tau[i] = 1.f / a.tau[c + i];
+        h[i] = a.state_in ? a.state_in[row + i] : 0.f;
+        lo[i] = 0.f;
+    }
+    if (a.ckpt) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) o[i] = h[i];
-        }
-        float x[V], s[V], gt[V];
-        unpack<DT, V>(*at<DT, V>(a.x, b, l, c), x);
-        unpack<DT, V>(*at<DT, V>(a.step, b, l, c), s);
-        unpack<DT, V>(*at<DT, V>(a.gate, b, l, c), gt);
+        for (int i = 0; i < V; ++i) a.ckpt[row + i] = h[i];
+    }
+    for (int l = 0; l < a.L; ++l) {
+        float x[V], s[V], g[V];
+        unpack<DT, V>(at<DT, V>(a.x, b, l, c), x);
+        unpack<DT, V>(at<DT, V>(a.step, b, l, c), s);
+        unpack<DT, V>(at<DT, V>(a.gate, b, l, c), g);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            float z, am1;
-            decay(s[i], inv_tau[i], z, am1);
-            const float n = __builtin_amdgcn_sqrtf(-am1 * (2.f + am1));
-            advance(h[i], lo[i], am1, n * sigmoid(gt[i]) * x[i]);
+            float am1, bt;
+            gates(x[i], s[i], g[i], inv_tau[i], am1, bt);
+            advance(h[i], lo[i], am1, bt);
         }
-        *at_out<DT, V>(a.y, b, l, c) = pack<DT, V>(h);
+        at_out<DT, V>(a.y, b, l, c) = pack<DT, V>(h);
     }
-    if (a.state_out && g == a.G - 1) {
+    if (a.state_out) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) a.state_out[static_cast<int64_t>(b) * a.C + c + i] = h[i];
+        for (int i = 0; i < V; ++i) a.state_out[row + i] = h[i];
     }
 }
 
 // ----------------------------------------------------------------- backward
 // With G_t the whole gradient of h_t, r_t = a_t G_t is what token t - 1 receives:
-//   G_t = dy_t + r_{t+1}, advanced as G <- G + (am1 G + dy) with the am1 of the token behind.
-// A segment folds into (sum of z, r of its first token from r = 0).
-template <int DT, int V>
-__global__ __launch_bounds__(kGatedThreads) void gated_bwd_summary_kernel(const GatedArgs a) {
-    int c, b, g;
-    if (!place<V>(a, c, b, g)) return;
-    float inv_tau[V], G[V], lo[V], am1[V], zs[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) inv_tau[i] = 1.f / a.tau[c + i], G[i] = lo[i] = am1[i] = zs[i] = 0.f;
-    const int l0 = g * a.seg_len, l1 = min(l0 + a.seg_len, a.L);
-#pragma unroll 4
-    for (int l = l1 - 1; l >= l0; --l) {
-        float s[V], dy[V];
-        unpack<DT, V>(*at<DT, V>(a.step, b, l, c), s);
-        unpack<DT, V>(*at<DT, V>(a.dy, b, l, c), dy);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            float z;
-            advance(G[i], lo[i], am1[i], dy[i]);
-            decay(s[i], inv_tau[i], z, am1[i]);
-            zs[i] += z;
-        }
-    }
-    const int64_t o = (static_cast<int64_t>(b) * a.G + g) * a.C + c;
-#pragma unroll
-    for (int i = 0; i < V; ++i) a.ws_z[o + i] = zs[i], a.ws_h[o + i] = fmaf(am1[i], G[i], G[i]);
-}
-
-// Gradients of one segment, a tile of kGatedTile tokens at a time from its end:
-// the tile's states come again from its checkpoint, then
+//   G_t = dy_t + r_{t+1},
+// the forward's recurrence in reversed time, with the decay of the token behind.  The
+// wave's states come again from its checkpoint, then
 //   dz = G (a^2 / n  sigmoid x - a h_{t-1}),  n = sqrt(1 - a^2).
 template <int DT, int V>
-__global__ __launch_bounds__(kGatedThreads) void gated_bwd_kernel(const GatedArgs a) {
-    int c, b, g;
-    if (!place<V>(a, c, b, g)) return;
+__global__ __launch_bounds__(kThreads) void gated_bwd_kernel(const GatedArgs a) {
+    __shared__ SpanShared<V> sh;
     constexpr int T = kGatedTile;
-    float inv_tau[V], G[V], lo[V], am1[V], dtau[V];
-    const int64_t row = static_cast<int64_t>(b) * a.C + c;
+    const Place p = place<V>(a, sh);
+    const int span = a.G - 1 - p.g, l0 = span * kSpan + p.wave * T, n = min(T, a.L - l0);
+    const int64_t row = static_cast<int64_t>(p.b) * a.C + p.c;
+    float inv_tau[V], A[V], R[V];
+    // a token: x, dy, a - 1, h_{t-1}, sigmoid(gate), sigmoid(gate) / n, z, d z / d step
+    float xs[T][V], dys[T][V], am1[T][V], h[T][V], sg[T][V], sn[T][V], z[T][V], dzds[T][V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        inv_tau[i] = 1.f / a.tau[c + i];
-        dtau[i] = lo[i] = am1[i] = 0.f;
-        G[i] = a.dstate_out ? a.dstate_out[row + i] : 0.f;
-    }
-    for (int j = a.G - 1; j > g; --j) {
-        const int64_t o = (static_cast<int64_t>(b) * a.G + j) * a.C + c;
-#pragma unroll
-        for (int i = 0; i < V; ++i) advance(G[i], lo[i], expm1_neg(a.ws_z[o + i]), a.ws_h[o + i]);
-    }
-    const int l0 = g * a.seg_len, l1 = min(l0 + a.seg_len, a.L);
-    for (int t0 = l0 + (l1 - 1 - l0) / T * T; t0 >= l0; t0 -= T) {
-        float h[T][V];  // the state before each token
+    for (int i = 0; i < V; ++i) inv_tau[i] = 1.f / a.tau[p.c + i], A[i] = R[i] = 0.f;
+    {
+        typename Packed<DT, V>::type px[T], ps[T], pg[T], pd[T];
         float hc[V], hl[V];
-        const float *ck = a.ckpt + (static_cast<int64_t>(b) * a.tiles + t0 / T) * a.C + c;
+        const float *ck = a.ckpt + (static_cast<int64_t>(p.b) * a.tiles + min(l0 / T, a.tiles - 1)) * a.C + p.c;
 #pragma unroll
         for (int i = 0; i < V; ++i) hc[i] = ck[i], hl[i] = 0.f;
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            const int l = min(t0 + t, l1 - 1);
-            float x[V], s[V], gt[V];
-            unpack<DT, V>(*at<DT, V>(a.x, b, l, c), x);
-            unpack<DT, V>(*at<DT, V>(a.step, b, l, c), s);
-            unpack<DT, V>(*at<DT, V>(a.gate, b, l, c), gt);
+            const int l = min(l0 + t, a.L - 1);
+            px[t] = at<DT, V>(a.x, p.b, l, p.c);
+            ps[t] = at<DT, V>(a.step, p.b, l, p.c);
+            pg[t] = at<DT, V>(a.gate, p.b, l, p.c);
+            pd[t] = at<DT, V>(a.dy, p.b, l, p.c);
+        }
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            float s[V], g[V];
+            unpack<DT, V>(px[t], xs[t]);
+            unpack<DT, V>(ps[t], s);
+            unpack<DT, V>(pg[t], g);
+            unpack<DT, V>(pd[t], dys[t]);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
+                float e;
+                const float soft = softplus(s[i], e);
+                const float sp = __builtin_amdgcn_rcpf(1.f + e) * (s[i] < 0.f ? e : 1.f);  // softplus'
+                dzds[t][i] = soft < kStepMin || soft > kStepMax ? 0.f : inv_tau[i] * sp;
+                z[t][i] = clamp_step(soft) * inv_tau[i];
+                am1[t][i] = expm1_neg(z[t][i]);
+                const float q = -am1[t][i] * (2.f + am1[t][i]);
+                sg[t][i] = sigmoid(g[i]);
+                sn[t][i] = sg[t][i] * __builtin_amdgcn_rsqf(q);
                 h[t][i] = hc[i];
-                float z, d;
-                decay(s[i], inv_tau[i], z, d);
-                advance(hc[i], hl[i], d, __builtin_amdgcn_sqrtf(-d * (2.f + d)) * sigmoid(gt[i]) * x[i]);
+                advance(hc[i], hl[i], am1[t][i], q * sn[t][i] * xs[t][i]);
+                if (t >= n) am1[t][i] = dys[t][i] = 0.f;
             }
         }
 #pragma unroll
         for (int t = T - 1; t >= 0; --t) {
-            const int l = t0 + t;
-            if (l >= l1) continue;
-            float x[V], s[V], gt[V], dy[V], dx[V], ds[V], dg[V];
-            unpack<DT, V>(*at<DT, V>(a.x, b, l, c), x);
-            unpack<DT, V>(*at<DT, V>(a.step, b, l, c), s);
-            unpack<DT, V>(*at<DT, V>(a.gate, b, l, c), gt);
-            unpack<DT, V>(*at<DT, V>(a.dy, b, l, c), dy);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                float e;
-                advance(G[i], lo[i], am1[i], dy[i]);
-                const float soft = softplus(s[i], e), z = clamp_step(soft) * inv_tau[i];
-                am1[i] = expm1_neg(z);
-                const float q = -am1[i] * (2.f + am1[i]), rq = __builtin_amdgcn_rsqf(q), n = q * rq, sg = sigmoid(gt[i]);
-                const float al = 1.f + am1[i], Gx = G[i] * x[i];
-                dx[i] = G[i] * n * sg;
-                dg[i] = Gx * n * sg * (1.f - sg);
-                const float dz = al * (al * rq * sg * Gx - G[i] * h[t][i]);
-                const float sp = __builtin_amdgcn_rcpf(1.f + e) * (s[i] < 0.f ? e : 1.f);  // softplus'
-                ds[i] = soft < kStepMin || soft > kStepMax ? 0.f : dz * inv_tau[i] * sp;
-                dtau[i] -= dz * z * inv_tau[i];
+                const float G = dys[t][i] + R[i];
+                R[i] = fmaf(am1[t][i], G, G);
+                A[i] += fmaf(am1[t][i], A[i], am1[t][i]);
             }
-            *at_out<DT, V>(a.dx, b, l, c) = pack<DT, V>(dx);
-            *at_out<DT, V>(a.dstep, b, l, c) = pack<DT, V>(ds);
-            *at_out<DT, V>(a.dgate, b, l, c) = pack<DT, V>(dg);
         }
     }
-    const int64_t o = (static_cast<int64_t>(b) * a.G + g) * a.C + c;
+    float G[V], lo[V], behind[V], dtau[V];
+    join<V, true>(a, sh, p, p.g, a.dstate_out, A, R, G, lo);
+#pragma unroll
+    for (int i = 0; i < V; ++i) behind[i] = dtau[i] = 0.f;
+#pragma unroll
+    for (int t = T - 1; t >= 0; --t) {
+        float dx[V], ds[V], dg[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            advance(G[i], lo[i], behind[i], dys[t][i]);
+            behind[i] = am1[t][i];
+            const float al = 1.f + am1[t][i], q = -am1[t][i] * (2.f + am1[t][i]);
+            dx[i] = G[i] * (q * sn[t][i]);
+            dg[i] = dx[i] * xs[t][i] * (1.f - sg[t][i]);
+            const float dz = al * G[i] * fmaf(al * sn[t][i], xs[t][i], -h[t][i]);
+            ds[i] = dz * dzds[t][i];
+            if (t < n) dtau[i] = fmaf(-dz, z[t][i], dtau[i]);
+        }
+        if (t < n && p.in) {
+            at_out<DT, V>(a.dx, p.b, l0 + t, p.c) = pack<DT, V>(dx);
+            at_out<DT, V>(a.dstep, p.b, l0 + t, p.c) = pack<DT, V>(ds);
+            at_out<DT, V>(a.dgate, p.b, l0 + t, p.c) = pack<DT, V>(dg);
+        }
+    }
+    if (l0 == 0 && a.dstate_in && p.in) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) a.dstate_in[row + i] = fmaf(behind[i], G[i], G[i]);
+    }
+    // the span's part of dtau, wave by wave
+    const int lane = threadIdx.x % kWave;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < V; ++i) sh.A[p.wave][lane * V + i] = dtau[i];
+    __syncthreads();
+    if (p.wave || !p.in) return;
+    float *part = a.dtau_part + (static_cast<int64_t>(p.b) * a.G + span) * a.C + p.c;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        a.dtau_part[o + i] = dtau[i];
-        if (g == 0 && a.dstate_in) a.dstate_in[row + i] = fmaf(am1[i], G[i], G[i]);
+        float sum = 0.f;
+        for (int w = 0; w < kWaves; ++w) sum += sh.A[w][lane * V + i];
+        part[i] = sum * inv_tau[i];
     }
 }
 
-// dtau[c] = the sum of the segments' parts, in order
-__global__ __launch_bounds__(kGatedThreads) void gated_dtau_kernel(const GatedArgs a) {
-    const int c = blockIdx.x * blockDim.x + threadIdx.x;
-    if (c >= a.C) return;
+// dtau[c] = the sum of the spans' parts: 16 waves each take every 16th, in order, then
+// their sums in order.
+__global__ __launch_bounds__(1024) void gated_dtau_kernel(const GatedArgs a) {
+    __shared__ float part[16][kWave];
+    const int c = blockIdx.x * kWave + threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int64_t n = static_cast<int64_t>(a.B) * a.G;
     float s = 0.f;
-    for (int64_t j = 0; j < static_cast<int64_t>(a.B) * a.G; ++j) s += a.dtau_part[j * a.C + c];
+    if (c < a.C) {
+#pragma unroll 8
+        for (int64_t j = wave; j < n; j += 16) s += a.dtau_part[j * a.C + c];
+    }
+    part[wave][threadIdx.x % kWave] = s;
+    __syncthreads();
+    if (wave || c >= a.C) return;
+    for (int w = 1; w < 16; ++w) s += part[w][threadIdx.x];
     a.dtau[c] = s;
+}
+
+// The chain's words and the counter before them, all ones.
+__global__ __launch_bounds__(256) void gated_fill_kernel(uint4 *p, int64_t n) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (i < n) p[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
 }
 
 // ------------------------------------------------------------------ launch
 namespace {
 
-// Channels a lane: 4 bytes where every row allows it.
-int lane_channels(const GatedArgs &a) {
-    const int es = a.dt == PRIME_F32 ? 4 : 2, v = 2;
-    if (a.C % v) return 1;
+constexpr int kStepTokens = 4;  // up to here a lane walks the tokens
+
+// Whether every row allows V channels a lane.
+bool lanes_of(const GatedArgs &a, int v) {
+    const int es = a.dt == PRIME_F32 ? 4 : 2;
+    if (a.C % v) return false;
     for (const GatedView *t : {&a.x, &a.step, &a.gate, &a.y, &a.dy, &a.dx, &a.dstep, &a.dgate})
-        if (t->data && (reinterpret_cast<uintptr_t>(t->data) % (v * es) || t->sb % v || t->sl % v)) return 1;
-    return v;
+        if (t->data && (reinterpret_cast<uintptr_t>(t->data) % (v * es) || t->sb % v || t->sl % v)) return false;
+    return true;
 }
 
-// whole waves, at most kGatedThreads
-dim3 threads(int lanes) { return dim3(lanes >= kGatedThreads ? kGatedThreads : (lanes + kWave - 1) / kWave * kWave); }
+int spans_grid(const GatedArgs &a, int v) { return a.B * ((a.C + kWave * v - 1) / (kWave * v)) * a.G; }
+
+void fill(const GatedArgs &a, hipStream_t s) {
+    if (a.G == 1) return;
+    const int64_t n = static_cast<int64_t>(gated_chain_bytes(a.B, a.L, a.C) / 16);
+    hipLaunchKernelGGL(gated_fill_kernel, dim3((n + 255) / 256), dim3(256), 0, s, reinterpret_cast<uint4 *>(a.counter), n);
+}
 
 template <int DT, int V>
 void forward(const GatedArgs &a, hipStream_t s) {
-    const dim3 block = threads(a.C / V), grid(a.B * a.G, (a.C / V + block.x - 1) / block.x);
-    if (a.G > 1) hipLaunchKernelGGL((gated_summary_kernel<DT, V>), grid, block, 0, s, a);
-    hipLaunchKernelGGL((gated_scan_kernel<DT, V>), grid, block, 0, s, a);
+    if (a.L <= kStepTokens) {
+        const int lanes = (a.C + V - 1) / V, block = lanes >= 256 ? 256 : (lanes + kWave - 1) / kWave * kWave;
+        hipLaunchKernelGGL((gated_step_kernel<DT, V>), dim3(a.B * ((lanes + block - 1) / block)), dim3(block), 0, s, a);
+        return;
+    }
+    fill(a, s);
+    hipLaunchKernelGGL((gated_scan_kernel<DT, V>), dim3(spans_grid(a, V)), dim3(kThreads), 0, s, a);
 }
 
-template <int DT, int V>
+template <int DT>
 void backward(const GatedArgs &a, hipStream_t s) {
-    const dim3 block = threads(a.C / V), grid(a.B * a.G, (a.C / V + block.x - 1) / block.x);
-    if (a.G > 1) hipLaunchKernelGGL((gated_bwd_summary_kernel<DT, V>), grid, block, 0, s, a);
-    hipLaunchKernelGGL((gated_bwd_kernel<DT, V>), grid, block, 0, s, a);
-    hipLaunchKernelGGL(gated_dtau_kernel, dim3((a.C + kGatedThreads - 1) / kGatedThreads), dim3(kGatedThreads), 0, s,
-                       a);
+    fill(a, s);
+    hipLaunchKernelGGL((gated_bwd_kernel<DT, 1>), dim3(spans_grid(a, 1)), dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL(gated_dtau_kernel, dim3((a.C + kWave - 1) / kWave), dim3(1024), 0, s, a);
 }
 
 template <int DT>
 void run(const GatedArgs &a, bool bwd, hipStream_t s) {
-    if (lane_channels(a) == 2) return bwd ? backward<DT, 2>(a, s) : forward<DT, 2>(a, s);
-    return bwd ? backward<DT, 1>(a, s) : forward<DT, 1>(a, s);
+    if (bwd) return backward<DT>(a, s);
+    if (DT != PRIME_F32 && lanes_of(a, 2)) return forward<DT, 2>(a, s);
+    return forward<DT, 1>(a, s);
 }
 
 }  // namespace
 
-int gated_segments(int B, int L, int C, int *seg_len) {
-    // about 4096 waves of 64 lanes with two channels each, segments of whole tiles
-    const int64_t lanes = static_cast<int64_t>(B) * ((C + 1) / 2), tiles = (L + kGatedTile - 1) / kGatedTile;
-    int64_t g = 4096 * 64 / lanes;
-    g = g < 1 ? 1 : g > 64 ? 64 : g;
-    if (g > tiles) g = tiles;
-    const int64_t per = (tiles + g - 1) / g;
-    *seg_len = static_cast<int>(per * kGatedTile);
-    return static_cast<int>((tiles + per - 1) / per);
+int gated_spans(int L) { return (L + kSpan - 1) / kSpan; }
+
+// a 16-byte head with the counter, and a word per span and channel; 0 for one span
+size_t gated_chain_bytes(int B, int L, int C) {
+    const int G = gated_spans(L);
+    return G == 1 ? 0 : 16 + (static_cast<size_t>(B) * G * C * sizeof(uint64_t) + 15) / 16 * 16;
 }
 
 hipError_t launch_gated_scan(const GatedArgs &a, bool bwd, hipStream_t s) {

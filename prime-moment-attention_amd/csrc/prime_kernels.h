@@ -435,13 +435,14 @@ struct GatedArgs {
     const float *dstate_out;          // [B, C] or null
     float *dstate_in;                 // [B, C] or null
     float *dtau;                      // [C]
-    int tiles, G, seg_len;            // ceil(L / kGatedTile); segments of seg_len tokens
-    float *ws_z, *ws_h;               // [B, G, C] each: the segments' folds (G > 1)
-    float *ws_h0;                     // [B, C] (G > 1)
+    int tiles, G;                     // ceil(L / kGatedTile); spans (gated_spans)
+    uint32_t *counter;                // G > 1: numbers the workgroups; all ones before
+    uint64_t *words;                  // G > 1: [B, G, C], the spans' folds and states; all ones before
     float *dtau_part;                 // [B, G, C]
 };
-constexpr int kGatedTile = 16, kGatedThreads = 256;
-int gated_segments(int B, int L, int C, int *seg_len);
+constexpr int kGatedTile = 16;
+int gated_spans(int L);
+size_t gated_chain_bytes(int B, int L, int C);
 hipError_t launch_gated_scan(const GatedArgs &a, bool bwd, hipStream_t stream);
 
 // Dropout with the residual add (dropout.hip).

@@ -12,7 +12,7 @@ from prime_moment_attention import GatedLinearRecurrence, _lib, dropout_add, gat
 
 BF, F32 = _lib.PRIME_BF16, _lib.PRIME_F32
 AT = [(i + 1) << 24 for i in range(20)]  # addresses far apart; never dereferenced
-B, L, C = 2, 40, 64
+B, L, C = 2, 400, 64
 
 
 def seq(addr, sl=C, sb=L * C):
