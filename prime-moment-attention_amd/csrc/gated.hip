@@ -140,7 +140,7 @@ __device__ __forceinline__ uint64_t peek(const uint64_t *w) {
 // are joined first, so that from one head's state to the next one's is one word's way.
 // `words` is this channel's word of span 0, `stride` apart; called for g > 0 only.
 __device__ __forceinline__ void chain_in(const uint64_t *words, int64_t stride, int g, float &h, float &lo) {
-    constexpr int U = 5;  // words in flight
+    constexpr int U = 3;  // words in flight; more spill the backward's registers
     const int head = (g - 1) / kChain * kChain, n = g - 1 - head;
     uint64_t first = peek(words + head * stride);
     float A = 0.f, H = 0.f;
