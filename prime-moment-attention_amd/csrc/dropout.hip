@@ -11,6 +11,8 @@
 
 namespace prime {
 
+constexpr int kDropThreads = 256;
+
 // Ten rounds; k is the same in every lane.
 __device__ __forceinline__ void philox(uint64_t block, uint64_t counter, uint64_t seed, uint32_t (&w)[4]) {
     uint32_t c0 = static_cast<uint32_t>(block), c1 = static_cast<uint32_t>(block >> 32);
@@ -29,8 +31,94 @@ __device__ __forceinline__ void philox(uint64_t block, uint64_t counter, uint64_
     w[0] = c0, w[1] = c1, w[2] = c2, w[3] = c3;
 }
 
-__global__ __launch_bounds__(256) void dropout_add_kernel(const DropoutArgs a) {
-    const int64_t block = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, total = a.rows * a.cols;
+__device__ __forceinline__ bool kept(const uint32_t (&w)[4], int j, uint32_t cut) {
+    return (j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xFFFFu) >= cut;
+}
+
+// One lane, eight elements: a 16-byte access in 16-bit types, two in fp32.
+template <int DT>
+struct Eight {
+    static constexpr int N = DT == PRIME_F32 ? 2 : 1;
+    u32x4 v[N];
+    __device__ __forceinline__ void load(const void *p, int64_t e) {
+        const u32x4 *q = reinterpret_cast<const u32x4 *>(static_cast<const char *>(p) + e * (2 * N));
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __builtin_nontemporal_load(q + i);
+    }
+    __device__ __forceinline__ void store(void *p, int64_t e) const {
+        u32x4 *q = reinterpret_cast<u32x4 *>(static_cast<char *>(p) + e * (2 * N));
+#pragma unroll
+        for (int i = 0; i < N; ++i) q[i] = v[i];
+    }
+    __device__ __forceinline__ float get(int j) const {
+        if constexpr (DT == PRIME_F32) return __uint_as_float(v[j / 4][j % 4]);
+        const uint32_t u = v[0][j / 2];
+        if constexpr (DT == PRIME_BF16) return __uint_as_float(j & 1 ? u & 0xFFFF0000u : u << 16);
+        return h16_bits_to_f32(static_cast<uint16_t>(j & 1 ? u >> 16 : u));
+    }
+    __device__ __forceinline__ void set(const float (&f)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; j += DT == PRIME_F32 ? 1 : 2) {
+            if constexpr (DT == PRIME_F32) v[j / 4][j % 4] = __float_as_uint(f[j]);
+            else if constexpr (DT == PRIME_BF16) v[0][j / 2] = f32_to_bf16_bits(f[j]) | static_cast<uint32_t>(f32_to_bf16_bits(f[j + 1])) << 16;
+            else v[0][j / 2] = f32_to_h16_bits(f[j]) | static_cast<uint32_t>(f32_to_h16_bits(f[j + 1])) << 16;
+        }
+    }
+};
+
+// Rows whose blocks of eight start on 16 bytes.  FLAT: the rows lie one after the other, so
+// the elements are one row of any length.  U blocks a lane, their loads first, the random
+// bits while they are under way.
+template <int DT, bool RES, bool FLAT>
+__global__ __launch_bounds__(kDropThreads) void dropout_add_kernel(const DropoutArgs a) {
+    constexpr int U = 2;
+    const int64_t total = a.rows * a.cols, j0 = static_cast<int64_t>(blockIdx.x) * (U * kDropThreads) + threadIdx.x;
+    const uint64_t counter = static_cast<uint64_t>(a.rng[1]) + static_cast<uint64_t>(a.call), seed = a.rng[0];
+    Eight<DT> x[U], r[U];
+    int64_t ox[U], orr[U], oo[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t e = (j0 + u * kDropThreads) * 8;
+        ox[u] = orr[u] = oo[u] = e;
+        if constexpr (!FLAT) {
+            const int64_t row = e / a.cols, col = e % a.cols;
+            ox[u] = row * a.ldx + col, orr[u] = row * a.ldr + col, oo[u] = row * a.ldo + col;
+        }
+        if (e + 8 <= total) {
+            x[u].load(a.x, ox[u]);
+            if constexpr (RES) r[u].load(a.residual, orr[u]);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t block = j0 + u * kDropThreads, e = block * 8;
+        if (e >= total) return;
+        uint32_t w[4];
+        philox(block, counter, seed, w);
+        if (e + 8 <= total) {
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                f[j] = kept(w, j, a.cut) ? x[u].get(j) * a.scale : 0.f;
+                if constexpr (RES) f[j] += r[u].get(j);
+            }
+            x[u].set(f);
+            x[u].store(a.out, oo[u]);
+        } else {  // the last elements of one long row
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (e + j >= total) continue;
+                float f = kept(w, j, a.cut) ? load_elem(a.x, e + j, DT) * a.scale : 0.f;
+                if constexpr (RES) f += load_elem(a.residual, e + j, DT);
+                store_elem(a.out, e + j, DT, f);
+            }
+        }
+    }
+}
+
+// Any rows: element by element.
+__global__ __launch_bounds__(kDropThreads) void dropout_any_kernel(const DropoutArgs a) {
+    const int64_t block = static_cast<int64_t>(blockIdx.x) * kDropThreads + threadIdx.x, total = a.rows * a.cols;
     if (block * 8 >= total) return;
     uint32_t w[4];
     philox(block, static_cast<uint64_t>(a.rng[1]) + static_cast<uint64_t>(a.call), static_cast<uint64_t>(a.rng[0]), w);
@@ -38,8 +126,7 @@ __global__ __launch_bounds__(256) void dropout_add_kernel(const DropoutArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         if (block * 8 + j < total) {
-            const uint32_t bits = j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xFFFFu;
-            float v = bits >= a.cut ? load_elem(a.x, row * a.ldx + col, a.dt) * a.scale : 0.f;
+            float v = kept(w, j, a.cut) ? load_elem(a.x, row * a.ldx + col, a.dt) * a.scale : 0.f;
             if (a.residual) v += load_elem(a.residual, row * a.ldr + col, a.dt);
             store_elem(a.out, row * a.ldo + col, a.dt, v);
         }
@@ -47,9 +134,32 @@ __global__ __launch_bounds__(256) void dropout_add_kernel(const DropoutArgs a) {
     }
 }
 
+namespace {
+
+template <int DT>
+void run(const DropoutArgs &a, bool flat, dim3 grid, hipStream_t s) {
+    const dim3 block(kDropThreads);
+    if (a.residual && flat) hipLaunchKernelGGL((dropout_add_kernel<DT, true, true>), grid, block, 0, s, a);
+    else if (a.residual) hipLaunchKernelGGL((dropout_add_kernel<DT, true, false>), grid, block, 0, s, a);
+    else if (flat) hipLaunchKernelGGL((dropout_add_kernel<DT, false, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((dropout_add_kernel<DT, false, false>), grid, block, 0, s, a);
+}
+
+}  // namespace
+
 hipError_t launch_dropout_add(const DropoutArgs &a, hipStream_t stream) {
-    const int64_t blocks = (a.rows * a.cols + 7) / 8;
-    hipLaunchKernelGGL(dropout_add_kernel, dim3(static_cast<unsigned>((blocks + 255) / 256)), dim3(256), 0, stream, a);
+    const int64_t blocks = (a.rows * a.cols + 7) / 8, es = a.dt == PRIME_F32 ? 4 : 2;
+    auto grid = [&](int per) { return dim3(static_cast<unsigned>((blocks + per - 1) / per)); };
+    auto starts = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    auto aligned = [&](const void *p, int64_t ld) { return starts(p) && ld * es % 16 == 0; };
+    const bool flat = a.rows == 1 || (a.ldx == a.cols && a.ldo == a.cols && (!a.residual || a.ldr == a.cols));
+    const bool wide = flat ? starts(a.x) && starts(a.out) && starts(a.residual)
+                           : a.cols % 8 == 0 && aligned(a.x, a.ldx) && aligned(a.out, a.ldo) &&
+                                 (!a.residual || aligned(a.residual, a.ldr));
+    if (!wide) hipLaunchKernelGGL(dropout_any_kernel, grid(kDropThreads), dim3(kDropThreads), 0, stream, a);
+    else if (a.dt == PRIME_BF16) run<PRIME_BF16>(a, flat, grid(2 * kDropThreads), stream);
+    else if (a.dt == PRIME_F16) run<PRIME_F16>(a, flat, grid(2 * kDropThreads), stream);
+    else run<PRIME_F32>(a, flat, grid(2 * kDropThreads), stream);
     return hipGetLastError();
 }
 
