@@ -23,7 +23,8 @@ namespace prime {
 constexpr uint64_t kMass = 1ull << 42;  // the largest token's
 constexpr int kBuckets = 2048, kList = 1024;
 constexpr int kSampleSmall = 4096;  // up to here a row takes 4 waves, else 16
-constexpr float kBucketSpan = 30.5f;  // a token this many T below the largest has mass 0
+constexpr double kLightest = -43.5;    // a token of weight 2^-43.5 or less has mass 0
+constexpr float kBucketSpan = 30.5f;  // so has one this many T below the largest
 constexpr float kInf = __builtin_inff();
 
 // order-preserving image of a logit, -0 as +0
@@ -35,37 +36,50 @@ __device__ __forceinline__ float key_logit(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
+// a b + c with c from scalar registers (left alone, the compiler copies c into the
+// accumulator first: a move for every multiply-add)
+__device__ __forceinline__ double fma_s(double a, double b, double c) {
+    double r;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+    return r;
+}
+
 // What the tokens of a row are weighed by.
 struct RowScale {
     float top;        // the largest logit
     double rate;      // log2(e) / T
-    double least;     // log2 of min_p; -infinity without
+    double least;     // log2 of min_p, at least kLightest
     float per_half;   // buckets per half a unit of the logit
 
     __device__ __forceinline__ double exponent(float x) const {  // of 2, at most 0
         return (static_cast<double>(x) - static_cast<double>(top)) * rate;
     }
-    // 2^t as a mass: 2^f on |f| <= 1/2 by its Chebyshev interpolant of degree 9 (1.4e-14
-    // off), scaled and rounded to a whole number by one addition to 2^52.
+    // 2^t as a mass, -44 <= t <= 0 (below, the result means nothing): 2^f on |f| <= 1/2 by
+    // its Chebyshev interpolant of degree 9 (1.4e-14 off), scaled and rounded to a whole
+    // number by one addition to 2^52.
     __device__ static __forceinline__ uint64_t mass_of(double t) {
         constexpr double kRound = 6755399441055744.0;  // 1.5 2^52: adding it rounds to a whole number
-        t = fmax(t, -64.0);
         const double r = t + kRound, f = t - (r - kRound);
-        double p = 1.0212097549811005e-07;
-        p = fma(p, f, 1.3259945262689143e-06);
-        p = fma(p, f, 1.5252640059770786e-05);
-        p = fma(p, f, 0.00015403432339553542);
-        p = fma(p, f, 0.001333355825801874);
-        p = fma(p, f, 0.009618129195951041);
-        p = fma(p, f, 0.05550410866428854);
-        p = fma(p, f, 0.24022650695631514);
-        p = fma(p, f, 0.6931471805599526);
+        double p = fma_s(1.0212097549811005e-07, f, 1.3259945262689143e-06);
+        p = fma_s(p, f, 1.5252640059770786e-05);
+        p = fma_s(p, f, 0.00015403432339553542);
+        p = fma_s(p, f, 0.001333355825801874);
+        p = fma_s(p, f, 0.009618129195951041);
+        p = fma_s(p, f, 0.05550410866428854);
+        p = fma_s(p, f, 0.24022650695631514);
+        p = fma_s(p, f, 0.6931471805599526);
         p = fma(p, f, 1.0);
         const uint32_t n = static_cast<uint32_t>(__builtin_bit_cast(uint64_t, r));  // low word: the whole number
         const double scale = __builtin_bit_cast(double, static_cast<uint64_t>((n + 1023u + 42u) << 20) << 32);
-        return __builtin_bit_cast(uint64_t, fma(p, scale, 4503599627370496.0)) - 0x4330000000000000ull;
+        uint64_t w = __builtin_bit_cast(uint64_t, fma(p, scale, 4503599627370496.0)) - 0x4330000000000000ull;
+        asm("" : "+v"(w));  // computed for every token: a branch around it costs more than it saves
+        return w;
     }
-    __device__ __forceinline__ uint64_t mass(float x) const { return mass_of(exponent(x)); }
+    __device__ __forceinline__ uint64_t mass(float x) const {
+        const double t = exponent(x);
+        return select(t >= kLightest, mass_of(t));
+    }
+    __device__ static __forceinline__ uint64_t select(bool keep, uint64_t w) { return keep ? w : 0; }
     // bucket of x, false for tokens whose mass is 0 (and for NaN); monotone: every step is
     __device__ __forceinline__ bool bucket(float x, int &b) const {
         const float f = fmaf(-0.5f, x, 0.5f * top) * per_half;
@@ -74,17 +88,26 @@ struct RowScale {
     }
 };
 
-__device__ __forceinline__ uint64_t shfl_u64(uint64_t v, int lane) {
-    return static_cast<uint64_t>(__shfl(static_cast<uint32_t>(v >> 32), lane, kWave)) << 32 |
-           __shfl(static_cast<uint32_t>(v), lane, kWave);
+// v of lane 63
+__device__ __forceinline__ uint64_t last_lane(uint64_t v) {
+    return static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), 63)) << 32 |
+           static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
 }
-__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {  // inclusive
-    const int lane = threadIdx.x % kWave;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-        const uint32_t lo = __shfl_up(static_cast<uint32_t>(v), o, kWave), hi = __shfl_up(static_cast<uint32_t>(v >> 32), o, kWave);
-        if (lane >= o) v += static_cast<uint64_t>(hi) << 32 | lo;
-    }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_u64(uint64_t v) {  // 0 where the move has no source
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CTRL, ROWS, 0xF, false);
+    return static_cast<uint64_t>(hi) << 32 | lo;
+}
+// inclusive sum over the lanes, on the vector unit: shifts within rows of 16, then the last
+// lane of row 0 (2) into row 1 (3), then lane 31 into rows 2 and 3
+__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {
+    v += dpp_u64<0x111, 0xF>(v);
+    v += dpp_u64<0x112, 0xF>(v);
+    v += dpp_u64<0x114, 0xF>(v);
+    v += dpp_u64<0x118, 0xF>(v);
+    v += dpp_u64<0x142, 0xA>(v);
+    v += dpp_u64<0x143, 0xC>(v);
     return v;
 }
 
@@ -96,38 +119,43 @@ struct SampleShared {
     uint64_t part[WAVES];
     uint64_t sum, ties;
     float last;
-    int bucket, n, index;
+    int bucket, n, index, owner;
+    bool whole;
 };
 
-// exclusive sum over the threads, and the total
+// exclusive sum over the threads, the sum over the waves before, and the total
 template <int WAVES>
-__device__ __forceinline__ uint64_t block_scan(SampleShared<WAVES> &sh, uint64_t v, uint64_t &total) {
+__device__ __forceinline__ uint64_t block_scan(SampleShared<WAVES> &sh, uint64_t v, uint64_t &waves, uint64_t &total) {
     const uint64_t inc = wave_scan_u64(v);
     const int wave = threadIdx.x / kWave;
     __syncthreads();
     if (threadIdx.x % kWave == kWave - 1) sh.part[wave] = inc;
     __syncthreads();
-    uint64_t before = 0;
-    total = 0;
+    waves = total = 0;
 #pragma unroll
     for (int i = 0; i < WAVES; ++i) {
-        if (i == wave) before = total;
-        total += sh.part[i];
+        const uint64_t p = sh.part[i];
+        waves += i < wave ? p : 0;
+        total += p;
     }
-    return before + inc - v;
+    return waves + inc - v;
 }
 
 // A row: wave w has the chunks [w per, (w + 1) per) of 64 lanes with VE elements each.
 // Elements past the vocabulary are -infinity.
+// The first `staged` chunks of every wave are in LDS once stage() has run.
 template <int DT>
 struct SampleRow {
     static constexpr int VE = DT == PRIME_F32 ? 4 : 8, es = DT == PRIME_F32 ? 4 : 2;
     const char *base;
     int vocab, per, start;  // start: the lane's first element
-    bool wide, infinite;    // 16-byte loads; some logit is +infinity: those are 0, all others -infinity
+    bool wide;              // 16-byte loads
+    u32x4 *lds;             // the lane's place in the staged chunks, `lds_step` between two
+    int staged, lds_step;
 
     __device__ __forceinline__ int index(int i) const { return start + i * (kWave * VE); }
-    __device__ __forceinline__ u32x4 fetch(int i) const {
+    __device__ __forceinline__ u32x4 fetch(int i) const { return i < staged ? lds[i * lds_step] : load(i); }
+    __device__ __forceinline__ u32x4 load(int i) const {
         constexpr uint32_t none = DT == PRIME_F32 ? 0xFF800000u : DT == PRIME_BF16 ? 0xFF80FF80u : 0xFC00FC00u;
         const int e = index(i);
         u32x4 v = {none, none, none, none};
@@ -153,36 +181,100 @@ struct SampleRow {
             if constexpr (DT == PRIME_F32) x[j] = __uint_as_float(v[j]);
             else if constexpr (DT == PRIME_BF16) x[j] = __uint_as_float(j & 1 ? v[j / 2] & 0xFFFF0000u : v[j / 2] << 16);
             else x[j] = h16_bits_to_f32(static_cast<uint16_t>(j & 1 ? v[j / 2] >> 16 : v[j / 2]));
-            if (infinite) x[j] = x[j] == kInf ? 0.f : -kInf;
         }
     }
-    // f(i, x) over the lane's chunks, the next ones under way
-    template <typename F>
+    // f(i, x) over the lane's chunks, U loads in flight
+    template <int U, typename F>
     __device__ __forceinline__ void each(F f) const {
-        constexpr int U = 2;
-        u32x4 next[U];
-#pragma unroll
-        for (int k = 0; k < U; ++k) next[k] = fetch(k);
         for (int i0 = 0; i0 < per; i0 += U) {
-            u32x4 now[U];
+            u32x4 v[U];
 #pragma unroll
-            for (int k = 0; k < U; ++k) now[k] = next[k], next[k] = fetch(i0 + U + k);
+            for (int k = 0; k < U; ++k)
+                if (i0 + k < per) v[k] = fetch(i0 + k);
 #pragma unroll
             for (int k = 0; k < U; ++k) {
-                float x[VE];
-                widen(now[k], x);
-                if (i0 + k < per) f(i0 + k, x);
+                if (i0 + k < per) {
+                    float x[VE];
+                    widen(v[k], x);
+                    f(i0 + k, x);
+                }
             }
+        }
+    }
+    // the first pass: f over the row as it comes from memory, into LDS what has place there
+    template <typename F>
+    __device__ __forceinline__ void stage(F f) {
+        constexpr int U = 8;
+        for (int i0 = 0; i0 < per; i0 += U) {
+            u32x4 v[U];
+#pragma unroll
+            for (int k = 0; k < U; ++k)
+                if (i0 + k < per) v[k] = load(i0 + k);
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                if (i0 + k >= per) continue;
+                if (i0 + k < staged) lds[(i0 + k) * lds_step] = v[k];
+                float x[VE];
+                widen(v[k], x);
+                f(i0 + k, x);
+            }
+        }
+    }
+    // the same for passes with much to compute, the next load under way
+    template <typename F>
+    __device__ __forceinline__ void each_heavy(F f) const {
+        u32x4 next = fetch(0);
+        for (int i = 0; i < per; ++i) {
+            const u32x4 now = next;
+            if (i + 1 < per) next = fetch(i + 1);
+            float x[VE];
+            widen(now, x);
+            f(i, x);
         }
     }
 };
 
+// How many tokens are equal to `value`; `nth` of that count gives n, and the index of the
+// n-th of them, from 1, is returned (any index where there are fewer).
+template <int DT, int WAVES, typename F>
+__device__ __forceinline__ int find_equal(SampleShared<WAVES> &sh, const SampleRow<DT> &row, float value, F nth) {
+    constexpr int VE = SampleRow<DT>::VE;
+    uint64_t count = 0, before, total;
+    row.template each<4>([&](int, const float (&x)[VE]) {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) count += x[j] == value;
+    });
+    block_scan(sh, count, before, total);
+    const uint64_t n = nth(total);
+    if (before < n && n <= before + sh.part[threadIdx.x / kWave]) {
+        // this wave's chunks one after the other, lanes in order within one
+        int left = static_cast<int>(n - before);
+        row.template each<4>([&](int i, const float (&x)[VE]) {
+            int all = 0, lower = 0;  // of the chunk, of the lanes below
+#pragma unroll
+            for (int j = 0; j < VE; ++j) {
+                const uint64_t b = __ballot(x[j] == value);
+                all += __popcll(b);
+                lower += __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(b >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(b), 0));
+            }
+            int skip = left - lower;  // the skip-th of this lane's is the one
+#pragma unroll
+            for (int j = 0; j < VE; ++j)
+                if (x[j] == value && --skip == 0) sh.index = row.index(i) + j;
+            left -= all;
+        });
+    }
+    __syncthreads();
+    return sh.index;
+}
+
 // The cut: over the tokens above `last` and `ties` tokens equal to it (none for -infinity),
 // in rank order, the shortest prefix with weight of at least wanted(sum of all weights).
-// WEIGH: masses, else ones.  Left as it is where all of them are needed.
+// WEIGH: masses, else ones.  Left as it is where all of them are needed.  whole: the tokens
+// equal to the new `last` are known to be all kept.
 template <bool WEIGH, int DT, int WAVES, typename F>
 __device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT> &row, const RowScale &rs,
-                                    float &last, uint64_t &ties, F wanted) {
+                                    float &last, uint64_t &ties, bool &whole, F wanted) {
     constexpr int kThreads = WAVES * kWave, kPer = kBuckets / kThreads, VE = SampleRow<DT>::VE;
     const int tid = threadIdx.x;
     const float floor = last;
@@ -194,7 +286,7 @@ __device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT>
     for (int b = tid; b < kBuckets; b += kThreads) sh.hist[b] = 0;
     if (tid == 0) sh.n = 0, sh.bucket = -1;
     __syncthreads();
-    row.each([&](int, const float (&x)[VE]) {
+    auto fill = [&](int, const float (&x)[VE]) {
         bool any = false;
 #pragma unroll
         for (int j = 0; j < VE; ++j) any |= x[j] > floor;
@@ -205,15 +297,17 @@ __device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT>
             const uint64_t w = WEIGH ? rs.mass(x[j]) : 1;
             if (rs.bucket(x[j], b) && x[j] > floor) add(&sh.hist[b], w);
         }
-    });
+    };
+    if constexpr (WEIGH) row.each_heavy(fill);
+    else row.template each<4>(fill);
     int floor_b = -1;
     if (floor_w && !rs.bucket(floor, floor_b)) floor_b = -1;
     if (tid == 0 && floor_b >= 0) add(&sh.hist[floor_b], floor_w);
     __syncthreads();
-    uint64_t mine = 0, total;
+    uint64_t mine = 0, waves, total;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) mine += sh.hist[tid * kPer + i];
-    uint64_t before = block_scan(sh, mine, total);
+    uint64_t before = block_scan(sh, mine, waves, total);
     const uint64_t want = wanted(total);
     if (want > total) return;  // (the same for every thread)
     if (before < want && want <= before + mine) {
@@ -227,7 +321,7 @@ __device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT>
     __syncthreads();
     const int bucket = sh.bucket;
     const uint64_t above = sh.sum;
-    row.each([&](int, const float (&x)[VE]) {
+    row.template each<4>([&](int, const float (&x)[VE]) {
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
             int b;
@@ -243,10 +337,12 @@ __device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT>
     }
     __syncthreads();
     const int n = sh.n;
-    auto found = [&](float x, uint64_t over) {  // `over`: the weight of the tokens above x
-        const uint64_t w = WEIGH ? rs.mass(x) : 1;
+    // `over`: the weight of the tokens above x; `equal`: of those equal to it, where known
+    auto found = [&](float x, uint64_t over, uint64_t equal) {
+        const uint64_t w = WEIGH ? rs.mass(x) : 1, n = (want - over + w - 1) / w;
         sh.last = x;
-        sh.ties = (want - over + w - 1) / w;
+        sh.ties = n;
+        sh.whole = x != floor && n * w == equal;
     };
     if (n <= kList) {
         for (int i = tid; i < n; i += kThreads) {
@@ -258,7 +354,7 @@ __device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT>
                 over += y > x ? w : 0;
                 equal += y == x ? w : 0;
             }
-            if (over < want && want <= over + equal) found(x, over);
+            if (over < want && want <= over + equal) found(x, over, equal);
         }
     } else {
         // the largest key with enough weight at and above it, eight bits at a time
@@ -270,7 +366,7 @@ __device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT>
             __syncthreads();
             if (tid < 256) sh.hist[tid] = 0;
             __syncthreads();
-            row.each([&](int, const float (&x)[VE]) {
+            row.each_heavy([&](int, const float (&x)[VE]) {
 #pragma unroll
                 for (int j = 0; j < VE; ++j) {
                     const uint32_t k = logit_key(x[j]);
@@ -289,16 +385,18 @@ __device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT>
             over = sh.sum;
             prefix = static_cast<uint32_t>(sh.n);
         }
-        if (tid == 0) found(key_logit(prefix), over);
+        if (tid == 0) found(key_logit(prefix), over, 0);
     }
     __syncthreads();
     last = sh.last;
     ties = sh.ties;
+    whole = sh.whole;
 }
 
-template <int DT, int WAVES>
+template <int DT, int WAVES, int STAGED>
 __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a) {
     __shared__ SampleShared<WAVES> sh;
+    __shared__ u32x4 stage[STAGED > 0 ? STAGED * WAVES * kWave : 1];
     using Row = SampleRow<DT>;
     constexpr int VE = Row::VE;
     const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave), r = blockIdx.x;
@@ -308,7 +406,9 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
     row.per = (a.vocab + WAVES * kWave * VE - 1) / (WAVES * kWave * VE);
     row.start = (wave * row.per * kWave + lane) * VE;
     row.wide = reinterpret_cast<uintptr_t>(row.base) % 16 == 0;
-    row.infinite = false;
+    row.staged = STAGED;
+    row.lds = stage + tid;
+    row.lds_step = WAVES * kWave;
     const float T = a.temperatures ? a.temperatures[r] : a.temperature;
     const float top_p = a.top_ps ? a.top_ps[r] : a.top_p, min_p = a.min_ps ? a.min_ps[r] : a.min_p;
     int top_k = a.top_ks ? a.top_ks[r] : a.top_k;
@@ -318,7 +418,7 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
     // the largest logit (fmaxf passes over NaN)
     RowScale rs;
     float top = -kInf;
-    row.each([&](int, const float (&x)[VE]) {
+    row.stage([&](int, const float (&x)[VE]) {
 #pragma unroll
         for (int j = 0; j < VE; ++j) top = fmaxf(top, x[j]);
     });
@@ -349,7 +449,7 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
     }
     if (!(T > 0.f) || top_k == 1 || top_p <= 0.f) {  // the first of the largest
         int first = a.vocab;
-        row.each([&](int i, const float (&x)[VE]) {
+        row.template each<4>([&](int i, const float (&x)[VE]) {
 #pragma unroll
             for (int j = VE - 1; j >= 0; --j)
                 if (x[j] == top) first = min(first, row.index(i) + j);
@@ -361,110 +461,122 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
         if (tid == 0) a.out[r] = sh.index;
         return;
     }
-    row.infinite = top == kInf;
-    rs.top = row.infinite ? 0.f : top;
+    if (top == kInf) {  // the infinite ones share the weight
+        const int index = find_equal(sh, row, top, [&](uint64_t n) {
+            if (n > static_cast<uint64_t>(top_k)) n = top_k;
+            if (top_p < 1.f) n = (share(n * kMass) + kMass - 1) / kMass;
+            return target_of(n * kMass) / kMass + 1;
+        });
+        if (tid == 0) a.out[r] = index;
+        return;
+    }
+    rs.top = top;
     rs.rate = 1.4426950408889634074 / static_cast<double>(T);
-    rs.least = min_p > 0.f ? log2(static_cast<double>(min_p < 1.f ? min_p : 1.f)) : -1e300;
+    rs.least = min_p > 0.f ? fmax(log2(static_cast<double>(min_p < 1.f ? min_p : 1.f)), kLightest) : kLightest;
     rs.per_half = fminf(2.f * (kBuckets - 1) / (kBucketSpan * T), 1e30f);
 
+    // kept are the tokens above `last`; where the cut runs through equal ones (split), also
+    // those equal to it up to tie_index
     float last = -kInf;
     uint64_t ties = 0;
-    if (top_k < a.vocab) cut<false>(sh, row, rs, last, ties, [&](uint64_t) { return static_cast<uint64_t>(top_k); });
-    if (top_p < 1.f) cut<true>(sh, row, rs, last, ties, share);
-
-    // the index up to which tokens equal to `last` are kept
+    bool whole = true;
+    if (top_k < a.vocab) cut<false>(sh, row, rs, last, ties, whole, [&](uint64_t) { return static_cast<uint64_t>(top_k); });
+    if (top_p < 1.f) cut<true>(sh, row, rs, last, ties, whole, share);
     int tie_index = -1;
-    if (ties) {
-        int mine = 0;
-        row.each([&](int, const float (&x)[VE]) {
-#pragma unroll
-            for (int j = 0; j < VE; ++j) mine += x[j] == last;
+    bool split = ties && !whole;
+    if (split)
+        tie_index = find_equal(sh, row, last, [&](uint64_t total) {
+            split = total > ties;
+            return ties;
         });
-        uint64_t total;
-        const uint64_t in_wave = wave_scan_u64(mine);
-        block_scan(sh, mine, total);
-        tie_index = a.vocab;
-        if (total > ties) {
-            uint64_t before = 0;
-            for (int i = 0; i < wave; ++i) before += sh.part[i];
-            if (before < ties && ties <= before + shfl_u64(in_wave, kWave - 1)) {
-                // this wave's chunks one after the other, lanes in order within one
-                int left = static_cast<int>(ties - before);
-                row.each([&](int i, const float (&x)[VE]) {
-                    int n = 0;
-#pragma unroll
-                    for (int j = 0; j < VE; ++j) n += x[j] == last;
-                    const int inc = static_cast<int>(wave_scan_u64(n)), all = __shfl(inc, kWave - 1, kWave);
-                    int skip = left - (inc - n);  // the skip-th of this lane's is the one
-                    if (left > 0 && skip >= 1 && skip <= n) {
-#pragma unroll
-                        for (int j = 0; j < VE; ++j)
-                            if (x[j] == last && --skip == 0) sh.index = row.index(i) + j;
-                    }
-                    left -= all;
-                });
-            }
-            __syncthreads();
-            tie_index = sh.index;
-        }
-    }
+    // all tokens equal to `last` are kept: the ones above the next value below it (below 0
+    // that is not -0)
+    if (ties && !split) last = key_logit(logit_key(last) - (last == 0.f ? 2 : 1));
 
-    auto chunk_masses = [&](int i, const float (&x)[VE], uint64_t (&m)[VE]) {
-        bool keep[VE], any = false;
-#pragma unroll
-        for (int j = 0; j < VE; ++j) {
-            keep[j] = x[j] > last || (x[j] == last && row.index(i) + j <= tie_index);
-            any |= keep[j];
-            m[j] = 0;
-        }
-        if (!any) return;
-#pragma unroll
-        for (int j = 0; j < VE; ++j) {
-            const double t = rs.exponent(x[j]);
-            const uint64_t w = RowScale::mass_of(t);
-            m[j] = keep[j] && t >= rs.least ? w : 0;
-        }
+    auto token_mass = [&](float x, int index, bool equals) -> uint64_t {
+        const double t = rs.exponent(x);
+        const uint64_t w = RowScale::mass_of(t);
+        bool keep = x > last;
+        if (equals) keep |= (x == last) & (index <= tie_index);
+        return RowScale::select(keep & (t >= rs.least), w);
     };
-    uint64_t mine = 0, total;
-    row.each([&](int i, const float (&x)[VE]) {
-        uint64_t m[VE];
-        chunk_masses(i, x, m);
+    auto chunk_mass = [&](int i, const float (&x)[VE]) {
+        float most = x[0];
+        uint64_t sum = 0;
 #pragma unroll
-        for (int j = 0; j < VE; ++j) mine += m[j];
-    });
-    block_scan(sh, mine, total);
+        for (int j = 1; j < VE; ++j) most = fmaxf(most, x[j]);
+        if (most >= last) {
+            if (split) {
+#pragma unroll
+                for (int j = 0; j < VE; ++j) sum += token_mass(x[j], row.index(i) + j, true);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VE; ++j) sum += token_mass(x[j], 0, false);
+            }
+        }
+        return sum;
+    };
+    uint64_t mine = 0, total, before;
+    row.each_heavy([&](int i, const float (&x)[VE]) { mine += chunk_mass(i, x); });
+    block_scan(sh, mine, before, total);
     const uint64_t target = target_of(total);
-    uint64_t before = 0;
-    for (int i = 0; i < wave; ++i) before += sh.part[i];
-    if (target < before || target - before >= sh.part[wave]) return;
-    // this wave has the token: its chunks one after the other
-    bool done = false;
-    row.each([&](int i, const float (&x)[VE]) {
-        if (done) return;  // the same in every lane
-        uint64_t m[VE], sum = 0;
-        chunk_masses(i, x, m);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) sum += m[j];
-        const uint64_t inc = wave_scan_u64(sum), all = shfl_u64(inc, kWave - 1);
-        if (target - before < all) {
-            uint64_t at = before + inc - sum;
+    // the wave with the token, then its chunks, taken by all waves 64 lanes' sums each
+    if (lane == 0 && before <= target && target - before < sh.part[wave]) sh.owner = wave, sh.sum = before;
+    __syncthreads();
+    before = sh.sum;
+    const int shift = sh.owner - wave;
+    row.start += shift * row.per * (kWave * VE);
+    row.lds += shift * kWave;
+    constexpr int kRound = kBuckets / kWave;  // chunks whose sums fit
+    for (int i0 = 0; i0 < row.per; i0 += kRound) {
+        const int n = min(kRound, row.per - i0);
+        __syncthreads();
+        for (int i = wave; i < n; i += WAVES) {
+            float x[VE];
+            row.widen(row.fetch(i0 + i), x);
+            sh.hist[i * kWave + lane] = chunk_mass(i0 + i, x);
+        }
+        __syncthreads();
+        if (wave) continue;
+        // in order: lane by lane, chunk by chunk; here a lane takes n sums in a row
+        uint64_t sum = 0;
+        for (int k = 0; k < n; ++k) sum += sh.hist[lane * n + k];
+        const uint64_t inc = wave_scan_u64(sum);
+        uint64_t at = before + inc - sum;
+        if (at <= target && target < before + inc) {
+            int k = lane * n;
+            while (target - at >= sh.hist[k]) at += sh.hist[k++];
+            // sum k is lane k % 64's of chunk k / 64
+            const int other = k % kWave - lane;
+            SampleRow<DT> its = row;
+            its.start += other * VE;
+            its.lds += other;
+            float x[VE];
+            its.widen(its.fetch(i0 + k / kWave), x);
 #pragma unroll
             for (int j = 0; j < VE; ++j) {
-                if (at <= target && target < at + m[j]) a.out[r] = row.index(i) + j;
-                at += m[j];
+                const int index = its.index(i0 + k / kWave) + j;
+                const uint64_t m = token_mass(x[j], index, split);
+                if (at <= target && target < at + m) a.out[r] = index;
+                at += m;
             }
-            done = true;
         }
-        before += all;
-    });
+        before += last_lane(inc);
+    }
 }
 
 namespace {
 
+template <int DT, int WAVES, int STAGED>
+void launch(const SampleArgs &a, hipStream_t s) {
+    hipLaunchKernelGGL((sample_kernel<DT, WAVES, STAGED>), dim3(a.n), dim3(WAVES * kWave), 0, s, a);
+}
+
 template <int DT>
 void run(const SampleArgs &a, hipStream_t s) {
-    if (a.vocab <= kSampleSmall) hipLaunchKernelGGL((sample_kernel<DT, 4>), dim3(a.n), dim3(4 * kWave), 0, s, a);
-    else hipLaunchKernelGGL((sample_kernel<DT, 16>), dim3(a.n), dim3(16 * kWave), 0, s, a);
+    if (a.vocab <= kSampleSmall) launch<DT, 4, DT == PRIME_F32 ? 4 : 2>(a, s);
+    else if (a.n <= 256) launch<DT, 16, 8>(a, s);
+    else launch<DT, 16, 0>(a, s);
 }
 
 }  // namespace
