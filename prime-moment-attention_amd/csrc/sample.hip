@@ -21,8 +21,7 @@
 namespace prime {
 
 constexpr uint64_t kMass = 1ull << 42;  // the largest token's
-constexpr int kBuckets = 2048, kList = 1024;
-constexpr int kSampleSmall = 4096;  // up to here a row takes 4 waves, else 16
+constexpr int kBuckets = 2048, kList = 1024, kFew = 256;
 constexpr double kLightest = -43.5;    // a token of weight 2^-43.5 or less has mass 0
 constexpr float kBucketSpan = 30.5f;  // so has one this many T below the largest
 constexpr float kInf = __builtin_inff();
@@ -117,10 +116,10 @@ struct SampleShared {
     uint64_t list_w[kList];
     float list_x[kList];
     uint64_t part[WAVES];
-    uint64_t sum, ties;
+    uint64_t sum, rest;
+    int list_i[kFew];
     float last;
-    int bucket, n, index, owner;
-    bool whole;
+    int bucket, n, index, owner, kept;
 };
 
 // exclusive sum over the threads, the sum over the waves before, and the total
@@ -141,39 +140,57 @@ __device__ __forceinline__ uint64_t block_scan(SampleShared<WAVES> &sh, uint64_t
     return waves + inc - v;
 }
 
-// A row: wave w has the chunks [w per, (w + 1) per) of 64 lanes with VE elements each.
-// Elements past the vocabulary are -infinity.
-// The first `staged` chunks of every wave are in LDS once stage() has run.
-template <int DT>
+// A row: wave w has the chunks [w per, (w + 1) per) of 64 lanes with VE elements each.  A
+// chunk past the vocabulary's end becomes the last VE elements, those that an earlier chunk
+// has as -infinity.  STAGED > 0: per is at most that, and after the first pass the row is in LDS.
+struct __attribute__((packed, aligned(2))) Raw {  // 16 bytes of a row, wherever it starts
+    u32x4 v;
+};
+template <int DT, int STAGED>
 struct SampleRow {
     static constexpr int VE = DT == PRIME_F32 ? 4 : 8, es = DT == PRIME_F32 ? 4 : 2;
     const char *base;
     int vocab, per, start;  // start: the lane's first element
-    bool wide;              // 16-byte loads
     u32x4 *lds;             // the lane's place in the staged chunks, `lds_step` between two
-    int staged, lds_step;
+    int lds_step;
 
-    __device__ __forceinline__ int index(int i) const { return start + i * (kWave * VE); }
-    __device__ __forceinline__ u32x4 fetch(int i) const { return i < staged ? lds[i * lds_step] : load(i); }
+    __device__ __forceinline__ int index(int i) const { return max(0, min(start + i * (kWave * VE), vocab - VE)); }
     __device__ __forceinline__ u32x4 load(int i) const {
-        constexpr uint32_t none = DT == PRIME_F32 ? 0xFF800000u : DT == PRIME_BF16 ? 0xFF80FF80u : 0xFC00FC00u;
-        const int e = index(i);
-        u32x4 v = {none, none, none, none};
-        if (wide && e + VE <= vocab) {
-            v = *reinterpret_cast<const u32x4 *>(base + static_cast<int64_t>(e) * es);
-        } else {
-#pragma unroll
-            for (int j = 0; j < VE; ++j) {
-                if (e + j >= vocab) continue;
-                if constexpr (DT == PRIME_F32) {
-                    v[j] = reinterpret_cast<const uint32_t *>(base)[e + j];
-                } else {
-                    const uint32_t h = reinterpret_cast<const uint16_t *>(base)[e + j];
-                    v[j / 2] = j & 1 ? (v[j / 2] & 0xFFFFu) | h << 16 : (v[j / 2] & 0xFFFF0000u) | h;
-                }
+        if constexpr (STAGED > 0) {
+            if (vocab < VE) {
+                uint16_t h[8] = {};
+                for (int k = 0; k < vocab * (es / 2); ++k) h[k] = reinterpret_cast<const uint16_t *>(base)[k];
+                return __builtin_bit_cast(u32x4, h);
             }
         }
-        return v;
+        return reinterpret_cast<const Raw *>(base + static_cast<int64_t>(index(i)) * es)->v;
+    }
+    __device__ __forceinline__ void mask(int i, u32x4 &v) const {
+        constexpr uint32_t none = DT == PRIME_F32 ? 0xFF800000u : DT == PRIME_BF16 ? 0xFF80u : 0xFC00u;  // -infinity
+        const int e = start + i * (kWave * VE), first = index(i);
+        if (first == e && first + VE <= vocab) return;
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+            if (first + j >= e && first + j < vocab) continue;
+            if constexpr (DT == PRIME_F32) v[j] = none;
+            else v[j / 2] = j & 1 ? (v[j / 2] & 0xFFFFu) | none << 16 : (v[j / 2] & 0xFFFF0000u) | none;
+        }
+    }
+    // chunk i as it was loaded or staged; what was loaded is masked after
+    template <bool FIRST = false>
+    __device__ __forceinline__ u32x4 get(int i) const {
+        if constexpr (STAGED > 0 && !FIRST) return lds[i * lds_step];
+        else return load(i);
+    }
+    template <bool FIRST = false>
+    __device__ __forceinline__ void finish(int i, u32x4 &v) const {
+        if constexpr (STAGED == 0 || FIRST) mask(i, v);
+        if constexpr (STAGED > 0 && FIRST) lds[i * lds_step] = v;
+    }
+    __device__ __forceinline__ void fetch(int i, float (&x)[VE]) const {
+        u32x4 v = get(i);
+        finish(i, v);
+        widen(v, x);
     }
     __device__ __forceinline__ void widen(const u32x4 &v, float (&x)[VE]) const {
 #pragma unroll
@@ -183,50 +200,22 @@ struct SampleRow {
             else x[j] = h16_bits_to_f32(static_cast<uint16_t>(j & 1 ? v[j / 2] >> 16 : v[j / 2]));
         }
     }
-    // f(i, x) over the lane's chunks, U loads in flight
-    template <int U, typename F>
+    // f(i, x) over the lane's chunks, the next ones on their way.  (One copy of f: with a row
+    // or two the time is in fetching instructions.)
+    template <bool FIRST = false, typename F>
     __device__ __forceinline__ void each(F f) const {
-        for (int i0 = 0; i0 < per; i0 += U) {
-            u32x4 v[U];
+        constexpr int D = STAGED == 0 ? 4 : !FIRST ? 2 : STAGED < 8 ? STAGED : 8;
+        u32x4 next[D];
 #pragma unroll
-            for (int k = 0; k < U; ++k)
-                if (i0 + k < per) v[k] = fetch(i0 + k);
-#pragma unroll
-            for (int k = 0; k < U; ++k) {
-                if (i0 + k < per) {
-                    float x[VE];
-                    widen(v[k], x);
-                    f(i0 + k, x);
-                }
-            }
-        }
-    }
-    // the first pass: f over the row as it comes from memory, into LDS what has place there
-    template <typename F>
-    __device__ __forceinline__ void stage(F f) {
-        constexpr int U = 8;
-        for (int i0 = 0; i0 < per; i0 += U) {
-            u32x4 v[U];
-#pragma unroll
-            for (int k = 0; k < U; ++k)
-                if (i0 + k < per) v[k] = load(i0 + k);
-#pragma unroll
-            for (int k = 0; k < U; ++k) {
-                if (i0 + k >= per) continue;
-                if (i0 + k < staged) lds[(i0 + k) * lds_step] = v[k];
-                float x[VE];
-                widen(v[k], x);
-                f(i0 + k, x);
-            }
-        }
-    }
-    // the same for passes with much to compute, the next load under way
-    template <typename F>
-    __device__ __forceinline__ void each_heavy(F f) const {
-        u32x4 next = fetch(0);
+        for (int k = 0; k < D; ++k)
+            if (k < per) next[k] = get<FIRST>(k);
+#pragma unroll 1
         for (int i = 0; i < per; ++i) {
-            const u32x4 now = next;
-            if (i + 1 < per) next = fetch(i + 1);
+            u32x4 now = next[0];
+#pragma unroll
+            for (int k = 0; k + 1 < D; ++k) next[k] = next[k + 1];
+            if (i + D < per) next[D - 1] = get<FIRST>(i + D);
+            finish<FIRST>(i, now);
             float x[VE];
             widen(now, x);
             f(i, x);
@@ -236,11 +225,11 @@ struct SampleRow {
 
 // How many tokens are equal to `value`; `nth` of that count gives n, and the index of the
 // n-th of them, from 1, is returned (any index where there are fewer).
-template <int DT, int WAVES, typename F>
-__device__ __forceinline__ int find_equal(SampleShared<WAVES> &sh, const SampleRow<DT> &row, float value, F nth) {
-    constexpr int VE = SampleRow<DT>::VE;
+template <int DT, int WAVES, int STAGED, typename F>
+__device__ __forceinline__ int find_equal(SampleShared<WAVES> &sh, const SampleRow<DT, STAGED> &row, float value, F nth) {
+    constexpr int VE = SampleRow<DT, STAGED>::VE;
     uint64_t count = 0, before, total;
-    row.template each<4>([&](int, const float (&x)[VE]) {
+    row.each([&](int, const float (&x)[VE]) {
 #pragma unroll
         for (int j = 0; j < VE; ++j) count += x[j] == value;
     });
@@ -249,7 +238,7 @@ __device__ __forceinline__ int find_equal(SampleShared<WAVES> &sh, const SampleR
     if (before < n && n <= before + sh.part[threadIdx.x / kWave]) {
         // this wave's chunks one after the other, lanes in order within one
         int left = static_cast<int>(n - before);
-        row.template each<4>([&](int i, const float (&x)[VE]) {
+        row.each([&](int i, const float (&x)[VE]) {
             int all = 0, lower = 0;  // of the chunk, of the lanes below
 #pragma unroll
             for (int j = 0; j < VE; ++j) {
@@ -268,86 +257,132 @@ __device__ __forceinline__ int find_equal(SampleShared<WAVES> &sh, const SampleR
     return sh.index;
 }
 
-// The cut: over the tokens above `last` and `ties` tokens equal to it (none for -infinity),
-// in rank order, the shortest prefix with weight of at least wanted(sum of all weights).
-// WEIGH: masses, else ones.  Left as it is where all of them are needed.  whole: the tokens
-// equal to the new `last` are known to be all kept.
-template <bool WEIGH, int DT, int WAVES, typename F>
-__device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT> &row, const RowScale &rs,
-                                    float &last, uint64_t &ties, bool &whole, F wanted) {
-    constexpr int kThreads = WAVES * kWave, kPer = kBuckets / kThreads, VE = SampleRow<DT>::VE;
-    const int tid = threadIdx.x;
-    const float floor = last;
-    const uint64_t floor_w = ties ? ties * (WEIGH ? rs.mass(floor) : 1) : 0;
-    auto add = [](uint64_t *p, uint64_t w) {
-        atomicAdd(reinterpret_cast<unsigned long long *>(p), static_cast<unsigned long long>(w));
-    };
-    __syncthreads();
-    for (int b = tid; b < kBuckets; b += kThreads) sh.hist[b] = 0;
-    if (tid == 0) sh.n = 0, sh.bucket = -1;
-    __syncthreads();
-    auto fill = [&](int, const float (&x)[VE]) {
-        bool any = false;
+// Thread t's sum over hist[t kPer ..], the sum before it, and the total.
+template <int WAVES>
+__device__ __forceinline__ uint64_t scan_hist(SampleShared<WAVES> &sh, uint64_t &mine, uint64_t &total) {
+    constexpr int kPer = kBuckets / (WAVES * kWave);
+    uint64_t waves;
+    mine = 0;
 #pragma unroll
-        for (int j = 0; j < VE; ++j) any |= x[j] > floor;
-        if (!any) return;
-#pragma unroll
-        for (int j = 0; j < VE; ++j) {
-            int b;
-            const uint64_t w = WEIGH ? rs.mass(x[j]) : 1;
-            if (rs.bucket(x[j], b) && x[j] > floor) add(&sh.hist[b], w);
-        }
-    };
-    if constexpr (WEIGH) row.each_heavy(fill);
-    else row.template each<4>(fill);
-    int floor_b = -1;
-    if (floor_w && !rs.bucket(floor, floor_b)) floor_b = -1;
-    if (tid == 0 && floor_b >= 0) add(&sh.hist[floor_b], floor_w);
-    __syncthreads();
-    uint64_t mine = 0, waves, total;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) mine += sh.hist[tid * kPer + i];
-    uint64_t before = block_scan(sh, mine, waves, total);
-    const uint64_t want = wanted(total);
-    if (want > total) return;  // (the same for every thread)
+    for (int i = 0; i < kPer; ++i) mine += sh.hist[threadIdx.x * kPer + i];
+    return block_scan(sh, mine, waves, total);
+}
+// The bucket in which the sum reaches `want` (at most the total) into sh.bucket, the sum
+// before it into sh.sum; `before`, `mine` as scan_hist gives them.
+template <int WAVES>
+__device__ __forceinline__ void locate(SampleShared<WAVES> &sh, uint64_t before, uint64_t mine, uint64_t want) {
+    constexpr int kPer = kBuckets / (WAVES * kWave);
     if (before < want && want <= before + mine) {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const uint64_t w = sh.hist[tid * kPer + i];
-            if (before < want && want <= before + w) sh.bucket = tid * kPer + i, sh.sum = before;
+            const uint64_t w = sh.hist[threadIdx.x * kPer + i];
+            if (before < want && want <= before + w) sh.bucket = threadIdx.x * kPer + i, sh.sum = before;
             before += w;
         }
     }
     __syncthreads();
-    const int bucket = sh.bucket;
-    const uint64_t above = sh.sum;
-    row.template each<4>([&](int, const float (&x)[VE]) {
+}
+__device__ __forceinline__ void lds_add(uint64_t *p, uint64_t w) {
+    atomicAdd(reinterpret_cast<unsigned long long *>(p), static_cast<unsigned long long>(w));
+}
+
+template <int N>
+__device__ __forceinline__ float largest(const float (&x)[N]) {
+    float m = x[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) m = fmaxf(m, x[j]);
+    return m;
+}
+
+// The cut: over the tokens above `last` and `ties` tokens equal to it (none for -infinity),
+// in rank order, the shortest prefix with weight of at least wanted(sum of all weights).
+// WEIGH: masses, else ones.  Left as it is where all of them are needed.  whole: the tokens
+// equal to the new `last` are known to be all kept.
+//
+// For top-k a first histogram, of the lanes' largest logits (lane_top), bounds the buckets
+// that matter: k lanes have a token at or above its `limit`, so at least as many tokens have.
+// kept: an upper bound of the tokens left.
+template <bool WEIGH, int DT, int WAVES, int STAGED, typename F>
+__device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT, STAGED> &row, const RowScale &rs, float lane_top,
+                                    float &last, uint64_t &ties, bool &whole, int &kept, F wanted) {
+    constexpr int kThreads = WAVES * kWave, VE = SampleRow<DT, STAGED>::VE;
+    const int tid = threadIdx.x;
+    const float floor = last;
+    const uint64_t floor_w = ties ? ties * (WEIGH ? rs.mass(floor) : 1) : 0;
+    uint64_t before, mine, total;
+    auto clear = [&]() {
+        __syncthreads();
+        for (int b = tid; b < kBuckets; b += kThreads) sh.hist[b] = 0;
+        if (tid == 0) sh.n = 0, sh.bucket = kBuckets, sh.kept = 0;
+        __syncthreads();
+    };
+    clear();
+    int limit = kBuckets;
+    if constexpr (!WEIGH) {
+        const uint64_t enough = wanted(0);
+        if (enough <= kThreads) {
+            int b;
+            if (rs.bucket(lane_top, b)) lds_add(&sh.hist[b], 1);
+            __syncthreads();
+            before = scan_hist(sh, mine, total);
+            locate(sh, before, mine, enough);
+            limit = sh.bucket;
+            clear();
+        }
+    }
+    auto fill = [&](int, const float (&x)[VE]) {
+        int b;
+        const float most = largest(x);
+        if (!(rs.bucket(most, b) & (b <= limit) & (most > floor))) return;
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
-            int b;
-            if (rs.bucket(x[j], b) && b == bucket && x[j] > floor) {
+            const bool in = rs.bucket(x[j], b) & (b <= limit) & (x[j] > floor);
+            const uint64_t w = WEIGH ? RowScale::mass_of(rs.exponent(x[j])) : 1;
+            if (in) lds_add(&sh.hist[b], w);
+        }
+    };
+    row.each(fill);
+    int floor_b = -1;
+    if (floor_w && !rs.bucket(floor, floor_b)) floor_b = -1;
+    if (tid == 0 && floor_b >= 0) lds_add(&sh.hist[floor_b], floor_w);
+    __syncthreads();
+    before = scan_hist(sh, mine, total);
+    const uint64_t want = wanted(total);
+    if (want > total) return;  // (the same for every thread)
+    locate(sh, before, mine, want);
+    const int bucket = sh.bucket;
+    const uint64_t above = sh.sum;
+    int higher = 0;
+    row.each([&](int, const float (&x)[VE]) {
+        int b;
+        const float most = largest(x);
+        if (!(rs.bucket(most, b) & (b <= bucket))) return;
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+            const bool in = rs.bucket(x[j], b) & (x[j] > floor);
+            higher += in & (b < bucket);
+            if (in & (b == bucket)) {
                 const int n = atomicAdd(&sh.n, 1);
                 if (n < kList) sh.list_x[n] = x[j], sh.list_w[n] = WEIGH ? rs.mass(x[j]) : 1;
             }
         }
     });
+    const int wave_higher = static_cast<int>(last_lane(wave_scan_u64(higher)));
+    if (tid % kWave == 0) atomicAdd(&sh.kept, wave_higher);
     if (tid == 0 && floor_b == bucket) {
         const int n = atomicAdd(&sh.n, 1);
         if (n < kList) sh.list_x[n] = floor, sh.list_w[n] = floor_w;
     }
     __syncthreads();
     const int n = sh.n;
+    kept = floor_b == bucket ? kept : min(kept, sh.kept + n);
     // `over`: the weight of the tokens above x; `equal`: of those equal to it, where known
-    auto found = [&](float x, uint64_t over, uint64_t equal) {
-        const uint64_t w = WEIGH ? rs.mass(x) : 1, n = (want - over + w - 1) / w;
-        sh.last = x;
-        sh.ties = n;
-        sh.whole = x != floor && n * w == equal;
-    };
+    auto found = [&](float x, uint64_t over, uint64_t equal) { sh.last = x, sh.sum = over, sh.rest = equal; };
     if (n <= kList) {
         for (int i = tid; i < n; i += kThreads) {
             const float x = sh.list_x[i];
             uint64_t over = above, equal = 0;
+#pragma unroll 8
             for (int j = 0; j < n; ++j) {
                 const float y = sh.list_x[j];
                 const uint64_t w = sh.list_w[j];
@@ -366,14 +401,14 @@ __device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT>
             __syncthreads();
             if (tid < 256) sh.hist[tid] = 0;
             __syncthreads();
-            row.each_heavy([&](int, const float (&x)[VE]) {
+            row.each([&](int, const float (&x)[VE]) {
 #pragma unroll
                 for (int j = 0; j < VE; ++j) {
                     const uint32_t k = logit_key(x[j]);
-                    if (x[j] > floor && inside(k)) add(&sh.hist[k >> shift & 255], WEIGH ? rs.mass(x[j]) : 1);
+                    if (x[j] > floor && inside(k)) lds_add(&sh.hist[k >> shift & 255], WEIGH ? rs.mass(x[j]) : 1);
                 }
             });
-            if (tid == 0 && floor_w && inside(floor_key)) add(&sh.hist[floor_key >> shift & 255], floor_w);
+            if (tid == 0 && floor_w && inside(floor_key)) lds_add(&sh.hist[floor_key >> shift & 255], floor_w);
             __syncthreads();
             if (tid == 0) {
                 int d = 255;
@@ -389,15 +424,16 @@ __device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT>
     }
     __syncthreads();
     last = sh.last;
-    ties = sh.ties;
-    whole = sh.whole;
+    const uint64_t w = WEIGH ? rs.mass(last) : 1;
+    ties = WEIGH ? (want - sh.sum + w - 1) / w : want - sh.sum;
+    whole = last != floor && ties * w == sh.rest;
 }
 
 template <int DT, int WAVES, int STAGED>
 __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a) {
     __shared__ SampleShared<WAVES> sh;
     __shared__ u32x4 stage[STAGED > 0 ? STAGED * WAVES * kWave : 1];
-    using Row = SampleRow<DT>;
+    using Row = SampleRow<DT, STAGED>;
     constexpr int VE = Row::VE;
     const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave), r = blockIdx.x;
     Row row;
@@ -405,8 +441,6 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
     row.vocab = a.vocab;
     row.per = (a.vocab + WAVES * kWave * VE - 1) / (WAVES * kWave * VE);
     row.start = (wave * row.per * kWave + lane) * VE;
-    row.wide = reinterpret_cast<uintptr_t>(row.base) % 16 == 0;
-    row.staged = STAGED;
     row.lds = stage + tid;
     row.lds_step = WAVES * kWave;
     const float T = a.temperatures ? a.temperatures[r] : a.temperature;
@@ -418,10 +452,11 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
     // the largest logit (fmaxf passes over NaN)
     RowScale rs;
     float top = -kInf;
-    row.stage([&](int, const float (&x)[VE]) {
+    row.template each<true>([&](int, const float (&x)[VE]) {
 #pragma unroll
         for (int j = 0; j < VE; ++j) top = fmaxf(top, x[j]);
     });
+    const float lane_top = top;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
     if (lane == 0) sh.list_x[wave] = top;
@@ -449,7 +484,7 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
     }
     if (!(T > 0.f) || top_k == 1 || top_p <= 0.f) {  // the first of the largest
         int first = a.vocab;
-        row.template each<4>([&](int i, const float (&x)[VE]) {
+        row.each([&](int i, const float (&x)[VE]) {
 #pragma unroll
             for (int j = VE - 1; j >= 0; --j)
                 if (x[j] == top) first = min(first, row.index(i) + j);
@@ -475,93 +510,142 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
     rs.least = min_p > 0.f ? fmax(log2(static_cast<double>(min_p < 1.f ? min_p : 1.f)), kLightest) : kLightest;
     rs.per_half = fminf(2.f * (kBuckets - 1) / (kBucketSpan * T), 1e30f);
 
-    // kept are the tokens above `last`; where the cut runs through equal ones (split), also
-    // those equal to it up to tie_index
+    // kept are the tokens above `last`, and of those equal to it the first `ties`
     float last = -kInf;
     uint64_t ties = 0;
     bool whole = true;
-    if (top_k < a.vocab) cut<false>(sh, row, rs, last, ties, whole, [&](uint64_t) { return static_cast<uint64_t>(top_k); });
-    if (top_p < 1.f) cut<true>(sh, row, rs, last, ties, whole, share);
-    int tie_index = -1;
-    bool split = ties && !whole;
-    if (split)
-        tie_index = find_equal(sh, row, last, [&](uint64_t total) {
-            split = total > ties;
-            return ties;
-        });
-    // all tokens equal to `last` are kept: the ones above the next value below it (below 0
-    // that is not -0)
-    if (ties && !split) last = key_logit(logit_key(last) - (last == 0.f ? 2 : 1));
+    int kept = a.vocab;
+    if (top_k < a.vocab)
+        cut<false>(sh, row, rs, lane_top, last, ties, whole, kept, [&](uint64_t) { return static_cast<uint64_t>(top_k); });
+    if (top_p < 1.f) cut<true>(sh, row, rs, lane_top, last, ties, whole, kept, share);
 
-    auto token_mass = [&](float x, int index, bool equals) -> uint64_t {
-        const double t = rs.exponent(x);
-        const uint64_t w = RowScale::mass_of(t);
-        bool keep = x > last;
-        if (equals) keep |= (x == last) & (index <= tie_index);
-        return RowScale::select(keep & (t >= rs.least), w);
-    };
-    auto chunk_mass = [&](int i, const float (&x)[VE]) {
-        float most = x[0];
-        uint64_t sum = 0;
+    // Few kept ones are compared with each other: a token's running mass is the sum over
+    // those with a lower index.  (min_p alone leaves few as a rule: tried, and given up at
+    // the first too many.)
+    if (kept <= kFew || (!ties && min_p > 0.f)) {
+        __syncthreads();
+        if (tid == 0) sh.n = 0;
+        __syncthreads();
+        row.each([&](int i, const float (&x)[VE]) {
+            if (!(largest(x) >= last) || sh.n > kFew) return;
 #pragma unroll
-        for (int j = 1; j < VE; ++j) most = fmaxf(most, x[j]);
-        if (most >= last) {
-            if (split) {
-#pragma unroll
-                for (int j = 0; j < VE; ++j) sum += token_mass(x[j], row.index(i) + j, true);
-            } else {
-#pragma unroll
-                for (int j = 0; j < VE; ++j) sum += token_mass(x[j], 0, false);
+            for (int j = 0; j < VE; ++j) {
+                const double t = rs.exponent(x[j]);
+                if (((x[j] > last) | (ties && x[j] == last)) & (t >= rs.least)) {
+                    const int n = atomicAdd(&sh.n, 1);
+                    if (n < kFew) sh.list_x[n] = x[j], sh.list_i[n] = row.index(i) + j, sh.list_w[n] = RowScale::mass_of(t);
+                }
             }
+        });
+        __syncthreads();
+        const int n = sh.n;
+        if (n <= kFew) {
+            if (ties && !whole) {  // of those equal to `last` only the first weigh
+                bool drop = false;
+                if (tid < n && sh.list_x[tid] == last) {
+                    uint64_t rank = 0;
+                    for (int k = 0; k < n; ++k) rank += (sh.list_x[k] == last) & (sh.list_i[k] < sh.list_i[tid]);
+                    drop = rank >= ties;
+                }
+                if (drop) sh.list_w[tid] = 0;
+                __syncthreads();
+            }
+            if (tid < n) {
+                const int index = sh.list_i[tid];
+                uint64_t at = 0, total = 0;
+#pragma unroll 8
+                for (int k = 0; k < n; ++k) {
+                    const uint64_t w = sh.list_w[k];
+                    total += w;
+                    at += sh.list_i[k] < index ? w : 0;
+                }
+                const uint64_t target = target_of(total);
+                if (at <= target && target < at + sh.list_w[tid]) a.out[r] = index;
+            }
+            return;
         }
-        return sum;
+    }
+
+    // Else the row is summed once more: the masses above `last`, and the tokens equal to it,
+    // of which the first `ties` weigh.  Where all of them are kept, they are the ones above the
+    // next value below it (below 0 that is not -0).
+    if (whole && ties) {
+        last = key_logit(logit_key(last) - (last == 0.f ? 2 : 1));
+        ties = 0;
+    }
+    const double tie_t = ties ? rs.exponent(last) : 0.0;
+    const uint64_t tie_w = ties && tie_t >= rs.least ? RowScale::mass_of(tie_t) : 0;
+    auto sum_of = [&](uint64_t mass, uint64_t count) { return mass + tie_w * (count < ties ? count : ties); };
+    auto token = [&](float x) {
+        const double t = rs.exponent(x);
+        return RowScale::select((x > last) & (t >= rs.least), RowScale::mass_of(t));
     };
-    uint64_t mine = 0, total, before;
-    row.each_heavy([&](int i, const float (&x)[VE]) { mine += chunk_mass(i, x); });
-    block_scan(sh, mine, before, total);
-    const uint64_t target = target_of(total);
+    auto add_chunk = [&](const float (&x)[VE], uint64_t &mass, uint64_t &count) {
+        if (!(largest(x) >= last)) return;
+#pragma unroll
+        for (int j = 0; j < VE; ++j) mass += token(x[j]);
+        if (ties) {
+#pragma unroll
+            for (int j = 0; j < VE; ++j) count += x[j] == last;
+        }
+    };
+    uint64_t mass = 0, count = 0, all_mass, all_count, mass0, count0;  // ..0: before the wave
+    row.each([&](int, const float (&x)[VE]) { add_chunk(x, mass, count); });
+    const uint64_t wave_count = ties ? last_lane(wave_scan_u64(count)) : 0;
+    count0 = all_count = 0;
+    if (ties) block_scan(sh, count, count0, all_count);
+    block_scan(sh, mass, mass0, all_mass);
+    const uint64_t target = target_of(sum_of(all_mass, all_count));
     // the wave with the token, then its chunks, taken by all waves 64 lanes' sums each
-    if (lane == 0 && before <= target && target - before < sh.part[wave]) sh.owner = wave, sh.sum = before;
+    if (lane == 0 && sum_of(mass0, count0) <= target && target < sum_of(mass0 + sh.part[wave], count0 + wave_count))
+        sh.owner = wave, sh.sum = mass0, sh.rest = count0;
     __syncthreads();
-    before = sh.sum;
+    mass0 = sh.sum, count0 = sh.rest;
     const int shift = sh.owner - wave;
     row.start += shift * row.per * (kWave * VE);
     row.lds += shift * kWave;
     constexpr int kRound = kBuckets / kWave;  // chunks whose sums fit
+    static_assert(sizeof(sh.list_w) >= kBuckets * sizeof(int), "the counts take the list's place");
+    int *counts = reinterpret_cast<int *>(sh.list_w);
     for (int i0 = 0; i0 < row.per; i0 += kRound) {
         const int n = min(kRound, row.per - i0);
         __syncthreads();
         for (int i = wave; i < n; i += WAVES) {
             float x[VE];
-            row.widen(row.fetch(i0 + i), x);
-            sh.hist[i * kWave + lane] = chunk_mass(i0 + i, x);
+            row.fetch(i0 + i, x);
+            uint64_t m = 0, c = 0;
+            add_chunk(x, m, c);
+            sh.hist[i * kWave + lane] = m;
+            counts[i * kWave + lane] = static_cast<int>(c);
         }
         __syncthreads();
         if (wave) continue;
         // in order: lane by lane, chunk by chunk; here a lane takes n sums in a row
-        uint64_t sum = 0;
-        for (int k = 0; k < n; ++k) sum += sh.hist[lane * n + k];
-        const uint64_t inc = wave_scan_u64(sum);
-        uint64_t at = before + inc - sum;
-        if (at <= target && target < before + inc) {
+        uint64_t m = 0, c = 0;
+#pragma unroll 8
+        for (int k = 0; k < n; ++k) m += sh.hist[lane * n + k], c += counts[lane * n + k];
+        const uint64_t mi = wave_scan_u64(m), ci = ties ? wave_scan_u64(c) : 0;
+        uint64_t am = mass0 + mi - m, ac = count0 + ci - c;
+        if (sum_of(am, ac) <= target && target < sum_of(mass0 + mi, count0 + ci)) {
             int k = lane * n;
-            while (target - at >= sh.hist[k]) at += sh.hist[k++];
+            while (target >= sum_of(am + sh.hist[k], ac + counts[k])) am += sh.hist[k], ac += counts[k], ++k;
             // sum k is lane k % 64's of chunk k / 64
             const int other = k % kWave - lane;
-            SampleRow<DT> its = row;
+            Row its = row;
             its.start += other * VE;
             its.lds += other;
             float x[VE];
-            its.widen(its.fetch(i0 + k / kWave), x);
+            its.fetch(i0 + k / kWave, x);
+            bool done = false;
 #pragma unroll
             for (int j = 0; j < VE; ++j) {
-                const int index = its.index(i0 + k / kWave) + j;
-                const uint64_t m = token_mass(x[j], index, split);
-                if (at <= target && target < at + m) a.out[r] = index;
-                at += m;
+                am += token(x[j]);
+                ac += ties && x[j] == last;
+                if (!done && target < sum_of(am, ac)) a.out[r] = its.index(i0 + k / kWave) + j, done = true;
             }
         }
-        before += last_lane(inc);
+        mass0 += last_lane(mi);
+        count0 += last_lane(ci);
     }
 }
 
@@ -572,10 +656,16 @@ void launch(const SampleArgs &a, hipStream_t s) {
     hipLaunchKernelGGL((sample_kernel<DT, WAVES, STAGED>), dim3(a.n), dim3(WAVES * kWave), 0, s, a);
 }
 
+// Up to 4096 tokens take 4 waves, more 16.  Rows go through LDS where they fit (131072 bytes)
+// and each has a CU to itself; with more rows than CUs, two smaller workgroups on each hide
+// one's memory behind the other's arithmetic (512 x 50304 fp32: 49 us, one workgroup at a
+// time 55).
 template <int DT>
 void run(const SampleArgs &a, hipStream_t s) {
-    if (a.vocab <= kSampleSmall) launch<DT, 4, DT == PRIME_F32 ? 4 : 2>(a, s);
-    else if (a.n <= 256) launch<DT, 16, 8>(a, s);
+    constexpr int kLds = 8, kChunk = kWave * (DT == PRIME_F32 ? 4 : 8);
+    if (a.vocab <= 4096) launch<DT, 4, 4096 / (4 * kChunk)>(a, s);
+    else if (a.n > 256) launch<DT, 8, 0>(a, s);
+    else if (a.vocab <= kLds * 16 * kChunk) launch<DT, 16, kLds>(a, s);
     else launch<DT, 16, 0>(a, s);
 }
 
