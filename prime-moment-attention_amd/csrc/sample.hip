@@ -363,19 +363,20 @@ __device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT,
             higher += in & (b < bucket);
             if (in & (b == bucket)) {
                 const int n = atomicAdd(&sh.n, 1);
-                if (n < kList) sh.list_x[n] = x[j], sh.list_w[n] = WEIGH ? rs.mass(x[j]) : 1;
+                if (n < kList) sh.list_x[n] = x[j];
             }
         }
     });
     const int wave_higher = static_cast<int>(last_lane(wave_scan_u64(higher)));
     if (tid % kWave == 0) atomicAdd(&sh.kept, wave_higher);
-    if (tid == 0 && floor_b == bucket) {
-        const int n = atomicAdd(&sh.n, 1);
-        if (n < kList) sh.list_x[n] = floor, sh.list_w[n] = floor_w;
-    }
     __syncthreads();
-    const int n = sh.n;
-    kept = floor_b == bucket ? kept : min(kept, sh.kept + n);
+    const int own = sh.n, n = own + (floor_b == bucket);  // the floor's tokens count as one more
+    if (n <= kList) {
+        for (int i = tid; i < own; i += kThreads) sh.list_w[i] = WEIGH ? rs.mass(sh.list_x[i]) : 1;
+        if (tid == 0 && n > own) sh.list_x[own] = floor, sh.list_w[own] = floor_w;
+        __syncthreads();
+    }
+    kept = n > own ? kept : min(kept, sh.kept + n);
     // `over`: the weight of the tokens above x; `equal`: of those equal to it, where known
     auto found = [&](float x, uint64_t over, uint64_t equal) { sh.last = x, sh.sum = over, sh.rest = equal; };
     if (n <= kList) {
@@ -523,33 +524,38 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
     // those with a lower index.  (min_p alone leaves few as a rule: tried, and given up at
     // the first too many.)
     if (kept <= kFew || (!ties && min_p > 0.f)) {
+        // nothing below this weighs: `last`, or what min_p leaves, with room for rounding
+        const float far = top + static_cast<float>(rs.least / rs.rate), room = 1e-5f * (fabsf(top) + fabsf(far));
+        const float least_x = ties ? last : fmaxf(far - room, -__FLT_MAX__);
         __syncthreads();
         if (tid == 0) sh.n = 0;
         __syncthreads();
         row.each([&](int i, const float (&x)[VE]) {
-            if (!(largest(x) >= last) || sh.n > kFew) return;
+            if (!(largest(x) >= least_x) || sh.n > kFew) return;
 #pragma unroll
             for (int j = 0; j < VE; ++j) {
-                const double t = rs.exponent(x[j]);
-                if (((x[j] > last) | (ties && x[j] == last)) & (t >= rs.least)) {
+                if (x[j] >= least_x) {
                     const int n = atomicAdd(&sh.n, 1);
-                    if (n < kFew) sh.list_x[n] = x[j], sh.list_i[n] = row.index(i) + j, sh.list_w[n] = RowScale::mass_of(t);
+                    if (n < kFew) sh.list_x[n] = x[j], sh.list_i[n] = row.index(i) + j;
                 }
             }
         });
         __syncthreads();
         const int n = sh.n;
         if (n <= kFew) {
-            if (ties && !whole) {  // of those equal to `last` only the first weigh
-                bool drop = false;
-                if (tid < n && sh.list_x[tid] == last) {
+            if (tid < n) {
+                const float x = sh.list_x[tid];
+                const double t = rs.exponent(x);
+                uint64_t w = t >= rs.least && (x > last || ties) ? RowScale::mass_of(t) : 0;
+                if (x == last && !whole) {  // of those equal to `last` only the first weigh
                     uint64_t rank = 0;
+#pragma unroll 8
                     for (int k = 0; k < n; ++k) rank += (sh.list_x[k] == last) & (sh.list_i[k] < sh.list_i[tid]);
-                    drop = rank >= ties;
+                    w = rank < ties ? w : 0;
                 }
-                if (drop) sh.list_w[tid] = 0;
-                __syncthreads();
+                sh.list_w[tid] = w;
             }
+            __syncthreads();
             if (tid < n) {
                 const int index = sh.list_i[tid];
                 uint64_t at = 0, total = 0;
