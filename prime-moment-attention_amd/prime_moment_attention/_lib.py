@@ -1094,21 +1094,29 @@ GATED_TILE = 16  # tokens between the checkpoints of the gated recurrence's back
 
 
 def _same_device(first: torch.Tensor, *ts) -> None:
+    d = first.get_device()
+    if d >= 0:
+        for t in ts:
+            if t is not None and t.get_device() != d:
+                break
+        else:
+            return
     _dev_check(first, *ts)
-    for t in ts:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"tensors on {first.device} and {t.device}: one device is needed")
+    raise ValueError("tensors on " + ", ".join(str(t.device) for t in (first, *ts) if t is not None)
+                     + ": one device is needed")
 
 
-def _launch(what: str, dev: torch.device, *args) -> None:
-    """The entry point ``what`` on the current stream of the tensors' device, which
-    need not be the current device."""
-    fn = getattr(load(), what)
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        _check(fn(*args, _stream(dev)), what)
-        return
-    with torch.cuda.device(dev):
-        _check(fn(*args, _stream(dev)), what)
+def _launch(fn, what: str, dev: torch.device, *args) -> None:
+    """The entry point fn on the current stream of the tensors' device, which need not be
+    the current device."""
+    index = dev.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream(dev))
+    if rc:
+        _check(rc, what)
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -1117,86 +1125,116 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def seq_desc(t: torch.Tensor) -> PrimeSeq:
     """Descriptor of a [B, L, C] view with contiguous channels."""
-    return PrimeSeq(t.data_ptr(), t.stride(0), t.stride(1))
+    sb, sl, _ = t.stride()
+    return PrimeSeq(t.data_ptr(), sb, sl)
 
 
-def _check_gated(x, step, gate, tau, state, *states) -> Tuple[int, int, int]:
+def _views_ok(x, *views) -> bool:
+    sh, dt, one = x.shape, x.dtype, x.shape[-1] <= 1
+    for t in views:
+        if t.shape != sh or t.dtype is not dt or not (t.stride(2) == 1 or one):
+            return False
+    return True
+
+
+def check_gated(x, step, gate, tau, state, state_out) -> Tuple[int, int, int]:
+    """(B, L, C) of the gated recurrence's operands, or the error that they have."""
     if x.dim() != 3:
         raise ValueError(f"x has shape {tuple(x.shape)}, expected [B, L, C]")
     if x.dtype not in _DTYPES:
         raise RuntimeError(f"unsupported dtype {x.dtype}")
     B, Lt, C = x.shape
-    for t, n in ((x, "x"), (step, "step"), (gate, "gate")):
-        _shape(t, (B, Lt, C), n)
-        if t.dtype != x.dtype:
-            raise ValueError(f"{n} is {t.dtype}, x is {x.dtype}: one dtype is needed")
-        if t.stride(2) != 1 and C > 1:
-            raise ValueError(f"{n}: channels must be contiguous")
-    if tau.dtype != torch.float32 or tuple(tau.shape) != (C,) or not tau.is_contiguous():
+    if not _views_ok(x, x, step, gate):
+        for t, n in ((x, "x"), (step, "step"), (gate, "gate")):
+            _shape(t, (B, Lt, C), n)
+            if t.dtype != x.dtype:
+                raise ValueError(f"{n} is {t.dtype}, x is {x.dtype}: one dtype is needed")
+        raise ValueError("channels must be contiguous")
+    if tau.dtype is not torch.float32 or tau.shape != (C,) or not tau.is_contiguous():
         raise ValueError(f"tau must be a contiguous fp32 tensor of {C} values")
-    for t, n in zip((state, *states), ("state", "state_out")):
-        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (B, C) or not t.is_contiguous()):
-            raise ValueError(f"{n} must be a contiguous fp32 [{B}, {C}] tensor")
-    _same_device(x, step, gate, tau, state, *states)
+    for t in (state, state_out):
+        if t is not None and (t.dtype is not torch.float32 or t.shape != (B, C) or not t.is_contiguous()):
+            raise ValueError(f"state and state_out must be contiguous fp32 [{B}, {C}] tensors")
+    _same_device(x, step, gate, tau, state, state_out)
     return B, Lt, C
 
 
-def gated_scan(x, step, gate, tau, state, y, state_out, checkpoints=None) -> None:
+def _check_checkpoints(ckpt, B: int, Lt: int, C: int) -> None:
+    if ckpt.dtype is not torch.float32 or not ckpt.is_contiguous() or ckpt.numel() != B * -(-Lt // GATED_TILE) * C:
+        raise ValueError("checkpoints must be a contiguous fp32 [B, ceil(L / 16), C] tensor")
+
+
+def gated_scan(x, step, gate, tau, state, y, state_out, checkpoints=None, checked: bool = False) -> None:
     """prime_gated_scan over [B, L, C] views of one dtype; tau fp32 [C]; states
     fp32 [B, C] or None (state_out may be state); checkpoints fp32
-    [B, ceil(L / GATED_TILE), C] for gated_scan_backward, or None."""
-    B, Lt, C = _check_gated(x, step, gate, tau, state, state_out)
-    _shape(y, (B, Lt, C), "y")
-    if y.dtype != x.dtype or (y.stride(2) != 1 and C > 1):
-        raise ValueError("y must have x's dtype and contiguous channels")
-    if checkpoints is not None and (checkpoints.dtype != torch.float32 or not checkpoints.is_contiguous()
-                                    or checkpoints.numel() != B * -(-Lt // GATED_TILE) * C):
-        raise ValueError("checkpoints must be a contiguous fp32 [B, ceil(L / 16), C] tensor")
-    _same_device(x, y, checkpoints)
-    n = load().prime_gated_scan_workspace_size(B, Lt, C)
+    [B, ceil(L / GATED_TILE), C] for gated_scan_backward, or None.  checked: the caller
+    has been through check_gated and made the outputs itself."""
+    if not checked:
+        B, Lt, C = check_gated(x, step, gate, tau, state, state_out)
+        _shape(y, (B, Lt, C), "y")
+        if not _views_ok(x, y):
+            raise ValueError("y must have x's dtype and contiguous channels")
+        if checkpoints is not None:
+            _check_checkpoints(checkpoints, B, Lt, C)
+        _same_device(x, y, checkpoints)
+    B, Lt, C = x.shape
+    L = load()
+    n = L.prime_gated_scan_workspace_size(B, Lt, C) if Lt > GATED_TILE else 0  # (fewer tokens need none)
     ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-    _launch("prime_gated_scan", x.device, seq_desc(x), seq_desc(step), seq_desc(gate), _DTYPES[x.dtype], B, Lt, C,
-            _ptr(tau), _ptr(state), seq_desc(y), _ptr(state_out), _ptr(checkpoints), _ptr(ws), n)
+    _launch(L.prime_gated_scan, "prime_gated_scan", x.device, seq_desc(x), seq_desc(step), seq_desc(gate),
+            _DTYPES[x.dtype], B, Lt, C, tau.data_ptr(), _ptr(state), seq_desc(y), _ptr(state_out), _ptr(checkpoints),
+            _ptr(ws), n)
 
 
-def gated_scan_backward(x, step, gate, tau, checkpoints, dy, dstate_out, dx, dstep, dgate, dtau, dstate_in) -> None:
+def gated_scan_backward(x, step, gate, tau, checkpoints, dy, dstate_out, dx, dstep, dgate, dtau, dstate_in,
+                        checked: bool = False) -> None:
     """prime_gated_scan_backward: dx, dstep, dgate [B, L, C] views of x's dtype, dtau
-    fp32 [C], dstate_in fp32 [B, C] or None."""
-    B, Lt, C = _check_gated(x, step, gate, tau, dstate_out, dstate_in)
-    for t, n in ((dy, "dy"), (dx, "dx"), (dstep, "dstep"), (dgate, "dgate")):
-        _shape(t, (B, Lt, C), n)
-        if t.dtype != x.dtype or (t.stride(2) != 1 and C > 1):
-            raise ValueError(f"{n} must have x's dtype and contiguous channels")
-    if checkpoints.dtype != torch.float32 or not checkpoints.is_contiguous() or (
-            checkpoints.numel() != B * -(-Lt // GATED_TILE) * C):
-        raise ValueError("checkpoints must be the forward's")
-    if dtau.dtype != torch.float32 or tuple(dtau.shape) != (C,) or not dtau.is_contiguous():
-        raise ValueError(f"dtau must be a contiguous fp32 tensor of {C} values")
-    _same_device(x, dy, dx, dstep, dgate, checkpoints, dtau)
-    n = load().prime_gated_scan_backward_workspace_size(B, Lt, C)
+    fp32 [C], dstate_in fp32 [B, C] or None.  checked: the operands are the forward's, the
+    outputs made by the caller."""
+    if not checked:
+        B, Lt, C = check_gated(x, step, gate, tau, dstate_out, dstate_in)
+        for t, n in ((dy, "dy"), (dx, "dx"), (dstep, "dstep"), (dgate, "dgate")):
+            _shape(t, (B, Lt, C), n)
+            if not _views_ok(x, t):
+                raise ValueError(f"{n} must have x's dtype and contiguous channels")
+        _check_checkpoints(checkpoints, B, Lt, C)
+        if dtau.dtype != torch.float32 or tuple(dtau.shape) != (C,) or not dtau.is_contiguous():
+            raise ValueError(f"dtau must be a contiguous fp32 tensor of {C} values")
+        _same_device(x, dy, dx, dstep, dgate, checkpoints, dtau)
+    B, Lt, C = x.shape
+    L = load()
+    n = L.prime_gated_scan_backward_workspace_size(B, Lt, C)
     ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-    _launch("prime_gated_scan_backward", x.device, seq_desc(x), seq_desc(step), seq_desc(gate), _DTYPES[x.dtype], B,
-            Lt, C, _ptr(tau), _ptr(checkpoints), seq_desc(dy), _ptr(dstate_out), seq_desc(dx), seq_desc(dstep),
-            seq_desc(dgate), _ptr(dtau), _ptr(dstate_in), _ptr(ws), n)
+    _launch(L.prime_gated_scan_backward, "prime_gated_scan_backward", x.device, seq_desc(x), seq_desc(step),
+            seq_desc(gate), _DTYPES[x.dtype], B, Lt, C, tau.data_ptr(), checkpoints.data_ptr(), seq_desc(dy),
+            _ptr(dstate_out), seq_desc(dx), seq_desc(dstep), seq_desc(dgate), dtau.data_ptr(), _ptr(dstate_in),
+            ws.data_ptr(), n)
 
 
 def dropout_add(x, residual, out, p: float, rng, call: int) -> None:
-    """prime_dropout_add over 2-D rows with contiguous columns; residual may be None."""
+    """prime_dropout_add; residual may be None.  Contiguous tensors of one shape, or 2-D
+    rows with contiguous columns."""
+    flat = x.is_contiguous() and out.is_contiguous() and (residual is None or residual.is_contiguous())
     for t, n in ((x, "x"), (residual, "residual"), (out, "out")):
         if t is None:
             continue
-        _shape(t, x.shape, n)
-        if t.dim() != 2 or t.dtype != x.dtype or (t.stride(1) != 1 and t.shape[1] > 1):
-            raise ValueError(f"{n} must be rows of x's dtype with contiguous columns")
+        if t.shape != x.shape or t.dtype is not x.dtype:
+            raise ValueError(f"{n} must have x's shape and dtype")
+        if not flat and (t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1)):
+            raise ValueError(f"{n} must be rows with contiguous columns")
     if x.dtype not in _DTYPES:
         raise RuntimeError(f"unsupported dtype {x.dtype}")
-    if rng.dtype != torch.int64 or rng.numel() != 2 or not rng.is_contiguous():
+    if rng.dtype is not torch.int64 or rng.numel() != 2 or not rng.is_contiguous():
         raise ValueError("rng must be a contiguous int64 tensor of two values (seed, offset)")
     _same_device(x, residual, out, rng)
-    rows, cols = x.shape
-    ld = lambda t: 0 if t is None else t.stride(0) if rows > 1 else cols
-    _launch("prime_dropout_add", x.device, _ptr(x), ld(x), _ptr(residual), ld(residual), _ptr(out), ld(out),
-            _DTYPES[x.dtype], rows, cols, float(p), _ptr(rng), int(call))
+    if flat:
+        rows, cols = 1, x.numel()
+        lds = (cols, cols, cols)
+    else:
+        rows, cols = x.shape
+        lds = [0 if t is None else t.stride(0) if rows > 1 else cols for t in (x, residual, out)]
+    _launch(load().prime_dropout_add, "prime_dropout_add", x.device, x.data_ptr(), lds[0], _ptr(residual), lds[1],
+            out.data_ptr(), lds[2], _DTYPES[x.dtype], rows, cols, p, rng.data_ptr(), call)
 
 
 def sample(logits, uniforms, temperature, top_k, top_p, min_p, out) -> None:
@@ -1208,20 +1246,23 @@ def sample(logits, uniforms, temperature, top_k, top_p, min_p, out) -> None:
     if logits.dtype not in _DTYPES:
         raise RuntimeError(f"unsupported dtype {logits.dtype}")
     n, vocab = logits.shape
-    args, keep = [], []
-    for v, name, dt in ((uniforms, "uniforms", torch.float32), (temperature, "temperature", torch.float32),
-                        (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
-                        (min_p, "min_p", torch.float32), (out, "out", torch.int64)):
-        if not torch.is_tensor(v):
+    dev, args = logits.get_device(), []
+    f32 = torch.float32
+    for v, name, dt, cast in ((out, "out", torch.int64, None), (uniforms, "uniforms", f32, None),
+                              (temperature, "temperature", f32, float), (top_k, "top_k", torch.int32, int),
+                              (top_p, "top_p", f32, float), (min_p, "min_p", f32, float)):
+        if cast is not None and not isinstance(v, torch.Tensor):
+            args += (cast(v), None)
             continue
-        if v.dtype != dt or v.numel() != n or not v.is_contiguous():
+        if v.dtype is not dt or v.numel() != n or not v.is_contiguous():
             raise ValueError(f"{name} must be a contiguous {dt} tensor of {n} values")
-        keep.append(v)
-    _same_device(logits, *keep)
-    for v, cast in ((temperature, float), (top_k, int), (top_p, float), (min_p, float)):
-        args += [cast(0), _ptr(v)] if torch.is_tensor(v) else [cast(v), None]
-    _launch("prime_sample", logits.device, _ptr(logits), _DTYPES[logits.dtype], n, vocab,
-            logits.stride(0) if n > 1 else vocab, _ptr(uniforms), *args, _ptr(out))
+        if dev < 0 or v.get_device() != dev:
+            _same_device(logits, v)
+        if cast is not None:
+            args.append(cast(0))
+        args.append(v.data_ptr())
+    _launch(load().prime_sample, "prime_sample", logits.device, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab,
+            logits.stride(0) if n > 1 else vocab, *args[1:], args[0])
 
 
 def timer_enable(*kernels: int) -> None:

@@ -30,6 +30,10 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _run(x, residual, p, rng, call) -> torch.Tensor:
+    if x.is_contiguous() and (residual is None or residual.is_contiguous()):
+        out = torch.empty_like(x)
+        _lib.dropout_add(x, residual, out, p, rng, call)
+        return out
     out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     _lib.dropout_add(_rows(x), None if residual is None else _rows(residual), out.view(-1, x.shape[-1]), p, rng, call)
     return out

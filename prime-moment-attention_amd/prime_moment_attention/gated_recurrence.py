@@ -51,7 +51,7 @@ class _GatedScanFn(torch.autograd.Function):
         y = torch.empty(B, L, C, device=x.device, dtype=x.dtype)
         last = torch.empty(B, C, device=x.device, dtype=torch.float32)
         ckpt = torch.empty(B, -(-L // _lib.GATED_TILE), C, device=x.device, dtype=torch.float32)
-        _lib.gated_scan(*parts, tau, state, y, last, ckpt)
+        _lib.gated_scan(*parts, tau, state, y, last, ckpt, checked=True)
         ctx.save_for_backward(x, step, gate, tau, ckpt)
         ctx.has_state = state is not None
         ctx.set_materialize_grads(False)
@@ -72,15 +72,15 @@ class _GatedScanFn(torch.autograd.Function):
             grads = out = tuple(new.view(3, B, L, C))
         dtau = torch.empty(C, device=x.device, dtype=torch.float32)
         dstate = torch.empty(B, C, device=x.device, dtype=torch.float32) if ctx.has_state else None
-        _lib.gated_scan_backward(*parts, tau, ckpt, dy, dlast, *grads, dtau, dstate)
+        _lib.gated_scan_backward(*parts, tau, ckpt, dy, dlast, *grads, dtau, dstate, checked=True)
         return (*out, dtau, dstate)
 
 
 def _scan(x, step, gate, tau, state, state_out):
     """(y, last state) of x, step, gate, or of x's thirds where step is None."""
     parts = (x, step, gate) if step is not None else _thirds(x)
-    B, L, C = _lib._check_gated(*parts, tau, state, state_out)
-    if L == 0 or B == 0 or C == 0:
+    B, L, C = _lib.check_gated(*parts, tau, state, state_out)
+    if not (L and B and C):
         h = parts[0].new_zeros(B, C, dtype=torch.float32) if state is None else state
         if state_out is not None:
             h = state_out.copy_(h)
@@ -89,10 +89,10 @@ def _scan(x, step, gate, tau, state, state_out):
         if state_out is not None:
             raise ValueError("state_out cannot be written while autograd records: take the returned state")
         return _GatedScanFn.apply(x, step, gate, tau, state)
-    y = torch.empty(B, L, C, device=x.device, dtype=x.dtype)
+    y = x.new_empty((B, L, C))
     if state_out is None:
-        state_out = torch.empty(B, C, device=x.device, dtype=torch.float32)
-    _lib.gated_scan(*parts, tau, state, y, state_out)
+        state_out = tau.new_empty((B, C))
+    _lib.gated_scan(*parts, tau, state, y, state_out, checked=True)
     return y, state_out
 
 
@@ -107,7 +107,8 @@ def gated_recurrence(x: torch.Tensor, step: torch.Tensor, gate: torch.Tensor, ta
     Differentiable once in x, step, gate, tau and state.  The given state is left as it
     is; without autograd, ``state_out`` names the tensor that receives the last state
     (it may be ``state``: a decode step in place)."""
-    x, step, gate = _channels(x), _channels(step), _channels(gate)
+    if not x.stride(-1) == step.stride(-1) == gate.stride(-1) == 1:
+        x, step, gate = _channels(x), _channels(step), _channels(gate)
     y, last = _scan(x, step, gate, tau, state, state_out)
     return y, (last if return_state else None)
 
