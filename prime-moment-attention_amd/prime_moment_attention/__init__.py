@@ -13,13 +13,13 @@ from .chunked_delta_prime import ChunkedGatedDeltaPrimeAttention
 from .chunked_ssd import ChunkedPrimeSSD, chunked_prime_ssd_core
 from .dropout import dropout_add, dropout_rng
 from .gated_recurrence import GatedLinearRecurrence, gated_recurrence
-from .model import GreedyDecoder, PrimeConfig, PrimeForCausalLM, prime_125m_config
+from .model import GreedyDecoder, PrimeConfig, PrimeForCausalLM, SamplingDecoder, prime_125m_config
 from .sampling import sample_tokens
 from .selective import PrimeSelectiveMomentAttention
 
 __version__ = "0.1.0"
 
 __all__ = ["PrimeMomentAttention", "PrimeMomentCache", "ChunkedPrimeSSD", "chunked_prime_ssd_core",
-           "PrimeConfig", "PrimeForCausalLM", "GreedyDecoder", "prime_125m_config",
+           "PrimeConfig", "PrimeForCausalLM", "GreedyDecoder", "SamplingDecoder", "prime_125m_config",
            "ChunkedGatedDeltaPrimeAttention", "PrimeSelectiveMomentAttention",
            "GatedLinearRecurrence", "gated_recurrence", "dropout_add", "dropout_rng", "sample_tokens"]

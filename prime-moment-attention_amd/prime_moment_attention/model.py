@@ -23,6 +23,15 @@ Additions for serving:
     place, the whole step (embedding, 12 layers, final norm, lm_head, argmax)
     captured in one HIP graph and replayed per token, so its tokens equal
     ``generate``'s at temperature 0.
+  * ``SamplingDecoder`` does the same with sampled tokens (temperature, top-k,
+    top-p, min-p); ``generate`` takes top_p and min_p.
+
+Additions for other layers and for training:
+  * ``PrimeConfig.gated_layers``: the layers whose mixer is a gated linear
+    recurrence (GatedLinearRecurrence) instead of moment attention; such a
+    layer's state is one fp32 tensor [B, heads * head_dim].
+  * ``PrimeConfig.dropout``: in training each block's two branches are dropped
+    out as they are added to the residual stream (dropout_add).
 """
 from __future__ import annotations
 
@@ -36,12 +45,15 @@ import torch.nn.functional as F
 
 from . import _lib
 from .attention import PrimeMomentAttention
+from .dropout import dropout_add, dropout_rng
+from .gated_recurrence import GatedLinearRecurrence
+from .sampling import sample_tokens
 from .selective import PrimeSelectiveMomentAttention
 
 
 @dataclass
 class PrimeConfig:
-    """model.py:20-44, plus ``mlp_type``."""
+    """model.py:20-44, plus ``mlp_type``, ``dropout`` and ``gated_layers``."""
     vocab_size: int = 32000
     hidden_size: int = 512
     num_layers: int = 6
@@ -59,6 +71,8 @@ class PrimeConfig:
     min_tau: float = 2.0
     max_tau: float = 2000.0
     mlp_type: str = "swiglu"
+    dropout: float = 0.0
+    gated_layers: Tuple[int, ...] = ()
 
     def __post_init__(self):
         if self.num_kv_heads is None:
@@ -67,6 +81,11 @@ class PrimeConfig:
             self.intermediate_size = int(2 * (4 * self.hidden_size) / 3)
         if self.mlp_type not in ("swiglu", "gelu"):
             raise ValueError(f"mlp_type must be 'swiglu' or 'gelu', not {self.mlp_type!r}")
+        if not 0.0 <= self.dropout <= 1.0:
+            raise ValueError(f"dropout={self.dropout} outside [0, 1]")
+        self.gated_layers = tuple(self.gated_layers)
+        if any(not 0 <= i < self.num_layers for i in self.gated_layers):
+            raise ValueError(f"gated_layers {self.gated_layers} outside the {self.num_layers} layers")
 
 
 def prime_125m_config(mlp_type: str = "gelu", vocab_size: int = 50304, use_selective: bool = False) -> PrimeConfig:
@@ -133,12 +152,18 @@ def _mlp_inner(mlp: nn.Module, x: torch.Tensor) -> torch.Tensor:
 
 
 class PrimeBlock(nn.Module):
-    """Pre-norm block, model.py:71-118: x + Attn(RMSNorm x); x + MLP(RMSNorm x)."""
+    """Pre-norm block, model.py:71-118: x + Attn(RMSNorm x); x + MLP(RMSNorm x).  `layer` is
+    its place in the model: whether it is a gated layer, and its calls of dropout."""
 
-    def __init__(self, config: PrimeConfig):
+    def __init__(self, config: PrimeConfig, layer: int = 0):
         super().__init__()
+        self.layer = layer
+        self.dropout = config.dropout
         self.input_layernorm = RMSNorm(config.hidden_size, eps=config.rms_norm_eps)
-        if config.use_selective:
+        if layer in config.gated_layers:
+            self.self_attn = GatedLinearRecurrence(config.hidden_size, config.num_heads * config.head_dim,
+                                                   min_tau=config.min_tau, max_tau=config.max_tau)
+        elif config.use_selective:
             self.self_attn = PrimeSelectiveMomentAttention(
                 hidden_size=config.hidden_size, num_heads=config.num_heads, head_dim=config.head_dim,
                 num_kv_heads=config.num_kv_heads, decay=config.decay, use_qk_norm=config.use_qk_norm,
@@ -152,13 +177,24 @@ class PrimeBlock(nn.Module):
         mlp = PrimeGeluMLP if config.mlp_type == "gelu" else PrimeMLP
         self.mlp = mlp(config.hidden_size, config.intermediate_size)
 
-    def forward(self, hidden_states, state=None, return_state=False):
+    def forward(self, hidden_states, state=None, return_state=False, rng=None):
+        """rng: the (seed, offset) of this pass's dropout (dropout_rng; one is drawn where
+        dropout applies and none is given)."""
         residual = hidden_states
         h, next_state = self.self_attn(self.input_layernorm(hidden_states), state=state,
                                        return_state=return_state)
+        if self.training and self.dropout > 0.0:
+            rng = dropout_rng(hidden_states.device) if rng is None else rng
+            hidden_states = self._drop(h, residual, rng, 0)
+            h = self.mlp(self.post_attention_layernorm(hidden_states))
+            return self._drop(h, hidden_states, rng, 1), next_state
         hidden_states = residual + h
         hidden_states = hidden_states + self.mlp(self.post_attention_layernorm(hidden_states))
         return hidden_states, next_state
+
+    def _drop(self, h, residual, rng, branch):
+        dtype = torch.promote_types(h.dtype, residual.dtype)  # as the sum would have (autocast)
+        return dropout_add(h.to(dtype), residual.to(dtype), self.dropout, rng, call=2 * self.layer + branch)
 
 
 class PrimeForCausalLM(nn.Module):
@@ -168,7 +204,7 @@ class PrimeForCausalLM(nn.Module):
         super().__init__()
         self.config = config
         self.embed_tokens = nn.Embedding(config.vocab_size, config.hidden_size)
-        self.layers = nn.ModuleList([PrimeBlock(config) for _ in range(config.num_layers)])
+        self.layers = nn.ModuleList([PrimeBlock(config, i) for i in range(config.num_layers)])
         self.norm = RMSNorm(config.hidden_size, eps=config.rms_norm_eps)
         self.lm_head = nn.Linear(config.hidden_size, config.vocab_size, bias=False)
         if config.tie_word_embeddings:
@@ -181,6 +217,8 @@ class PrimeForCausalLM(nn.Module):
             layer.mlp.down_proj.weight.data.normal_(mean=0.0, std=scale)
             if hasattr(layer.self_attn, "init_selective_weights"):  # model.py:148-149
                 layer.self_attn.init_selective_weights()
+            if hasattr(layer.self_attn, "init_gate_weights"):
+                layer.self_attn.init_gate_weights()
 
     @classmethod
     def from_pretrained_base_to_selective(cls, checkpoint_path: str,
@@ -207,7 +245,8 @@ class PrimeForCausalLM(nn.Module):
             num_heads=get("num_heads"), head_dim=get("head_dim"), num_kv_heads=get("num_kv_heads"),
             intermediate_size=get("intermediate_size"), decay=get("decay"), use_qk_norm=get("use_qk_norm"),
             rms_norm_eps=get("rms_norm_eps"), eps=get("eps"), tie_word_embeddings=get("tie_word_embeddings"),
-            initializer_range=get("initializer_range"), use_selective=True, mlp_type=get("mlp_type", "swiglu"))
+            initializer_range=get("initializer_range"), use_selective=True, mlp_type=get("mlp_type", "swiglu"),
+            dropout=get("dropout", 0.0), gated_layers=get("gated_layers", ()))
         model = cls(sel_config).to(device)
         sd = ckpt["model_state_dict"]
         missing_keys, unexpected_keys = model.load_state_dict(sd, strict=False)
@@ -231,7 +270,8 @@ class PrimeForCausalLM(nn.Module):
     def forward(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None,
                 states: Optional[List[Tuple[torch.Tensor, ...]]] = None, return_states: bool = False,
                 logits_to_keep: int = 0) -> Dict[str, Any]:
-        if torch.is_grad_enabled() and any(p.requires_grad for p in self.parameters()):
+        if (self.training and self.config.dropout > 0.0) or (
+                torch.is_grad_enabled() and any(p.requires_grad for p in self.parameters())):
             return self._forward_graph(input_ids, labels, states, return_states, logits_to_keep)
         if input_ids.shape[-1] == 1 and _fused_step_supported(self):
             # one token per sequence (the generate loop, model.py:238): the fused
@@ -285,8 +325,9 @@ class PrimeForCausalLM(nn.Module):
         the differentiable prefill."""
         x = self.embed_tokens(input_ids)
         next_states = [] if return_states else None
+        rng = dropout_rng(x.device) if self.training and self.config.dropout > 0.0 else None
         for i, layer in enumerate(self.layers):
-            x, ns = layer(x, state=states[i] if states is not None else None, return_state=return_states)
+            x, ns = layer(x, state=states[i] if states is not None else None, return_state=return_states, rng=rng)
             if return_states:
                 next_states.append(ns)
         if logits_to_keep:
@@ -301,14 +342,31 @@ class PrimeForCausalLM(nn.Module):
 
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int = 50, temperature: float = 1.0,
-                 top_k: int = 50, eos_token_id: Optional[int] = None) -> torch.Tensor:
-        """model.py:202-242: prefill, then one recurrent step per token."""
+                 top_k: int = 50, eos_token_id: Optional[int] = None, top_p: float = 1.0, min_p: float = 0.0,
+                 generator: Optional[torch.Generator] = None) -> torch.Tensor:
+        """model.py:202-242: prefill, then one recurrent step per token.
+
+        With top_p below 1, min_p above 0 or a generator (on the model's device), tokens
+        at temperature > 0 come from sample_tokens and one uniform number each of that
+        generator: exactly top_k tokens, of equal ones the first, and NaN or -infinity
+        never chosen.  Otherwise they are the reference's torch.multinomial."""
+        own_sampler = temperature > 0.0 and (top_p < 1.0 or min_p > 0.0 or generator is not None)
         self.eval()
         out = self.forward(input_ids, return_states=True, logits_to_keep=1)
         states = out["states"]
         next_logits = out["logits"][:, -1, :]
         generated = input_ids
         for _ in range(max_new_tokens):
+            if own_sampler:
+                u = torch.rand(next_logits.shape[0], device=next_logits.device, generator=generator)
+                next_token = sample_tokens(next_logits, u, max(temperature, 1e-4), top_k, top_p, min_p).unsqueeze(1)
+                generated = torch.cat([generated, next_token], dim=-1)
+                if eos_token_id is not None and (next_token == eos_token_id).all():
+                    break
+                step = self.forward(next_token, states=states, return_states=True)
+                states = step["states"]
+                next_logits = step["logits"][:, -1, :]
+                continue
             next_logits = torch.nan_to_num(next_logits, nan=0.0, posinf=50.0, neginf=-50.0)
             if temperature > 0.0:
                 logits = next_logits / max(temperature, 1e-4)
@@ -351,6 +409,11 @@ class _LayerStep:
 
     def __init__(self, layer: "PrimeBlock", dtype: torch.dtype, device: torch.device):
         at = layer.self_attn
+        self.gated = isinstance(at, GatedLinearRecurrence)
+        if self.gated:  # runs as the module it is
+            self.qkv_g = self.up_g = self.frag = None
+            self.folded = False
+            return
         self.qkv = torch.cat([at.q_proj.weight, at.k_proj.weight, at.v_proj.weight], dim=0)
         self.norm = _lib.qk_norm(at.q_norm if at.use_qk_norm else None, at.k_norm if at.use_qk_norm else None,
                                  at.scaling, dtype)
@@ -463,11 +526,24 @@ def _fused_step_supported(model: "PrimeForCausalLM") -> bool:
         return False
     for layer in model.layers:
         at = layer.self_attn
+        if isinstance(at, GatedLinearRecurrence):
+            continue
         if at.use_qk_norm:
             for t in (at.q_norm.weight, at.q_norm.bias, at.k_norm.weight, at.k_norm.bias):
                 if t is None or t.dtype != w.dtype or t.device != w.device or not t.is_contiguous():
                     return False
     return True
+
+
+def _finish_step(layer: "PrimeBlock", x: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
+    """The block behind its mixer's y [B, H*D]: the output projection added to x in
+    place, and the MLP of its norm, still to be added."""
+    a = _decode_linear(y, layer.self_attn.o_proj.weight)
+    n2 = torch.empty_like(x)
+    _lib.add_rmsnorm(x, a, layer.post_attention_layernorm.weight, n2, layer.post_attention_layernorm.eps)
+    if isinstance(layer.mlp, PrimeGeluMLP):
+        return _decode_linear(_decode_linear(n2, layer.mlp.up_proj.weight, gelu=True), layer.mlp.down_proj.weight)
+    return layer.mlp(n2)
 
 
 @torch.no_grad()
@@ -504,6 +580,14 @@ def _fused_step(model: "PrimeForCausalLM", tokens: torch.Tensor, states, consts:
     next_states = []
     for i, (layer, c) in enumerate(zip(model.layers, consts)):
         at = layer.self_attn
+        if c.gated:
+            n1 = torch.empty_like(x)
+            _lib.add_rmsnorm(x, pending, layer.input_layernorm.weight, n1, layer.input_layernorm.eps)
+            y, st_out = at.mix(n1.unsqueeze(1), state=states[i] if states is not None else None, return_state=True,
+                               in_place=inplace)
+            next_states.append(st_out)
+            pending = _finish_step(layer, x, y.view(B, -1))
+            continue
         H, Hk, D = at.num_heads, at.num_kv_heads, at.head_dim
         if folded:
             qkv = _lib.linear_fused(x, c.qkv_g, torch.empty(B, c.qkv_g.shape[0], device=dev, dtype=x.dtype),
@@ -540,14 +624,7 @@ def _fused_step(model: "PrimeForCausalLM", tokens: torch.Tensor, states, consts:
                                   _lib.EPILOGUE_GELU, layer.post_attention_layernorm.eps)
             x.addmm_(t, layer.mlp.down_proj.weight.t())
             continue
-        a = _decode_linear(y.view(B, -1), at.o_proj.weight)
-        n2 = torch.empty_like(x)
-        _lib.add_rmsnorm(x, a, layer.post_attention_layernorm.weight, n2, layer.post_attention_layernorm.eps)
-        if isinstance(layer.mlp, PrimeGeluMLP):
-            pending = _decode_linear(_decode_linear(n2, layer.mlp.up_proj.weight, gelu=True),
-                                     layer.mlp.down_proj.weight)
-        else:
-            pending = layer.mlp(n2)
+        pending = _finish_step(layer, x, y.view(B, -1))
     nf = torch.empty_like(x)
     _lib.add_rmsnorm(x, pending, model.norm.weight, nf, model.norm.eps)
     return model.lm_head(nf), next_states
@@ -659,13 +736,17 @@ class GreedyDecoder:
         """Run the prompt; returns the first generated token [B, 1]."""
         m = self.model
         out = m.forward(input_ids, return_states=True, logits_to_keep=1)
-        self.states = [tuple(s) for s in out["states"]]
+        self.states = [s if torch.is_tensor(s) else tuple(s) for s in out["states"]]
         self.token = torch.empty(input_ids.shape[0], 1, dtype=torch.int64, device=input_ids.device)
-        _lib.argmax(out["logits"][:, -1, :], self.token)
+        self._choose(out["logits"][:, -1, :])
         # the step's per-layer constants, taken from the modules now
         self.consts = _step_constants(m)
         self.graph = None
         return self.token
+
+    def _choose(self, logits: torch.Tensor) -> None:
+        """The next tokens [B, 1] of logits [B, V], into self.token."""
+        _lib.argmax(logits, self.token)
 
     @torch.no_grad()
     def _step_eager(self) -> torch.Tensor:
@@ -676,7 +757,7 @@ class GreedyDecoder:
                        tokens_out=self.token.view(-1))
             return self.token
         logits, _ = _fused_step(self.model, self.token, self.states, self.consts, inplace=True)
-        _lib.argmax(logits, self.token)  # the embedding above has consumed the old token
+        self._choose(logits)  # the embedding above has consumed the old token
         return self.token
 
     @torch.no_grad()
@@ -692,14 +773,15 @@ class GreedyDecoder:
     def _capture(self):
         # warm up on a side stream (allocator pools, cached decay tensors), on a
         # copy of the states so that the real states advance only by replays
-        saved = [tuple(t.clone() for t in st) for st in self.states]
+        states = [(st,) if torch.is_tensor(st) else st for st in self.states]
+        saved = [tuple(t.clone() for t in st) for st in states]
         tok = self.token.clone()
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
             self._step_eager()
         torch.cuda.current_stream().wait_stream(s)
-        for st, sv in zip(self.states, saved):
+        for st, sv in zip(states, saved):
             for t, x in zip(st, sv):
                 t.copy_(x)
         self.token.copy_(tok)
@@ -715,3 +797,44 @@ class GreedyDecoder:
         for _ in range(max_new_tokens - 1):
             toks.append(self.step().clone())
         return torch.cat([input_ids] + toks, dim=-1)
+
+
+class SamplingDecoder(GreedyDecoder):
+    """GreedyDecoder with sampled tokens: temperature, top_k, top_p and min_p as
+    sample_tokens takes them, numbers or one value per sequence (0, 1 and 0 cut
+    nothing; temperature 0 is greedy), and one uniform number per token from
+    ``generator`` (on the model's device; None: torch's own).  The numbers are drawn
+    before each step into a fixed buffer, so that replays of the captured step sample
+    anew and a seeded generator gives the same tokens with and without a graph."""
+
+    def __init__(self, model: PrimeForCausalLM, temperature=1.0, top_k=50, top_p=1.0, min_p=0.0,
+                 generator: Optional[torch.Generator] = None, use_graph: bool = True):
+        super().__init__(model, use_graph)
+        self.cuts = (temperature, top_k, top_p, min_p)
+        self.generator = generator
+
+    @torch.no_grad()
+    def prefill(self, input_ids: torch.Tensor) -> torch.Tensor:
+        dev = input_ids.device
+        self.uniforms = torch.rand(input_ids.shape[0], device=dev, generator=self.generator)
+        # held here in the kernel's types: a captured step reads these tensors
+        self.params = [v.to(device=dev, dtype=dt).contiguous() if torch.is_tensor(v) else v
+                       for v, dt in zip(self.cuts, (torch.float32, torch.int32, torch.float32, torch.float32))]
+        return super().prefill(input_ids)
+
+    def _choose(self, logits: torch.Tensor) -> None:
+        sample_tokens(logits, self.uniforms, *self.params, out=self.token.view(-1))
+
+    @torch.no_grad()
+    def _step_eager(self) -> torch.Tensor:
+        if _frag_step_ready(self.consts):
+            logits, _ = _frag_step(self.model, self.token, self.states, self.consts, inplace=True)
+        else:
+            logits, _ = _fused_step(self.model, self.token, self.states, self.consts, inplace=True)
+        self._choose(logits)
+        return self.token
+
+    @torch.no_grad()
+    def step(self) -> torch.Tensor:
+        self.uniforms.uniform_(generator=self.generator)
+        return super().step()
