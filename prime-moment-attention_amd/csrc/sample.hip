@@ -87,6 +87,10 @@ struct RowScale {
     }
 };
 
+__device__ __forceinline__ uint64_t shfl_u64(uint64_t v, int lane) {
+    return static_cast<uint64_t>(__shfl(static_cast<uint32_t>(v >> 32), lane, kWave)) << 32 |
+           __shfl(static_cast<uint32_t>(v), lane, kWave);
+}
 // v of lane 63
 __device__ __forceinline__ uint64_t last_lane(uint64_t v) {
     return static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), 63)) << 32 |
@@ -119,7 +123,8 @@ struct SampleShared {
     uint64_t sum, rest;
     int list_i[kFew];
     float last;
-    int bucket, n, index, owner, kept;
+    int bucket, n, index, owner, kept, low, high;
+    uint8_t list_wave[kList];
 };
 
 // exclusive sum over the threads, the sum over the waves before, and the total
@@ -430,6 +435,137 @@ __device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT,
     whole = last != floor && ties * w == sh.rest;
 }
 
+// The cut by masses over all tokens (no top-k before it, no min_p behind) with each one's mass
+// computed once, which gives the kept masses of the lanes' waves along with the cut (mass: of
+// tokens above `last`, or equal to it where all of those are kept; count: of the tokens equal
+// to it otherwise).
+//
+// A token in bucket b weighs between 2^(-(b + 1) step) and 2^(-b step), with a hundredth of a
+// bucket for roundings, so the buckets' counts bound every prefix's mass, and the bucket where
+// top_p falls, to a few of them: low .. high.  Masses of higher tokens are added up in the
+// lanes, only those between go into shared sums, one for each wave and bucket.
+// False, and nothing decided, where those are more than kRange buckets (few tokens, of which
+// one comparison with each other is cheaper), or one holds too many tokens to compare.
+template <int DT, int WAVES, int STAGED, typename F>
+__device__ __forceinline__ bool cut_once(SampleShared<WAVES> &sh, const SampleRow<DT, STAGED> &row, const RowScale &rs,
+                                         float top_p, F share, float &last, uint64_t &ties, bool &whole, uint64_t &mass,
+                                         uint64_t &count) {
+    constexpr int kThreads = WAVES * kWave, kPer = kBuckets / kThreads, VE = SampleRow<DT, STAGED>::VE;
+    constexpr int kRange = 64;
+    static_assert(WAVES * kRange <= kBuckets, "the waves' sums take the histogram's place");
+    const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
+    const float step = static_cast<float>(2.0 * rs.rate / static_cast<double>(rs.per_half));
+    if (!(step < 1.f)) return false;  // (T above any use: one bucket for all)
+    uint32_t *counts = reinterpret_cast<uint32_t *>(sh.hist);
+    __syncthreads();
+    for (int b = tid; b < kBuckets; b += kThreads) counts[b] = 0;
+    if (tid == 0) sh.n = 0, sh.low = sh.high = kBuckets - 1;
+    __syncthreads();
+    row.each([&](int, const float (&x)[VE]) {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+            int b;
+            if (rs.bucket(x[j], b)) atomicAdd(&counts[b], 1u);
+        }
+    });
+    __syncthreads();
+    uint64_t most[kPer], least[kPer], all_most, all_least, waves;  // in 2^-30 of the largest mass
+    uint64_t to_most = 0, to_least = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int b = tid * kPer + i;
+        const float n = static_cast<float>(counts[b]) * 1073741824.f, at = static_cast<float>(b);
+        most[i] = static_cast<uint64_t>(n * __builtin_amdgcn_exp2f(step * (0.01f - at)) * 1.0001f) + (counts[b] ? 1 : 0);
+        least[i] = static_cast<uint64_t>(n * __builtin_amdgcn_exp2f(-step * (at + 1.01f)) * 0.9999f);
+        to_most += most[i];
+        to_least += least[i];
+    }
+    to_most = block_scan(sh, to_most, waves, all_most), to_least = block_scan(sh, to_least, waves, all_least);
+    const double from = 0.9999 * top_p * static_cast<double>(all_least), to = 1.0001 * top_p * static_cast<double>(all_most);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int b = tid * kPer + i;
+        const double m0 = static_cast<double>(to_most), l0 = static_cast<double>(to_least);
+        to_most += most[i], to_least += least[i];
+        if (m0 < from && from <= static_cast<double>(to_most)) sh.low = b;
+        if (l0 < to && to <= static_cast<double>(to_least)) sh.high = b;
+    }
+    __syncthreads();
+    const int low = sh.low, range = sh.high - low + 1;
+    if (range < 1 || range > kRange) return false;
+    uint64_t *sums = sh.hist;  // [wave][kRange]
+    for (int b = tid; b < WAVES * kRange; b += kThreads) sums[b] = 0;
+    __syncthreads();
+    uint64_t rest = 0;
+    mass = count = 0;
+    row.each([&](int, const float (&x)[VE]) {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+            int b;
+            const bool in = rs.bucket(x[j], b);
+            const uint64_t w = RowScale::select(in, rs.mass_of(rs.exponent(x[j])));
+            b -= low;
+            rest += w;
+            mass += b < 0 ? w : 0;
+            if (in & (static_cast<uint32_t>(b) < static_cast<uint32_t>(range))) lds_add(&sums[wave * kRange + b], w);
+        }
+    });
+    uint64_t all, above;
+    block_scan(sh, rest, waves, all);
+    block_scan(sh, mass, waves, above);
+    const uint64_t want = share(all);
+    // every wave finds the bucket for itself: lane b has bucket low + b
+    uint64_t sum = 0;
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) sum += sums[k * kRange + lane];
+    const uint64_t to_b = above + wave_scan_u64(sum);
+    const uint64_t hit = __ballot(to_b - sum < want && want <= to_b);
+    if (!hit) return false;
+    const int found = __builtin_ctzll(hit), bucket = low + found;
+    const uint64_t over0 = shfl_u64(to_b - sum, found);
+    row.each([&](int, const float (&x)[VE]) {
+        int b;
+        if (!(rs.bucket(largest(x), b) & (b <= bucket))) return;
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+            if (rs.bucket(x[j], b) & (b == bucket)) {
+                const int n = atomicAdd(&sh.n, 1);
+                if (n < kList) sh.list_x[n] = x[j], sh.list_wave[n] = static_cast<uint8_t>(wave);
+            }
+        }
+    });
+    __syncthreads();
+    const int n = sh.n;
+    if (n > kList) return false;
+    for (int i = tid; i < n; i += kThreads) sh.list_w[i] = rs.mass(sh.list_x[i]);
+    __syncthreads();
+    for (int i = tid; i < n; i += kThreads) {
+        const float x = sh.list_x[i];
+        uint64_t over = over0, equal = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) {
+            const float y = sh.list_x[j];
+            const uint64_t w = sh.list_w[j];
+            over += y > x ? w : 0;
+            equal += y == x ? w : 0;
+        }
+        if (over < want && want <= over + equal) sh.last = x, sh.sum = over, sh.rest = equal;
+    }
+    __syncthreads();
+    last = sh.last;
+    const uint64_t w = rs.mass(last);
+    ties = (want - sh.sum + w - 1) / w;
+    whole = ties * w == sh.rest;
+    if (lane < found) mass += sums[wave * kRange + lane];
+    for (int i = lane; i < n; i += kWave) {
+        const float x = sh.list_x[i];
+        if (sh.list_wave[i] != wave) continue;
+        if (x > last || (whole && x == last)) mass += sh.list_w[i];
+        else count += x == last;
+    }
+    return true;
+}
+
 template <int DT, int WAVES, int STAGED>
 __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a) {
     __shared__ SampleShared<WAVES> sh;
@@ -518,12 +654,15 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
     int kept = a.vocab;
     if (top_k < a.vocab)
         cut<false>(sh, row, rs, lane_top, last, ties, whole, kept, [&](uint64_t) { return static_cast<uint64_t>(top_k); });
-    if (top_p < 1.f) cut<true>(sh, row, rs, lane_top, last, ties, whole, kept, share);
+    uint64_t mass = 0, count = 0;  // the lane's kept ones, once summed
+    const bool summed = top_p < 1.f && !ties && !(min_p > 0.f) &&
+                        cut_once(sh, row, rs, top_p, share, last, ties, whole, mass, count);
+    if (top_p < 1.f && !summed) cut<true>(sh, row, rs, lane_top, last, ties, whole, kept, share);
 
     // Few kept ones are compared with each other: a token's running mass is the sum over
     // those with a lower index.  (min_p alone leaves few as a rule: tried, and given up at
     // the first too many.)
-    if (kept <= kFew || (!ties && min_p > 0.f)) {
+    if (!summed && (kept <= kFew || (!ties && min_p > 0.f))) {
         // nothing below this weighs: `last`, or what min_p leaves, with room for rounding
         const float far = top + static_cast<float>(rs.least / rs.rate), room = 1e-5f * (fabsf(top) + fabsf(far));
         const float least_x = ties ? last : fmaxf(far - room, -__FLT_MAX__);
@@ -572,7 +711,7 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
         }
     }
 
-    // Else the row is summed once more: the masses above `last`, and the tokens equal to it,
+    // Else the row is summed (once more): the masses above `last`, and the tokens equal to it,
     // of which the first `ties` weigh.  Where all of them are kept, they are the ones above the
     // next value below it (below 0 that is not -0).
     if (whole && ties) {
@@ -595,8 +734,11 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
             for (int j = 0; j < VE; ++j) count += x[j] == last;
         }
     };
-    uint64_t mass = 0, count = 0, all_mass, all_count, mass0, count0;  // ..0: before the wave
-    row.each([&](int, const float (&x)[VE]) { add_chunk(x, mass, count); });
+    uint64_t all_mass, all_count, mass0, count0;  // ..0: before the wave
+    if (!summed) {
+        mass = count = 0;
+        row.each([&](int, const float (&x)[VE]) { add_chunk(x, mass, count); });
+    }
     const uint64_t wave_count = ties ? last_lane(wave_scan_u64(count)) : 0;
     count0 = all_count = 0;
     if (ties) block_scan(sh, count, count0, all_count);
