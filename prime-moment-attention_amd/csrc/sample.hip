@@ -21,7 +21,7 @@
 namespace prime {
 
 constexpr uint64_t kMass = 1ull << 42;  // the largest token's
-constexpr int kBuckets = 2048, kList = 1024, kFew = 256;
+constexpr int kBuckets = 2048, kList = 1024;
 constexpr double kLightest = -43.5;    // a token of weight 2^-43.5 or less has mass 0
 constexpr float kBucketSpan = 30.5f;  // so has one this many T below the largest
 constexpr float kInf = __builtin_inff();
@@ -121,7 +121,6 @@ struct SampleShared {
     float list_x[kList];
     uint64_t part[WAVES];
     uint64_t sum, rest;
-    int list_i[kFew];
     float last;
     int bucket, n, index, owner, kept, low, high;
     uint8_t list_wave[kList];
@@ -304,11 +303,11 @@ __device__ __forceinline__ float largest(const float (&x)[N]) {
 // WEIGH: masses, else ones.  Left as it is where all of them are needed.  whole: the tokens
 // equal to the new `last` are known to be all kept.
 //
-// For top-k a first histogram, of the lanes' largest logits (lane_top), bounds the buckets
-// that matter: k lanes have a token at or above its `limit`, so at least as many tokens have.
+// For top-k a first histogram, of the chunks' largest logits, bounds the buckets that matter:
+// k chunks have a token at or above its `limit`, so at least as many tokens have.
 // kept: an upper bound of the tokens left.
 template <bool WEIGH, int DT, int WAVES, int STAGED, typename F>
-__device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT, STAGED> &row, const RowScale &rs, float lane_top,
+__device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT, STAGED> &row, const RowScale &rs,
                                     float &last, uint64_t &ties, bool &whole, int &kept, F wanted) {
     constexpr int kThreads = WAVES * kWave, VE = SampleRow<DT, STAGED>::VE;
     const int tid = threadIdx.x;
@@ -325,15 +324,15 @@ __device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT,
     int limit = kBuckets;
     if constexpr (!WEIGH) {
         const uint64_t enough = wanted(0);
-        if (enough <= kThreads) {
+        row.each([&](int, const float (&x)[VE]) {
             int b;
-            if (rs.bucket(lane_top, b)) lds_add(&sh.hist[b], 1);
-            __syncthreads();
-            before = scan_hist(sh, mine, total);
-            locate(sh, before, mine, enough);
-            limit = sh.bucket;
-            clear();
-        }
+            if (rs.bucket(largest(x), b)) atomicAdd(reinterpret_cast<uint32_t *>(&sh.hist[b]), 1u);
+        });
+        __syncthreads();
+        before = scan_hist(sh, mine, total);
+        locate(sh, before, mine, enough);
+        limit = sh.bucket;  // (kBuckets where there are not as many chunks)
+        clear();
     }
     auto fill = [&](int, const float (&x)[VE]) {
         int b;
@@ -593,7 +592,6 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
 #pragma unroll
         for (int j = 0; j < VE; ++j) top = fmaxf(top, x[j]);
     });
-    const float lane_top = top;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
     if (lane == 0) sh.list_x[wave] = top;
@@ -653,63 +651,98 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
     bool whole = true;
     int kept = a.vocab;
     if (top_k < a.vocab)
-        cut<false>(sh, row, rs, lane_top, last, ties, whole, kept, [&](uint64_t) { return static_cast<uint64_t>(top_k); });
-    uint64_t mass = 0, count = 0;  // the lane's kept ones, once summed
-    const bool summed = top_p < 1.f && !ties && !(min_p > 0.f) &&
-                        cut_once(sh, row, rs, top_p, share, last, ties, whole, mass, count);
-    if (top_p < 1.f && !summed) cut<true>(sh, row, rs, lane_top, last, ties, whole, kept, share);
-
-    // Few kept ones are compared with each other: a token's running mass is the sum over
-    // those with a lower index.  (min_p alone leaves few as a rule: tried, and given up at
-    // the first too many.)
-    if (!summed && (kept <= kFew || (!ties && min_p > 0.f))) {
+        cut<false>(sh, row, rs, last, ties, whole, kept, [&](uint64_t) { return static_cast<uint64_t>(top_k); });
+    // After top-k, or where min_p alone cuts, few are left as a rule: one thread takes each, in
+    // the order of their indices, and the rest is a few sums over the threads.
+    const bool top_k_cut = ties > 0;
+    if (top_k_cut ? kept <= WAVES * kWave : top_p >= 1.f && min_p > 0.f) {
         // nothing below this weighs: `last`, or what min_p leaves, with room for rounding
         const float far = top + static_cast<float>(rs.least / rs.rate), room = 1e-5f * (fabsf(top) + fabsf(far));
         const float least_x = ties ? last : fmaxf(far - room, -__FLT_MAX__);
-        __syncthreads();
-        if (tid == 0) sh.n = 0;
-        __syncthreads();
-        row.each([&](int i, const float (&x)[VE]) {
-            if (!(largest(x) >= least_x) || sh.n > kFew) return;
+        uint64_t n = 0, first, all;
+        row.each([&](int, const float (&x)[VE]) {
 #pragma unroll
-            for (int j = 0; j < VE; ++j) {
-                if (x[j] >= least_x) {
-                    const int n = atomicAdd(&sh.n, 1);
-                    if (n < kFew) sh.list_x[n] = x[j], sh.list_i[n] = row.index(i) + j;
-                }
-            }
+            for (int j = 0; j < VE; ++j) n += x[j] >= least_x;
         });
-        __syncthreads();
-        const int n = sh.n;
-        if (n <= kFew) {
-            if (tid < n) {
-                const float x = sh.list_x[tid];
-                const double t = rs.exponent(x);
-                uint64_t w = t >= rs.least && (x > last || ties) ? RowScale::mass_of(t) : 0;
-                if (x == last && !whole) {  // of those equal to `last` only the first weigh
-                    uint64_t rank = 0;
-#pragma unroll 8
-                    for (int k = 0; k < n; ++k) rank += (sh.list_x[k] == last) & (sh.list_i[k] < sh.list_i[tid]);
-                    w = rank < ties ? w : 0;
+        block_scan(sh, n, first, all);
+        if (all <= WAVES * kWave) {
+            int *list_i = reinterpret_cast<int *>(sh.list_w);
+            int at = static_cast<int>(first);
+            row.each([&](int i, const float (&x)[VE]) {
+                if (!__any(largest(x) >= least_x)) return;
+                int chunk = 0, place = at;
+#pragma unroll
+                for (int j = 0; j < VE; ++j) {
+                    const uint64_t b = __ballot(x[j] >= least_x);
+                    chunk += __popcll(b);
+                    place += __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(b >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(b), 0));
                 }
-                sh.list_w[tid] = w;
-            }
+#pragma unroll
+                for (int j = 0; j < VE; ++j) {
+                    if (x[j] >= least_x) {
+                        sh.list_x[place] = x[j], list_i[place] = row.index(i) + j;
+                        ++place;
+                    }
+                }
+                at += chunk;
+            });
             __syncthreads();
-            if (tid < n) {
-                const int index = sh.list_i[tid];
-                uint64_t at = 0, total = 0;
-#pragma unroll 8
-                for (int k = 0; k < n; ++k) {
-                    const uint64_t w = sh.list_w[k];
-                    total += w;
-                    at += sh.list_i[k] < index ? w : 0;
-                }
-                const uint64_t target = target_of(total);
-                if (at <= target && target < at + sh.list_w[tid]) a.out[r] = index;
+            const bool mine = tid < static_cast<int>(all);
+            const float x = mine ? sh.list_x[tid] : -kInf;
+            const int index = mine ? list_i[tid] : 0;
+            const double t = rs.exponent(mine ? x : top);
+            uint64_t waves, total, w = RowScale::select(mine & (t >= kLightest), RowScale::mass_of(t));
+            if (ties && !whole) {  // of those equal to `last` only the first
+                const uint64_t rank = block_scan(sh, x == last, waves, total);
+                w = x == last && rank >= ties ? 0 : w;
             }
+            if (top_p < 1.f) {
+                // the cut of these by their masses: its bucket, and the tokens in it with each other
+                __syncthreads();
+                for (int b = tid; b < kBuckets; b += WAVES * kWave) sh.hist[b] = 0;
+                if (tid == 0) sh.n = 0;
+                __syncthreads();
+                int b;
+                if (!rs.bucket(x, b)) b = -1, w = 0;
+                if (w) lds_add(&sh.hist[b], w);
+                __syncthreads();
+                uint64_t part, over, equal;
+                const uint64_t before = scan_hist(sh, part, total), want = share(total);
+                locate(sh, before, part, want);
+                const bool in = w && b == sh.bucket;
+                if (in) {
+                    const int k = atomicAdd(&sh.n, 1);
+                    sh.list_x[k] = x, sh.list_w[k] = w;
+                }
+                __syncthreads();
+                if (in) {
+                    over = sh.sum, equal = 0;
+                    const int m = sh.n;
+#pragma unroll 8
+                    for (int k = 0; k < m; ++k) {
+                        const float y = sh.list_x[k];
+                        const uint64_t v = sh.list_w[k];
+                        over += y > x ? v : 0;
+                        equal += y == x ? v : 0;
+                    }
+                    if (over < want && want <= over + equal) sh.last = x, sh.rest = (want - over + w - 1) / w;
+                }
+                __syncthreads();
+                const float end = sh.last;
+                const uint64_t rank = block_scan(sh, w && x == end, waves, total);
+                w = x > end || (x == end && rank < sh.rest) ? w : 0;
+            }
+            w = RowScale::select(t >= rs.least, w);
+            const uint64_t to = block_scan(sh, w, waves, total), target = target_of(total);
+            if (to <= target && target < to + w) a.out[r] = index;
             return;
         }
     }
+
+    uint64_t mass = 0, count = 0;  // the lane's kept ones, once summed
+    const bool summed = top_p < 1.f && !ties && !(min_p > 0.f) &&
+                        cut_once(sh, row, rs, top_p, share, last, ties, whole, mass, count);
+    if (top_p < 1.f && !summed) cut<true>(sh, row, rs, last, ties, whole, kept, share);
 
     // Else the row is summed (once more): the masses above `last`, and the tokens equal to it,
     // of which the first `ties` weigh.  Where all of them are kept, they are the ones above the
