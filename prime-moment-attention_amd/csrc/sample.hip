@@ -49,6 +49,7 @@ struct RowScale {
     double rate;      // log2(e) / T
     double least;     // log2 of min_p, at least kLightest
     float per_half;   // buckets per half a unit of the logit
+    float step;       // log2 of the weight from one bucket to the next
 
     __device__ __forceinline__ double exponent(float x) const {  // of 2, at most 0
         return (static_cast<double>(x) - static_cast<double>(top)) * rate;
@@ -80,8 +81,9 @@ struct RowScale {
     }
     __device__ static __forceinline__ uint64_t select(bool keep, uint64_t w) { return keep ? w : 0; }
     // bucket of x, false for tokens whose mass is 0 (and for NaN); monotone: every step is
+    __device__ __forceinline__ float place(float x) const { return fmaf(-0.5f, x, 0.5f * top) * per_half; }
     __device__ __forceinline__ bool bucket(float x, int &b) const {
-        const float f = fmaf(-0.5f, x, 0.5f * top) * per_half;
+        const float f = place(x);
         b = static_cast<int>(f);
         return f < static_cast<float>(kBuckets - 1);
     }
@@ -122,7 +124,7 @@ struct SampleShared {
     uint64_t part[WAVES];
     uint64_t sum, rest;
     float last;
-    int bucket, n, index, owner, kept, low, high;
+    int bucket, n, index, owner, low, high;
     uint8_t list_wave[kList];
 };
 
@@ -302,45 +304,25 @@ __device__ __forceinline__ float largest(const float (&x)[N]) {
 // in rank order, the shortest prefix with weight of at least wanted(sum of all weights).
 // WEIGH: masses, else ones.  Left as it is where all of them are needed.  whole: the tokens
 // equal to the new `last` are known to be all kept.
-//
-// For top-k a first histogram, of the chunks' largest logits, bounds the buckets that matter:
-// k chunks have a token at or above its `limit`, so at least as many tokens have.
-// kept: an upper bound of the tokens left.
 template <bool WEIGH, int DT, int WAVES, int STAGED, typename F>
 __device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT, STAGED> &row, const RowScale &rs,
-                                    float &last, uint64_t &ties, bool &whole, int &kept, F wanted) {
+                                    float &last, uint64_t &ties, bool &whole, F wanted) {
     constexpr int kThreads = WAVES * kWave, VE = SampleRow<DT, STAGED>::VE;
     const int tid = threadIdx.x;
     const float floor = last;
     const uint64_t floor_w = ties ? ties * (WEIGH ? rs.mass(floor) : 1) : 0;
     uint64_t before, mine, total;
-    auto clear = [&]() {
-        __syncthreads();
-        for (int b = tid; b < kBuckets; b += kThreads) sh.hist[b] = 0;
-        if (tid == 0) sh.n = 0, sh.bucket = kBuckets, sh.kept = 0;
-        __syncthreads();
-    };
-    clear();
-    int limit = kBuckets;
-    if constexpr (!WEIGH) {
-        const uint64_t enough = wanted(0);
-        row.each([&](int, const float (&x)[VE]) {
-            int b;
-            if (rs.bucket(largest(x), b)) atomicAdd(reinterpret_cast<uint32_t *>(&sh.hist[b]), 1u);
-        });
-        __syncthreads();
-        before = scan_hist(sh, mine, total);
-        locate(sh, before, mine, enough);
-        limit = sh.bucket;  // (kBuckets where there are not as many chunks)
-        clear();
-    }
+    __syncthreads();
+    for (int b = tid; b < kBuckets; b += kThreads) sh.hist[b] = 0;
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
     auto fill = [&](int, const float (&x)[VE]) {
         int b;
         const float most = largest(x);
-        if (!(rs.bucket(most, b) & (b <= limit) & (most > floor))) return;
+        if (!(rs.bucket(most, b) & (most > floor))) return;
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
-            const bool in = rs.bucket(x[j], b) & (b <= limit) & (x[j] > floor);
+            const bool in = rs.bucket(x[j], b) & (x[j] > floor);
             const uint64_t w = WEIGH ? RowScale::mass_of(rs.exponent(x[j])) : 1;
             if (in) lds_add(&sh.hist[b], w);
         }
@@ -356,23 +338,17 @@ __device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT,
     locate(sh, before, mine, want);
     const int bucket = sh.bucket;
     const uint64_t above = sh.sum;
-    int higher = 0;
     row.each([&](int, const float (&x)[VE]) {
         int b;
-        const float most = largest(x);
-        if (!(rs.bucket(most, b) & (b <= bucket))) return;
+        if (!(rs.bucket(largest(x), b) & (b <= bucket))) return;
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
-            const bool in = rs.bucket(x[j], b) & (x[j] > floor);
-            higher += in & (b < bucket);
-            if (in & (b == bucket)) {
+            if (rs.bucket(x[j], b) & (b == bucket) & (x[j] > floor)) {
                 const int n = atomicAdd(&sh.n, 1);
                 if (n < kList) sh.list_x[n] = x[j];
             }
         }
     });
-    const int wave_higher = static_cast<int>(last_lane(wave_scan_u64(higher)));
-    if (tid % kWave == 0) atomicAdd(&sh.kept, wave_higher);
     __syncthreads();
     const int own = sh.n, n = own + (floor_b == bucket);  // the floor's tokens count as one more
     if (n <= kList) {
@@ -380,7 +356,6 @@ __device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT,
         if (tid == 0 && n > own) sh.list_x[own] = floor, sh.list_w[own] = floor_w;
         __syncthreads();
     }
-    kept = n > own ? kept : min(kept, sh.kept + n);
     // `over`: the weight of the tokens above x; `equal`: of those equal to it, where known
     auto found = [&](float x, uint64_t over, uint64_t equal) { sh.last = x, sh.sum = over, sh.rest = equal; };
     if (n <= kList) {
@@ -434,31 +409,16 @@ __device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT,
     whole = last != floor && ties * w == sh.rest;
 }
 
-// The cut by masses over all tokens (no top-k before it, no min_p behind) with each one's mass
-// computed once, which gives the kept masses of the lanes' waves along with the cut (mass: of
-// tokens above `last`, or equal to it where all of those are kept; count: of the tokens equal
-// to it otherwise).
-//
-// A token in bucket b weighs between 2^(-(b + 1) step) and 2^(-b step), with a hundredth of a
-// bucket for roundings, so the buckets' counts bound every prefix's mass, and the bucket where
-// top_p falls, to a few of them: low .. high.  Masses of higher tokens are added up in the
-// lanes, only those between go into shared sums, one for each wave and bucket.
-// False, and nothing decided, where those are more than kRange buckets (few tokens, of which
-// one comparison with each other is cheaper), or one holds too many tokens to compare.
-template <int DT, int WAVES, int STAGED, typename F>
-__device__ __forceinline__ bool cut_once(SampleShared<WAVES> &sh, const SampleRow<DT, STAGED> &row, const RowScale &rs,
-                                         float top_p, F share, float &last, uint64_t &ties, bool &whole, uint64_t &mass,
-                                         uint64_t &count) {
-    constexpr int kThreads = WAVES * kWave, kPer = kBuckets / kThreads, VE = SampleRow<DT, STAGED>::VE;
-    constexpr int kRange = 64;
-    static_assert(WAVES * kRange <= kBuckets, "the waves' sums take the histogram's place");
-    const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
-    const float step = static_cast<float>(2.0 * rs.rate / static_cast<double>(rs.per_half));
-    if (!(step < 1.f)) return false;  // (T above any use: one bucket for all)
+// The buckets' token counts, in the histogram's place.  False where all of a row is one bucket
+// (a temperature above any use).
+template <int DT, int WAVES, int STAGED>
+__device__ __forceinline__ bool count_buckets(SampleShared<WAVES> &sh, const SampleRow<DT, STAGED> &row, const RowScale &rs) {
+    constexpr int VE = SampleRow<DT, STAGED>::VE;
+    if (!(rs.step < 1.f)) return false;
     uint32_t *counts = reinterpret_cast<uint32_t *>(sh.hist);
     __syncthreads();
-    for (int b = tid; b < kBuckets; b += kThreads) counts[b] = 0;
-    if (tid == 0) sh.n = 0, sh.low = sh.high = kBuckets - 1;
+    for (int b = threadIdx.x; b < kBuckets; b += WAVES * kWave) counts[b] = 0;
+    if (threadIdx.x == 0) sh.low = 0, sh.high = kBuckets - 1, sh.n = 1 << 30;
     __syncthreads();
     row.each([&](int, const float (&x)[VE]) {
 #pragma unroll
@@ -468,30 +428,91 @@ __device__ __forceinline__ bool cut_once(SampleShared<WAVES> &sh, const SampleRo
         }
     });
     __syncthreads();
-    uint64_t most[kPer], least[kPer], all_most, all_least, waves;  // in 2^-30 of the largest mass
-    uint64_t to_most = 0, to_least = 0;
+    return true;
+}
+
+// Where a cut falls, from the counts: in one of the buckets low .. high, with `above` tokens
+// above those and `tokens` up to their end.
+struct Bounds {
+    int low, high, above, tokens;
+};
+
+// top-k: one bucket, or (false) none, where no more than k tokens weigh anything.
+template <int WAVES>
+__device__ __forceinline__ bool bound_count(SampleShared<WAVES> &sh, int k, Bounds &out) {
+    constexpr int kPer = kBuckets / (WAVES * kWave);
+    const uint32_t *counts = reinterpret_cast<uint32_t *>(sh.hist);
+    uint64_t n = 0, waves, total;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) n += counts[threadIdx.x * kPer + i];
+    int to = static_cast<int>(block_scan(sh, n, waves, total));
+    if (static_cast<uint64_t>(k) >= total) return false;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const int b = tid * kPer + i;
-        const float n = static_cast<float>(counts[b]) * 1073741824.f, at = static_cast<float>(b);
-        most[i] = static_cast<uint64_t>(n * __builtin_amdgcn_exp2f(step * (0.01f - at)) * 1.0001f) + (counts[b] ? 1 : 0);
-        least[i] = static_cast<uint64_t>(n * __builtin_amdgcn_exp2f(-step * (at + 1.01f)) * 0.9999f);
+        const int c = counts[threadIdx.x * kPer + i];
+        if (to < k && k <= to + c) sh.high = threadIdx.x * kPer + i, sh.low = to, sh.n = to + c;
+        to += c;
+    }
+    __syncthreads();
+    out = {sh.high, sh.high, sh.low, sh.n};
+    return true;
+}
+
+// top_p: a token in bucket b weighs between 2^(-(b + 1) step) and 2^(-b step), with a hundredth
+// of a bucket for roundings, so the counts bound every prefix's mass.
+template <int WAVES>
+__device__ __forceinline__ void bound_mass(SampleShared<WAVES> &sh, const RowScale &rs, float top_p, Bounds &out) {
+    constexpr int kPer = kBuckets / (WAVES * kWave);
+    const uint32_t *counts = reinterpret_cast<uint32_t *>(sh.hist);
+    // the most and the least, in 2^-30 of the largest mass (below 2^50 in all)
+    uint64_t most[kPer], least[kPer], all_most, all_least, waves, to_most = 0, to_least = 0, to_n = 0, all_n;
+    uint32_t n[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int b = threadIdx.x * kPer + i;
+        n[i] = counts[b];
+        const float w = static_cast<float>(n[i]) * 1073741824.f, at = static_cast<float>(b);
+        most[i] = static_cast<uint64_t>(w * __builtin_amdgcn_exp2f(rs.step * (0.01f - at)) * 1.0001f) + (n[i] ? 1 : 0);
+        least[i] = static_cast<uint64_t>(w * __builtin_amdgcn_exp2f(-rs.step * (at + 1.01f)) * 0.9999f);
         to_most += most[i];
         to_least += least[i];
+        to_n += n[i];
     }
-    to_most = block_scan(sh, to_most, waves, all_most), to_least = block_scan(sh, to_least, waves, all_least);
+    to_most = block_scan(sh, to_most, waves, all_most);
+    to_least = block_scan(sh, to_least, waves, all_least);
+    to_n = block_scan(sh, to_n, waves, all_n);
     const double from = 0.9999 * top_p * static_cast<double>(all_least), to = 1.0001 * top_p * static_cast<double>(all_most);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const int b = tid * kPer + i;
+        const int b = threadIdx.x * kPer + i;
         const double m0 = static_cast<double>(to_most), l0 = static_cast<double>(to_least);
-        to_most += most[i], to_least += least[i];
+        to_most += most[i], to_least += least[i], to_n += n[i];
         if (m0 < from && from <= static_cast<double>(to_most)) sh.low = b;
-        if (l0 < to && to <= static_cast<double>(to_least)) sh.high = b;
+        if (l0 < to && to <= static_cast<double>(to_least)) sh.high = b, sh.n = static_cast<int>(to_n);
     }
     __syncthreads();
-    const int low = sh.low, range = sh.high - low + 1;
+    out = {sh.low, sh.high, 0, sh.n};
+}
+
+// The cut by masses over all tokens (no top-k before it, no min_p behind) with each one's mass
+// computed once, which gives the kept masses of the lanes' waves along with the cut (mass: of
+// tokens above `last`, or equal to it where all of those are kept; count: of the tokens equal
+// to it otherwise).  Masses of tokens above the bounds are added up in the lanes, only those
+// between them go into shared sums, one for each wave and bucket.
+// False, and nothing decided, where those are more than kRange buckets, or one holds too many
+// tokens to compare.
+template <int DT, int WAVES, int STAGED, typename F>
+__device__ __forceinline__ bool cut_once(SampleShared<WAVES> &sh, const SampleRow<DT, STAGED> &row, const RowScale &rs,
+                                         const Bounds &bounds, F share, float &last, uint64_t &ties, bool &whole,
+                                         uint64_t &mass, uint64_t &count) {
+    constexpr int kThreads = WAVES * kWave, VE = SampleRow<DT, STAGED>::VE, kRange = 64;
+    static_assert(WAVES * kRange <= kBuckets, "the waves' sums take the histogram's place");
+    const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
+    const int low = bounds.low, range = bounds.high - low + 1;
     if (range < 1 || range > kRange) return false;
+    uint64_t waves;
+    __syncthreads();
+    if (tid == 0) sh.n = 0;
     uint64_t *sums = sh.hist;  // [wave][kRange]
     for (int b = tid; b < WAVES * kRange; b += kThreads) sums[b] = 0;
     __syncthreads();
@@ -644,42 +665,57 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
     rs.rate = 1.4426950408889634074 / static_cast<double>(T);
     rs.least = min_p > 0.f ? fmax(log2(static_cast<double>(min_p < 1.f ? min_p : 1.f)), kLightest) : kLightest;
     rs.per_half = fminf(2.f * (kBuckets - 1) / (kBucketSpan * T), 1e30f);
+    rs.step = static_cast<float>(2.0 * rs.rate / static_cast<double>(rs.per_half));
 
-    // kept are the tokens above `last`, and of those equal to it the first `ties`
-    float last = -kInf;
-    uint64_t ties = 0;
-    bool whole = true;
-    int kept = a.vocab;
-    if (top_k < a.vocab)
-        cut<false>(sh, row, rs, last, ties, whole, kept, [&](uint64_t) { return static_cast<uint64_t>(top_k); });
-    // After top-k, or where min_p alone cuts, few are left as a rule: one thread takes each, in
-    // the order of their indices, and the rest is a few sums over the threads.
-    const bool top_k_cut = ties > 0;
-    if (top_k_cut ? kept <= WAVES * kWave : top_p >= 1.f && min_p > 0.f) {
-        // nothing below this weighs: `last`, or what min_p leaves, with room for rounding
+    // Few tokens are left as a rule by top-k, where min_p alone cuts, or above top_p's bounds:
+    // one thread takes each, in the order of their indices, and the rest is a few sums over the
+    // threads.  (top_p alone also needs the mass of all.)
+    Bounds bounds{0, kBuckets - 1, 0, 1 << 30};
+    const bool counted = (top_k < a.vocab || top_p < 1.f) && count_buckets(sh, row, rs);
+    const bool by_count = counted && top_k < a.vocab && bound_count(sh, top_k, bounds);
+    if (counted && !by_count) top_k = a.vocab;
+    const bool by_mass = counted && !by_count && top_p < 1.f;
+    if (by_mass) bound_mass(sh, rs, top_p, bounds);
+    if (by_count || by_mass ? bounds.tokens <= WAVES * kWave : top_k == a.vocab && top_p >= 1.f && min_p > 0.f) {
+        uint64_t all_mass = 0, waves, total;
+        if (by_mass) {
+            uint64_t sum = 0;
+            row.each([&](int, const float (&x)[VE]) {
+#pragma unroll
+                for (int j = 0; j < VE; ++j) {
+                    const double t = rs.exponent(x[j]);
+                    sum += RowScale::select(t >= kLightest, RowScale::mass_of(t));
+                }
+            });
+            block_scan(sh, sum, waves, all_mass);
+        }
+        // nothing below this weighs: what min_p leaves, with room for rounding, or the bounds'
+        // end, in buckets
         const float far = top + static_cast<float>(rs.least / rs.rate), room = 1e-5f * (fabsf(top) + fabsf(far));
-        const float least_x = ties ? last : fmaxf(far - room, -__FLT_MAX__);
+        const float least_x = counted ? -__FLT_MAX__ : fmaxf(far - room, -__FLT_MAX__);
+        const float end = static_cast<float>(bounds.high + 1);
+        auto stays = [&](float x) { return (x >= least_x) & (rs.place(x) < end); };
         uint64_t n = 0, first, all;
         row.each([&](int, const float (&x)[VE]) {
 #pragma unroll
-            for (int j = 0; j < VE; ++j) n += x[j] >= least_x;
+            for (int j = 0; j < VE; ++j) n += stays(x[j]);
         });
         block_scan(sh, n, first, all);
         if (all <= WAVES * kWave) {
             int *list_i = reinterpret_cast<int *>(sh.list_w);
             int at = static_cast<int>(first);
             row.each([&](int i, const float (&x)[VE]) {
-                if (!__any(largest(x) >= least_x)) return;
+                if (!__any(stays(largest(x)))) return;
                 int chunk = 0, place = at;
 #pragma unroll
                 for (int j = 0; j < VE; ++j) {
-                    const uint64_t b = __ballot(x[j] >= least_x);
+                    const uint64_t b = __ballot(stays(x[j]));
                     chunk += __popcll(b);
                     place += __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(b >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(b), 0));
                 }
 #pragma unroll
                 for (int j = 0; j < VE; ++j) {
-                    if (x[j] >= least_x) {
+                    if (stays(x[j])) {
                         sh.list_x[place] = x[j], list_i[place] = row.index(i) + j;
                         ++place;
                     }
@@ -691,46 +727,48 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
             const float x = mine ? sh.list_x[tid] : -kInf;
             const int index = mine ? list_i[tid] : 0;
             const double t = rs.exponent(mine ? x : top);
-            uint64_t waves, total, w = RowScale::select(mine & (t >= kLightest), RowScale::mass_of(t));
-            if (ties && !whole) {  // of those equal to `last` only the first
-                const uint64_t rank = block_scan(sh, x == last, waves, total);
-                w = x == last && rank >= ties ? 0 : w;
-            }
-            if (top_p < 1.f) {
-                // the cut of these by their masses: its bucket, and the tokens in it with each other
+            uint64_t w = RowScale::select(mine & (t >= kLightest), RowScale::mass_of(t));
+            int b;
+            if (!rs.bucket(x, b)) b = kBuckets, w = 0;
+            // the weight ranked before this token within its bucket, among those `in` it
+            auto before_in_bucket = [&](bool in, uint64_t weight) {
+                uint64_t over = 0;
                 __syncthreads();
-                for (int b = tid; b < kBuckets; b += WAVES * kWave) sh.hist[b] = 0;
                 if (tid == 0) sh.n = 0;
                 __syncthreads();
-                int b;
-                if (!rs.bucket(x, b)) b = -1, w = 0;
-                if (w) lds_add(&sh.hist[b], w);
-                __syncthreads();
-                uint64_t part, over, equal;
-                const uint64_t before = scan_hist(sh, part, total), want = share(total);
-                locate(sh, before, part, want);
-                const bool in = w && b == sh.bucket;
                 if (in) {
                     const int k = atomicAdd(&sh.n, 1);
-                    sh.list_x[k] = x, sh.list_w[k] = w;
+                    sh.list_x[k] = x, sh.list_w[k] = weight << 10 | tid;  // (a mass is below 2^43)
                 }
                 __syncthreads();
                 if (in) {
-                    over = sh.sum, equal = 0;
                     const int m = sh.n;
 #pragma unroll 8
                     for (int k = 0; k < m; ++k) {
                         const float y = sh.list_x[k];
                         const uint64_t v = sh.list_w[k];
-                        over += y > x ? v : 0;
-                        equal += y == x ? v : 0;
+                        over += y > x || (y == x && static_cast<int>(v & 1023) < tid) ? v >> 10 : 0;
                     }
-                    if (over < want && want <= over + equal) sh.last = x, sh.rest = (want - over + w - 1) / w;
                 }
+                return over;
+            };
+            if (by_count) {
+                const bool in = b == bounds.high;
+                const uint64_t rank = bounds.above + before_in_bucket(in, 1);
+                w = b > bounds.high || (in && rank >= static_cast<uint64_t>(top_k)) ? 0 : w;
+            }
+            if (top_p < 1.f) {
                 __syncthreads();
-                const float end = sh.last;
-                const uint64_t rank = block_scan(sh, w && x == end, waves, total);
-                w = x > end || (x == end && rank < sh.rest) ? w : 0;
+                for (int k = tid; k < kBuckets; k += WAVES * kWave) sh.hist[k] = 0;
+                __syncthreads();
+                if (w) lds_add(&sh.hist[b], w);
+                __syncthreads();
+                uint64_t part;
+                const uint64_t before = scan_hist(sh, part, total), want = share(by_mass ? all_mass : total);
+                locate(sh, before, part, want);
+                const int bucket = sh.bucket;
+                const uint64_t over = sh.sum + before_in_bucket(w && b == bucket, w);
+                w = b > bucket || (b == bucket && over >= want) ? 0 : w;
             }
             w = RowScale::select(t >= rs.least, w);
             const uint64_t to = block_scan(sh, w, waves, total), target = target_of(total);
@@ -739,12 +777,16 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
         }
     }
 
-    uint64_t mass = 0, count = 0;  // the lane's kept ones, once summed
-    const bool summed = top_p < 1.f && !ties && !(min_p > 0.f) &&
-                        cut_once(sh, row, rs, top_p, share, last, ties, whole, mass, count);
-    if (top_p < 1.f && !summed) cut<true>(sh, row, rs, last, ties, whole, kept, share);
+    // Else: kept are the tokens above `last`, and of those equal to it the first `ties`
+    float last = -kInf;
+    uint64_t ties = 0, mass = 0, count = 0;  // mass, count: the lane's kept ones, once summed
+    bool whole = true;
+    if (top_k < a.vocab) cut<false>(sh, row, rs, last, ties, whole, [&](uint64_t) { return static_cast<uint64_t>(top_k); });
+    const bool summed =
+        by_mass && !(min_p > 0.f) && cut_once(sh, row, rs, bounds, share, last, ties, whole, mass, count);
+    if (top_p < 1.f && !summed) cut<true>(sh, row, rs, last, ties, whole, share);
 
-    // Else the row is summed (once more): the masses above `last`, and the tokens equal to it,
+    // The row is summed (once more): the masses above `last`, and the tokens equal to it,
     // of which the first `ties` weigh.  Where all of them are kept, they are the ones above the
     // next value below it (below 0 that is not -0).
     if (whole && ties) {
