@@ -83,9 +83,9 @@ def _scan(x, step, gate, tau, state, state_out):
     parts = (x, step, gate) if step is not None else _thirds(x)
     B, L, C = _lib.check_gated(*parts, tau, state, state_out)
     if not (L and B and C):
-        h = parts[0].new_zeros(B, C, dtype=torch.float32) if state is None else state
+        h = parts[0].new_zeros((B, C), dtype=torch.float32) if state is None else state
         if state_out is not None:
-            h = state_out.copy_(h)
+            return torch.zeros_like(parts[0]), state_out.copy_(h)
         return torch.zeros_like(parts[0]) + 0 * (parts[1] + parts[2]), h + 0
     if needs_grad(x, step, gate, tau, state) or forward_ad._current_level >= 0:
         if state_out is not None:

@@ -54,8 +54,10 @@ def sample_row(row, u, T=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if top_k > 0:
         order = order[:top_k]
     top = row[order[0]]
-    with np.errstate(invalid="ignore"):
-        weigh = lambda i: np.where(row[i] == top, 1.0, np.exp(np.nan_to_num((row[i] - top) / T, nan=-np.inf)))
+
+    def weigh(i):
+        with np.errstate(invalid="ignore"):
+            return np.where(row[i] == top, 1.0, np.exp(np.nan_to_num((row[i] - top) / T, nan=-np.inf)))
     w = weigh(order)
     if top_p < 1:
         before = np.concatenate([[0.0], np.cumsum(w)[:-1]])

@@ -149,3 +149,34 @@ def test_refusals():
     with pytest.raises(ValueError, match="rng"):
         dropout_add(x, None, 0.1, torch.zeros(2, device=dev()))
     assert dropout_add(x[:0], None, 0.1, rng_of(0, 0)).shape == (0, 8)
+
+
+def test_more_than_32_bits_of_elements():
+    """The elements behind 2^31 have their own bits, and so do the last ones of a ragged end."""
+    n = (1 << 31) + 8 * 1000 + 5
+    x = torch.ones(n, dtype=BF16, device=dev())
+    y = dropout_add(x, None, 0.5, rng_of(21, 22))
+    del x
+    for block in (0, (1 << 28) - 1, 1 << 28, (1 << 28) + 999, (1 << 28) + 1000):
+        words = philox_words(block, 22, 21)
+        bits = [h for w in words for h in (w & 0xFFFF, w >> 16)]
+        got = y[8 * block:8 * block + 8].cpu()
+        assert got.tolist() == [2.0 if b >= 32768 else 0.0 for b in bits[:got.numel()]]
+
+
+def test_expanded_gradient_and_same_tensor_twice():
+    x = torch.randn(12, 40, device=dev(), requires_grad=True)
+    y = dropout_add(x, x, 0.3, rng_of(1, 9))
+    g, = torch.autograd.grad(y.sum(), x)  # the upstream gradient is one number, expanded
+    keep, scale = keep_mask(480, 0.3, 1, 9, 0)
+    want = 1 + torch.from_numpy(keep * scale).view(12, 40)
+    assert (g.double().cpu() - want).abs().max() <= 4 * 2.0 ** -24 * 3
+
+
+def test_create_graph_once():
+    """First gradients with create_graph are had; a second derivative is refused."""
+    x = torch.randn(100, device=dev(), requires_grad=True)
+    g, = torch.autograd.grad(dropout_add(x, None, 0.3, rng_of(1, 9)).sum(), x, create_graph=True)
+    assert torch.isfinite(g).all()
+    with pytest.raises(RuntimeError):
+        g.sum().backward()

@@ -343,3 +343,77 @@ def test_module_tau_follows_its_parameter():
         b = m(h)[0]
         m.log_tau.sub_(0.5)
     assert not torch.equal(a, b)
+
+
+def test_offsets_past_32_bits():
+    """Sequences further apart than 2^31 elements, and tokens further apart than 2^27."""
+    big = torch.zeros((1 << 31) + (1 << 20), dtype=BF16, device=dev())
+    x, step, gate, tau, st, dy, dlast = inputs(2, 10, 64, BF16, 12)
+
+    def apart(t, offset, sb, sl):
+        v = big.as_strided(t.shape, (sb, sl, 1), offset)
+        return v.copy_(t)
+    views = [apart(t, 4096 * i, (1 << 31) + 32768, 256) for i, t in enumerate((x, step, gate))]
+    tau_d, st_d = tau.to(dev()), st.to(dev())
+    ref = gated_recurrence(*(t.to(dev()) for t in (x, step, gate)), tau_d, st_d, True)
+    got = gated_recurrence(*views, tau_d, st_d, True)
+    assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+    big.zero_()
+    views = [apart(t, 4096 * i, 128, (1 << 27) + 64) for i, t in enumerate((x, step, gate))]
+    leaves = [v.detach().requires_grad_() for v in views]
+    flat = [t.to(dev()).requires_grad_() for t in (x, step, gate)]
+    g = [torch.autograd.grad(gated_recurrence(*l, tau_d, st_d)[0], l, dy.to(dev())) for l in (leaves, flat)]
+    assert all(torch.equal(a, b) for a, b in zip(*g))
+
+
+def test_two_streams_at_once():
+    """Split calls that run beside each other, each with its own chain."""
+    args = [[t.to(dev()) for t in inputs(1, 9000, 200, F32, 40 + i)[:5]] for i in range(4)]
+    want = [gated_recurrence(*a, True) for a in args]
+    streams = [torch.cuda.Stream() for _ in args]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        for a, s in zip(args, streams):
+            with torch.cuda.stream(s):
+                got.append(gated_recurrence(*a, True))
+    torch.cuda.synchronize()
+    for i, (y, last) in enumerate(got):
+        assert torch.equal(y, want[i % 4][0]) and torch.equal(last, want[i % 4][1])
+
+
+def test_same_result_every_time():
+    """Many spans in flight: which of them is first does not show."""
+    args = [t.to(dev()) for t in inputs(2, 20000, 320, BF16, 50)]
+    leaves = [t.detach().requires_grad_() for t in args[:5]]
+
+    def run():
+        y, last = gated_recurrence(*leaves, True)
+        return (y.detach(), last.detach(), *torch.autograd.grad([y, last], leaves, args[5:]))
+    first = run()
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(run(), first))
+
+
+def test_a_length_of_many_chains():
+    """Spans of several chain heads against one segment's reference, state and gradient through all of them."""
+    run_case(1, 128 * 35 + 3, 64, F32, 60, True)
+
+
+def test_retained_graph_backward_twice():
+    args = [t.to(dev()) for t in inputs(1, 700, 64, F32, 13)]
+    leaves = [t.detach().requires_grad_() for t in args[:5]]
+    y, last = gated_recurrence(*leaves, True)
+    a = torch.autograd.grad([y, last], leaves, args[5:], retain_graph=True)
+    b = torch.autograd.grad([y, last], leaves, args[5:])
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_the_same_tensor_in_every_place():
+    """x, step and gate one tensor: its gradient is the sum of the three."""
+    x, _, _, tau, st, dy, dlast = inputs(2, 50, 64, F32, 14)
+    one = x.to(dev()).requires_grad_()
+    got, = torch.autograd.grad(gated_recurrence(one, one, one, tau.to(dev()))[0], one, dy.to(dev()))
+    _, _, rg = reference(x, x, x, tau, None, dy, torch.zeros_like(dlast))
+    check(got, rg[0] + rg[1] + rg[2], F32, 2 * f_tol(50) * 3 + 2 ** -23, "sum")

@@ -192,3 +192,63 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="vocab"):
         sample_tokens(torch.zeros(1, (1 << 20) + 1, device=dev()), u[:1])
     assert sample_tokens(logits[:0], u[:0]).shape == (0,)
+
+
+def test_offsets_past_32_bits():
+    V = 5000
+    big = torch.zeros((1 << 31) + 2 * V, dtype=BF16, device=dev())
+    logits, u = make(2, V, BF16, 13)
+    view = big.as_strided((2, V), ((1 << 31) + 100, 1), 7)
+    view.copy_(logits)
+    assert sample_tokens(view, u.to(dev()), top_p=0.9).tolist() == check(logits, u, top_p=0.9)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("scale", [0.01, 0.5, 1.0, 2.0, 4.0, 30.0])
+def test_flat_to_peaked(scale, dtype):
+    """From one bucket full of tokens to a handful of them that weigh anything: every way
+    through the cuts."""
+    logits, u = make(10, 20011, dtype, 14, scale)
+    check(logits, u)
+    for p in (0.05, 0.5, 0.9, 0.99, 0.9999):
+        check(logits, u, top_p=p)
+        check(logits, u, top_p=p, min_p=0.01)
+    for k in (1, 2, 100, 1000, 1024, 1025, 5000, 20010, 20011):
+        check(logits, u, top_k=k)
+        check(logits, u, top_k=k, top_p=0.8, temperature=1.7)
+    for m in (1e-6, 1e-3, 0.3, 0.999):
+        check(logits, u, min_p=m)
+
+
+@pytest.mark.parametrize("n", [255, 257, 700])
+def test_more_rows_than_compute_units(n):
+    logits, u = make(n, 4500, BF16, 15)
+    rng = np.random.default_rng(n)
+    check(logits, u, temperature=rng.uniform(0.3, 2.0, n), top_k=rng.choice([0, 1, 50, 1000, 3000], n),
+          top_p=rng.choice([1.0, 0.9, 0.5], n), min_p=rng.choice([0.0, 0.05], n))
+
+
+def test_ties_through_the_top_k_border():
+    """A thousand tokens of one value at the border of every cut."""
+    logits = torch.full((6, 3000), -1.0)
+    logits[:, 500:520] = 2.0
+    logits[:, 1000:2400] = 1.0
+    u = torch.tensor([0.0, 0.1, 0.5, 0.9, 0.99, 1 - 2.0 ** -24])
+    for kw in (dict(top_k=700), dict(top_k=1400), dict(top_k=21, top_p=0.99), dict(top_p=0.6), dict(top_p=0.9),
+               dict(top_k=1420, min_p=0.2), dict(top_k=1421)):
+        check(logits, u, **kw)
+        check(logits.to(BF16), u, **kw)
+
+
+def test_two_streams_at_once():
+    logits, u = make(8, 50304, BF16, 16)
+    logits, u = logits.to(dev()), u.to(dev())
+    want = sample_tokens(logits, u, top_p=0.9)
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(sample_tokens(logits, u, top_p=0.9))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
