@@ -22,8 +22,7 @@ namespace prime {
 
 constexpr uint64_t kMass = 1ull << 42;  // the largest token's
 constexpr int kBuckets = 2048, kList = 1024;
-constexpr double kLightest = -43.5;    // a token of weight 2^-43.5 or less has mass 0
-constexpr float kBucketSpan = 30.5f;  // so has one this many T below the largest
+constexpr float kBucketSpan = 30.5f;  // a token this many T below the largest has mass 0
 constexpr float kInf = __builtin_inff();
 
 // order-preserving image of a logit, -0 as +0
@@ -47,18 +46,19 @@ __device__ __forceinline__ double fma_s(double a, double b, double c) {
 struct RowScale {
     float top;        // the largest logit
     double rate;      // log2(e) / T
-    double least;     // log2 of min_p, at least kLightest
+    double least;     // log2 of min_p; below every exponent without
     float per_half;   // buckets per half a unit of the logit
     float step;       // log2 of the weight from one bucket to the next
 
     __device__ __forceinline__ double exponent(float x) const {  // of 2, at most 0
         return (static_cast<double>(x) - static_cast<double>(top)) * rate;
     }
-    // 2^t as a mass, -44 <= t <= 0 (below, the result means nothing): 2^f on |f| <= 1/2 by
-    // its Chebyshev interpolant of degree 9 (1.4e-14 off), scaled and rounded to a whole
-    // number by one addition to 2^52.
+    // 2^t as a mass, t <= 0: 2^f on |f| <= 1/2 by its Chebyshev interpolant of degree 9
+    // (1.4e-14 off), scaled and rounded to a whole number by one addition to 2^52.  Below
+    // 2^-44 (and for NaN, of a NaN or of -infinity times a rate of 0) that is 0.
     __device__ static __forceinline__ uint64_t mass_of(double t) {
         constexpr double kRound = 6755399441055744.0;  // 1.5 2^52: adding it rounds to a whole number
+        t = fmax(t, -44.0);
         const double r = t + kRound, f = t - (r - kRound);
         double p = fma_s(1.0212097549811005e-07, f, 1.3259945262689143e-06);
         p = fma_s(p, f, 1.5252640059770786e-05);
@@ -75,13 +75,18 @@ struct RowScale {
         asm("" : "+v"(w));  // computed for every token: a branch around it costs more than it saves
         return w;
     }
-    __device__ __forceinline__ uint64_t mass(float x) const {
-        const double t = exponent(x);
-        return select(t >= kLightest, mass_of(t));
-    }
+    __device__ __forceinline__ uint64_t mass(float x) const { return mass_of(exponent(x)); }
     __device__ static __forceinline__ uint64_t select(bool keep, uint64_t w) { return keep ? w : 0; }
     // bucket of x, false for tokens whose mass is 0 (and for NaN); monotone: every step is
-    __device__ __forceinline__ float place(float x) const { return fmaf(-0.5f, x, 0.5f * top) * per_half; }
+    __device__ __forceinline__ float place(float x) const {
+#pragma clang fp contract(off)  // the same number wherever it is asked for
+        return fmaf(-0.5f, x, 0.5f * top) * per_half;
+    }
+    // a part of a bucket: the place behind `low`, `fine` parts to a bucket
+    __device__ __forceinline__ float part(float x, float low, float fine) const {
+#pragma clang fp contract(off)
+        return (place(x) - low) * fine;
+    }
     __device__ __forceinline__ bool bucket(float x, int &b) const {
         const float f = place(x);
         b = static_cast<int>(f);
@@ -464,31 +469,29 @@ template <int WAVES>
 __device__ __forceinline__ void bound_mass(SampleShared<WAVES> &sh, const RowScale &rs, float top_p, Bounds &out) {
     constexpr int kPer = kBuckets / (WAVES * kWave);
     const uint32_t *counts = reinterpret_cast<uint32_t *>(sh.hist);
-    // the most and the least, in 2^-30 of the largest mass (below 2^50 in all)
-    uint64_t most[kPer], least[kPer], all_most, all_least, waves, to_most = 0, to_least = 0, to_n = 0, all_n;
-    uint32_t n[kPer];
+    // the most and the least, in 2^-22 of the largest mass (below 2^43 in all), the least with
+    // the tokens' number behind it, so that two sums over the threads do
+    uint64_t most[kPer], least[kPer], all_most, all_least, waves, to_most = 0, to_least = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int b = threadIdx.x * kPer + i;
-        n[i] = counts[b];
-        const float w = static_cast<float>(n[i]) * 1073741824.f, at = static_cast<float>(b);
-        most[i] = static_cast<uint64_t>(w * __builtin_amdgcn_exp2f(rs.step * (0.01f - at)) * 1.0001f) + (n[i] ? 1 : 0);
-        least[i] = static_cast<uint64_t>(w * __builtin_amdgcn_exp2f(-rs.step * (at + 1.01f)) * 0.9999f);
+        const uint32_t n = counts[b];
+        const float w = static_cast<float>(n) * 4194304.f, at = static_cast<float>(b);
+        most[i] = static_cast<uint64_t>(w * __builtin_amdgcn_exp2f(rs.step * (0.01f - at)) * 1.0001f) + (n ? 1 : 0);
+        least[i] = static_cast<uint64_t>(w * __builtin_amdgcn_exp2f(-rs.step * (at + 1.01f)) * 0.9999f) << 21 | n;
         to_most += most[i];
         to_least += least[i];
-        to_n += n[i];
     }
     to_most = block_scan(sh, to_most, waves, all_most);
     to_least = block_scan(sh, to_least, waves, all_least);
-    to_n = block_scan(sh, to_n, waves, all_n);
-    const double from = 0.9999 * top_p * static_cast<double>(all_least), to = 1.0001 * top_p * static_cast<double>(all_most);
+    const double from = 0.9999 * top_p * static_cast<double>(all_least >> 21), to = 1.0001 * top_p * static_cast<double>(all_most);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int b = threadIdx.x * kPer + i;
-        const double m0 = static_cast<double>(to_most), l0 = static_cast<double>(to_least);
-        to_most += most[i], to_least += least[i], to_n += n[i];
+        const double m0 = static_cast<double>(to_most), l0 = static_cast<double>(to_least >> 21);
+        to_most += most[i], to_least += least[i];
         if (m0 < from && from <= static_cast<double>(to_most)) sh.low = b;
-        if (l0 < to && to <= static_cast<double>(to_least)) sh.high = b, sh.n = static_cast<int>(to_n);
+        if (l0 < to && to <= static_cast<double>(to_least >> 21)) sh.high = b, sh.n = static_cast<int>(to_least & 0x1FFFFF);
     }
     __syncthreads();
     out = {sh.low, sh.high, 0, sh.n};
@@ -498,9 +501,9 @@ __device__ __forceinline__ void bound_mass(SampleShared<WAVES> &sh, const RowSca
 // computed once, which gives the kept masses of the lanes' waves along with the cut (mass: of
 // tokens above `last`, or equal to it where all of those are kept; count: of the tokens equal
 // to it otherwise).  Masses of tokens above the bounds are added up in the lanes, only those
-// between them go into shared sums, one for each wave and bucket.
-// False, and nothing decided, where those are more than kRange buckets, or one holds too many
-// tokens to compare.
+// between them go into shared sums, kRange parts of the bounds for each wave.
+// False, and nothing decided, where the bounds are more than kRange buckets apart, or a part
+// holds too many tokens to compare.
 template <int DT, int WAVES, int STAGED, typename F>
 __device__ __forceinline__ bool cut_once(SampleShared<WAVES> &sh, const SampleRow<DT, STAGED> &row, const RowScale &rs,
                                          const Bounds &bounds, F share, float &last, uint64_t &ties, bool &whole,
@@ -516,39 +519,40 @@ __device__ __forceinline__ bool cut_once(SampleShared<WAVES> &sh, const SampleRo
     uint64_t *sums = sh.hist;  // [wave][kRange]
     for (int b = tid; b < WAVES * kRange; b += kThreads) sums[b] = 0;
     __syncthreads();
+    const float from = static_cast<float>(low), fine = static_cast<float>(kRange / range);
+    const float end = static_cast<float>(range * (kRange / range));
     uint64_t rest = 0;
     mass = count = 0;
     row.each([&](int, const float (&x)[VE]) {
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
-            int b;
-            const bool in = rs.bucket(x[j], b);
-            const uint64_t w = RowScale::select(in, rs.mass_of(rs.exponent(x[j])));
-            b -= low;
+            const uint64_t w = rs.mass(x[j]);
+            const float f = rs.part(x[j], from, fine);
             rest += w;
-            mass += b < 0 ? w : 0;
-            if (in & (static_cast<uint32_t>(b) < static_cast<uint32_t>(range))) lds_add(&sums[wave * kRange + b], w);
+            mass += f < 0.f ? w : 0;
+            if ((f >= 0.f) & (f < end)) lds_add(&sums[wave * kRange + static_cast<int>(f)], w);
         }
     });
     uint64_t all, above;
     block_scan(sh, rest, waves, all);
     block_scan(sh, mass, waves, above);
     const uint64_t want = share(all);
-    // every wave finds the bucket for itself: lane b has bucket low + b
+    // every wave finds the part for itself: lane k has part k
     uint64_t sum = 0;
 #pragma unroll
     for (int k = 0; k < WAVES; ++k) sum += sums[k * kRange + lane];
     const uint64_t to_b = above + wave_scan_u64(sum);
     const uint64_t hit = __ballot(to_b - sum < want && want <= to_b);
     if (!hit) return false;
-    const int found = __builtin_ctzll(hit), bucket = low + found;
+    const int found = __builtin_ctzll(hit);
     const uint64_t over0 = shfl_u64(to_b - sum, found);
+    const float at = static_cast<float>(found);
     row.each([&](int, const float (&x)[VE]) {
-        int b;
-        if (!(rs.bucket(largest(x), b) & (b <= bucket))) return;
+        if (!(rs.part(largest(x), from, fine) < at + 1.f)) return;
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
-            if (rs.bucket(x[j], b) & (b == bucket)) {
+            const float f = rs.part(x[j], from, fine);
+            if ((f >= at) & (f < at + 1.f)) {
                 const int n = atomicAdd(&sh.n, 1);
                 if (n < kList) sh.list_x[n] = x[j], sh.list_wave[n] = static_cast<uint8_t>(wave);
             }
@@ -663,7 +667,7 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
     }
     rs.top = top;
     rs.rate = 1.4426950408889634074 / static_cast<double>(T);
-    rs.least = min_p > 0.f ? fmax(log2(static_cast<double>(min_p < 1.f ? min_p : 1.f)), kLightest) : kLightest;
+    rs.least = min_p > 0.f ? log2(static_cast<double>(min_p < 1.f ? min_p : 1.f)) : -1e300;
     rs.per_half = fminf(2.f * (kBuckets - 1) / (kBucketSpan * T), 1e30f);
     rs.step = static_cast<float>(2.0 * rs.rate / static_cast<double>(rs.per_half));
 
@@ -683,8 +687,7 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
             row.each([&](int, const float (&x)[VE]) {
 #pragma unroll
                 for (int j = 0; j < VE; ++j) {
-                    const double t = rs.exponent(x[j]);
-                    sum += RowScale::select(t >= kLightest, RowScale::mass_of(t));
+                    sum += rs.mass(x[j]);
                 }
             });
             block_scan(sh, sum, waves, all_mass);
@@ -727,7 +730,7 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
             const float x = mine ? sh.list_x[tid] : -kInf;
             const int index = mine ? list_i[tid] : 0;
             const double t = rs.exponent(mine ? x : top);
-            uint64_t w = RowScale::select(mine & (t >= kLightest), RowScale::mass_of(t));
+            uint64_t w = RowScale::select(mine, RowScale::mass_of(t));
             int b;
             if (!rs.bucket(x, b)) b = kBuckets, w = 0;
             // the weight ranked before this token within its bucket, among those `in` it
