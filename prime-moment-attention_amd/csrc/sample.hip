@@ -22,6 +22,7 @@ namespace prime {
 
 constexpr uint64_t kMass = 1ull << 42;  // the largest token's
 constexpr int kBuckets = 2048, kList = 1024;
+constexpr int kCells = 2 * kBuckets;     // half buckets, for counts
 constexpr float kBucketSpan = 30.5f;  // a token this many T below the largest has mass 0
 constexpr float kInf = __builtin_inff();
 
@@ -48,7 +49,7 @@ struct RowScale {
     double rate;      // log2(e) / T
     double least;     // log2 of min_p; below every exponent without
     float per_half;   // buckets per half a unit of the logit
-    float step;       // log2 of the weight from one bucket to the next
+    float step;       // log2 of the weight from one cell to the next
 
     __device__ __forceinline__ double exponent(float x) const {  // of 2, at most 0
         return (static_cast<double>(x) - static_cast<double>(top)) * rate;
@@ -81,6 +82,12 @@ struct RowScale {
     __device__ __forceinline__ float place(float x) const {
 #pragma clang fp contract(off)  // the same number wherever it is asked for
         return fmaf(-0.5f, x, 0.5f * top) * per_half;
+    }
+    // cell of x, as bucket()
+    __device__ __forceinline__ bool cell(float x, int &c) const {
+        const float f = place(x) * 2.f;
+        c = static_cast<int>(f);
+        return f < static_cast<float>(kCells - 2);
     }
     // a part of a bucket: the place behind `low`, `fine` parts to a bucket
     __device__ __forceinline__ float part(float x, float low, float fine) const {
@@ -414,38 +421,38 @@ __device__ __forceinline__ void cut(SampleShared<WAVES> &sh, const SampleRow<DT,
     whole = last != floor && ties * w == sh.rest;
 }
 
-// The buckets' token counts, in the histogram's place.  False where all of a row is one bucket
+// The cells' token counts, in the histogram's place.  False where all of a row is one cell
 // (a temperature above any use).
 template <int DT, int WAVES, int STAGED>
-__device__ __forceinline__ bool count_buckets(SampleShared<WAVES> &sh, const SampleRow<DT, STAGED> &row, const RowScale &rs) {
+__device__ __forceinline__ bool count_cells(SampleShared<WAVES> &sh, const SampleRow<DT, STAGED> &row, const RowScale &rs) {
     constexpr int VE = SampleRow<DT, STAGED>::VE;
     if (!(rs.step < 1.f)) return false;
     uint32_t *counts = reinterpret_cast<uint32_t *>(sh.hist);
     __syncthreads();
-    for (int b = threadIdx.x; b < kBuckets; b += WAVES * kWave) counts[b] = 0;
-    if (threadIdx.x == 0) sh.low = 0, sh.high = kBuckets - 1, sh.n = 1 << 30;
+    for (int b = threadIdx.x; b < kCells; b += WAVES * kWave) counts[b] = 0;
+    if (threadIdx.x == 0) sh.low = 0, sh.high = kCells - 1, sh.n = 1 << 30;
     __syncthreads();
     row.each([&](int, const float (&x)[VE]) {
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
             int b;
-            if (rs.bucket(x[j], b)) atomicAdd(&counts[b], 1u);
+            if (rs.cell(x[j], b)) atomicAdd(&counts[b], 1u);
         }
     });
     __syncthreads();
     return true;
 }
 
-// Where a cut falls, from the counts: in one of the buckets low .. high, with `above` tokens
+// Where a cut falls, from the counts: in one of the cells low .. high, with `above` tokens
 // above those and `tokens` up to their end.
 struct Bounds {
     int low, high, above, tokens;
 };
 
-// top-k: one bucket, or (false) none, where no more than k tokens weigh anything.
+// top-k: one cell, or (false) none, where no more than k tokens weigh anything.
 template <int WAVES>
 __device__ __forceinline__ bool bound_count(SampleShared<WAVES> &sh, int k, Bounds &out) {
-    constexpr int kPer = kBuckets / (WAVES * kWave);
+    constexpr int kPer = kCells / (WAVES * kWave);
     const uint32_t *counts = reinterpret_cast<uint32_t *>(sh.hist);
     uint64_t n = 0, waves, total;
 #pragma unroll
@@ -463,11 +470,11 @@ __device__ __forceinline__ bool bound_count(SampleShared<WAVES> &sh, int k, Boun
     return true;
 }
 
-// top_p: a token in bucket b weighs between 2^(-(b + 1) step) and 2^(-b step), with a hundredth
-// of a bucket for roundings, so the counts bound every prefix's mass.
+// top_p: a token in cell c weighs between 2^(-(c + 1) step) and 2^(-c step), with a hundredth
+// of a cell for roundings, so the counts bound every prefix's mass.
 template <int WAVES>
 __device__ __forceinline__ void bound_mass(SampleShared<WAVES> &sh, const RowScale &rs, float top_p, Bounds &out) {
-    constexpr int kPer = kBuckets / (WAVES * kWave);
+    constexpr int kPer = kCells / (WAVES * kWave);
     const uint32_t *counts = reinterpret_cast<uint32_t *>(sh.hist);
     // the most and the least, in 2^-22 of the largest mass (below 2^43 in all), the least with
     // the tokens' number behind it, so that two sums over the threads do
@@ -502,13 +509,13 @@ __device__ __forceinline__ void bound_mass(SampleShared<WAVES> &sh, const RowSca
 // tokens above `last`, or equal to it where all of those are kept; count: of the tokens equal
 // to it otherwise).  Masses of tokens above the bounds are added up in the lanes, only those
 // between them go into shared sums, kRange parts of the bounds for each wave.
-// False, and nothing decided, where the bounds are more than kRange buckets apart, or a part
+// False, and nothing decided, where the bounds are more than kRange cells apart, or a part
 // holds too many tokens to compare.
 template <int DT, int WAVES, int STAGED, typename F>
 __device__ __forceinline__ bool cut_once(SampleShared<WAVES> &sh, const SampleRow<DT, STAGED> &row, const RowScale &rs,
                                          const Bounds &bounds, F share, float &last, uint64_t &ties, bool &whole,
                                          uint64_t &mass, uint64_t &count) {
-    constexpr int kThreads = WAVES * kWave, VE = SampleRow<DT, STAGED>::VE, kRange = 64;
+    constexpr int kThreads = WAVES * kWave, VE = SampleRow<DT, STAGED>::VE, kRange = 2 * kWave;
     static_assert(WAVES * kRange <= kBuckets, "the waves' sums take the histogram's place");
     const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
     const int low = bounds.low, range = bounds.high - low + 1;
@@ -519,7 +526,7 @@ __device__ __forceinline__ bool cut_once(SampleShared<WAVES> &sh, const SampleRo
     uint64_t *sums = sh.hist;  // [wave][kRange]
     for (int b = tid; b < WAVES * kRange; b += kThreads) sums[b] = 0;
     __syncthreads();
-    const float from = static_cast<float>(low), fine = static_cast<float>(kRange / range);
+    const float from = 0.5f * static_cast<float>(low), fine = static_cast<float>(2 * (kRange / range));
     const float end = static_cast<float>(range * (kRange / range));
     uint64_t rest = 0;
     mass = count = 0;
@@ -537,15 +544,16 @@ __device__ __forceinline__ bool cut_once(SampleShared<WAVES> &sh, const SampleRo
     block_scan(sh, rest, waves, all);
     block_scan(sh, mass, waves, above);
     const uint64_t want = share(all);
-    // every wave finds the part for itself: lane k has part k
-    uint64_t sum = 0;
+    // every wave finds the part for itself: lane k has the parts 2 k and 2 k + 1
+    uint64_t even = 0, odd = 0;
 #pragma unroll
-    for (int k = 0; k < WAVES; ++k) sum += sums[k * kRange + lane];
-    const uint64_t to_b = above + wave_scan_u64(sum);
-    const uint64_t hit = __ballot(to_b - sum < want && want <= to_b);
-    if (!hit) return false;
-    const int found = __builtin_ctzll(hit);
-    const uint64_t over0 = shfl_u64(to_b - sum, found);
+    for (int k = 0; k < WAVES; ++k) even += sums[k * kRange + 2 * lane], odd += sums[k * kRange + 2 * lane + 1];
+    const uint64_t to_even = above + wave_scan_u64(even + odd) - odd, to_odd = to_even + odd;
+    const uint64_t hit_even = __ballot(to_even - even < want && want <= to_even);
+    const uint64_t hit_odd = __ballot(to_even < want && want <= to_odd);
+    if (!(hit_even | hit_odd)) return false;
+    const int owner = __builtin_ctzll(hit_even | hit_odd), found = 2 * owner + (hit_even ? 0 : 1);
+    const uint64_t over0 = shfl_u64(hit_even ? to_even - even : to_even, owner);
     const float at = static_cast<float>(found);
     row.each([&](int, const float (&x)[VE]) {
         if (!(rs.part(largest(x), from, fine) < at + 1.f)) return;
@@ -580,7 +588,7 @@ __device__ __forceinline__ bool cut_once(SampleShared<WAVES> &sh, const SampleRo
     const uint64_t w = rs.mass(last);
     ties = (want - sh.sum + w - 1) / w;
     whole = ties * w == sh.rest;
-    if (lane < found) mass += sums[wave * kRange + lane];
+    for (int k = lane; k < found; k += kWave) mass += sums[wave * kRange + k];
     for (int i = lane; i < n; i += kWave) {
         const float x = sh.list_x[i];
         if (sh.list_wave[i] != wave) continue;
@@ -669,13 +677,13 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
     rs.rate = 1.4426950408889634074 / static_cast<double>(T);
     rs.least = min_p > 0.f ? log2(static_cast<double>(min_p < 1.f ? min_p : 1.f)) : -1e300;
     rs.per_half = fminf(2.f * (kBuckets - 1) / (kBucketSpan * T), 1e30f);
-    rs.step = static_cast<float>(2.0 * rs.rate / static_cast<double>(rs.per_half));
+    rs.step = static_cast<float>(rs.rate / static_cast<double>(rs.per_half));
 
     // Few tokens are left as a rule by top-k, where min_p alone cuts, or above top_p's bounds:
     // one thread takes each, in the order of their indices, and the rest is a few sums over the
     // threads.  (top_p alone also needs the mass of all.)
-    Bounds bounds{0, kBuckets - 1, 0, 1 << 30};
-    const bool counted = (top_k < a.vocab || top_p < 1.f) && count_buckets(sh, row, rs);
+    Bounds bounds{0, kCells - 1, 0, 1 << 30};
+    const bool counted = (top_k < a.vocab || top_p < 1.f) && count_cells(sh, row, rs);
     const bool by_count = counted && top_k < a.vocab && bound_count(sh, top_k, bounds);
     if (counted && !by_count) top_k = a.vocab;
     const bool by_mass = counted && !by_count && top_p < 1.f;
@@ -693,11 +701,11 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
             block_scan(sh, sum, waves, all_mass);
         }
         // nothing below this weighs: what min_p leaves, with room for rounding, or the bounds'
-        // end, in buckets
+        // end, in cells
         const float far = top + static_cast<float>(rs.least / rs.rate), room = 1e-5f * (fabsf(top) + fabsf(far));
         const float least_x = counted ? -__FLT_MAX__ : fmaxf(far - room, -__FLT_MAX__);
         const float end = static_cast<float>(bounds.high + 1);
-        auto stays = [&](float x) { return (x >= least_x) & (rs.place(x) < end); };
+        auto stays = [&](float x) { return (x >= least_x) & (rs.place(x) * 2.f < end); };
         uint64_t n = 0, first, all;
         row.each([&](int, const float (&x)[VE]) {
 #pragma unroll
@@ -756,9 +764,10 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
                 return over;
             };
             if (by_count) {
-                const bool in = b == bounds.high;
+                int c;
+                const bool in = rs.cell(x, c) && c == bounds.high;
                 const uint64_t rank = bounds.above + before_in_bucket(in, 1);
-                w = b > bounds.high || (in && rank >= static_cast<uint64_t>(top_k)) ? 0 : w;
+                w = in && rank >= static_cast<uint64_t>(top_k) ? 0 : w;
             }
             if (top_p < 1.f) {
                 __syncthreads();
