@@ -538,7 +538,8 @@ int prime_argmax(const void *logits, int dtype, int n, int vocab, int64_t stride
  *                      before every 16th token, for the backward
  *   workspace        : prime_gated_scan_workspace_size bytes (0: may be NULL), this
  *                      call's own until it has run on `stream`
- * A non-finite x, step or gate leaves its channel non-finite from that token on.
+ * An infinite step or gate acts as its limit; an infinite x, or a NaN anywhere, leaves
+ * its channel non-finite from that token on.
  *
  * prime_gated_scan_backward: gradients for dy (view like y) and dstate_out (fp32
  * [B, C] or NULL), from the forward's inputs and its checkpoints:
@@ -547,7 +548,7 @@ int prime_argmax(const void *logits, int dtype, int n, int vocab, int64_t stride
  *   dtau             : fp32 [C], summed over sequences and tokens in a fixed order
  *   dstate_in        : fp32 [B, C] or NULL
  * Where softplus(step) lies outside the clamp dstep is 0, as torch.clamp's gradient.
- * L <= 2^30; C up to 2^23.
+ * L <= 2^30, C <= 2^23, B * ceil(C / 64) * ceil(L / 128) < 2^23.
  */
 typedef struct prime_seq {
     void   *data;
@@ -576,7 +577,7 @@ int prime_gated_scan_backward(const prime_seq_t *x, const prime_seq_t *step, con
  *   x, residual, out : rows of cols contiguous elements, ld* elements apart; out may
  *                      be x or residual (the same rows), else it overlaps neither
  *   rng              : int64 [2] on the device, read when the kernel runs
- *   rows * cols <= 2^40, 0 <= p <= 1
+ *   rows * cols <= 2^34, 0 <= p <= 1
  */
 int prime_dropout_add(const void *x, int64_t ldx, const void *residual, int64_t ldr, void *out, int64_t ldo, int dtype,
                       int64_t rows, int64_t cols, float p, const int64_t *rng, int64_t call, void *stream);
@@ -593,7 +594,8 @@ int prime_dropout_add(const void *x, int64_t ldx, const void *residual, int64_t 
  * which is never chosen; a row with nothing else is sampled as if all its logits
  * were equal.  Several +infinity share the weight among them.
  * Weights are held to 2^-42 of the largest; the result does not depend on timing.
- *   logits : n rows of `vocab` <= 2^20 elements (F32 / BF16 / F16), stride_n apart
+ *   logits : n < 2^22 rows of `vocab` <= 2^20 elements (F32 / BF16 / F16), stride_n >= 0
+ *            apart (0: the same logits for every row)
  *   temperature, top_k, top_p, min_p : one value, or, where the pointer behind it is
  *            not NULL, one per row on the device
  *   out    : int64 [n]

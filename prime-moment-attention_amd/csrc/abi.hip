@@ -1517,7 +1517,7 @@ bool seq_overlap(const prime_seq_t *p, const prime_seq_t *q, int B, int L, int C
     return m < w || row - m < w;
 }
 
-int check_seq(const prime_seq_t *t, int es, int B, int L, int C, const char *name) {
+int check_seq(const prime_seq_t *t, int es, const char *name) {
     if (!t || !t->data) return fail(PRIME_ERR_INVALID_ARG, "%s is null", name);
     if (t->stride_b < 0 || t->stride_l < 0) return fail(PRIME_ERR_INVALID_ARG, "%s has negative strides", name);
     if (reinterpret_cast<uintptr_t>(t->data) % es) return fail(PRIME_ERR_MISALIGNED, "%s is misaligned", name);
@@ -1526,7 +1526,7 @@ int check_seq(const prime_seq_t *t, int es, int B, int L, int C, const char *nam
 
 // an output's rows must not share memory with each other
 int check_seq_out(const prime_seq_t *t, int es, int B, int L, int C, const char *name) {
-    int rc = check_seq(t, es, B, L, C, name);
+    int rc = check_seq(t, es, name);
     if (rc) return rc;
     if ((L > 1 && t->stride_l < C) || (B > 1 && t->stride_b < C) ||
         (B > 1 && L > 1 && t->stride_b < t->stride_l * L && t->stride_l < t->stride_b * B))
@@ -1543,7 +1543,8 @@ int gated_sizes(int dtype, int B, int L, int C) {
     if (B <= 0 || L <= 0 || C <= 0 || L > (1 << 30) || C > (1 << 23))
         return fail(PRIME_ERR_INVALID_ARG, "bad sizes B=%d L=%d C=%d", B, L, C);
     if (!valid_dtype(dtype)) return fail(PRIME_ERR_UNSUPPORTED_DTYPE, "unsupported dtype");
-    if (static_cast<int64_t>(B) * ((C + 63) / 64) * prime::gated_spans(L) >= (int64_t(1) << 31))
+    // (a launch has below 2^32 threads, a span of 128 tokens by 64 channels 512 of them)
+    if (static_cast<int64_t>(B) * ((C + 63) / 64) * prime::gated_spans(L) >= (1 << 23))
         return fail(PRIME_ERR_INVALID_ARG, "B=%d L=%d C=%d above the grid's limit", B, L, C);
     return PRIME_OK;
 }
@@ -1579,8 +1580,8 @@ int prime_gated_scan(const prime_seq_t *x, const prime_seq_t *step, const prime_
     int rc = gated_sizes(dtype, B, L, C);
     if (rc) return rc;
     const int es = elem_size(dtype);
-    if ((rc = check_seq(x, es, B, L, C, "x")) || (rc = check_seq(step, es, B, L, C, "step")) ||
-        (rc = check_seq(gate, es, B, L, C, "gate")) || (rc = check_seq_out(y, es, B, L, C, "y")))
+    if ((rc = check_seq(x, es, "x")) || (rc = check_seq(step, es, "step")) ||
+        (rc = check_seq(gate, es, "gate")) || (rc = check_seq_out(y, es, B, L, C, "y")))
         return rc;
     if (!tau) return fail(PRIME_ERR_INVALID_ARG, "tau is null");
     if ((rc = check_floats(tau, "tau")) || (rc = check_floats(state_in, "state_in")) ||
@@ -1623,8 +1624,8 @@ int prime_gated_scan_backward(const prime_seq_t *x, const prime_seq_t *step, con
     int rc = gated_sizes(dtype, B, L, C);
     if (rc) return rc;
     const int es = elem_size(dtype);
-    if ((rc = check_seq(x, es, B, L, C, "x")) || (rc = check_seq(step, es, B, L, C, "step")) ||
-        (rc = check_seq(gate, es, B, L, C, "gate")) || (rc = check_seq(dy, es, B, L, C, "dy")) ||
+    if ((rc = check_seq(x, es, "x")) || (rc = check_seq(step, es, "step")) ||
+        (rc = check_seq(gate, es, "gate")) || (rc = check_seq(dy, es, "dy")) ||
         (rc = check_seq_out(dx, es, B, L, C, "dx")) || (rc = check_seq_out(dstep, es, B, L, C, "dstep")) ||
         (rc = check_seq_out(dgate, es, B, L, C, "dgate")))
         return rc;
@@ -1676,7 +1677,7 @@ int prime_dropout_add(const void *x, int64_t ldx, const void *residual, int64_t 
     g_err[0] = 0;
     if (!x || !out || !rng) return fail(PRIME_ERR_INVALID_ARG, "prime_dropout_add: null argument");
     if (!valid_dtype(dtype)) return fail(PRIME_ERR_UNSUPPORTED_DTYPE, "unsupported dtype");
-    if (rows <= 0 || cols <= 0 || rows > (int64_t(1) << 40) || cols > (int64_t(1) << 40) / rows)
+    if (rows <= 0 || cols <= 0 || rows > (int64_t(1) << 34) || cols > (int64_t(1) << 34) / rows)
         return fail(PRIME_ERR_INVALID_ARG, "bad sizes rows=%lld cols=%lld", static_cast<long long>(rows),
                     static_cast<long long>(cols));
     if (ldx < cols || ldo < cols || (residual && ldr < cols))
@@ -1705,9 +1706,10 @@ int prime_sample(const void *logits, int dtype, int n, int vocab, int64_t stride
                  const float *top_ps, float min_p, const float *min_ps, int64_t *out, void *stream) {
     g_err[0] = 0;
     if (!logits || !uniforms || !out) return fail(PRIME_ERR_INVALID_ARG, "prime_sample: null argument");
-    if (n <= 0 || vocab <= 0 || vocab > prime::kSampleMaxVocab || stride_n < vocab)
-        return fail(PRIME_ERR_INVALID_ARG, "bad sizes n=%d vocab=%d (at most %d) stride=%lld", n, vocab,
-                    prime::kSampleMaxVocab, static_cast<long long>(stride_n));
+    // (a launch has below 2^32 threads, a row up to 1024 of them)
+    if (n <= 0 || n >= (1 << 22) || vocab <= 0 || vocab > prime::kSampleMaxVocab || stride_n < 0)
+        return fail(PRIME_ERR_INVALID_ARG, "bad sizes n=%d (below %d) vocab=%d (at most %d) stride=%lld", n, 1 << 22,
+                    vocab, prime::kSampleMaxVocab, static_cast<long long>(stride_n));
     if (!valid_dtype(dtype)) return fail(PRIME_ERR_UNSUPPORTED_DTYPE, "unsupported logits dtype");
     const int es = elem_size(dtype);
     if (reinterpret_cast<uintptr_t>(logits) % es || (reinterpret_cast<uintptr_t>(out) & 7u))

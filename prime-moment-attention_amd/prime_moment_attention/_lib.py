@@ -1246,6 +1246,8 @@ def sample(logits, uniforms, temperature, top_k, top_p, min_p, out) -> None:
     if logits.dtype not in _DTYPES:
         raise RuntimeError(f"unsupported dtype {logits.dtype}")
     n, vocab = logits.shape
+    if not isinstance(top_k, torch.Tensor):
+        top_k = min(max(int(top_k), 0), vocab)
     dev, args = logits.get_device(), []
     f32 = torch.float32
     for v, name, dt, cast in ((out, "out", torch.int64, None), (uniforms, "uniforms", f32, None),

@@ -104,11 +104,14 @@ def gated_recurrence(x: torch.Tensor, step: torch.Tensor, gate: torch.Tensor, ta
     """The recurrence over x, step, gate [B, L, C] (fp32, bf16 or fp16 alike; any batch
     and token strides) with tau fp32 [C], positive and finite, and state fp32 [B, C] or
     None (zero): (y [B, L, C] of x's dtype, last state fp32 [B, C] or None without
-    return_state).
+    return_state).  Every token counts: the last state of a padded sequence has taken its
+    padding in.
 
     Differentiable once in x, step, gate, tau and state.  The given state is left as it
     is; without autograd, ``state_out`` names the tensor that receives the last state
-    (it may be ``state``: a decode step in place)."""
+    (it may be ``state``: a decode step in place).  Forward and backward can be captured
+    into a graph; as for any operator, no eager autograd graph of the same leaves may live
+    meanwhile (torch would run a part of the captured backward on that graph's stream)."""
     if not x.stride(-1) == step.stride(-1) == gate.stride(-1) == 1:
         x, step, gate = _channels(x), _channels(step), _channels(gate)
     y, last = _scan(x, step, gate, tau, state, state_out)
@@ -145,21 +148,6 @@ class GatedLinearRecurrence(nn.Module):
     def get_tau(self, device: torch.device) -> torch.Tensor:
         return torch.clamp(torch.exp(self.log_tau.to(device).float()), min=self.min_tau, max=self.max_tau)
 
-    def _tau(self, device: torch.device) -> torch.Tensor:
-        """tau for the kernels; without autograd cached until log_tau changes."""
-        p = self.log_tau
-        if torch.is_grad_enabled() and p.requires_grad:
-            return self.get_tau(device)
-        key = (p.data_ptr(), p._version, str(device), self.min_tau, self.max_tau)
-        cached = self.__dict__.get("_tau_cache")
-        if cached is not None and cached[0] is p and cached[1] == key and (
-                not cached[2].is_inference() or torch.is_inference_mode_enabled()):
-            return cached[2]
-        with torch.no_grad():
-            tau = self.get_tau(device).contiguous()
-        self.__dict__["_tau_cache"] = (p, key, tau)
-        return tau
-
     def mix(self, hidden_states: torch.Tensor, state: Optional[torch.Tensor] = None, return_state: bool = False,
             in_place: bool = False):
         """The layer up to its output projection: (y [B, L, width], next state or None).
@@ -171,7 +159,7 @@ class GatedLinearRecurrence(nn.Module):
             if ((in_place or self.inplace_state) and return_state and state is given
                     and not needs_grad(proj, state, self.log_tau)):
                 state_out = state
-        y, last = _scan(proj, None, None, self._tau(proj.device), state, state_out)
+        y, last = _scan(proj, None, None, self.get_tau(proj.device), state, state_out)
         return y.to(hidden_states.dtype), (last if return_state else None)
 
     def forward(self, hidden_states: torch.Tensor, state: Optional[torch.Tensor] = None, return_state: bool = False):

@@ -47,7 +47,7 @@ from . import _lib
 from .attention import PrimeMomentAttention
 from .dropout import dropout_add, dropout_rng
 from .gated_recurrence import GatedLinearRecurrence
-from .sampling import sample_tokens
+from .sampling import _per_row, sample_tokens
 from .selective import PrimeSelectiveMomentAttention
 
 
@@ -735,6 +735,8 @@ class GreedyDecoder:
     def prefill(self, input_ids: torch.Tensor) -> torch.Tensor:
         """Run the prompt; returns the first generated token [B, 1]."""
         m = self.model
+        if m.training and m.config.dropout > 0.0:
+            raise ValueError("the model drops out while it trains: call its eval() before decoding")
         out = m.forward(input_ids, return_states=True, logits_to_keep=1)
         self.states = [s if torch.is_tensor(s) else tuple(s) for s in out["states"]]
         self.token = torch.empty(input_ids.shape[0], 1, dtype=torch.int64, device=input_ids.device)
@@ -818,7 +820,7 @@ class SamplingDecoder(GreedyDecoder):
         dev = input_ids.device
         self.uniforms = torch.rand(input_ids.shape[0], device=dev, generator=self.generator)
         # held here in the kernel's types: a captured step reads these tensors
-        self.params = [v.to(device=dev, dtype=dt).contiguous() if torch.is_tensor(v) else v
+        self.params = [_per_row(v, dt, dev)
                        for v, dt in zip(self.cuts, (torch.float32, torch.int32, torch.float32, torch.float32))]
         return super().prefill(input_ids)
 

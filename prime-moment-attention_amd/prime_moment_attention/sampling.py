@@ -16,14 +16,17 @@ def _per_row(v, dtype, device):
     """A per-row parameter in the kernel's type (a number as it is)."""
     if not torch.is_tensor(v):
         return v
+    if dtype is torch.int32 and v.dtype is not dtype:
+        v = v.clamp(0, (1 << 31) - 1)  # more than int32 holds: all
     return v.to(device=device, dtype=dtype).contiguous()
 
 
 def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Param = 1.0,
                   top_k: Union[int, torch.Tensor] = 0, top_p: Param = 1.0, min_p: Param = 0.0,
                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """One token per row of logits [n, vocab] (fp32, bf16 or fp16; vocab at most 2^20):
-    int64 [n], or written into ``out`` (int64 of n values).
+    """One token per row of logits [n, vocab] (fp32, bf16 or fp16; vocab at most 2^20; one
+    row expanded to n gives n draws of it): int64 [n], or written into ``out`` (int64 of n
+    values).
 
     Tokens are ranked by logit, equal ones by index, and weigh exp((logit - largest) /
     temperature).  In this order: top_k keeps the first top_k (0: all); top_p of these

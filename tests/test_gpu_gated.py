@@ -335,14 +335,36 @@ def test_module_matches_its_composition():
 
 
 def test_module_tau_follows_its_parameter():
+    """However the parameter is written, behind autograd's back too."""
     m = GatedLinearRecurrence(16).to(dev())
     h = torch.randn(1, 5, 16, device=dev())
     with torch.no_grad():
         a = m(h)[0]
         m.log_tau.add_(0.5)
         b = m(h)[0]
-        m.log_tau.sub_(0.5)
-    assert not torch.equal(a, b)
+        m.log_tau.data.fill_(3.0)
+        c = m(h)[0]
+        m.log_tau.data.copy_(GatedLinearRecurrence(16).log_tau)
+        d = m(h)[0]
+    assert not torch.equal(a, b) and not torch.equal(b, c) and torch.equal(a, d)
+
+
+def test_infinite_steps_and_gates_act_as_their_limits():
+    """step +-infinity as +-1e5 (clamped both), gate +-infinity as +-1e4 (1 and 0): the same
+    values, and finite gradients that are 0 there."""
+    x, step, gate, tau, st, dy, dlast = inputs(2, 200, 48, F32, 6)
+    at = torch.zeros(2, 200, 48, dtype=torch.int64)
+    at[0, 3, 5], at[1, 130, 7], at[0, 60, 0], at[1, 199, 47] = 1, 2, 3, 4
+    runs = []
+    for s, g in ((math.inf, math.inf), (1e5, 1e4)):
+        step[at == 1], step[at == 2], gate[at == 3], gate[at == 4] = s, -s, g, -g
+        leaves = [t.to(dev()).clone().requires_grad_() for t in (x, step, gate, tau, st)]
+        y, last = gated_recurrence(*leaves, True)
+        runs.append([y, last, *torch.autograd.grad([y, last], leaves, [dy.to(dev()), dlast.to(dev())])])
+    for a, b in zip(*runs):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+    dstep, dgate = runs[0][3].cpu(), runs[0][4].cpu()
+    assert not dstep[(at == 1) | (at == 2)].any() and not dgate[at > 2].any()
 
 
 def test_offsets_past_32_bits():

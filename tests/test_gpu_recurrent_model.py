@@ -129,6 +129,17 @@ def test_greedy_decoder(gated, dtype):
         assert torch.equal(GreedyDecoder(model, use_graph=graph).generate(ids, 8), want)
 
 
+def test_decoders_refuse_a_model_that_drops_out():
+    """A decoder puts its model into eval mode; back in training it is refused."""
+    model = model_of((1,), dropout=0.2)
+    ids = torch.randint(0, 120, (2, 5), device=dev())
+    for d in (GreedyDecoder(model), SamplingDecoder(model)):
+        model.train()
+        with pytest.raises(ValueError, match="eval"):
+            d.generate(ids, 3)
+    assert GreedyDecoder(model.eval()).generate(ids, 3).shape == (2, 8)
+
+
 @pytest.mark.parametrize("gated", [(), (0, 1), (1,)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_sampling_decoder(gated, dtype):

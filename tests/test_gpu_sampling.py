@@ -194,6 +194,18 @@ def test_refusals():
     assert sample_tokens(logits[:0], u[:0]).shape == (0,)
 
 
+def test_draws_of_one_row():
+    """One row expanded to many, and a top_k beyond 32 bits: all."""
+    logits, u = make(1, 5003, BF16, 21)
+    u = torch.rand(300, generator=torch.Generator().manual_seed(3))
+    got = sample_tokens(logits.to(dev()).expand(300, -1), u.to(dev()), 0.8, top_k=200).tolist()
+    assert got == check(logits.expand(300, -1).contiguous(), u, temperature=0.8, top_k=200)
+    each = sample_tokens(logits.to(dev()).expand(300, -1), u.to(dev()), 0.8).tolist()
+    many = torch.full((300,), (1 << 32) + 5, device=dev())
+    for k in ((1 << 32) + 5, -(1 << 32) + 5, many):
+        assert sample_tokens(logits.to(dev()).expand(300, -1), u.to(dev()), 0.8, top_k=k).tolist() == each
+
+
 def test_offsets_past_32_bits():
     V = 5000
     big = torch.zeros((1 << 31) + 2 * V, dtype=BF16, device=dev())

@@ -32,6 +32,7 @@ def scan_bwd(x=seq(AT[0]), s=seq(AT[1]), g=seq(AT[2]), dt=BF, tau=AT[3], ck=AT[4
 
 def test_gated_scan_refuses_before_device_work():
     assert scan(x=None) == -1 and scan(tau=None) == -1 and scan(y=seq(None)) == -1
+    assert scan(b=1 << 23, l=5) == -1 and "grid" in _lib.last_error()
     assert scan(b=0) == -1 and scan(l=0) == -1 and scan(c=-1) == -1 and scan(l=(1 << 30) + 1) == -1
     assert scan(dt=9) == -3
     assert scan(x=seq(AT[0], sl=-1)) == -1 and "stride" in _lib.last_error()
@@ -61,6 +62,7 @@ def test_dropout_refuses_before_device_work():
         return _lib.load().prime_dropout_add(x, ldx, r, ldr, o, ldo, dt, rows, cols, p, rng, 0, None)
     assert call(x=None) == -1 and call(o=None) == -1 and call(rng=None) == -1
     assert call(rows=0) == -1 and call(cols=-2) == -1 and call(rows=1 << 30, cols=1 << 30) == -1
+    assert call(rows=(1 << 28) + 1, ldx=1 << 20) == -1
     assert call(ldx=63) == -1 and call(ldr=1) == -1 and call(ldo=0) == -1
     for p in (-0.1, 1.1, float("nan")):
         assert call(p=p) == -1 and "outside" in _lib.last_error()
@@ -74,7 +76,8 @@ def test_sample_refuses_before_device_work():
     def call(lg=AT[0], dt=BF, n=4, V=100, st=100, u=AT[1], T=None, k=None, p=None, m=None, out=AT[2]):
         return _lib.load().prime_sample(lg, dt, n, V, st, u, 1.0, T, 0, k, 1.0, p, 0.0, m, out, None)
     assert call(lg=None) == -1 and call(u=None) == -1 and call(out=None) == -1
-    assert call(n=0) == -1 and call(V=0) == -1 and call(V=(1 << 20) + 1, st=1 << 21) == -1 and call(st=99) == -1
+    assert call(n=0) == -1 and call(V=0) == -1 and call(V=(1 << 20) + 1, st=1 << 21) == -1 and call(st=-1) == -1
+    assert call(n=1 << 22) == -1
     assert call(dt=3) == -3
     assert call(lg=AT[0] + 1) == -4 and call(out=AT[2] + 4) == -4 and call(T=AT[3] + 1) == -4 and call(k=AT[3] + 2) == -4
     assert call(out=AT[0] + 8) == -5 and call(out=AT[1]) == -5 and call(k=AT[2]) == -5
