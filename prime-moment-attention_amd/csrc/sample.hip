@@ -57,7 +57,13 @@ struct RowScale {
     // 2^t as a mass, t <= 0: 2^f on |f| <= 1/2 by its Chebyshev interpolant of degree 9
     // (1.4e-14 off), scaled and rounded to a whole number by one addition to 2^52.  Below
     // 2^-44 (and for NaN, of a NaN or of -infinity times a rate of 0) that is 0.
+    static constexpr uint64_t kBits = 0x4330000000000000ull;  // of 2^52
     __device__ static __forceinline__ uint64_t mass_of(double t) {
+        uint64_t w = mass_bits(t) - kBits;
+        asm("" : "+v"(w));  // computed for every token: a branch around it costs more than it saves
+        return w;
+    }
+    __device__ static __forceinline__ uint64_t mass_bits(double t) {  // the mass and kBits
         constexpr double kRound = 6755399441055744.0;  // 1.5 2^52: adding it rounds to a whole number
         t = fmax(t, -44.0);
         const double r = t + kRound, f = t - (r - kRound);
@@ -72,9 +78,7 @@ struct RowScale {
         p = fma(p, f, 1.0);
         const uint32_t n = static_cast<uint32_t>(__builtin_bit_cast(uint64_t, r));  // low word: the whole number
         const double scale = __builtin_bit_cast(double, static_cast<uint64_t>((n + 1023u + 42u) << 20) << 32);
-        uint64_t w = __builtin_bit_cast(uint64_t, fma(p, scale, 4503599627370496.0)) - 0x4330000000000000ull;
-        asm("" : "+v"(w));  // computed for every token: a branch around it costs more than it saves
-        return w;
+        return __builtin_bit_cast(uint64_t, fma(p, scale, 4503599627370496.0));
     }
     __device__ __forceinline__ uint64_t mass(float x) const { return mass_of(exponent(x)); }
     __device__ static __forceinline__ uint64_t select(bool keep, uint64_t w) { return keep ? w : 0; }
@@ -169,10 +173,18 @@ struct SampleRow {
     static constexpr int VE = DT == PRIME_F32 ? 4 : 8, es = DT == PRIME_F32 ? 4 : 2;
     const char *base;
     int vocab, per, start;  // start: the lane's first element
+    int whole;              // the wave's chunks that lie before the vocabulary's end
+    __device__ __forceinline__ void place(int wave, int lane) {
+        whole = (vocab - wave * per * (kWave * VE)) / (kWave * VE);
+        start = (wave * per * kWave + lane) * VE;
+    }
     u32x4 *lds;             // the lane's place in the staged chunks, `lds_step` between two
     int lds_step;
 
-    __device__ __forceinline__ int index(int i) const { return max(0, min(start + i * (kWave * VE), vocab - VE)); }
+    __device__ __forceinline__ int index(int i) const {
+        const int e = start + i * (kWave * VE);
+        return i < whole ? e : max(0, min(e, vocab - VE));
+    }
     __device__ __forceinline__ u32x4 load(int i) const {
         if constexpr (STAGED > 0) {
             if (vocab < VE) {
@@ -185,6 +197,7 @@ struct SampleRow {
     }
     __device__ __forceinline__ void mask(int i, u32x4 &v) const {
         constexpr uint32_t none = DT == PRIME_F32 ? 0xFF800000u : DT == PRIME_BF16 ? 0xFF80u : 0xFC00u;  // -infinity
+        if (i < whole) return;
         const int e = start + i * (kWave * VE), first = index(i);
         if (first == e && first + VE <= vocab) return;
 #pragma unroll
@@ -220,23 +233,24 @@ struct SampleRow {
     }
     // f(i, x) over the lane's chunks, the next ones on their way.  (One copy of f: with a row
     // or two the time is in fetching instructions.)
-    template <bool FIRST = false, typename F>
+    template <bool FIRST = false, bool BACK = false, typename F>
     __device__ __forceinline__ void each(F f) const {
+        auto at = [&](int i) { return BACK ? per - 1 - i : i; };
         constexpr int D = STAGED == 0 ? 4 : !FIRST ? 2 : STAGED < 8 ? STAGED : 8;
         u32x4 next[D];
 #pragma unroll
         for (int k = 0; k < D; ++k)
-            if (k < per) next[k] = get<FIRST>(k);
+            if (k < per) next[k] = get<FIRST>(at(k));
 #pragma unroll 1
         for (int i = 0; i < per; ++i) {
             u32x4 now = next[0];
 #pragma unroll
             for (int k = 0; k + 1 < D; ++k) next[k] = next[k + 1];
-            if (i + D < per) next[D - 1] = get<FIRST>(i + D);
-            finish<FIRST>(i, now);
+            if (i + D < per) next[D - 1] = get<FIRST>(at(i + D));
+            finish<FIRST>(at(i), now);
             float x[VE];
             widen(now, x);
-            f(i, x);
+            f(at(i), x);
         }
     }
 };
@@ -470,35 +484,87 @@ __device__ __forceinline__ bool bound_count(SampleShared<WAVES> &sh, int k, Boun
     return true;
 }
 
-// top_p: a token in cell c weighs between 2^(-(c + 1) step) and 2^(-c step), with a hundredth
-// of a cell for roundings, so the counts bound every prefix's mass.
+// The cut by top-k, from its cell's tokens.  False, and nothing decided, where those are too many
+// to compare.
+template <int DT, int WAVES, int STAGED>
+__device__ __forceinline__ bool cut_cell(SampleShared<WAVES> &sh, const SampleRow<DT, STAGED> &row, const RowScale &rs,
+                                         const Bounds &bounds, int k, float &last, uint64_t &ties, bool &whole) {
+    constexpr int VE = SampleRow<DT, STAGED>::VE;
+    __syncthreads();
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
+    row.each([&](int, const float (&x)[VE]) {
+        int c;
+        if (!(rs.cell(largest(x), c) & (c <= bounds.high))) return;
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+            if (rs.cell(x[j], c) & (c == bounds.high)) {
+                const int n = atomicAdd(&sh.n, 1);
+                if (n < kList) sh.list_x[n] = x[j];
+            }
+        }
+    });
+    __syncthreads();
+    const int n = sh.n;
+    if (n > kList) return false;
+    for (int i = threadIdx.x; i < n; i += WAVES * kWave) {
+        const float x = sh.list_x[i];
+        int over = bounds.above, equal = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) {
+            const float y = sh.list_x[j];
+            over += y > x;
+            equal += y == x;
+        }
+        if (over < k && k <= over + equal) sh.last = x, sh.sum = over, sh.rest = equal;
+    }
+    __syncthreads();
+    last = sh.last;
+    ties = k - sh.sum;
+    whole = ties == sh.rest;
+    return true;
+}
+
+// top_p: a token of cell c weighs 2^(-(c + 1/2) step) give or take 0.2 step of that (a uniform
+// place in the cell), so the counts give every prefix's mass up to 0.2 step sqrt(sum of the
+// cells' squared masses); the bounds leave six times that, and 5e-5 of the total for roundings.
+// They may miss, where tokens lie in their cells other than by chance: what comes after finds
+// out, and falls back.
 template <int WAVES>
 __device__ __forceinline__ void bound_mass(SampleShared<WAVES> &sh, const RowScale &rs, float top_p, Bounds &out) {
     constexpr int kPer = kCells / (WAVES * kWave);
     const uint32_t *counts = reinterpret_cast<uint32_t *>(sh.hist);
-    // the most and the least, in 2^-22 of the largest mass (below 2^43 in all), the least with
-    // the tokens' number behind it, so that two sums over the threads do
-    uint64_t most[kPer], least[kPer], all_most, all_least, waves, to_most = 0, to_least = 0;
+    // masses in 2^-22 of the largest (below 2^42 in all) with the tokens' number behind, so that
+    // one sum over the threads does
+    uint64_t mass[kPer], to = 0, all, waves;
+    float squares = 0.f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int b = threadIdx.x * kPer + i;
         const uint32_t n = counts[b];
-        const float w = static_cast<float>(n) * 4194304.f, at = static_cast<float>(b);
-        most[i] = static_cast<uint64_t>(w * __builtin_amdgcn_exp2f(rs.step * (0.01f - at)) * 1.0001f) + (n ? 1 : 0);
-        least[i] = static_cast<uint64_t>(w * __builtin_amdgcn_exp2f(-rs.step * (at + 1.01f)) * 0.9999f) << 21 | n;
-        to_most += most[i];
-        to_least += least[i];
+        const float w = static_cast<float>(n) * __builtin_amdgcn_exp2f(-rs.step * (static_cast<float>(b) + 0.5f));
+        mass[i] = static_cast<uint64_t>(w * 4194304.f + 0.5f) << 21 | n;
+        squares += w * w;
+        to += mass[i];
     }
-    to_most = block_scan(sh, to_most, waves, all_most);
-    to_least = block_scan(sh, to_least, waves, all_least);
-    const double from = 0.9999 * top_p * static_cast<double>(all_least >> 21), to = 1.0001 * top_p * static_cast<double>(all_most);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) squares += __shfl_xor(squares, o, kWave);
+    if (threadIdx.x % kWave == 0) sh.list_x[threadIdx.x / kWave] = squares;
+    to = block_scan(sh, to, waves, all);
+    squares = 0.f;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) squares += sh.list_x[i];
+    const float sum = static_cast<float>(all >> 21), want = top_p * sum;
+    const float margin = 1.2f * rs.step * 4194304.f * __builtin_amdgcn_sqrtf(squares) + 5e-5f * sum;
+    const float from = want - margin, end = want + margin;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int b = threadIdx.x * kPer + i;
-        const double m0 = static_cast<double>(to_most), l0 = static_cast<double>(to_least >> 21);
-        to_most += most[i], to_least += least[i];
-        if (m0 < from && from <= static_cast<double>(to_most)) sh.low = b;
-        if (l0 < to && to <= static_cast<double>(to_least >> 21)) sh.high = b, sh.n = static_cast<int>(to_least & 0x1FFFFF);
+        const float before = static_cast<float>(to >> 21);
+        to += mass[i];
+        const float after = static_cast<float>(to >> 21);
+        if (before < from && from <= after) sh.low = b;
+        if (before < end && end <= after) sh.high = b, sh.n = static_cast<int>(to & 0x1FFFFF);
     }
     __syncthreads();
     out = {sh.low, sh.high, 0, sh.n};
@@ -508,9 +574,9 @@ __device__ __forceinline__ void bound_mass(SampleShared<WAVES> &sh, const RowSca
 // computed once, which gives the kept masses of the lanes' waves along with the cut (mass: of
 // tokens above `last`, or equal to it where all of those are kept; count: of the tokens equal
 // to it otherwise).  Masses of tokens above the bounds are added up in the lanes, only those
-// between them go into shared sums, kRange parts of the bounds for each wave.
-// False, and nothing decided, where the bounds are more than kRange cells apart, or a part
-// holds too many tokens to compare.
+// between them go into shared sums, at most kRange parts of the bounds for each wave.
+// False, and nothing decided, where the bounds miss the cut, or a part holds too many tokens to
+// compare.
 template <int DT, int WAVES, int STAGED, typename F>
 __device__ __forceinline__ bool cut_once(SampleShared<WAVES> &sh, const SampleRow<DT, STAGED> &row, const RowScale &rs,
                                          const Bounds &bounds, F share, float &last, uint64_t &ties, bool &whole,
@@ -519,15 +585,16 @@ __device__ __forceinline__ bool cut_once(SampleShared<WAVES> &sh, const SampleRo
     static_assert(WAVES * kRange <= kBuckets, "the waves' sums take the histogram's place");
     const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
     const int low = bounds.low, range = bounds.high - low + 1;
-    if (range < 1 || range > kRange) return false;
+    if (range < 1) return false;
     uint64_t waves;
     __syncthreads();
     if (tid == 0) sh.n = 0;
     uint64_t *sums = sh.hist;  // [wave][kRange]
     for (int b = tid; b < WAVES * kRange; b += kThreads) sums[b] = 0;
     __syncthreads();
-    const float from = 0.5f * static_cast<float>(low), fine = static_cast<float>(2 * (kRange / range));
-    const float end = static_cast<float>(range * (kRange / range));
+    const int join = (range + kRange - 1) / kRange;  // cells in a part
+    const float from = 0.5f * static_cast<float>(low), end = static_cast<float>(join > 1 ? (range + join - 1) / join : range * (kRange / range));
+    const float fine = join > 1 ? 2.f / static_cast<float>(join) : static_cast<float>(2 * (kRange / range));
     uint64_t rest = 0;
     mass = count = 0;
     row.each([&](int, const float (&x)[VE]) {
@@ -609,7 +676,7 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
     row.base = static_cast<const char *>(a.logits) + r * a.stride_n * Row::es;
     row.vocab = a.vocab;
     row.per = (a.vocab + WAVES * kWave * VE - 1) / (WAVES * kWave * VE);
-    row.start = (wave * row.per * kWave + lane) * VE;
+    row.place(wave, lane);
     row.lds = stage + tid;
     row.lds_step = WAVES * kWave;
     const float T = a.temperatures ? a.temperatures[r] : a.temperature;
@@ -679,6 +746,12 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
     rs.per_half = fminf(2.f * (kBuckets - 1) / (kBucketSpan * T), 1e30f);
     rs.step = static_cast<float>(rs.rate / static_cast<double>(rs.per_half));
 
+    auto masses = [&](const float (&x)[VE]) {  // of a chunk
+        uint64_t sum = 0;
+#pragma unroll
+        for (int j = 0; j < VE; ++j) sum += RowScale::mass_bits(rs.exponent(x[j]));
+        return sum - VE * RowScale::kBits;
+    };
     // Few tokens are left as a rule by top-k, where min_p alone cuts, or above top_p's bounds:
     // one thread takes each, in the order of their indices, and the rest is a few sums over the
     // threads.  (top_p alone also needs the mass of all.)
@@ -690,29 +763,22 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
     if (by_mass) bound_mass(sh, rs, top_p, bounds);
     if (by_count || by_mass ? bounds.tokens <= WAVES * kWave : top_k == a.vocab && top_p >= 1.f && min_p > 0.f) {
         uint64_t all_mass = 0, waves, total;
-        if (by_mass) {
-            uint64_t sum = 0;
-            row.each([&](int, const float (&x)[VE]) {
-#pragma unroll
-                for (int j = 0; j < VE; ++j) {
-                    sum += rs.mass(x[j]);
-                }
-            });
-            block_scan(sh, sum, waves, all_mass);
-        }
         // nothing below this weighs: what min_p leaves, with room for rounding, or the bounds'
         // end, in cells
         const float far = top + static_cast<float>(rs.least / rs.rate), room = 1e-5f * (fabsf(top) + fabsf(far));
         const float least_x = counted ? -__FLT_MAX__ : fmaxf(far - room, -__FLT_MAX__);
         const float end = static_cast<float>(bounds.high + 1);
         auto stays = [&](float x) { return (x >= least_x) & (rs.place(x) * 2.f < end); };
-        uint64_t n = 0, first, all;
+        uint64_t n = 0, sum = 0, first, all;
         row.each([&](int, const float (&x)[VE]) {
 #pragma unroll
             for (int j = 0; j < VE; ++j) n += stays(x[j]);
+            if (by_mass) sum += masses(x);
         });
         block_scan(sh, n, first, all);
-        if (all <= WAVES * kWave) {
+        if (by_mass) block_scan(sh, sum, waves, all_mass);
+        bool closed = all <= WAVES * kWave;
+        if (closed) {
             int *list_i = reinterpret_cast<int *>(sh.list_w);
             int at = static_cast<int>(first);
             row.each([&](int i, const float (&x)[VE]) {
@@ -777,23 +843,27 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
                 __syncthreads();
                 uint64_t part;
                 const uint64_t before = scan_hist(sh, part, total), want = share(by_mass ? all_mass : total);
-                locate(sh, before, part, want);
-                const int bucket = sh.bucket;
-                const uint64_t over = sh.sum + before_in_bucket(w && b == bucket, w);
-                w = b > bucket || (b == bucket && over >= want) ? 0 : w;
+                closed = want <= total;  // (else the bounds have missed)
+                if (closed) {
+                    locate(sh, before, part, want);
+                    const int bucket = sh.bucket;
+                    const uint64_t over = sh.sum + before_in_bucket(w && b == bucket, w);
+                    w = b > bucket || (b == bucket && over >= want) ? 0 : w;
+                }
             }
             w = RowScale::select(t >= rs.least, w);
             const uint64_t to = block_scan(sh, w, waves, total), target = target_of(total);
-            if (to <= target && target < to + w) a.out[r] = index;
-            return;
+            if (closed && to <= target && target < to + w) a.out[r] = index;
         }
+        if (closed) return;
     }
 
     // Else: kept are the tokens above `last`, and of those equal to it the first `ties`
     float last = -kInf;
     uint64_t ties = 0, mass = 0, count = 0;  // mass, count: the lane's kept ones, once summed
     bool whole = true;
-    if (top_k < a.vocab) cut<false>(sh, row, rs, last, ties, whole, [&](uint64_t) { return static_cast<uint64_t>(top_k); });
+    if (top_k < a.vocab && !(by_count && cut_cell(sh, row, rs, bounds, top_k, last, ties, whole)))
+        cut<false>(sh, row, rs, last, ties, whole, [&](uint64_t) { return static_cast<uint64_t>(top_k); });
     const bool summed =
         by_mass && !(min_p > 0.f) && cut_once(sh, row, rs, bounds, share, last, ties, whole, mass, count);
     if (top_p < 1.f && !summed) cut<true>(sh, row, rs, last, ties, whole, share);
@@ -812,7 +882,12 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
         const double t = rs.exponent(x);
         return RowScale::select((x > last) & (t >= rs.least), RowScale::mass_of(t));
     };
+    const bool plain = last == -kInf && !(min_p > 0.f);
     auto add_chunk = [&](const float (&x)[VE], uint64_t &mass, uint64_t &count) {
+        if (plain) {
+            mass += masses(x);
+            return;
+        }
         if (!(largest(x) >= last)) return;
 #pragma unroll
         for (int j = 0; j < VE; ++j) mass += token(x[j]);
@@ -824,7 +899,7 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
     uint64_t all_mass, all_count, mass0, count0;  // ..0: before the wave
     if (!summed) {
         mass = count = 0;
-        row.each([&](int, const float (&x)[VE]) { add_chunk(x, mass, count); });
+        row.template each<false, true>([&](int, const float (&x)[VE]) { add_chunk(x, mass, count); });
     }
     const uint64_t wave_count = ties ? last_lane(wave_scan_u64(count)) : 0;
     count0 = all_count = 0;
@@ -837,7 +912,7 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
     __syncthreads();
     mass0 = sh.sum, count0 = sh.rest;
     const int shift = sh.owner - wave;
-    row.start += shift * row.per * (kWave * VE);
+    row.place(__builtin_amdgcn_readfirstlane(sh.owner), lane);
     row.lds += shift * kWave;
     constexpr int kRound = kBuckets / kWave;  // chunks whose sums fit
     static_assert(sizeof(sh.list_w) >= kBuckets * sizeof(int), "the counts take the list's place");
