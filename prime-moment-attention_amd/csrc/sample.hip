@@ -16,6 +16,8 @@
 // bucket with each other; should it hold too many, a radix descent over the
 // order-preserving keys of all tokens takes its place.
 
+#include <type_traits>
+
 #include "prime_kernels.h"
 
 namespace prime {
@@ -92,11 +94,6 @@ struct RowScale {
         const float f = place(x) * 2.f;
         c = static_cast<int>(f);
         return f < static_cast<float>(kCells - 2);
-    }
-    // a part of a bucket: the place behind `low`, `fine` parts to a bucket
-    __device__ __forceinline__ float part(float x, float low, float fine) const {
-#pragma clang fp contract(off)
-        return (place(x) - low) * fine;
     }
     __device__ __forceinline__ bool bucket(float x, int &b) const {
         const float f = place(x);
@@ -222,6 +219,17 @@ struct SampleRow {
         u32x4 v = get(i);
         finish(i, v);
         widen(v, x);
+    }
+    // element j of chunk i
+    __device__ __forceinline__ float one(int i, int j) const {
+        using P = typename std::conditional<DT == PRIME_F32, float, uint16_t>::type;
+        const int e = start + i * (kWave * VE), at = index(i) + j;
+        if (at < e || at >= vocab) return -kInf;
+        P p;
+        if constexpr (STAGED > 0) p = reinterpret_cast<const P *>(lds + i * lds_step)[j];
+        else p = reinterpret_cast<const P *>(base)[at];
+        if constexpr (DT == PRIME_F32) return p;
+        else return DT == PRIME_BF16 ? bf16_bits_to_f32(p) : h16_bits_to_f32(p);
     }
     __device__ __forceinline__ void widen(const u32x4 &v, float (&x)[VE]) const {
 #pragma unroll
@@ -592,20 +600,23 @@ __device__ __forceinline__ bool cut_once(SampleShared<WAVES> &sh, const SampleRo
     uint64_t *sums = sh.hist;  // [wave][kRange]
     for (int b = tid; b < WAVES * kRange; b += kThreads) sums[b] = 0;
     __syncthreads();
-    const int join = (range + kRange - 1) / kRange;  // cells in a part
-    const float from = 0.5f * static_cast<float>(low), end = static_cast<float>(join > 1 ? (range + join - 1) / join : range * (kRange / range));
-    const float fine = join > 1 ? 2.f / static_cast<float>(join) : static_cast<float>(2 * (kRange / range));
+    // the bounds as logits, and the parts between them: `width` cells each
+    const int join = (range + kRange - 1) / kRange, parts = join > 1 ? (range + join - 1) / join : range * (kRange / range);
+    const float width = join > 1 ? static_cast<float>(join) : 1.f / static_cast<float>(kRange / range);
+    const float cell = 1.f / rs.per_half, from = static_cast<float>(low), fine = 1.f / width;
+    const float high_x = rs.top - from * cell, low_x = rs.top - static_cast<float>(bounds.high + 1) * cell;
+    auto part = [&](float x) { return max(0, min(parts - 1, static_cast<int>((rs.place(x) * 2.f - from) * fine))); };
     uint64_t rest = 0;
-    mass = count = 0;
+    mass = 0;
     row.each([&](int, const float (&x)[VE]) {
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
-            const uint64_t w = rs.mass(x[j]);
-            const float f = rs.part(x[j], from, fine);
+            const uint64_t w = RowScale::mass_bits(rs.exponent(x[j]));
             rest += w;
-            mass += f < 0.f ? w : 0;
-            if ((f >= 0.f) & (f < end)) lds_add(&sums[wave * kRange + static_cast<int>(f)], w);
+            mass += x[j] > high_x ? w - RowScale::kBits : 0;
+            if ((x[j] <= high_x) & (x[j] >= low_x)) lds_add(&sums[wave * kRange + part(x[j])], w - RowScale::kBits);
         }
+        rest -= VE * RowScale::kBits;
     });
     uint64_t all, above;
     block_scan(sh, rest, waves, all);
@@ -621,13 +632,14 @@ __device__ __forceinline__ bool cut_once(SampleShared<WAVES> &sh, const SampleRo
     if (!(hit_even | hit_odd)) return false;
     const int owner = __builtin_ctzll(hit_even | hit_odd), found = 2 * owner + (hit_even ? 0 : 1);
     const uint64_t over0 = shfl_u64(hit_even ? to_even - even : to_even, owner);
-    const float at = static_cast<float>(found);
+    // (half a cell around the part: nearly all tokens are told by two comparisons)
+    const float part_high = fminf(high_x, rs.top - (from + static_cast<float>(found) * width - 0.5f) * cell);
+    const float part_low = fmaxf(low_x, rs.top - (from + static_cast<float>(found + 1) * width + 0.5f) * cell);
     row.each([&](int, const float (&x)[VE]) {
-        if (!(rs.part(largest(x), from, fine) < at + 1.f)) return;
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
-            const float f = rs.part(x[j], from, fine);
-            if ((f >= at) & (f < at + 1.f)) {
+            if (!((x[j] <= part_high) & (x[j] >= part_low))) continue;
+            if (part(x[j]) == found) {
                 const int n = atomicAdd(&sh.n, 1);
                 if (n < kList) sh.list_x[n] = x[j], sh.list_wave[n] = static_cast<uint8_t>(wave);
             }
@@ -655,6 +667,7 @@ __device__ __forceinline__ bool cut_once(SampleShared<WAVES> &sh, const SampleRo
     const uint64_t w = rs.mass(last);
     ties = (want - sh.sum + w - 1) / w;
     whole = ties * w == sh.rest;
+    count = 0;
     for (int k = lane; k < found; k += kWave) mass += sums[wave * kRange + k];
     for (int i = lane; i < n; i += kWave) {
         const float x = sh.list_x[i];
@@ -896,7 +909,7 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
             for (int j = 0; j < VE; ++j) count += x[j] == last;
         }
     };
-    uint64_t all_mass, all_count, mass0, count0;  // ..0: before the wave
+    uint64_t all_mass, all_count, mass0, count0;  // ..0: before what is looked at
     if (!summed) {
         mass = count = 0;
         row.template each<false, true>([&](int, const float (&x)[VE]) { add_chunk(x, mass, count); });
@@ -914,9 +927,20 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
     const int shift = sh.owner - wave;
     row.place(__builtin_amdgcn_readfirstlane(sh.owner), lane);
     row.lds += shift * kWave;
+    // the lane that has the target among its (mass, count), which follow each other lane by lane,
+    // or -1; mass0, count0 move to before that lane, or behind all
+    auto pick = [&](uint64_t m, uint64_t c) {
+        const uint64_t mi = wave_scan_u64(m), ci = ties ? wave_scan_u64(c) : 0;
+        const uint64_t hit = __ballot(target < sum_of(mass0 + mi, count0 + ci));
+        const int l = hit ? __builtin_ctzll(hit) : kWave - 1;
+        mass0 += shfl_u64(hit ? mi - m : mi, l);
+        count0 += ties ? shfl_u64(hit ? ci - c : ci, l) : 0;
+        return hit ? l : -1;
+    };
     constexpr int kRound = kBuckets / kWave;  // chunks whose sums fit
     static_assert(sizeof(sh.list_w) >= kBuckets * sizeof(int), "the counts take the list's place");
     int *counts = reinterpret_cast<int *>(sh.list_w);
+    bool done = false;
     for (int i0 = 0; i0 < row.per; i0 += kRound) {
         const int n = min(kRound, row.per - i0);
         __syncthreads();
@@ -929,33 +953,23 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
             counts[i * kWave + lane] = static_cast<int>(c);
         }
         __syncthreads();
-        if (wave) continue;
-        // in order: lane by lane, chunk by chunk; here a lane takes n sums in a row
+        if (wave || done) continue;
+        // in order, chunk by chunk: the lane whose n sums in a row have the target, then the sum,
+        // then the token
         uint64_t m = 0, c = 0;
 #pragma unroll 8
         for (int k = 0; k < n; ++k) m += sh.hist[lane * n + k], c += counts[lane * n + k];
-        const uint64_t mi = wave_scan_u64(m), ci = ties ? wave_scan_u64(c) : 0;
-        uint64_t am = mass0 + mi - m, ac = count0 + ci - c;
-        if (sum_of(am, ac) <= target && target < sum_of(mass0 + mi, count0 + ci)) {
-            int k = lane * n;
-            while (target >= sum_of(am + sh.hist[k], ac + counts[k])) am += sh.hist[k], ac += counts[k], ++k;
-            // sum k is lane k % 64's of chunk k / 64
-            const int other = k % kWave - lane;
-            Row its = row;
-            its.start += other * VE;
-            its.lds += other;
-            float x[VE];
-            its.fetch(i0 + k / kWave, x);
-            bool done = false;
-#pragma unroll
-            for (int j = 0; j < VE; ++j) {
-                am += token(x[j]);
-                ac += ties && x[j] == last;
-                if (!done && target < sum_of(am, ac)) a.out[r] = its.index(i0 + k / kWave) + j, done = true;
-            }
-        }
-        mass0 += last_lane(mi);
-        count0 += last_lane(ci);
+        const int l = pick(m, c);
+        if (l < 0) continue;
+        const bool one = lane < n;
+        const int k = l * n + pick(one ? sh.hist[l * n + lane] : 0, one ? counts[l * n + lane] : 0);
+        const int i = i0 + k / kWave, other = k % kWave - lane;  // lane k % 64's of chunk k / 64
+        Row its = row;
+        its.start += other * VE;
+        its.lds += other;
+        const float x = lane < VE ? its.one(i, lane) : -kInf;
+        if (pick(token(x), ties && x == last) == lane) a.out[r] = its.index(i) + lane;
+        done = true;
     }
 }
 
