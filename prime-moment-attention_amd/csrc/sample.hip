@@ -774,16 +774,30 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
     if (counted && !by_count) top_k = a.vocab;
     const bool by_mass = counted && !by_count && top_p < 1.f;
     if (by_mass) bound_mass(sh, rs, top_p, bounds);
-    if (by_count || by_mass ? bounds.tokens <= WAVES * kWave : top_k == a.vocab && top_p >= 1.f && min_p > 0.f) {
+    // kept are the tokens above `last`, and of those equal to it the first `ties`
+    float last = -kInf;
+    uint64_t ties = 0;
+    bool whole = true;
+    // where the last cell holds too many tokens, as it does with many equal ones, top-k's cut first
+    const bool celled = by_count && bounds.tokens > WAVES * kWave && cut_cell(sh, row, rs, bounds, top_k, last, ties, whole);
+    const bool exact = celled && top_k <= WAVES * kWave;
+    const int last_tie = exact && !whole ? find_equal(sh, row, last, [&](uint64_t) { return ties; }) : a.vocab;
+    if (by_count || by_mass ? exact || bounds.tokens <= WAVES * kWave : top_k == a.vocab && top_p >= 1.f && min_p > 0.f) {
         uint64_t all_mass = 0, waves, total;
         // nothing below this weighs: what min_p leaves, with room for rounding, or the bounds'
         // end, in cells
         const float far = top + static_cast<float>(rs.least / rs.rate), room = 1e-5f * (fabsf(top) + fabsf(far));
-        const float least_x = counted ? -__FLT_MAX__ : fmaxf(far - room, -__FLT_MAX__);
+        const float least_x = exact ? last : counted ? -__FLT_MAX__ : fmaxf(far - room, -__FLT_MAX__);
         const float end = static_cast<float>(bounds.high + 1);
         auto stays = [&](float x) { return (x >= least_x) & (rs.place(x) * 2.f < end); };
+        auto drop_ties = [&](int i, float (&x)[VE]) {
+            if (last_tie >= a.vocab) return;
+#pragma unroll
+            for (int j = 0; j < VE; ++j) x[j] = x[j] == last && row.index(i) + j > last_tie ? -kInf : x[j];
+        };
         uint64_t n = 0, sum = 0, first, all;
-        row.each([&](int, const float (&x)[VE]) {
+        row.each([&](int i, float (&x)[VE]) {
+            drop_ties(i, x);
 #pragma unroll
             for (int j = 0; j < VE; ++j) n += stays(x[j]);
             if (by_mass) sum += masses(x);
@@ -794,8 +808,9 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
         if (closed) {
             int *list_i = reinterpret_cast<int *>(sh.list_w);
             int at = static_cast<int>(first);
-            row.each([&](int i, const float (&x)[VE]) {
+            row.each([&](int i, float (&x)[VE]) {
                 if (!__any(stays(largest(x)))) return;
+                drop_ties(i, x);
                 int chunk = 0, place = at;
 #pragma unroll
                 for (int j = 0; j < VE; ++j) {
@@ -842,7 +857,7 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
                 }
                 return over;
             };
-            if (by_count) {
+            if (by_count && !exact) {
                 int c;
                 const bool in = rs.cell(x, c) && c == bounds.high;
                 const uint64_t rank = bounds.above + before_in_bucket(in, 1);
@@ -871,11 +886,9 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
         if (closed) return;
     }
 
-    // Else: kept are the tokens above `last`, and of those equal to it the first `ties`
-    float last = -kInf;
-    uint64_t ties = 0, mass = 0, count = 0;  // mass, count: the lane's kept ones, once summed
-    bool whole = true;
-    if (top_k < a.vocab && !(by_count && cut_cell(sh, row, rs, bounds, top_k, last, ties, whole)))
+    // Else
+    uint64_t mass = 0, count = 0;  // the lane's kept ones, once summed
+    if (top_k < a.vocab && !celled)
         cut<false>(sh, row, rs, last, ties, whole, [&](uint64_t) { return static_cast<uint64_t>(top_k); });
     const bool summed =
         by_mass && !(min_p > 0.f) && cut_once(sh, row, rs, bounds, share, last, ties, whole, mass, count);

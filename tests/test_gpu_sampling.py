@@ -252,6 +252,17 @@ def test_ties_through_the_top_k_border():
         check(logits.to(BF16), u, **kw)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V,ks", [(50304, (1000, 1010, 1023, 1024, 1025, 3000)), (4000, (240, 250, 255, 256, 257, 900))])
+def test_top_k_near_the_threads(V, ks, dtype):
+    """As many kept tokens as a workgroup has threads, and ties that reach past them."""
+    logits, u = make(24, V, dtype, V + 2)
+    if dtype is F32:
+        logits = (logits * 32).round() / 32
+    for kw in ({}, {"top_p": 0.93, "min_p": 0.001}):
+        check(logits, u, temperature=0.9, top_k=np.array(ks * 4), **kw)
+
+
 def test_two_streams_at_once():
     logits, u = make(8, 50304, BF16, 16)
     logits, u = logits.to(dev()), u.to(dev())
