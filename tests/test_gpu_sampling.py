@@ -263,6 +263,21 @@ def test_top_k_near_the_threads(V, ks, dtype):
         check(logits, u, temperature=0.9, top_k=np.array(ks * 4), **kw)
 
 
+@pytest.mark.parametrize("V", [900, 4000, 40000])
+def test_mass_estimates_that_are_off(V):
+    """top_p where the heavier tokens lie at the upper ends of equal steps of the logit and
+    the lighter ones at the lower ends: what counts alone tell of the masses is off."""
+    n = 64
+    step = torch.arange(V) * 2000 // V
+    for edge in (40, 150, 400):
+        x = -(step + torch.where(step < edge, 0.03, 0.97)) * (30.5 / 4094)
+        perm = torch.randperm(V, generator=torch.Generator().manual_seed(edge))
+        logits = x[perm].expand(n, V).contiguous()
+        u = torch.rand(n, generator=torch.Generator().manual_seed(V))
+        check(logits, u, top_p=np.linspace(0.02, 0.9999, n))
+        check(logits, u, top_p=np.linspace(0.02, 0.9999, n), min_p=0.01)
+
+
 def test_two_streams_at_once():
     logits, u = make(8, 50304, BF16, 16)
     logits, u = logits.to(dev()), u.to(dev())
