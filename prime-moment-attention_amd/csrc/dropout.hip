@@ -67,51 +67,41 @@ struct Eight {
 };
 
 // Rows whose blocks of eight start on 16 bytes.  FLAT: the rows lie one after the other, so
-// the elements are one row of any length.  U blocks a lane, their loads first, the random
-// bits while they are under way.
+// the elements are one row of any length.  The loads first, the random bits while they are
+// under way.
 template <int DT, bool RES, bool FLAT>
 __global__ __launch_bounds__(kDropThreads) void dropout_add_kernel(const DropoutArgs a) {
-    constexpr int U = 2;
-    const int64_t total = a.rows * a.cols, j0 = static_cast<int64_t>(blockIdx.x) * (U * kDropThreads) + threadIdx.x;
-    const uint64_t counter = static_cast<uint64_t>(a.rng[1]) + static_cast<uint64_t>(a.call), seed = a.rng[0];
-    Eight<DT> x[U], r[U];
-    int64_t ox[U], orr[U], oo[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int64_t e = (j0 + u * kDropThreads) * 8;
-        ox[u] = orr[u] = oo[u] = e;
-        if constexpr (!FLAT) {
-            const int64_t row = e / a.cols, col = e % a.cols;
-            ox[u] = row * a.ldx + col, orr[u] = row * a.ldr + col, oo[u] = row * a.ldo + col;
-        }
-        if (e + 8 <= total) {
-            x[u].load(a.x, ox[u]);
-            if constexpr (RES) r[u].load(a.residual, orr[u]);
-        }
+    const int64_t block = static_cast<int64_t>(blockIdx.x) * kDropThreads + threadIdx.x, e = block * 8, total = a.rows * a.cols;
+    if (e >= total) return;
+    int64_t ox = e, orr = e, oo = e;
+    if constexpr (!FLAT) {
+        const int64_t row = e / a.cols, col = e % a.cols;
+        ox = row * a.ldx + col, orr = row * a.ldr + col, oo = row * a.ldo + col;
     }
+    const bool all = !FLAT || e + 8 <= total;
+    Eight<DT> x, r;
+    if (all) {
+        x.load(a.x, ox);
+        if constexpr (RES) r.load(a.residual, orr);
+    }
+    uint32_t w[4];
+    philox(block, static_cast<uint64_t>(a.rng[1]) + static_cast<uint64_t>(a.call), static_cast<uint64_t>(a.rng[0]), w);
+    if (all) {
+        float f[8];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int64_t block = j0 + u * kDropThreads, e = block * 8;
-        if (e >= total) return;
-        uint32_t w[4];
-        philox(block, counter, seed, w);
-        if (e + 8 <= total) {
-            float f[8];
+        for (int j = 0; j < 8; ++j) {
+            f[j] = kept(w, j, a.cut) ? x.get(j) * a.scale : 0.f;
+            if constexpr (RES) f[j] += r.get(j);
+        }
+        x.set(f);
+        x.store(a.out, oo);
+    } else {  // the last elements of one long row
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                f[j] = kept(w, j, a.cut) ? x[u].get(j) * a.scale : 0.f;
-                if constexpr (RES) f[j] += r[u].get(j);
-            }
-            x[u].set(f);
-            x[u].store(a.out, oo[u]);
-        } else {  // the last elements of one long row
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (e + j >= total) continue;
-                float f = kept(w, j, a.cut) ? load_elem(a.x, e + j, DT) * a.scale : 0.f;
-                if constexpr (RES) f += load_elem(a.residual, e + j, DT);
-                store_elem(a.out, e + j, DT, f);
-            }
+        for (int j = 0; j < 8; ++j) {
+            if (e + j >= total) continue;
+            float f = kept(w, j, a.cut) ? load_elem(a.x, e + j, DT) * a.scale : 0.f;
+            if constexpr (RES) f += load_elem(a.residual, e + j, DT);
+            store_elem(a.out, e + j, DT, f);
         }
     }
 }
@@ -149,17 +139,17 @@ void run(const DropoutArgs &a, bool flat, dim3 grid, hipStream_t s) {
 
 hipError_t launch_dropout_add(const DropoutArgs &a, hipStream_t stream) {
     const int64_t blocks = (a.rows * a.cols + 7) / 8, es = a.dt == PRIME_F32 ? 4 : 2;
-    auto grid = [&](int per) { return dim3(static_cast<unsigned>((blocks + per - 1) / per)); };
+    const dim3 grid(static_cast<unsigned>((blocks + kDropThreads - 1) / kDropThreads));
     auto starts = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
     auto aligned = [&](const void *p, int64_t ld) { return starts(p) && ld * es % 16 == 0; };
     const bool flat = a.rows == 1 || (a.ldx == a.cols && a.ldo == a.cols && (!a.residual || a.ldr == a.cols));
     const bool wide = flat ? starts(a.x) && starts(a.out) && starts(a.residual)
                            : a.cols % 8 == 0 && aligned(a.x, a.ldx) && aligned(a.out, a.ldo) &&
                                  (!a.residual || aligned(a.residual, a.ldr));
-    if (!wide) hipLaunchKernelGGL(dropout_any_kernel, grid(kDropThreads), dim3(kDropThreads), 0, stream, a);
-    else if (a.dt == PRIME_BF16) run<PRIME_BF16>(a, flat, grid(2 * kDropThreads), stream);
-    else if (a.dt == PRIME_F16) run<PRIME_F16>(a, flat, grid(2 * kDropThreads), stream);
-    else run<PRIME_F32>(a, flat, grid(2 * kDropThreads), stream);
+    if (!wide) hipLaunchKernelGGL(dropout_any_kernel, grid, dim3(kDropThreads), 0, stream, a);
+    else if (a.dt == PRIME_BF16) run<PRIME_BF16>(a, flat, grid, stream);
+    else if (a.dt == PRIME_F16) run<PRIME_F16>(a, flat, grid, stream);
+    else run<PRIME_F32>(a, flat, grid, stream);
     return hipGetLastError();
 }
 

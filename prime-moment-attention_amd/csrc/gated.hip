@@ -246,11 +246,11 @@ __device__ __forceinline__ void join(const GatedArgs &a, SpanShared &sh, const P
 }
 
 // A wave's tokens: all kGatedTile of them (the loops below then have no branch in them),
-// or the n < kGatedTile before the sequence's end.
+// or the n < kGatedTile before the sequence's end, if any.
 template <typename F>
 __device__ __forceinline__ void for_tokens(int n, F f) {
     if (n >= kGatedTile) f(std::true_type{}, kGatedTile);
-    else f(std::false_type{}, n);
+    else if (n > 0) f(std::false_type{}, n);
 }
 
 // ------------------------------------------------------------------ forward
@@ -263,8 +263,7 @@ __global__ __launch_bounds__(kThreads) void gated_scan_kernel(const GatedArgs a)
     const int l0 = p.g * kSpan + p.wave * T, left = a.L - l0;  // left <= 0: nothing of the wave's is left
     float h[T], prod[T], zs = 0.f, H = 0.f;                    // state from zero, product of a, per token
     for_tokens(left, [&](auto full, int n) {
-        const int l = min(l0, a.L - 1);
-        Rows rx(a.x, es, p.b, l), rs(a.step, es, p.b, l), rg(a.gate, es, p.b, l);
+        Rows rx(a.x, es, p.b, l0), rs(a.step, es, p.b, l0), rg(a.gate, es, p.b, l0);
         const uint32_t o = here(p.c * es);
         P px[T], ps[T], pg[T];
 #pragma unroll
@@ -312,7 +311,8 @@ __device__ __forceinline__ P *elem(const GatedView &v, int b, uint32_t c) {
     return static_cast<P *>(v.data) + b * v.sb + c;
 }
 
-// Few tokens: a lane walks them.
+// Few tokens: a lane walks them, kWalk on their way at a time.
+constexpr int kWalk = 4;
 template <int DT>
 __global__ __launch_bounds__(256) void gated_step_kernel(const GatedArgs a) {
     using P = Elem<DT>;
@@ -324,13 +324,24 @@ __global__ __launch_bounds__(256) void gated_step_kernel(const GatedArgs a) {
     P *ry = elem<P>(a.y, b, c);
     const float rate = kLog2e / a.tau[c];
     float h = a.state_in ? a.state_in[row] : 0.f, lo = 0.f;
-    if (a.ckpt) a.ckpt[row] = h;
-    for (int l = 0; l < a.L; ++l) {
-        float z, am1, bt;
-        gates(widen<DT>(*rx), widen<DT>(*rs), widen<DT>(*rg), rate, z, am1, bt);
-        advance(h, lo, am1, bt);
-        *ry = narrow<DT>(h);
-        rx += a.x.sl, rs += a.step.sl, rg += a.gate.sl, ry += a.y.sl;
+    for (int l0 = 0; l0 < a.L; l0 += kWalk) {
+        if (a.ckpt && l0 % kGatedTile == 0) a.ckpt[(static_cast<int64_t>(b) * a.tiles + l0 / kGatedTile) * a.C + c] = h;
+        P px[kWalk], ps[kWalk], pg[kWalk];
+#pragma unroll
+        for (int t = 0; t < kWalk; ++t) {
+            if (l0 + t >= a.L) break;
+            px[t] = *rx, ps[t] = *rs, pg[t] = *rg;
+            rx += a.x.sl, rs += a.step.sl, rg += a.gate.sl;
+        }
+#pragma unroll
+        for (int t = 0; t < kWalk; ++t) {
+            if (l0 + t >= a.L) break;
+            float z, am1, bt;
+            gates(widen<DT>(px[t]), widen<DT>(ps[t]), widen<DT>(pg[t]), rate, z, am1, bt);
+            advance(h, lo, am1, bt);
+            *ry = narrow<DT>(h);
+            ry += a.y.sl;
+        }
     }
     if (a.state_out) a.state_out[row] = h;
 }
@@ -357,10 +368,9 @@ __global__ __launch_bounds__(kThreads, 4) void gated_bwd_kernel(const GatedArgs 
     float zs = 0.f, R = 0.f;
     for_tokens(left, [&](auto full, int n) {
         P px[T], ps[T], pg[T], pd[T];
-        const int l = min(l0, a.L - 1);
-        Rows rx(a.x, es, p.b, l), rs(a.step, es, p.b, l), rg(a.gate, es, p.b, l), rd(a.dy, es, p.b, l);
+        Rows rx(a.x, es, p.b, l0), rs(a.step, es, p.b, l0), rg(a.gate, es, p.b, l0), rd(a.dy, es, p.b, l0);
         const uint32_t o = here(p.c * es);
-        float h = a.ckpt[(static_cast<int64_t>(p.b) * a.tiles + l / T) * a.C + p.c], pr = 1.f;
+        float h = a.ckpt[(static_cast<int64_t>(p.b) * a.tiles + l0 / T) * a.C + p.c], pr = 1.f;
 #pragma unroll
         for (int t = 0; t < T; ++t) {
             px[t] = rx.load<P>(o), ps[t] = rs.load<P>(o), pg[t] = rg.load<P>(o), pd[t] = rd.load<P>(o);
@@ -456,7 +466,12 @@ __global__ __launch_bounds__(256) void gated_fill_kernel(uint4 *p, int64_t n) {
 // ------------------------------------------------------------------ launch
 namespace {
 
-constexpr int kStepTokens = 4;  // up to here a lane walks the tokens
+// Whether a lane walks the tokens: a few always (8 tokens of 768 bf16 channels: 1 sequence 4.3
+// us, spans 5.0; 256 sequences 6.0, 16.3), more where the sequences fill the chip without the
+// waves that share a span (32 tokens: 256 sequences 18 us, 23; 16 sequences 9.4, 4.9).
+bool walks(const GatedArgs &a) {
+    return a.L <= 8 || (a.L <= 32 && static_cast<int64_t>(a.B) * ((a.C + kWave - 1) / kWave) >= 2048);
+}
 
 int spans_grid(const GatedArgs &a) { return a.B * ((a.C + kWave - 1) / kWave) * a.G; }
 
@@ -472,7 +487,7 @@ void run(const GatedArgs &a, bool bwd, hipStream_t s) {
         fill(a, s);
         hipLaunchKernelGGL(gated_bwd_kernel<DT>, dim3(spans_grid(a)), dim3(kThreads), 0, s, a);
         hipLaunchKernelGGL(gated_dtau_kernel, dim3((a.C + kWave - 1) / kWave), dim3(1024), 0, s, a);
-    } else if (a.L <= kStepTokens) {
+    } else if (walks(a)) {
         const int block = a.C >= 256 ? 256 : (a.C + kWave - 1) / kWave * kWave;
         hipLaunchKernelGGL(gated_step_kernel<DT>, dim3(a.B * ((a.C + block - 1) / block)), dim3(block), 0, s, a);
     } else {

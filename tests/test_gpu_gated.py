@@ -108,6 +108,14 @@ def test_split_over_time(B, L, C, dtype):
     run_case(B, L, C, dtype, 200 + L, state=True)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("L", [4, 8, 9, 16, 17, 20, 32, 33])
+@pytest.mark.parametrize("B", [2, 520])
+def test_short_prompts(B, L, dtype):
+    """Few tokens of few and of many sequences: walked, or split over a span's waves."""
+    run_case(B, L, 250, dtype, L, True)
+
+
 @pytest.mark.parametrize("B", [1, 5000])
 def test_long_memory_keeps_its_value(B):
     """One token of input, then 6,000 with almost no decay: z = 1e-4 / 2000 = 5e-8 lies
