@@ -6,6 +6,13 @@
 // low halves first, of one block of Philox4x32-10 (J. Salmon, M. Moraes, R. Dror,
 // D. Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011: the rounds and the
 // constants are the paper's) with counter (j, offset + call) and key seed.
+//
+// Bound by memory: 65536 x 768 bf16 moves 302 MB in 47 us (6.4 TB/s) with a residual and 201 MB
+// in 33 us (6.0 TB/s) without; the ten rounds, some 60 integer instructions for eight
+// elements, hide behind the loads.  Two or four blocks a lane: 48 and 49 us, and 0.4 and 0.9 us
+// more at 1000 x 513 (3.3 us).  Element by element, as rows take that start anywhere: 179 us.
+// The loads past the caches: 106 us for fp32 with plain ones, 105 with these (without a
+// residual 73, 68; for bf16 31, 33); stores past them too: 111.
 
 #include "prime_kernels.h"
 

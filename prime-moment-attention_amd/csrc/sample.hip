@@ -9,12 +9,23 @@
 // token every time, and a border is missed by at most 2^-42 of the largest mass per
 // token.  A vocabulary of up to 2^20 keeps every sum below 2^62.
 //
-// One workgroup a row, a contiguous part a wave; every pass reads the row again, from the
-// caches after the first.  The ranking is never sorted.  A cut
-// adds weights (ones for top-k, masses for top-p) into buckets of equal width in the logit,
-// finds the bucket in which the wanted sum is reached, and compares the tokens of that one
-// bucket with each other; should it hold too many, a radix descent over the
-// order-preserving keys of all tokens takes its place.
+// One workgroup a row, a contiguous part a wave.  The first pass finds the largest logit and
+// puts the row into LDS where it fits (else the later ones read the caches).  The ranking is
+// never sorted: tokens are counted in cells of equal width in the logit (count_cells), and the
+// counts tell in which cell top-k ends, and between which cells top_p ends.  Where no more
+// tokens are left than the workgroup has threads, they are gathered in the order of their
+// indices, one a thread, and compared only within the cell or bucket in which a cut falls.
+// Where more are left, the masses of all are summed once, those near top_p's border in
+// separate parts (cut_once).  What either cannot decide (a border in a cell of more than kList
+// tokens) is left to buckets of masses and, at the last, a radix descent over the tokens'
+// order-preserving keys (cut).
+//
+// What bounds it.  A row belongs to one CU, whose fp64 rate is the floor of a pass over masses
+// (21 instructions a token, 4.9 cycles each: 50304 tokens 9 us); the rest is fetching code that
+// runs once and barriers.  One row of 50304 bf16: 19 us without cuts, 23 with top_k 50, 34 with
+// top_p 0.9 (of these: 5 to load, 7 for counts and bounds, 14 for the masses, 9 for the border,
+// 6 for the token).  256 rows, one a CU, take what the slowest takes: 45 us.  512 x 50304 fp32
+// without cuts: 103 MB, 20 us to read, 44 us.
 
 #include <type_traits>
 
@@ -993,10 +1004,12 @@ void launch(const SampleArgs &a, hipStream_t s) {
     hipLaunchKernelGGL((sample_kernel<DT, WAVES, STAGED>), dim3(a.n), dim3(WAVES * kWave), 0, s, a);
 }
 
-// Up to 4096 tokens take 4 waves, more 16.  Rows go through LDS where they fit (131072 bytes)
-// and each has a CU to itself; with more rows than CUs, two smaller workgroups on each hide
-// one's memory behind the other's arithmetic (512 x 50304 fp32: 49 us, one workgroup at a
-// time 55).
+// Up to 4096 tokens take 4 waves, more 16: 256 x 4000 bf16 without cuts 7.2 us (16 waves 10.1),
+// top_k 10.3 (11.3), top_p 16.4 (16.3); one row fp32 6.9 (8.2), 10.2 (9.2), 14.8 (13.2).  Rows go
+// through LDS where they fit (131072 bytes) and each has a CU to itself: 64 x 50304 bf16 20, 23
+// and 42 us (8 waves without LDS 21, 28, 46).  With more rows than CUs, two smaller workgroups
+// on each hide one's memory behind the other's arithmetic: 512 x 50304 bf16 35, 42 and 71 us
+// (one of 16 waves at a time 44, 47, 86), fp32 42, 61 and 79 (49, 70, 101).
 template <int DT>
 void run(const SampleArgs &a, hipStream_t s) {
     constexpr int kLds = 8, kChunk = kWave * (DT == PRIME_F32 ? 4 : 8);
