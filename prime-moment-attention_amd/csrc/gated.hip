@@ -19,8 +19,8 @@
 // What bounds it.  A token is read once and written once: 8 x 8192 x 768 bf16 is 403 MB, 79
 // us at the 5.1 TB/s of a large copy; its 46 vector instructions, five of them at a quarter of
 // the rate, take as long again.  Together 104 us (3.9 TB/s); 65536 x 512 fp32, twice the bytes
-// a token, 106 us (5.1 TB/s).  The backward, 32 x 2048 x 768 bf16: 704 MB with the checkpoints,
-// 138 us, takes 155-165.  Tried before the last steps, in us for that bf16 forward, that fp32
+// a token, 106 us (5.1 TB/s).  The backward, 32 x 2048 x 768 bf16: 717 MB with the checkpoints,
+// 141 us, takes 157-164.  Tried before the last steps, in us for that bf16 forward, that fp32
 // one and the backward, then 112, 113 and 174: 4 waves a span 116, 138, 181; 16 waves 125, 106,
 // 179; tiles of 8 tokens 161, 128, 187; a state published every 32nd span 123, 117, 171.
 //
