@@ -1,5 +1,7 @@
 """Plain float64 forms of the gated linear recurrence, of Philox4x32-10 dropout and of
 the sampled token, for the tests (not collected: no test_ prefix)."""
+import math
+
 import numpy as np
 import torch
 
@@ -63,6 +65,10 @@ def sample_row(row, u, T=1.0, top_k=0, top_p=1.0, min_p=0.0):
         before = np.concatenate([[0.0], np.cumsum(w)[:-1]])
         n = max(1, int((before < top_p * w.sum()).sum()))
         order, w = order[:n], w[:n]
-    kept = np.sort(order[w >= min(max(min_p, 0.0), 1.0)])
+    if min_p > 0:  # in exponents: next to a weight of 1, exp itself rounds to 1
+        with np.errstate(invalid="ignore"):
+            e = np.where(row[order] == top, 0.0, np.nan_to_num((row[order] - top) / T, nan=-np.inf))
+        order = order[e >= math.log(min(min_p, 1.0))]
+    kept = np.sort(order)
     mass = np.cumsum(weigh(kept))
     return int(kept[min(np.searchsorted(mass, u * mass[-1], side="right"), len(kept) - 1)])

@@ -278,6 +278,18 @@ def test_mass_estimates_that_are_off(V):
         check(logits, u, top_p=np.linspace(0.02, 0.9999, n), min_p=0.01)
 
 
+@pytest.mark.parametrize("T", [1e-38, 1e-6, 1e6, 3e38, INF])
+@pytest.mark.parametrize("V", [300, 5003, 50304])
+def test_ends_of_the_temperature(V, T):
+    logits, u = make(8, V, F32, 5)
+    logits[1, ::3] = -INF
+    logits[2, ::5] = float("nan")
+    logits[3] *= 1e37
+    for kw in ({}, {"top_k": 40}, {"top_k": 2000}, {"top_p": 0.7}, {"min_p": 0.5}, {"min_p": 1.0},
+               {"top_k": 100, "top_p": 0.9, "min_p": 0.1}):
+        check(logits, u, temperature=T, **kw)
+
+
 def test_two_streams_at_once():
     logits, u = make(8, 50304, BF16, 16)
     logits, u = logits.to(dev()), u.to(dev())
