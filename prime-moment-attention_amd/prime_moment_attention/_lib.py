@@ -1139,6 +1139,18 @@ def _views_ok(x, *views) -> bool:
 
 def check_gated(x, step, gate, tau, state, state_out) -> Tuple[int, int, int]:
     """(B, L, C) of the gated recurrence's operands, or the error that they have."""
+    sh, dt, d, f32 = x.shape, x.dtype, x.get_device(), torch.float32
+    if (len(sh) == 3 and dt in _DTYPES and step.shape == sh and gate.shape == sh and step.dtype is dt
+            and gate.dtype is dt and x.stride(2) == step.stride(2) == gate.stride(2) == 1 and tau.dtype is f32
+            and tau.shape == sh[2:] and tau.is_contiguous()
+            and d >= 0 and step.get_device() == gate.get_device() == tau.get_device() == d):
+        for t in (state, state_out):
+            if t is not None and not (t.dtype is f32 and t.shape == (sh[0], sh[2]) and t.is_contiguous()
+                                      and t.get_device() == d):
+                break
+        else:
+            return sh
+    # some operand is not as it has to be (or one channel, or none)
     if x.dim() != 3:
         raise ValueError(f"x has shape {tuple(x.shape)}, expected [B, L, C]")
     if x.dtype not in _DTYPES:

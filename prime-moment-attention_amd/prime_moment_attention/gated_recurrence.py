@@ -87,13 +87,15 @@ def _scan(x, step, gate, tau, state, state_out):
         if state_out is not None:
             return torch.zeros_like(parts[0]), state_out.copy_(h)
         return torch.zeros_like(parts[0]) + 0 * (parts[1] + parts[2]), h + 0
-    if needs_grad(x, step, gate, tau, state) or forward_ad._current_level >= 0:
+    leaves = x.requires_grad or tau.requires_grad or (step is not None and (step.requires_grad or gate.requires_grad)) or (
+        state is not None and state.requires_grad)
+    if (leaves and torch.is_grad_enabled()) or forward_ad._current_level >= 0:
         if state_out is not None:
             raise ValueError("state_out cannot be written while autograd records: take the returned state")
         return _GatedScanFn.apply(x, step, gate, tau, state)
     y = x.new_empty((B, L, C))
     if state_out is None:
-        state_out = tau.new_empty((B, C))
+        state_out = tau.new_empty((B, C)) if state is None else torch.empty_like(state)
     _lib.gated_scan(*parts, tau, state, y, state_out, checked=True)
     return y, state_out
 
