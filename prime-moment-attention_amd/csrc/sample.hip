@@ -117,11 +117,12 @@ __device__ __forceinline__ uint64_t shfl_u64(uint64_t v, int lane) {
     return static_cast<uint64_t>(__shfl(static_cast<uint32_t>(v >> 32), lane, kWave)) << 32 |
            __shfl(static_cast<uint32_t>(v), lane, kWave);
 }
-// v of lane 63
-__device__ __forceinline__ uint64_t last_lane(uint64_t v) {
-    return static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), 63)) << 32 |
-           static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
+// v of one lane, the same for all
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int lane) {
+    return static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane)) << 32 |
+           static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
 }
+__device__ __forceinline__ uint64_t last_lane(uint64_t v) { return lane_u64(v, kWave - 1); }
 template <int CTRL, int ROWS>
 __device__ __forceinline__ uint64_t dpp_u64(uint64_t v) {  // 0 where the move has no source
     const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false);
@@ -839,6 +840,31 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
                 at += chunk;
             });
             __syncthreads();
+            // One wave can do without barriers (8 x 32000 fp32, top_k 50: 17.0 -> 15.9 us; with top_p
+            // behind it 18.8 -> 19.2, so not there)
+            if (all <= kWave && !(top_p < 1.f)) {
+                if (wave) return;
+                const int number = static_cast<int>(all);
+                const bool mine = lane < number;
+                const float x = mine ? sh.list_x[lane] : -kInf;
+                const double t = rs.exponent(mine ? x : top);
+                uint64_t w = RowScale::select(mine && rs.place(x) < static_cast<float>(kBuckets - 1), RowScale::mass_of(t));
+                if (by_count && !exact) {
+                    int c;
+                    const bool in = rs.cell(x, c) && c == bounds.high;
+                    int rank = bounds.above;
+                    for (uint64_t set = __ballot(in); set; set &= set - 1) {
+                        const int j = __builtin_ctzll(set);
+                        const float y = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), j));
+                        rank += (y > x) | ((y == x) & (j < lane));
+                    }
+                    w = RowScale::select(!in || rank < top_k, w);
+                }
+                w = RowScale::select(t >= rs.least, w);
+                const uint64_t to = wave_scan_u64(w), target = target_of(last_lane(to));
+                if (to <= target + w && target < to && w) a.out[r] = list_i[lane];
+                return;
+            }
             const bool mine = tid < static_cast<int>(all);
             const float x = mine ? sh.list_x[tid] : -kInf;
             const int index = mine ? list_i[tid] : 0;
