@@ -149,7 +149,7 @@ struct SampleShared {
     uint64_t part[WAVES];
     uint64_t sum, rest;
     float last;
-    int bucket, n, index, owner, low, high;
+    int bucket, n, index, owner, low, high, found;
     uint8_t list_wave[kList];
 };
 
@@ -464,7 +464,7 @@ __device__ __forceinline__ bool count_cells(SampleShared<WAVES> &sh, const Sampl
     uint32_t *counts = reinterpret_cast<uint32_t *>(sh.hist);
     __syncthreads();
     for (int b = threadIdx.x; b < kCells; b += WAVES * kWave) counts[b] = 0;
-    if (threadIdx.x == 0) sh.low = 0, sh.high = kCells - 1, sh.n = 1 << 30;
+    if (threadIdx.x == 0) sh.low = 0, sh.high = kCells - 1, sh.n = 1 << 30, sh.found = 0;
     __syncthreads();
     row.each([&](int, const float (&x)[VE]) {
 #pragma unroll
@@ -807,20 +807,45 @@ __global__ __launch_bounds__(WAVES *kWave) void sample_kernel(const SampleArgs a
 #pragma unroll
             for (int j = 0; j < VE; ++j) x[j] = x[j] == last && row.index(i) + j > last_tie ? -kInf : x[j];
         };
-        uint64_t n = 0, sum = 0, first, all;
-        row.each([&](int i, float (&x)[VE]) {
-            drop_ties(i, x);
+        uint64_t n = 0, sum = 0, first = 0, all;
+        int *list_i = reinterpret_cast<int *>(sh.list_w);
+        // Up to 64 are gathered as they come and put in order by one wave, which saves the pass that
+        // counts them (top_k 50, 8 x 32000 fp32: 15.8 -> 13.9 us, 64 x 50304 bf16 21.7 -> 17.9; a pass
+        // over 4096 tokens costs less than the ordering, 1 x 4000 9.7 -> 10.6).
+        const bool few = WAVES > 4 && by_count && !exact && bounds.tokens <= kWave;
+        if (few) {
+            row.each([&](int i, const float (&x)[VE]) {
+                if (!stays(largest(x))) return;
 #pragma unroll
-            for (int j = 0; j < VE; ++j) n += stays(x[j]);
-            if (by_mass) sum += masses(x);
-        });
-        block_scan(sh, n, first, all);
-        if (by_mass) block_scan(sh, sum, waves, all_mass);
+                for (int j = 0; j < VE; ++j) {
+                    if (!stays(x[j])) continue;
+                    const int k = atomicAdd(&sh.found, 1);
+                    sh.list_x[k] = x[j], list_i[k] = row.index(i) + j;
+                }
+            });
+            __syncthreads();
+            all = bounds.tokens;
+            if (wave == 0) {
+                const float x = sh.list_x[lane];
+                const int index = list_i[lane];
+                int place = 0;
+                for (int j = 0; j < bounds.tokens; ++j) place += __builtin_amdgcn_readlane(index, j) < index;
+                if (lane < bounds.tokens) sh.list_x[place] = x, list_i[place] = index;
+            }
+        } else {
+            row.each([&](int i, float (&x)[VE]) {
+                drop_ties(i, x);
+#pragma unroll
+                for (int j = 0; j < VE; ++j) n += stays(x[j]);
+                if (by_mass) sum += masses(x);
+            });
+            block_scan(sh, n, first, all);
+            if (by_mass) block_scan(sh, sum, waves, all_mass);
+        }
         bool closed = all <= WAVES * kWave;
         if (closed) {
-            int *list_i = reinterpret_cast<int *>(sh.list_w);
             int at = static_cast<int>(first);
-            row.each([&](int i, float (&x)[VE]) {
+            if (!few) row.each([&](int i, float (&x)[VE]) {
                 if (!__any(stays(largest(x)))) return;
                 drop_ties(i, x);
                 int chunk = 0, place = at;
