@@ -14,7 +14,8 @@
 // never sorted: tokens are counted in cells of equal width in the logit (count_cells), and the
 // counts tell in which cell top-k ends, and between which cells top_p ends.  Where no more
 // tokens are left than the workgroup has threads, they are gathered in the order of their
-// indices, one a thread, and compared only within the cell or bucket in which a cut falls.
+// indices, one a thread, and compared only within the cell or bucket in which a cut falls
+// (equal tokens that top-k cuts away past that number are found by their indices before).
 // Where more are left, the masses of all are summed once, those near top_p's border in
 // separate parts (cut_once).  What either cannot decide (a border in a cell of more than kList
 // tokens) is left to buckets of masses and, at the last, a radix descent over the tokens'
@@ -22,7 +23,7 @@
 //
 // What bounds it.  A row belongs to one CU, whose fp64 rate is the floor of a pass over masses
 // (21 instructions a token, 4.9 cycles each: 50304 tokens 9 us); the rest is fetching code that
-// runs once and barriers.  One row of 50304 bf16: 19 us without cuts, 23 with top_k 50, 34 with
+// runs once and barriers.  One row of 50304 bf16: 19 us without cuts, 17 with top_k 50, 34 with
 // top_p 0.9 (of these: 5 to load, 7 for counts and bounds, 14 for the masses, 9 for the border,
 // 6 for the token).  256 rows, one a CU, take what the slowest takes: 45 us.  512 x 50304 fp32
 // without cuts: 103 MB, 20 us to read, 44 us.
@@ -1055,12 +1056,12 @@ void launch(const SampleArgs &a, hipStream_t s) {
     hipLaunchKernelGGL((sample_kernel<DT, WAVES, STAGED>), dim3(a.n), dim3(WAVES * kWave), 0, s, a);
 }
 
-// Up to 4096 tokens take 4 waves, more 16: 256 x 4000 bf16 without cuts 7.2 us (16 waves 10.1),
-// top_k 10.3 (11.3), top_p 16.4 (16.3); one row fp32 6.9 (8.2), 10.2 (9.2), 14.8 (13.2).  Rows go
-// through LDS where they fit (131072 bytes) and each has a CU to itself: 64 x 50304 bf16 20, 23
-// and 42 us (8 waves without LDS 21, 28, 46).  With more rows than CUs, two smaller workgroups
-// on each hide one's memory behind the other's arithmetic: 512 x 50304 bf16 35, 42 and 71 us
-// (one of 16 waves at a time 44, 47, 86), fp32 42, 61 and 79 (49, 70, 101).
+// Up to 4096 tokens take 4 waves, more 16: 256 x 4000 bf16 without cuts 7.3 us (16 waves 9.9),
+// top_k 50 9.6 (10.3), top_p 0.9 16.5 (17.2); one row fp32 6.9 (8.2), 9.6 (8.3), 14.6 (13.7).  Rows
+// go through LDS where they fit (131072 bytes) and each has a CU to itself: 64 x 50304 bf16 20,
+// 18 and 42 us (8 waves without LDS 21, 22, 47).  With more rows than CUs, two smaller
+// workgroups on each hide one's memory behind the other's arithmetic: 512 x 50304 bf16 36, 33
+// and 71 us (one of 16 waves at a time 45, 38, 86), fp32 42, 49 and 80 (49, 55, 100).
 template <int DT>
 void run(const SampleArgs &a, hipStream_t s) {
     constexpr int kLds = 8, kChunk = kWave * (DT == PRIME_F32 ? 4 : 8);
