@@ -290,6 +290,29 @@ def test_ends_of_the_temperature(V, T):
         check(logits, u, temperature=T, **kw)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("kw", [{}, {"top_k": 60}, {"top_k": 700, "top_p": 0.9}, {"top_p": 0.97}, {"min_p": 0.02}])
+def test_a_row_alone_and_among_many(kw, dtype):
+    """The launches for few and for many rows of a long vocabulary give the same tokens."""
+    logits, u = (t.to(dev()) for t in make(300, 20000, dtype, 31, scale=2.0))
+    a = sample_tokens(logits, u, 1.1, **kw)
+    for i in range(0, 300, 23):
+        assert torch.equal(sample_tokens(logits[i:i + 1], u[i:i + 1], 1.1, **kw), a[i:i + 1])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [16, 272])
+def test_top_k_near_the_lanes(n, dtype):
+    """As many kept tokens as a wave has lanes, ties around that number among them."""
+    logits, u = make(n, 9000, dtype, 33)
+    if dtype is F32:
+        logits = (logits * 8).round() / 8
+    ks = np.resize([1, 2, 60, 62, 63, 64, 65, 66], n)
+    check(logits, u, top_k=ks)
+    check(logits, u, temperature=1.7, top_k=ks, top_p=0.8)
+    check(logits, u, temperature=1.7, top_k=ks, min_p=0.05)
+
+
 def test_two_streams_at_once():
     logits, u = make(8, 50304, BF16, 16)
     logits, u = logits.to(dev()), u.to(dev())
