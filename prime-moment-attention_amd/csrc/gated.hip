@@ -114,15 +114,18 @@ struct Rows {
     int64_t step;
     __device__ __forceinline__ Rows(const GatedView &v, int es, int b, int l)
         : row(static_cast<char *>(v.data) + (b * v.sb + l * v.sl) * es), step(v.sl * es) {}
-    // (nontemporal: each element is used once, by one wave; 8 x 8192 x 768 bf16 took 110 us
-    // with plain accesses, now 104, the backward at 32 x 2048 x 768 166 us, now 159)
-    template <typename P>
+    // PAST: past the caches, each element being used once
+    template <typename P, bool PAST>
     __device__ __forceinline__ P load(uint32_t offset) const {
-        return __builtin_nontemporal_load(reinterpret_cast<const P *>(row + offset));
+        const P *p = reinterpret_cast<const P *>(row + offset);
+        if constexpr (PAST) return __builtin_nontemporal_load(p);
+        else return *p;
     }
-    template <typename P>
-    __device__ __forceinline__ void store(uint32_t offset, P p) const {
-        __builtin_nontemporal_store(p, reinterpret_cast<P *>(row + offset));
+    template <bool PAST, typename P>
+    __device__ __forceinline__ void store(uint32_t offset, P v) const {
+        P *p = reinterpret_cast<P *>(row + offset);
+        if constexpr (PAST) __builtin_nontemporal_store(v, p);
+        else *p = v;
     }
     __device__ __forceinline__ void next(bool more = true) { row += more ? step : 0; }
 };
@@ -262,7 +265,7 @@ __device__ __forceinline__ void for_tokens(int n, F f) {
 }
 
 // ------------------------------------------------------------------ forward
-template <int DT>
+template <int DT, bool LINES>
 __global__ __launch_bounds__(kThreads) void gated_scan_kernel(const GatedArgs a) {
     __shared__ SpanShared sh;
     constexpr int T = kGatedTile, es = sizeof(Elem<DT>);
@@ -276,7 +279,7 @@ __global__ __launch_bounds__(kThreads) void gated_scan_kernel(const GatedArgs a)
         P px[T], ps[T], pg[T];
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            px[t] = rx.load<P>(o), ps[t] = rs.load<P>(o), pg[t] = rg.load<P>(o);
+            px[t] = rx.load<P, LINES>(o), ps[t] = rs.load<P, LINES>(o), pg[t] = rg.load<P, LINES>(o);
             const bool more = full || t + 1 < n;
             rx.next(more), rs.next(more), rg.next(more);
             __builtin_amdgcn_sched_barrier(0);  // else all rows' addresses are held at once, and spilled
@@ -304,7 +307,7 @@ __global__ __launch_bounds__(kThreads) void gated_scan_kernel(const GatedArgs a)
         const uint32_t o = here(p.c * es);
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            if (full || t < n) ry.store<P>(o, narrow<DT>(fmaf(prod[t], carry, h[t])));
+            if (full || t < n) ry.store<true>(o, narrow<DT>(fmaf(prod[t], carry, h[t])));
             ry.next();
         }
     });
@@ -364,7 +367,7 @@ __global__ __launch_bounds__(256) void gated_step_kernel(const GatedArgs a) {
 //   dstep = dz d z / d step                          dtau = -sum dz z / tau
 // so a wave takes its states again from its checkpoint, keeps those four numbers a token
 // instead of the inputs, and multiplies once its G is known (125 registers, 4 waves a SIMD).
-template <int DT>
+template <int DT, bool LINES>
 __global__ __launch_bounds__(kThreads, 4) void gated_bwd_kernel(const GatedArgs a) {
     __shared__ SpanShared sh;
     constexpr int T = kGatedTile, es = sizeof(Elem<DT>);
@@ -382,7 +385,7 @@ __global__ __launch_bounds__(kThreads, 4) void gated_bwd_kernel(const GatedArgs 
         float h = a.ckpt[(static_cast<int64_t>(p.b) * a.tiles + l0 / T) * a.C + p.c], pr = 1.f;
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            px[t] = rx.load<P>(o), ps[t] = rs.load<P>(o), pg[t] = rg.load<P>(o), pd[t] = rd.load<P>(o);
+            px[t] = rx.load<P, LINES>(o), ps[t] = rs.load<P, LINES>(o), pg[t] = rg.load<P, LINES>(o), pd[t] = rd.load<P, LINES>(o);
             const bool more = full || t + 1 < n;
             rx.next(more), rs.next(more), rg.next(more), rd.next(more);
             __builtin_amdgcn_sched_barrier(0);
@@ -426,9 +429,9 @@ __global__ __launch_bounds__(kThreads, 4) void gated_bwd_kernel(const GatedArgs 
                 const float Gt = fmaf(prod[t], carry, G[t]);
                 if (full || t < n) {
                     dtau = fmaf(-Gt, cz[t], dtau);
-                    rx.store<P>(o, narrow<DT>(Gt * cx[t]));
-                    rs.store<P>(o, narrow<DT>(Gt * cs[t]));
-                    rg.store<P>(o, narrow<DT>(Gt * cg[t]));
+                    rx.store<LINES>(o, narrow<DT>(Gt * cx[t]));
+                    rs.store<LINES>(o, narrow<DT>(Gt * cs[t]));
+                    rg.store<LINES>(o, narrow<DT>(Gt * cg[t]));
                 }
                 rx.next(), rs.next(), rg.next();
             }
@@ -490,19 +493,38 @@ void fill(const GatedArgs &a, hipStream_t s) {
     hipLaunchKernelGGL(gated_fill_kernel, dim3((n + 255) / 256), dim3(256), 0, s, reinterpret_cast<uint4 *>(a.counter), n);
 }
 
+// Whether every row starts on a 128-byte line.
+bool lines(const GatedArgs &a, bool bwd) {
+    const int es = a.dt == PRIME_F32 ? 4 : 2;
+    auto one = [&](const GatedView &v) {
+        return reinterpret_cast<uintptr_t>(v.data) % 128 == 0 && (a.L == 1 || v.sl * es % 128 == 0) &&
+               (a.B == 1 || v.sb * es % 128 == 0);
+    };
+    return one(a.x) && one(a.step) && one(a.gate) && (bwd ? one(a.dy) && one(a.dx) && one(a.dstep) && one(a.dgate) : one(a.y));
+}
+
+template <int DT, bool LINES>
+void run_spans(const GatedArgs &a, bool bwd, hipStream_t s) {
+    fill(a, s);
+    if (bwd) hipLaunchKernelGGL((gated_bwd_kernel<DT, LINES>), dim3(spans_grid(a)), dim3(kThreads), 0, s, a);
+    else hipLaunchKernelGGL((gated_scan_kernel<DT, LINES>), dim3(spans_grid(a)), dim3(kThreads), 0, s, a);
+}
+
+// Accesses go past the caches where every row starts on a line: 8 x 8192 x 768 bf16 took 110 us
+// with plain ones, 104 so, the backward at 32 x 2048 x 768 166, 159.  Else neighbouring channel
+// groups share lines, which the caches then put together: 8 x 8192 x 1000 bf16 203 us past them,
+// 168 through them, the backward 427, 291; fp32 287, 246 and 553, 474; 501 channels bf16 114, 85
+// and 235, 162.  (The forward's stores go past them in either case: up to 5 us less.)
 template <int DT>
 void run(const GatedArgs &a, bool bwd, hipStream_t s) {
-    if (bwd) {
-        fill(a, s);
-        hipLaunchKernelGGL(gated_bwd_kernel<DT>, dim3(spans_grid(a)), dim3(kThreads), 0, s, a);
-        hipLaunchKernelGGL(gated_dtau_kernel, dim3((a.C + kWave - 1) / kWave), dim3(1024), 0, s, a);
-    } else if (walks(a)) {
+    if (!bwd && walks(a)) {
         const int block = a.C >= 256 ? 256 : (a.C + kWave - 1) / kWave * kWave;
         hipLaunchKernelGGL(gated_step_kernel<DT>, dim3(a.B * ((a.C + block - 1) / block)), dim3(block), 0, s, a);
-    } else {
-        fill(a, s);
-        hipLaunchKernelGGL(gated_scan_kernel<DT>, dim3(spans_grid(a)), dim3(kThreads), 0, s, a);
+        return;
     }
+    if (lines(a, bwd)) run_spans<DT, true>(a, bwd, s);
+    else run_spans<DT, false>(a, bwd, s);
+    if (bwd) hipLaunchKernelGGL(gated_dtau_kernel, dim3((a.C + kWave - 1) / kWave), dim3(1024), 0, s, a);
 }
 
 }  // namespace
