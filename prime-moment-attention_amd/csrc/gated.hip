@@ -24,9 +24,11 @@
 // one and the backward, then 112, 113 and 174: 4 waves a span 116, 138, 181; 16 waves 125, 106,
 // 179; tiles of 8 tokens 161, 128, 187; a state published every 32nd span 123, 117, 171.
 //
-// a is carried as a - 1 = expm1(-z): next to 1 (long memories) a itself has
-// lost the decay's low bits, and with it the error of h grows by 2^-25 times
-// the memory's length in tokens.  1 - a^2 = -(a - 1)(2 + (a - 1)) loses nothing.
+// A decay is held in one of two forms.  Next to 1 (long memories) a itself has lost the low bits
+// of 1 - a, and with it the error of h grows by 2^-25 times the memory's length in tokens:
+// there it is a - 1 = expm1(-z), and h + ((a - 1) h + b).  Far from 1 that sum rounds b at the
+// spacing of the h that is to be forgotten (h = 1e7 and a = e^-25 leave nothing of b = 0.3):
+// there it is a, and a h + b.  So a token is off by roundings of |a h| + |b| in either form.
 
 #include <type_traits>
 
@@ -40,16 +42,29 @@ constexpr int kWaves = 8, kThreads = kWaves * kWave, kSpan = kWaves * kGatedTile
 constexpr int kChain = 16;
 
 // ------------------------------------------------------------------- gates
-// z in binary logarithms (z = D log2(e) / tau, a = 2^-z): a - 1, the Taylor polynomial below
-// 1/16 (next term 3e-8 of the value), else exp2 (its rounding is 2^-24 / (ln(2) / 16) of the value at most).
-__device__ __forceinline__ float decay_m1(float z) {
+// z in binary logarithms: z = D log2(e) / tau, a = 2^-z.  1 - a below 1/16, its Taylor
+// polynomial (next term 3e-8 of the value).
+constexpr float kNear = 0.0625f;
+__device__ __forceinline__ float loss(float z) {
     constexpr float l = 0.693147180559945f;
     float p = fmaf(-l * l * l * l / 24.f, z, l * l * l / 6.f);
     p = fmaf(p, z, -l * l / 2.f);
     p = fmaf(p, z, l);
-    const float far = __builtin_amdgcn_exp2f(-z) - 1.f;
-    return z < 0.0625f ? -z * p : far;
+    return z * p;
 }
+
+// A decay's number m: a - 1 (negative or -0) where it is near 1, else a (positive or +0).
+__device__ __forceinline__ bool near_one(float m) { return __float_as_int(m) < 0; }
+
+// of a run of tokens: exp2 - 1 is exact up to z = 1
+__device__ __forceinline__ float decay(float z) {
+    const float e = __builtin_amdgcn_exp2f(-z);
+    return z < kNear ? -loss(z) : z <= 1.f ? e - 1.f : e;
+}
+
+// a h + b, and a h, for a token
+__device__ __forceinline__ float step_on(float h, bool near, float m, float b) { return (near ? h : 0.f) + fmaf(m, h, b); }
+__device__ __forceinline__ float decayed(float h, bool near, float m) { return fmaf(m, h, near ? h : 0.f); }
 
 // softplus, unclamped, and e = exp(-|s|) for its derivative: max(s, 0) + log(1 + e), with
 // log(1 + e) / e on [0, 1] its Chebyshev interpolant of degree 7 (2.2e-7 off at most), so
@@ -75,21 +90,34 @@ __device__ __forceinline__ float sigmoid(float g) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-g * kLog2e));
 }
 
-// z, a - 1 and b = sqrt(1 - a^2) sigmoid(g) x of one token; rate = log2(e) / tau
-__device__ __forceinline__ void gates(float x, float s, float g, float rate, float &z, float &am1, float &b) {
-    float e;
-    z = clamp_step(softplus(s, e)) * rate;
-    am1 = decay_m1(z);
-    b = __builtin_amdgcn_sqrtf(-am1 * (2.f + am1)) * sigmoid(g) * x;
+// A token's decay, and 1 - a^2: d (2 - d) with d = 1 - a near 1, else 1 - a a (exp2's rounding is
+// 2^-24 / (ln(2) / 16) of it at most).
+__device__ __forceinline__ float token_decay(float z, bool &near, float &m) {
+    const float d = loss(z), a = __builtin_amdgcn_exp2f(-z);
+    near = z < kNear;
+    m = near ? -d : a;
+    return fmaf(-m, m, near ? d + d : 1.f);
 }
 
-// h <- h + (am1 h + b), `lo` keeping what the sum's rounding drops.  Without it a state
-// that hardly changes is rounded the same way every time: h = 3 at z = 5e-8 moves by
+// z, the decay and b = sqrt(1 - a^2) sigmoid(g) x of one token, of none (a = 1, b = 0) without
+// `in`; rate = log2(e) / tau
+__device__ __forceinline__ void gates(bool in, float x, float s, float g, float rate, float &z, bool &near, float &m,
+                                      float &b) {
+    float e;
+    z = clamp_step(softplus(s, e)) * rate;
+    z = in ? z : 0.f;
+    b = __builtin_amdgcn_sqrtf(token_decay(z, near, m)) * sigmoid(g) * x;
+    b = in ? b : 0.f;
+}
+
+// h <- a h + b, `lo` keeping what a decay near 1 would drop of it by rounding.  Without it a
+// state that hardly changes is rounded the same way every time: h = 3 at z = 5e-8 moves by
 // 0.63 of its spacing a token, which rounds to 1, and decays 1.6 times too fast.
-__device__ __forceinline__ void advance(float &h, float &lo, float am1, float b) {
-    const float d = fmaf(am1, h, b) + lo, next = h + d;
-    lo = d - (next - h);
-    h = next;
+__device__ __forceinline__ void advance(float &h, float &lo, float m, float b) {
+    const bool near = near_one(m);
+    const float d = fmaf(m, h, b), dl = d + lo, next = h + dl;
+    lo = near ? dl - (next - h) : 0.f;
+    h = near ? next : d;
 }
 
 // ------------------------------------------------------------------- access
@@ -152,6 +180,12 @@ __device__ __forceinline__ uint64_t peek(const uint64_t *w) {
     return __hip_atomic_load(w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// v computed before what follows: before the wait for a state that others wait for in turn.
+__device__ __forceinline__ float ready(float v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 // What reaches span g (counted from where the recurrence starts): the published end state
 // of the last chain head before it, then the folds between.  The folds are there early and
 // are joined first, so that from one head's state to the next one's is one word's way.
@@ -160,7 +194,7 @@ __device__ __forceinline__ void chain_in(const uint64_t *words, int64_t stride, 
     constexpr int U = 3;  // words in flight; more spill the backward's registers
     const int head = (g - 1) / kChain * kChain, n = g - 1 - head;
     uint64_t first = peek(words + head * stride);
-    float A = 0.f, H = 0.f;
+    float Z = 0.f, H = 0.f;
     for (int j0 = 0; j0 < n; j0 += U) {
         uint64_t w[U];
 #pragma unroll
@@ -173,23 +207,24 @@ __device__ __forceinline__ void chain_in(const uint64_t *words, int64_t stride, 
                 __builtin_amdgcn_s_sleep(1);
                 w[j] = peek(words + (head + 1 + j0 + j) * stride);
             }
-            const float wa = __uint_as_float(static_cast<uint32_t>(w[j] >> 32));
-            A += fmaf(wa, A, wa);
-            H += fmaf(wa, H, __uint_as_float(static_cast<uint32_t>(w[j])));
+            const float z = __uint_as_float(static_cast<uint32_t>(w[j] >> 32)), m = decay(z);
+            Z += z;
+            H = step_on(H, near_one(m), m, __uint_as_float(static_cast<uint32_t>(w[j])));
         }
     }
+    const float m = ready(decay(Z));
     while (first == kEmpty) {
         __builtin_amdgcn_s_sleep(1);
         first = peek(words + head * stride);
     }
     h = __uint_as_float(static_cast<uint32_t>(first));
     lo = __uint_as_float(static_cast<uint32_t>(first >> 32));
-    advance(h, lo, A, H);
+    advance(h, lo, m, H);
 }
 
-// A fold (A, H): the tokens take a state h to h + (A h + H).
+// A fold (z, H): the tokens take a state h to 2^-z h + H.
 struct SpanShared {
-    float A[kWaves][kWave], H[kWaves][kWave];  // the waves' folds
+    float z[kWaves][kWave], m[kWaves][kWave], H[kWaves][kWave];  // the waves' folds, m = decay(z)
     float h[kWave], lo[kWave];                 // what reaches the span
     int span;
 };
@@ -223,22 +258,23 @@ __device__ __forceinline__ Place place(const GatedArgs &a, SpanShared &sh) {
 // of the waves before it in the recurrence's order.  Wave 0 gets what the span needs from the
 // chain and publishes what the chain needs from the span.
 template <bool REVERSE>
-__device__ __forceinline__ void join(const GatedArgs &a, SpanShared &sh, const Place &p, const float *start, float A,
-                                     float H, float &h, float &lo) {
+__device__ __forceinline__ void join(const GatedArgs &a, SpanShared &sh, const Place &p, const float *start, float z,
+                                     float m, float H, float &h, float &lo) {
     const int order = REVERSE ? kWaves - 1 - p.wave : p.wave;
-    sh.A[order][p.lane] = A, sh.H[order][p.lane] = H;
+    sh.z[order][p.lane] = z, sh.m[order][p.lane] = m, sh.H[order][p.lane] = H;
     __syncthreads();
     if (p.wave == 0) {
         uint64_t *words = a.words + static_cast<int64_t>(p.b) * a.G * a.C + p.c, *mine = words + static_cast<int64_t>(p.g) * a.C;
         const bool on = p.g + 1 < a.G && p.in, head = p.g % kChain == 0;
-        float fa = 0.f, fh = 0.f;
+        float fz = 0.f, fh = 0.f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            const float wa = sh.A[w][p.lane];
-            fa += fmaf(wa, fa, wa);
-            fh += fmaf(wa, fh, sh.H[w][p.lane]);
+            const float wm = sh.m[w][p.lane];
+            fz += sh.z[w][p.lane];
+            fh = step_on(fh, near_one(wm), wm, sh.H[w][p.lane]);
         }
-        if (on && !head) publish(mine, fa, fh);
+        const float m = ready(decay(fz));
+        if (on && !head) publish(mine, fz, fh);
         h = lo = 0.f;
         if (p.g == 0) {
             if (start) h = start[static_cast<int64_t>(p.b) * a.C + p.c];
@@ -247,13 +283,13 @@ __device__ __forceinline__ void join(const GatedArgs &a, SpanShared &sh, const P
         }
         sh.h[p.lane] = h, sh.lo[p.lane] = lo;
         if (on && head) {
-            advance(h, lo, fa, fh);
+            advance(h, lo, m, fh);
             publish(mine, lo, h);
         }
     }
     __syncthreads();
     h = sh.h[p.lane], lo = sh.lo[p.lane];
-    for (int w = 0; w < order; ++w) advance(h, lo, sh.A[w][p.lane], sh.H[w][p.lane]);
+    for (int w = 0; w < order; ++w) advance(h, lo, sh.m[w][p.lane], sh.H[w][p.lane]);
 }
 
 // A wave's tokens: all kGatedTile of them (the loops below then have no branch in them),
@@ -288,18 +324,18 @@ __global__ __launch_bounds__(kThreads) void gated_scan_kernel(const GatedArgs a)
         float pr = 1.f;
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            float z, am1, b;
-            gates(widen<DT>(px[t]), widen<DT>(ps[t]), widen<DT>(pg[t]), rate, z, am1, b);
-            if (!full && t >= n) z = am1 = b = 0.f;
-            H += fmaf(am1, H, b);
-            pr = fmaf(pr, am1, pr);
+            float z, m, b;
+            bool near;
+            gates(full || t < n, widen<DT>(px[t]), widen<DT>(ps[t]), widen<DT>(pg[t]), rate, z, near, m, b);
+            H = step_on(H, near, m, b);
+            pr = decayed(pr, near, m);
             zs += z;
             h[t] = H, prod[t] = pr;
         }
     });
-    const float A = decay_m1(zs);
+    const float m = decay(zs);
     float carry, lo;
-    join<false>(a, sh, p, a.state_in, A, H, carry, lo);
+    join<false>(a, sh, p, a.state_in, zs, m, H, carry, lo);
     if (!p.in || left <= 0) return;
     if (a.ckpt) a.ckpt[(static_cast<int64_t>(p.b) * a.tiles + l0 / T) * a.C + p.c] = carry;
     for_tokens(left, [&](auto full, int n) {
@@ -312,7 +348,7 @@ __global__ __launch_bounds__(kThreads) void gated_scan_kernel(const GatedArgs a)
         }
     });
     if (a.state_out && left <= T) {
-        advance(carry, lo, A, H);
+        advance(carry, lo, m, H);
         a.state_out[static_cast<int64_t>(p.b) * a.C + p.c] = carry;
     }
 }
@@ -348,9 +384,10 @@ __global__ __launch_bounds__(256) void gated_step_kernel(const GatedArgs a) {
 #pragma unroll
         for (int t = 0; t < kWalk; ++t) {
             if (l0 + t >= a.L) break;
-            float z, am1, bt;
-            gates(widen<DT>(px[t]), widen<DT>(ps[t]), widen<DT>(pg[t]), rate, z, am1, bt);
-            advance(h, lo, am1, bt);
+            float z, m, bt;
+            bool near;
+            gates(true, widen<DT>(px[t]), widen<DT>(ps[t]), widen<DT>(pg[t]), rate, z, near, m, bt);
+            advance(h, lo, m, bt);
             *ry = narrow<DT>(h);
             ry += a.y.sl;
         }
@@ -394,32 +431,35 @@ __global__ __launch_bounds__(kThreads, 4) void gated_bwd_kernel(const GatedArgs 
         for (int t = 0; t < T; ++t) {
             const float x = widen<DT>(px[t]), s = widen<DT>(ps[t]), d = widen<DT>(pd[t]);
             float e;
-            const float soft = softplus(s, e), step = clamp_step(soft), z = step * rate, am1 = decay_m1(z);
+            const float soft = softplus(s, e), step = clamp_step(soft), z = step * rate;
+            bool near;
+            float m;
+            const float q = token_decay(z, near, m), rq = __builtin_amdgcn_rsqf(q), al = near ? 1.f + m : m;
             const float sp = __builtin_amdgcn_rcpf(1.f + e) * (s < 0.f ? e : 1.f);  // softplus'
-            const float al = 1.f + am1, q = -am1 * (2.f + am1), rq = __builtin_amdgcn_rsqf(q), sg = sigmoid(widen<DT>(pg[t]));
-            const float sn = sg * rq;
+            const float sg = sigmoid(widen<DT>(pg[t])), sn = sg * rq;
             cx[t] = q * sn;
             const float b = cx[t] * x, w = al * fmaf(al * sn, x, -h);
             cg[t] = b - b * sg;
             cs[t] = step == soft ? w * inv_tau * sp : 0.f;
             cz[t] = w * step;
-            h += fmaf(am1, h, b);
+            h = step_on(h, near, m, b);
             const bool in = full || t < n;
             zs += in ? z : 0.f;
-            G[t] = in ? d : 0.f, prod[t] = in ? am1 : 0.f;
+            G[t] = in ? d : 0.f, prod[t] = in ? m : -0.f;
         }
 #pragma unroll
         for (int t = T - 1; t >= 0; --t) {
-            const float am1 = prod[t];
+            const float m = prod[t];
+            const bool near = near_one(m);
             G[t] += R;
             prod[t] = pr;
-            R = fmaf(am1, G[t], G[t]);
-            pr = fmaf(pr, am1, pr);
+            R = decayed(G[t], near, m);
+            pr = decayed(pr, near, m);
         }
     });
     float carry, lo, dtau = 0.f;
-    const float A = decay_m1(zs);
-    join<true>(a, sh, p, a.dstate_out, A, R, carry, lo);
+    const float m = decay(zs);
+    join<true>(a, sh, p, a.dstate_out, zs, m, R, carry, lo);
     if (left > 0 && p.in) {
         for_tokens(left, [&](auto full, int n) {
             Rows rx(a.dx, es, p.b, l0), rs(a.dstep, es, p.b, l0), rg(a.dgate, es, p.b, l0);
@@ -437,17 +477,17 @@ __global__ __launch_bounds__(kThreads, 4) void gated_bwd_kernel(const GatedArgs 
             }
         });
         if (l0 == 0 && a.dstate_in) {
-            advance(carry, lo, A, R);
+            advance(carry, lo, m, R);
             a.dstate_in[static_cast<int64_t>(p.b) * a.C + p.c] = carry;
         }
     }
     // the span's part of dtau = -sum dz D / tau^2, wave by wave
     __syncthreads();
-    sh.A[p.wave][p.lane] = dtau;
+    sh.z[p.wave][p.lane] = dtau;
     __syncthreads();
     if (p.wave || !p.in) return;
     float sum = 0.f;
-    for (int w = 0; w < kWaves; ++w) sum += sh.A[w][p.lane];
+    for (int w = 0; w < kWaves; ++w) sum += sh.z[w][p.lane];
     a.dtau_part[(static_cast<int64_t>(p.b) * a.G + span) * a.C + p.c] = sum * inv_tau * inv_tau;
 }
 
