@@ -86,8 +86,11 @@ __device__ __forceinline__ float clamp_step(float d) {
     return __builtin_elementwise_minimum(__builtin_elementwise_maximum(d, kStepMin), kStepMax);
 }
 
-__device__ __forceinline__ float sigmoid(float g) {
-    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-g * kLog2e));
+// sigmoid, and e = exp(-g): 1 - sigmoid is e sigmoid, which an open gate does not cancel (at
+// g = 12 a subtraction is off by a hundredth of it)
+__device__ __forceinline__ float sigmoid(float g, float &e) {
+    e = __builtin_amdgcn_exp2f(-g * kLog2e);
+    return __builtin_amdgcn_rcpf(1.f + e);
 }
 
 // A token's decay, and 1 - a^2: d (2 - d) with d = 1 - a near 1, else 1 - a a (exp2's rounding is
@@ -103,10 +106,10 @@ __device__ __forceinline__ float token_decay(float z, bool &near, float &m) {
 // `in`; rate = log2(e) / tau
 __device__ __forceinline__ void gates(bool in, float x, float s, float g, float rate, float &z, bool &near, float &m,
                                       float &b) {
-    float e;
+    float e, eg;
     z = clamp_step(softplus(s, e)) * rate;
     z = in ? z : 0.f;
-    b = __builtin_amdgcn_sqrtf(token_decay(z, near, m)) * sigmoid(g) * x;
+    b = __builtin_amdgcn_sqrtf(token_decay(z, near, m)) * sigmoid(g, eg) * x;
     b = in ? b : 0.f;
 }
 
@@ -430,16 +433,16 @@ __global__ __launch_bounds__(kThreads, 4) void gated_bwd_kernel(const GatedArgs 
 #pragma unroll
         for (int t = 0; t < T; ++t) {
             const float x = widen<DT>(px[t]), s = widen<DT>(ps[t]), d = widen<DT>(pd[t]);
-            float e;
+            float e, eg;
             const float soft = softplus(s, e), step = clamp_step(soft), z = step * rate;
             bool near;
             float m;
             const float q = token_decay(z, near, m), rq = __builtin_amdgcn_rsqf(q), al = near ? 1.f + m : m;
             const float sp = __builtin_amdgcn_rcpf(1.f + e) * (s < 0.f ? e : 1.f);  // softplus'
-            const float sg = sigmoid(widen<DT>(pg[t])), sn = sg * rq;
+            const float sg = sigmoid(widen<DT>(pg[t]), eg), sn = sg * rq;
             cx[t] = q * sn;
             const float b = cx[t] * x, w = al * fmaf(al * sn, x, -h);
-            cg[t] = b - b * sg;
+            cg[t] = b * fminf(eg * sg, 1.f);  // (an infinite e times 0 is the 1 of a shut gate)
             cs[t] = step == soft ? w * inv_tau * sp : 0.f;
             cz[t] = w * step;
             h = step_on(h, near, m, b);

@@ -95,3 +95,22 @@ def test_what_comes_after_is_kept(kind, L):
     within(got[1], rg[1], bound, "dstep")
     within(got[3], rg[3].sum((0, 1)), (bound * soft / tau + U * L * rg[3].abs()).sum((0, 1)), "dtau")
     within(got[4], rg[4], a[:, 0] * (eG[:, 0] + K * U * (1 + z[:, 0]) * G[:, 0]), "dstate")
+
+
+def test_open_gates_keep_their_gradient():
+    """dgate = G n x s (1 - s) where 1 - s is far below a rounding of s.  x and dy of one sign,
+    so that G has no cancellation.  1 - s = e s with e = exp(-gate): 2 u |gate| of it from the
+    exponent; G as a state of 40 tokens.  (Float64's own sigmoid loses 1 - s too: the reference is
+    dx x sigmoid(-gate).)"""
+    g = torch.Generator().manual_seed(6)
+    r = lambda *s: torch.rand(*s, generator=g)
+    x, dy, step, tau = 0.5 + r(2, 40, 64), 0.5 + r(2, 40, 64), 4 * r(2, 40, 64) - 2, 2.0 * 1000.0 ** r(64)
+    gate = 8.0 + 12.0 * r(2, 40, 64)
+    gate[0, ::7], gate[1, ::7] = 60.0, -60.0
+    leaves = [t.to(dev()).requires_grad_() for t in (x, step, gate, tau)]
+    got = torch.autograd.grad(gated_recurrence(*leaves)[0], leaves[2], dy.to(dev()))[0]
+    ref = [t.double().requires_grad_() for t in (x, step, gate, tau)]
+    dx, = torch.autograd.grad(gated_forward(*ref)[0], ref[0], dy.double())
+    want = (dx * ref[0] * torch.sigmoid(-ref[2])).detach()
+    off = ((got.double().cpu() - want) / want).abs()
+    assert (off <= U * (64 + 2 * 40 ** 0.5 + 2 * gate.abs())).all(), off.max()
