@@ -532,7 +532,8 @@ int prime_argmax(const void *logits, int dtype, int n, int vocab, int64_t stride
  * in fp32, y rounded once to `dtype` (F32 / BF16 / F16).
  *   x, step, gate, y : [B, L, C] views of one dtype, any batch and token strides,
  *                      contiguous channels; y overlaps none of the inputs
- *   tau              : fp32 [C], positive and finite, in tokens
+ *   tau              : fp32 [C], positive, in tokens; below 1e-30 it acts as 1e-30,
+ *                      above 1e33 as 1e33
  *   state_in, state_out : fp32 [B, C] or NULL; state_out may be state_in
  *   checkpoints      : NULL, or fp32 [B, ceil(L / 16), C] that receives the state
  *                      before every 16th token, for the backward

@@ -86,6 +86,12 @@ __device__ __forceinline__ float clamp_step(float d) {
     return __builtin_elementwise_minimum(__builtin_elementwise_maximum(d, kStepMin), kStepMax);
 }
 
+// tau between 1e-30 and 1e33: past them 1 / tau, or 1 - a^2 >= 2e-4 / tau, is no normal number and
+// a gradient the product of 0 and infinity.
+__device__ __forceinline__ float held(float tau) {
+    return __builtin_elementwise_minimum(__builtin_elementwise_maximum(tau, 1e-30f), 1e33f);
+}
+
 // sigmoid, and e = exp(-g): 1 - sigmoid is e sigmoid, which an open gate does not cancel (at
 // g = 12 a subtraction is off by a hundredth of it)
 __device__ __forceinline__ float sigmoid(float g, float &e) {
@@ -323,7 +329,7 @@ __global__ __launch_bounds__(kThreads) void gated_scan_kernel(const GatedArgs a)
             rx.next(more), rs.next(more), rg.next(more);
             __builtin_amdgcn_sched_barrier(0);  // else all rows' addresses are held at once, and spilled
         }
-        const float rate = kLog2e / a.tau[p.c];
+        const float rate = kLog2e / held(a.tau[p.c]);
         float pr = 1.f;
 #pragma unroll
         for (int t = 0; t < T; ++t) {
@@ -373,7 +379,7 @@ __global__ __launch_bounds__(256) void gated_step_kernel(const GatedArgs a) {
     const int64_t row = static_cast<int64_t>(b) * a.C + c;
     const P *rx = elem<P>(a.x, b, c), *rs = elem<P>(a.step, b, c), *rg = elem<P>(a.gate, b, c);
     P *ry = elem<P>(a.y, b, c);
-    const float rate = kLog2e / a.tau[c];
+    const float rate = kLog2e / held(a.tau[c]);
     float h = a.state_in ? a.state_in[row] : 0.f, lo = 0.f;
     for (int l0 = 0; l0 < a.L; l0 += kWalk) {
         if (a.ckpt && l0 % kGatedTile == 0) a.ckpt[(static_cast<int64_t>(b) * a.tiles + l0 / kGatedTile) * a.C + c] = h;
@@ -414,7 +420,7 @@ __global__ __launch_bounds__(kThreads, 4) void gated_bwd_kernel(const GatedArgs 
     using P = Elem<DT>;
     const Place p = place(a, sh);
     const int span = a.G - 1 - p.g, l0 = span * kSpan + p.wave * T, left = a.L - l0;
-    const float inv_tau = 1.f / a.tau[p.c], rate = inv_tau * kLog2e;
+    const float inv_tau = 1.f / held(a.tau[p.c]), rate = inv_tau * kLog2e;
     float cx[T], cg[T], cs[T], cz[T];  // what G is multiplied by for dx, dgate, dstep, -dtau tau^2
     float G[T], prod[T];               // G from r = 0 behind the wave; the product of the a behind a token
     float zs = 0.f, R = 0.f;

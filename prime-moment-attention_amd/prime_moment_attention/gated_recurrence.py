@@ -104,8 +104,8 @@ def gated_recurrence(x: torch.Tensor, step: torch.Tensor, gate: torch.Tensor, ta
                      state: Optional[torch.Tensor] = None, return_state: bool = False,
                      state_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """The recurrence over x, step, gate [B, L, C] (fp32, bf16 or fp16 alike; any batch
-    and token strides) with tau fp32 [C], positive and finite, and state fp32 [B, C] or
-    None (zero): (y [B, L, C] of x's dtype, last state fp32 [B, C] or None without
+    and token strides) with tau fp32 [C], positive (below 1e-30 and above 1e33 it acts as
+    these), and state fp32 [B, C] or None (zero): (y [B, L, C] of x's dtype, last state fp32 [B, C] or None without
     return_state).  Every token counts: the last state of a padded sequence has taken its
     padding in.
 

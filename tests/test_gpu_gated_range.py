@@ -114,3 +114,27 @@ def test_open_gates_keep_their_gradient():
     want = (dx * ref[0] * torch.sigmoid(-ref[2])).detach()
     off = ((got.double().cpu() - want) / want).abs()
     assert (off <= U * (64 + 2 * 40 ** 0.5 + 2 * gate.abs())).all(), off.max()
+
+
+@pytest.mark.parametrize("L", [1, 5, 200])
+def test_the_ends_of_tau(L):
+    """tau below 1e-30 forgets everything at once (no gradient but in x and gate), tau above
+    1e30 nothing, and takes in next to nothing: no infinity comes of either, and no NaN."""
+    g = torch.Generator().manual_seed(7)
+    r = lambda *s: torch.randn(*s, generator=g)
+    tau = torch.tensor([1e-45, 1e-39, 1.2e-38, 1e-31, 1e-29, 1e-20, 1e20, 1e29, 1e33, 1e36, 1e38, 3.4e38])
+    C = tau.numel()
+    x, step, gate, dy, state, dlast = r(2, L, C), r(2, L, C), r(2, L, C), r(2, L, C), r(2, C), r(2, C)
+    step[:, ::3] = -20.0
+    leaves = [t.to(dev()).requires_grad_() for t in (x, step, gate, tau, state)]
+    y, last = gated_recurrence(*leaves, return_state=True)
+    got = [t.double().cpu() for t in torch.autograd.grad([y, last], leaves, [dy.to(dev()), dlast.to(dev())])]
+    ref = [t.double().requires_grad_() for t in (x, step, gate, tau, state)]
+    ry, rlast = gated_forward(*ref)
+    want = torch.autograd.grad([ry, rlast], ref, [dy.double(), dlast.double()])
+    for a, b, n in zip([y, last, *got], [ry, rlast, *want], ["y", "last", "dx", "dstep", "dgate", "dtau", "dstate"]):
+        a, b = a.detach().double().cpu(), b.detach()
+        assert torch.isfinite(a).all(), n
+        # n = sqrt(2 D / tau) is below 1e-14 for the large ones: within that of the reference, and of
+        # a first-order bound elsewhere
+        assert (a - b).abs().max() <= 1e-13 + (64 + 2 * L ** 0.5) * 2 * U * b.abs().max(), n
