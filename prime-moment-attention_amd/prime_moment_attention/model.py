@@ -225,7 +225,7 @@ class PrimeForCausalLM(nn.Module):
                                           device: Any = "cpu") -> "PrimeForCausalLM":
         """Identity-preserving warm start of a selective model from a base PRIME
         checkpoint (model.py:269-310): every pretrained tensor (embeddings,
-        projections, norms, MLP, lm_head) is kept; the selective parameters the
+        projections, norms, MLP, lm_head, gated layers) is kept; the selective parameters the
         checkpoint lacks keep their initialisation (init_selective_weights:
         zero step weights and a step bias that reproduces the base decay, so
         the warm-started model computes the base model at step 0).
@@ -240,16 +240,27 @@ class PrimeForCausalLM(nn.Module):
         if base is None:
             raise ValueError(f"Checkpoint at {checkpoint_path} has no saved config.")
         get = (lambda k, d=None: base.get(k, d)) if isinstance(base, dict) else (lambda k, d=None: getattr(base, k, d))
+        tau_range, held = {}, None
+        if get("gated_layers", ()):
+            # the gated layers keep the range of their tau, widened where the decay of the moment
+            # layers, from now on a tau of that range too, lies outside it
+            held = get("min_tau", 2.0), get("max_tau", 2000.0)
+            base_tau = -1.0 / math.log(max(1e-5, min(0.9999, get("decay"))))
+            tau_range = {"min_tau": min(held[0], base_tau), "max_tau": max(held[1], base_tau)}
         sel_config = PrimeConfig(
             vocab_size=get("vocab_size"), hidden_size=get("hidden_size"), num_layers=get("num_layers"),
             num_heads=get("num_heads"), head_dim=get("head_dim"), num_kv_heads=get("num_kv_heads"),
             intermediate_size=get("intermediate_size"), decay=get("decay"), use_qk_norm=get("use_qk_norm"),
             rms_norm_eps=get("rms_norm_eps"), eps=get("eps"), tie_word_embeddings=get("tie_word_embeddings"),
             initializer_range=get("initializer_range"), use_selective=True, mlp_type=get("mlp_type", "swiglu"),
-            dropout=get("dropout", 0.0), gated_layers=get("gated_layers", ()))
+            dropout=get("dropout", 0.0), gated_layers=get("gated_layers", ()), **tau_range)
         model = cls(sel_config).to(device)
         sd = ckpt["model_state_dict"]
         missing_keys, unexpected_keys = model.load_state_dict(sd, strict=False)
+        if held is not None and held != (sel_config.min_tau, sel_config.max_tau):
+            with torch.no_grad():  # what the narrower range held at its ends stays there
+                for i in sel_config.gated_layers:
+                    model.layers[i].self_attn.log_tau.clamp_(math.log(held[0]), math.log(held[1]))
         print(f"[Selective Warm-Start] Loaded {len(sd)} pretrained tensors from {checkpoint_path}")
         print(f"    Missing keys initialized to identity: {len(missing_keys)}")
         print(f"    Unexpected keys: {len(unexpected_keys)}")

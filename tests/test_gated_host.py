@@ -1,0 +1,37 @@
+"""CPU tests of the gated layers' host side: the warm start of a model that has some."""
+import dataclasses
+
+import pytest
+import torch
+
+from prime_moment_attention import PrimeConfig, PrimeForCausalLM
+
+
+@pytest.mark.parametrize("min_tau,max_tau,decay", [(1.0, 8000.0, 0.99), (2.0, 2000.0, 0.99), (3.0, 50.0, 0.995),
+                                                   (200.0, 900.0, 0.9)])
+@pytest.mark.parametrize("config_as_dict", [False, True])
+def test_warm_start_keeps_the_gated_layers(tmp_path, min_tau, max_tau, decay, config_as_dict):
+    """The same tau as the base's in every channel, those that training has moved past the ends
+    too (off by the rounding of log and exp where the range had to be widened), and selective
+    layers that begin with the base's decay though its tau lies outside that range."""
+    cfg = PrimeConfig(vocab_size=96, hidden_size=128, num_layers=3, num_heads=2, head_dim=64, decay=decay,
+                      min_tau=min_tau, max_tau=max_tau, gated_layers=(0, 2))
+    torch.manual_seed(0)
+    base = PrimeForCausalLM(cfg)
+    with torch.no_grad():
+        base.layers[2].self_attn.log_tau.add_(torch.randn(128))
+    path = tmp_path / "base.pt"
+    torch.save({"config": dataclasses.asdict(cfg) if config_as_dict else cfg,
+                "model_state_dict": base.state_dict()}, path)
+    sel = PrimeForCausalLM.from_pretrained_base_to_selective(str(path))
+    cpu = torch.device("cpu")
+    for i in (0, 2):
+        a, b = base.layers[i].self_attn, sel.layers[i].self_attn
+        assert torch.equal(a.in_proj.weight, b.in_proj.weight) and torch.equal(a.in_proj.bias, b.in_proj.bias)
+        # log(2000) = 7.6 rounded to fp32: 2^-22 of tau
+        assert torch.allclose(a.get_tau(cpu), b.get_tau(cpu), rtol=2.0 ** -21, atol=0)
+        if min_tau < 10 and max_tau > 250:
+            assert torch.equal(a.log_tau, b.log_tau) and (sel.config.min_tau, sel.config.max_tau) == (min_tau, max_tau)
+    at = sel.layers[1].self_attn
+    lam = torch.exp(-torch.nn.functional.softplus(at.delta_proj.bias) / at.get_tau(cpu))
+    assert torch.allclose(lam, torch.full_like(lam, decay), rtol=1e-5)
