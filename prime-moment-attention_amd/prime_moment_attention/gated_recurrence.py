@@ -140,12 +140,16 @@ class GatedLinearRecurrence(nn.Module):
         self.init_gate_weights()
 
     def init_gate_weights(self):
-        """Step size 1 and open-half gates at zero input, memories from min_tau to max_tau."""
+        """Step size 1 and open-half gates at zero input, memories from min_tau to max_tau: a
+        hundred thousandth inside, as fp32's log and exp end up to 4e-6 beyond for any range of
+        floats, where get_tau's clamp gives log_tau no gradient."""
         W = self.width
+        low, high = math.log(self.min_tau), math.log(self.max_tau)
+        inside = min(1e-5, (high - low) / 4)
         with torch.no_grad():
             self.in_proj.bias.zero_()
             self.in_proj.bias[W:2 * W].fill_(math.log(math.exp(1.0) - 1.0))
-            self.log_tau.copy_(torch.linspace(math.log(self.min_tau), math.log(self.max_tau), W))
+            self.log_tau.copy_(torch.linspace(low + inside, high - inside, W))
 
     def get_tau(self, device: torch.device) -> torch.Tensor:
         return torch.clamp(torch.exp(self.log_tau.to(device).float()), min=self.min_tau, max=self.max_tau)

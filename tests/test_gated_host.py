@@ -1,10 +1,11 @@
-"""CPU tests of the gated layers' host side: the warm start of a model that has some."""
+"""CPU tests of the gated layers' host side: what they begin with, and the warm start of a model
+that has some."""
 import dataclasses
 
 import pytest
 import torch
 
-from prime_moment_attention import PrimeConfig, PrimeForCausalLM
+from prime_moment_attention import GatedLinearRecurrence, PrimeConfig, PrimeForCausalLM
 
 
 @pytest.mark.parametrize("min_tau,max_tau,decay", [(1.0, 8000.0, 0.99), (2.0, 2000.0, 0.99), (3.0, 50.0, 0.995),
@@ -35,3 +36,19 @@ def test_warm_start_keeps_the_gated_layers(tmp_path, min_tau, max_tau, decay, co
     at = sel.layers[1].self_attn
     lam = torch.exp(-torch.nn.functional.softplus(at.delta_proj.bias) / at.get_tau(cpu))
     assert torch.allclose(lam, torch.full_like(lam, decay), rtol=1e-5)
+
+
+@pytest.mark.parametrize("width", [1, 2, 64, 1000])
+@pytest.mark.parametrize("min_tau,max_tau", [(2.0, 2000.0), (4.0, 1000.0), (2.0, 500.0), (3.0, 3000.0), (1.0, 4096.0),
+                                             (0.3, 0.7), (1e-20, 1e30)])
+def test_every_tau_begins_with_a_gradient(width, min_tau, max_tau):
+    m = GatedLinearRecurrence(8, width=width, min_tau=min_tau, max_tau=max_tau)
+    tau = m.get_tau(torch.device("cpu"))
+    tau.sum().backward()
+    assert torch.allclose(m.log_tau.grad, tau.detach(), rtol=1e-6) and (m.log_tau.grad > 0).all()
+    assert tau[0] < min_tau * (1 + 2e-5) and (width == 1 or tau[-1] > max_tau * (1 - 2e-5))
+
+
+def test_a_range_of_one_tau():
+    tau = GatedLinearRecurrence(8, min_tau=5.0, max_tau=5.0).get_tau(torch.device("cpu"))
+    assert torch.equal(tau, torch.full((8,), 5.0))
