@@ -336,9 +336,10 @@ class PrimeForCausalLM(nn.Module):
         the differentiable prefill."""
         x = self.embed_tokens(input_ids)
         next_states = [] if return_states else None
-        rng = dropout_rng(x.device) if self.training and self.config.dropout > 0.0 else None
+        # without dropout a block needs no more than (hidden_states, state, return_state)
+        drop = {"rng": dropout_rng(x.device)} if self.training and self.config.dropout > 0.0 else {}
         for i, layer in enumerate(self.layers):
-            x, ns = layer(x, state=states[i] if states is not None else None, return_state=return_states, rng=rng)
+            x, ns = layer(x, state=states[i] if states is not None else None, return_state=return_states, **drop)
             if return_states:
                 next_states.append(ns)
         if logits_to_keep:

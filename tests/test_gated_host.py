@@ -1,5 +1,5 @@
-"""CPU tests of the gated layers' host side: what they begin with, and the warm start of a model
-that has some."""
+"""CPU tests of the host side of gated layers, dropout and sampling: what layers begin with, the
+warm start of a model that has some, blocks of a model without dropout."""
 import dataclasses
 
 import pytest
@@ -52,3 +52,19 @@ def test_every_tau_begins_with_a_gradient(width, min_tau, max_tau):
 def test_a_range_of_one_tau():
     tau = GatedLinearRecurrence(8, min_tau=5.0, max_tau=5.0).get_tau(torch.device("cpu"))
     assert torch.equal(tau, torch.full((8,), 5.0))
+
+
+def test_a_block_without_rng_trains():
+    """A block of the three-argument form in a model without dropout."""
+    class Block(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.proj = torch.nn.Linear(16, 16)
+
+        def forward(self, hidden_states, state=None, return_state=False):
+            return hidden_states + self.proj(hidden_states), None
+    model = PrimeForCausalLM(PrimeConfig(vocab_size=20, hidden_size=16, num_layers=2, num_heads=1, head_dim=16)).train()
+    model.layers[1] = model.layers[0] = Block()
+    ids = torch.arange(12).view(2, 6)
+    model(ids, labels=ids)["loss"].backward()
+    assert model.layers[0].proj.weight.grad.any()
