@@ -17,7 +17,7 @@ def _per_row(v, dtype, device):
     if not torch.is_tensor(v):
         return v
     if dtype is torch.int32 and v.dtype is not dtype:
-        v = v.clamp(0, (1 << 31) - 1)  # more than int32 holds: all
+        v = v.to(torch.int64).clamp(0, (1 << 31) - 1)  # more than int32 holds: all
     return v.to(device=device, dtype=dtype).contiguous()
 
 

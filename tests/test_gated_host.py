@@ -1,11 +1,12 @@
 """CPU tests of the host side of gated layers, dropout and sampling: what layers begin with, the
-warm start of a model that has some, blocks of a model without dropout."""
+warm start of a model that has some, blocks of a model without dropout, types of top_k."""
 import dataclasses
 
 import pytest
 import torch
 
 from prime_moment_attention import GatedLinearRecurrence, PrimeConfig, PrimeForCausalLM
+from prime_moment_attention.sampling import _per_row
 
 
 @pytest.mark.parametrize("min_tau,max_tau,decay", [(1.0, 8000.0, 0.99), (2.0, 2000.0, 0.99), (3.0, 50.0, 0.995),
@@ -68,3 +69,16 @@ def test_a_block_without_rng_trains():
     ids = torch.arange(12).view(2, 6)
     model(ids, labels=ids)["loss"].backward()
     assert model.layers[0].proj.weight.grad.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64, torch.uint16,
+                                   torch.uint32, torch.float16, torch.float32])
+def test_top_k_of_every_type(dtype):
+    """As int32: none below 0, what int32 does not hold as its largest."""
+    k = torch.tensor([0, 1, 50, 127]).to(dtype)
+    got = _per_row(k, torch.int32, k.device)
+    assert got.dtype == torch.int32 and got.tolist() == [0, 1, 50, 127]
+    if dtype in (torch.int64, torch.uint32, torch.float32):
+        assert _per_row(torch.tensor([4294967040]).to(dtype), torch.int32, k.device).tolist() == [(1 << 31) - 1]
+    if dtype.is_signed:
+        assert _per_row(torch.tensor([-3]).to(dtype), torch.int32, k.device).item() <= 0
