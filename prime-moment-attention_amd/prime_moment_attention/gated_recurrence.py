@@ -86,7 +86,7 @@ def _scan(x, step, gate, tau, state, state_out):
         h = parts[0].new_zeros((B, C), dtype=torch.float32) if state is None else state
         if state_out is not None:
             return torch.zeros_like(parts[0]), state_out.copy_(h)
-        return torch.zeros_like(parts[0]) + 0 * (parts[1] + parts[2]), h + 0
+        return (0 * (parts[0] + parts[1] + parts[2] + tau + h.unsqueeze(1))).to(x.dtype), h + 0
     leaves = x.requires_grad or tau.requires_grad or (step is not None and (step.requires_grad or gate.requires_grad)) or (
         state is not None and state.requires_grad)
     if (leaves and torch.is_grad_enabled()) or forward_ad._current_level >= 0:
