@@ -154,13 +154,14 @@ def _mlp_inner(mlp: nn.Module, x: torch.Tensor) -> torch.Tensor:
 class PrimeBlock(nn.Module):
     """Pre-norm block, model.py:71-118: x + Attn(RMSNorm x); x + MLP(RMSNorm x).  `layer` is
     its place in the model: whether it is a gated layer, and its calls of dropout."""
+    layer, dropout = 0, 0.0  # (of a block pickled without them)
 
     def __init__(self, config: PrimeConfig, layer: int = 0):
         super().__init__()
         self.layer = layer
-        self.dropout = config.dropout
+        self.dropout = getattr(config, "dropout", 0.0)  # a config of another class may lack it
         self.input_layernorm = RMSNorm(config.hidden_size, eps=config.rms_norm_eps)
-        if layer in config.gated_layers:
+        if layer in getattr(config, "gated_layers", ()):
             self.self_attn = GatedLinearRecurrence(config.hidden_size, config.num_heads * config.head_dim,
                                                    min_tau=config.min_tau, max_tau=config.max_tau)
         elif config.use_selective:
@@ -272,6 +273,11 @@ class PrimeForCausalLM(nn.Module):
             if getattr(module, "bias", None) is not None:
                 nn.init.zeros_(module.bias)
 
+    @property
+    def drops_out(self) -> bool:
+        """Whether forward applies dropout."""
+        return self.training and getattr(self.config, "dropout", 0.0) > 0.0
+
     def get_input_embeddings(self) -> nn.Embedding:
         return self.embed_tokens
 
@@ -281,8 +287,7 @@ class PrimeForCausalLM(nn.Module):
     def forward(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None,
                 states: Optional[List[Tuple[torch.Tensor, ...]]] = None, return_states: bool = False,
                 logits_to_keep: int = 0) -> Dict[str, Any]:
-        if (self.training and self.config.dropout > 0.0) or (
-                torch.is_grad_enabled() and any(p.requires_grad for p in self.parameters())):
+        if self.drops_out or (torch.is_grad_enabled() and any(p.requires_grad for p in self.parameters())):
             return self._forward_graph(input_ids, labels, states, return_states, logits_to_keep)
         if input_ids.shape[-1] == 1 and _fused_step_supported(self):
             # one token per sequence (the generate loop, model.py:238): the fused
@@ -337,7 +342,7 @@ class PrimeForCausalLM(nn.Module):
         x = self.embed_tokens(input_ids)
         next_states = [] if return_states else None
         # without dropout a block needs no more than (hidden_states, state, return_state)
-        drop = {"rng": dropout_rng(x.device)} if self.training and self.config.dropout > 0.0 else {}
+        drop = {"rng": dropout_rng(x.device)} if self.drops_out else {}
         for i, layer in enumerate(self.layers):
             x, ns = layer(x, state=states[i] if states is not None else None, return_state=return_states, **drop)
             if return_states:
@@ -747,7 +752,7 @@ class GreedyDecoder:
     def prefill(self, input_ids: torch.Tensor) -> torch.Tensor:
         """Run the prompt; returns the first generated token [B, 1]."""
         m = self.model
-        if m.training and m.config.dropout > 0.0:
+        if m.drops_out:
             raise ValueError("the model drops out while it trains: call its eval() before decoding")
         out = m.forward(input_ids, return_states=True, logits_to_keep=1)
         self.states = [s if torch.is_tensor(s) else tuple(s) for s in out["states"]]

@@ -1,6 +1,7 @@
 """CPU tests of the host side of gated layers, dropout and sampling: what layers begin with, the
-warm start of a model that has some, blocks of a model without dropout, types of top_k."""
+warm start of a model that has some, blocks and configurations without dropout, types of top_k."""
 import dataclasses
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -82,3 +83,17 @@ def test_top_k_of_every_type(dtype):
         assert _per_row(torch.tensor([4294967040]).to(dtype), torch.int32, k.device).tolist() == [(1 << 31) - 1]
     if dtype.is_signed:
         assert _per_row(torch.tensor([-3]).to(dtype), torch.int32, k.device).item() <= 0
+
+
+def test_a_config_without_the_new_fields():
+    """A configuration of another class, and a block pickled without its place and its dropout."""
+    fields = dataclasses.asdict(PrimeConfig(vocab_size=20, hidden_size=16, num_layers=1, num_heads=1, head_dim=16))
+    del fields["dropout"], fields["gated_layers"]
+    model = PrimeForCausalLM(SimpleNamespace(**fields)).train()
+    assert not model.drops_out
+    block = model.layers[0]
+    del block.layer, block.dropout
+    block.self_attn.forward = lambda h, state=None, return_state=False: (h, None)
+    ids = torch.arange(12).view(2, 6)
+    model(ids, labels=ids)["loss"].backward()
+    assert block.mlp.up_proj.weight.grad.any()
