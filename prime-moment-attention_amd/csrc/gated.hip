@@ -17,11 +17,12 @@
 // that started before it, so every wait ends.
 //
 // What bounds it.  A token is read once and written once: 8 x 8192 x 768 bf16 is 403 MB, 79
-// us at the 5.1 TB/s of a large copy; its 46 vector instructions, five of them at a quarter of
-// the rate, take as long again.  Together 104 us (3.9 TB/s); 65536 x 512 fp32, twice the bytes
-// a token, 106 us (5.1 TB/s).  The backward, 32 x 2048 x 768 bf16: 717 MB with the checkpoints,
-// 141 us, takes 157-164.  Tried before the last steps, in us for that bf16 forward, that fp32
-// one and the backward, then 112, 113 and 174: 4 waves a span 116, 138, 181; 16 waves 125, 106,
+// us at the 5.1 TB/s of a large copy; its 49 vector instructions, five of them at a quarter of
+// the rate, take as long again.  Together 111 us (3.6 TB/s); 65536 x 512 fp32, twice the bytes
+// a token, 107 us (5.0 TB/s).  The backward, 32 x 2048 x 768 bf16, 79 instructions a token: 717 MB
+// with the checkpoints, 141 us, takes 158-175.  (With a - 1 alone, which is wrong for quick
+// forgetting, 46 and 71 instructions: 106, 106 and 154-166 us.)  Tried early, in us for that bf16
+// forward, that fp32 one and the backward, then 112, 113 and 174: 4 waves a span 116, 138, 181; 16 waves 125, 106,
 // 179; tiles of 8 tokens 161, 128, 187; a state published every 32nd span 123, 117, 171.
 //
 // A decay is held in one of two forms.  Next to 1 (long memories) a itself has lost the low bits
@@ -368,7 +369,7 @@ __device__ __forceinline__ P *elem(const GatedView &v, int b, uint32_t c) {
 }
 
 // Few tokens: a lane walks them, kWalk on their way at a time.  One token of 256 x 768 bf16:
-// 3.3 us, all of it the launch and one way through memory (3.1 MB are 0.6 us).
+// 3.5 us, all of it the launch and one way through memory (3.1 MB are 0.6 us).
 constexpr int kWalk = 4;
 template <int DT>
 __global__ __launch_bounds__(256) void gated_step_kernel(const GatedArgs a) {
@@ -528,8 +529,10 @@ __global__ __launch_bounds__(256) void gated_fill_kernel(uint4 *p, int64_t n) {
 namespace {
 
 // Whether a lane walks the tokens: a few always (8 tokens of 768 bf16 channels: 1 sequence 4.3
-// us, spans 5.0; 256 sequences 6.0, 16.3), more where the sequences fill the chip without the
-// waves that share a span (32 tokens: 256 sequences 18 us, 23; 16 sequences 9.4, 4.9).
+// us, spans 5.1; 256 sequences 6.2, 17.3), more where the sequences fill the chip without the
+// waves that share a span (32 tokens: 256 sequences 18.3 us, 22.8; 171, which are 2052 waves,
+// 16.2, 16.5; 128 14.2, 13.6; 16 9.4, 5.0).  16 tokens could be walked from 1032 waves on: 86
+// sequences 6.8 us, the spans that they get here 8.6; 64 6.3, 5.9.
 bool walks(const GatedArgs &a) {
     return a.L <= 8 || (a.L <= 32 && static_cast<int64_t>(a.B) * ((a.C + kWave - 1) / kWave) >= 2048);
 }
@@ -559,11 +562,12 @@ void run_spans(const GatedArgs &a, bool bwd, hipStream_t s) {
     else hipLaunchKernelGGL((gated_scan_kernel<DT, LINES>), dim3(spans_grid(a)), dim3(kThreads), 0, s, a);
 }
 
-// Accesses go past the caches where every row starts on a line: 8 x 8192 x 768 bf16 took 110 us
-// with plain ones, 104 so, the backward at 32 x 2048 x 768 166, 159.  Else neighbouring channel
-// groups share lines, which the caches then put together: 8 x 8192 x 1000 bf16 203 us past them,
-// 168 through them, the backward 427, 291; fp32 287, 246 and 553, 474; 501 channels bf16 114, 85
-// and 235, 162.  (The forward's stores go past them in either case: up to 5 us less.)
+// Accesses go past the caches where every row starts on a line: 65536 x 512 fp32 takes 115 us
+// with plain ones, 110 so, the backwards of that and of 32 x 2048 x 768 bf16 192, 177 and 175, 165
+// (8 x 8192 x 768 bf16 117 either way).  Else neighbouring channel groups share lines, which the
+// caches then put together: 8 x 8192 x 1000 bf16 202 us past them, 169 through them, the backward
+// 410, 284; fp32 285, 241 and 544, 465; 501 channels bf16 113, 86 and 236, 161.  (The forward's
+// stores go past them in either case: up to 5 us less.)
 template <int DT>
 void run(const GatedArgs &a, bool bwd, hipStream_t s) {
     if (!bwd && walks(a)) {

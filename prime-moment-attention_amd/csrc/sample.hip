@@ -23,10 +23,11 @@
 //
 // What bounds it.  A row belongs to one CU, whose fp64 rate is the floor of a pass over masses
 // (21 instructions a token, 4.9 cycles each: 50304 tokens 9 us); the rest is fetching code that
-// runs once and barriers.  One row of 50304 bf16: 19 us without cuts, 17 with top_k 50, 34 with
-// top_p 0.9 (of these: 5 to load, 7 for counts and bounds, 14 for the masses, 9 for the border,
-// 6 for the token).  256 rows, one a CU, take what the slowest takes: 45 us.  512 x 50304 fp32
-// without cuts: 103 MB, 20 us to read, 44 us.
+// runs once and barriers.  One row of 50304 bf16: 19 us without cuts, 17 with top_k 50, 13 with
+// min_p 0.1, 34 with top_p 0.9 where the tokens down to its border can be gathered, else 38 (of
+// these: 4 to load, 7 for counts and bounds, 14 for the masses, 7 for the border, 6 for the token).
+// 256 rows, one a CU, take what the slowest takes: 45 us with every kind of cut, 22 with min_p 0.1.
+// 512 x 50304 fp32 without cuts: 103 MB, 20 us to read, but the row comes in nearly twice: 44 us.
 
 #include <type_traits>
 
@@ -1056,8 +1057,10 @@ void launch(const SampleArgs &a, hipStream_t s) {
     hipLaunchKernelGGL((sample_kernel<DT, WAVES, STAGED>), dim3(a.n), dim3(WAVES * kWave), 0, s, a);
 }
 
-// Up to 4096 tokens take 4 waves, more 16: 256 x 4000 bf16 without cuts 7.3 us (16 waves 9.9),
-// top_k 50 9.6 (10.3), top_p 0.9 16.5 (17.2); one row fp32 6.9 (8.2), 9.6 (8.3), 14.6 (13.7).  Rows
+// Up to 4096 tokens take 4 waves, more 16.  Without cuts, with top_k 50 and with top_p 0.9: 256 x 4000
+// bf16 7.4, 9.7 and 16.7 us (16 waves 10.0, 10.3 and 21.5), one row 6.7, 9.1 and 15.6 (8.7, 9.4 and
+// 20.2); fp32 7.6, 10.3 and 15.6 (9.3, 9.4 and 18.4), one row 6.9, 9.6 and 14.6 (8.1, 8.4 and 17.0):
+// of these only fp32 with top_k would take less with 16.  Rows
 // go through LDS where they fit (131072 bytes) and each has a CU to itself: 64 x 50304 bf16 20,
 // 18 and 42 us (8 waves without LDS 21, 22, 47).  With more rows than CUs, two smaller
 // workgroups on each hide one's memory behind the other's arithmetic: 512 x 50304 bf16 36, 33
