@@ -606,6 +606,75 @@ int prime_sample(const void *logits, int dtype, int n, int vocab, int64_t stride
                  const float *top_ps, float min_p, const float *min_ps, int64_t *out, void *stream);
 
 /*
+ * Embedding lookup: out[i] = scale * weight[ids[i]], rounded once to `dtype` (F32 / BF16 /
+ * F16; a copy where scale is 1).  An id outside [0, V) gives a row of zeros.
+ *   ids    : n <= 2^30 of int64 (ids64) or int32
+ *   weight : V < 2^31 rows of C <= 2^20 contiguous elements, ldw >= C apart
+ *   out    : [n, C], apart from weight and ids
+ *
+ * prime_embedding_backward: dweight[v] = scale * sum of the rows dy[i] with ids[i] = v, all
+ * V rows written.  Ids outside [0, V) and `padding` (-1: none) have no gradient.  Sums are in
+ * fp32 in a fixed order, rounded once.
+ *   dy        : n rows of C contiguous elements, ldy >= C apart
+ *   dweight   : [V, C], apart from the inputs
+ *   workspace : prime_embedding_backward_workspace_size bytes, 16-byte aligned, this call's
+ *               own until it has run on `stream`
+ */
+int prime_embedding(const void *ids, int ids64, int64_t n, const void *weight, int64_t ldw, int64_t V, int C,
+                    int dtype, float scale, void *out, void *stream);
+size_t prime_embedding_backward_workspace_size(int64_t n, int64_t V, int C);
+int prime_embedding_backward(const void *ids, int ids64, int64_t n, const void *dy, int64_t ldy, int64_t V, int C,
+                             int dtype, float scale, int64_t padding, void *dweight, void *workspace,
+                             size_t workspace_bytes, void *stream);
+
+/*
+ * Log probabilities of given tokens: per row of logits, in fp32, with p = softmax(logits),
+ *   logprobs = log p[token]     0 where token is `ignore`, NaN for another one outside the
+ *                               vocabulary
+ *   entropy  = -sum p log p     (or NULL)
+ *   top_tokens, top_logprobs    the `top` <= 64 largest logits, equal ones by index, NaN last
+ *                               ([n, top]; NULL where top is 0)
+ *   stats                       [n, 2] for the backward, or NULL
+ * A logit of -infinity has probability 0; a row with nothing else has log probabilities of
+ * -infinity, entropy 0 and no gradient.  Logits of +infinity share the probability among
+ * them.  A NaN makes its row's results NaN.
+ *   logits : n rows of vocab <= 2^24 contiguous elements (F32 / BF16 / F16), stride_n >= 0
+ *            apart
+ *   tokens : int64 [n]
+ *
+ * prime_token_logprobs_backward: with g = dlogprobs (0 where the token is `ignore`) and
+ * h = dentropy (fp32 [n], either may be NULL),
+ *   dlogits_j = g (delta_j,token - p_j) - h p_j (log p_j + entropy)
+ * in logits' dtype, rounded once; stats, and with h entropy, are the forward's.  dlogits:
+ * rows stride_d >= vocab apart, apart from logits.
+ */
+int prime_token_logprobs(const void *logits, int dtype, int n, int vocab, int64_t stride_n, const int64_t *tokens,
+                         int64_t ignore, float *logprobs, float *entropy, float *stats, int top, float *top_logprobs,
+                         int64_t *top_tokens, void *stream);
+int prime_token_logprobs_backward(const void *logits, int dtype, int n, int vocab, int64_t stride_n,
+                                  const int64_t *tokens, int64_t ignore, const float *stats, const float *entropy,
+                                  const float *dlogprobs, const float *dentropy, void *dlogits, int64_t stride_d,
+                                  void *stream);
+
+/*
+ * The norm over many tensors, and clipping by it.  tensors, sizes, dtypes: host arrays of
+ * `count` device addresses, numbers of elements (0: skipped, below 2^35 in all) and types
+ * (F32 / BF16 / F16, mixed as they come), contiguous tensors that do not overlap.
+ *   prime_grad_norm : norm (fp32, on the device) = sqrt(sum of all squares), in 64 bits
+ *   prime_grad_clip : the same, and every element times min(1, max_norm / (norm + 1e-6)),
+ *                     in fp32, rounded once; nothing is written where that is 1.  given: norm
+ *                     is read instead (one that other processes share in) and no workspace
+ *                     needed.  An infinite norm scales by 0, a NaN one by NaN; an infinite max_norm clips nothing.
+ * workspace: prime_grad_norm_workspace_size bytes, 16-byte aligned, this call's own until it
+ * has run on `stream`.
+ */
+size_t prime_grad_norm_workspace_size(const int64_t *sizes, int count);
+int prime_grad_norm(const void *const *tensors, const int64_t *sizes, const int32_t *dtypes, int count, float *norm,
+                    void *workspace, size_t workspace_bytes, void *stream);
+int prime_grad_clip(void *const *tensors, const int64_t *sizes, const int32_t *dtypes, int count, double max_norm,
+                    float *norm, int given, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
  * Hybrid window-PRIME pieces (hybrid.py:98-170 calls them through the JIT
  * extension of prime_cpp_kernel.cpp).  The reference's prime_prefill_cpp
  * (prime_cpp_kernel.cpp:6-46) is prime_chunked_prefill with eps = 1e-3 and a

@@ -7,6 +7,8 @@
 #include <chrono>
 #include <mutex>
 #include <random>
+#include <utility>
+#include <vector>
 
 #include "prime_kernels.h"
 
@@ -1730,6 +1732,267 @@ int prime_sample(const void *logits, int dtype, int n, int vocab, int64_t stride
     a.temperature = temperature; a.temperatures = temperatures; a.top_k = top_k; a.top_ks = top_ks;
     a.top_p = top_p; a.top_ps = top_ps; a.min_p = min_p; a.min_ps = min_ps; a.out = out;
     return check_hip(prime::launch_sample(a, static_cast<hipStream_t>(stream)), "sample launch");
+}
+
+}  // extern "C"
+
+namespace {
+
+// n rows of `cols` elements, `ld` apart
+size_t rows_span(int64_t n, int64_t cols, int64_t ld, int es) {
+    return n > 0 ? static_cast<size_t>(((n - 1) * ld + cols) * es) : 0;
+}
+
+int embedding_checks(const char *who, const void *ids, int ids64, int64_t n, const void *rows, int64_t ld, int64_t V,
+                     int C, int dtype, const void *out) {
+    if (!ids || !rows || !out) return fail(PRIME_ERR_INVALID_ARG, "%s: null argument", who);
+    if (!valid_dtype(dtype)) return fail(PRIME_ERR_UNSUPPORTED_DTYPE, "unsupported dtype");
+    if (n <= 0 || n > (1 << 30) || V <= 0 || V >= (int64_t{1} << 31) || C <= 0 || C > (1 << 20) || ld < C ||
+        ld > (int64_t{1} << 40))
+        return fail(PRIME_ERR_INVALID_ARG, "%s: bad sizes n=%lld V=%lld C=%d row stride=%lld", who,
+                    static_cast<long long>(n), static_cast<long long>(V), C, static_cast<long long>(ld));
+    const int es = elem_size(dtype);
+    if (reinterpret_cast<uintptr_t>(ids) % (ids64 ? 8 : 4) || reinterpret_cast<uintptr_t>(rows) % es ||
+        reinterpret_cast<uintptr_t>(out) % es)
+        return fail(PRIME_ERR_MISALIGNED, "%s: misaligned argument", who);
+    return PRIME_OK;
+}
+
+// The tensors of a call in tables of at most kGradTable, those without elements left out.
+// next() fills the one after the last, false behind the last.
+struct GradTables {
+    const void *const *tensors;
+    const int64_t *sizes;
+    const int32_t *dtypes;
+    int count, at = 0;
+    static constexpr uint32_t kMinSpan = 512, kMaxBlocks = 2048;
+    prime::GradTable t;
+    int blocks = 0;
+
+    bool next() {
+        t.count = 0;
+        uint64_t slots = 0;
+        for (; at < count && t.count < prime::kGradTable; ++at) {
+            if (sizes[at] == 0) continue;
+            if (tensors) t.data[t.count] = reinterpret_cast<uintptr_t>(tensors[at]) | static_cast<uint64_t>(dtypes[at]) << 62;
+            t.size[t.count] = sizes[at];
+            t.first[t.count++] = static_cast<uint32_t>(slots);
+            slots += static_cast<uint64_t>(sizes[at] + 7) / 8;
+        }
+        t.first[t.count] = static_cast<uint32_t>(slots);
+        const uint64_t span = std::max<uint64_t>(kMinSpan, (slots + kMaxBlocks - 1) / kMaxBlocks);
+        t.span = static_cast<uint32_t>(span);
+        blocks = static_cast<int>((slots + span - 1) / span);
+        return t.count > 0;
+    }
+};
+
+int grad_checks(const void *const *tensors, const int64_t *sizes, const int32_t *dtypes, int count, const float *norm,
+                const void *workspace, size_t workspace_bytes, bool given) {
+    if (count < 0 || (count && (!tensors || !sizes || !dtypes)) || !norm)
+        return fail(PRIME_ERR_INVALID_ARG, "null tensors, sizes, dtypes or norm");
+    int rc = check_floats(norm, "norm");
+    if (rc) return rc;
+    int64_t slots = 0;
+    for (int i = 0; i < count; ++i) {
+        if (!valid_dtype(dtypes[i])) return fail(PRIME_ERR_UNSUPPORTED_DTYPE, "unsupported dtype of tensor %d", i);
+        if (sizes[i] < 0 || sizes[i] >= (int64_t{1} << 35) || (sizes[i] && !tensors[i]))
+            return fail(PRIME_ERR_INVALID_ARG, "tensor %d: null, or %lld elements", i, static_cast<long long>(sizes[i]));
+        if (sizes[i] && reinterpret_cast<uintptr_t>(tensors[i]) % elem_size(dtypes[i]))
+            return fail(PRIME_ERR_MISALIGNED, "tensor %d is misaligned", i);
+        slots += (sizes[i] + 7) / 8;
+        if (slots >= (int64_t{1} << 32)) return fail(PRIME_ERR_INVALID_ARG, "too many elements");
+    }
+    const size_t need = given ? 0 : prime_grad_norm_workspace_size(sizes, count);
+    if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
+        return fail(PRIME_ERR_INVALID_ARG, "workspace of %zu bytes needed, 16-byte aligned", need);
+    // no two of the tensors, norm and the workspace overlap
+    try {
+        std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+        spans.reserve(static_cast<size_t>(count) + 2);
+        auto add = [&](const void *p, size_t bytes) {
+            if (bytes) spans.emplace_back(reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes);
+        };
+        for (int i = 0; i < count; ++i) add(tensors[i], static_cast<size_t>(sizes[i]) * elem_size(dtypes[i]));
+        add(norm, sizeof(float));
+        add(workspace, need);
+        if (!std::is_sorted(spans.begin(), spans.end())) std::sort(spans.begin(), spans.end());
+        for (size_t i = 1; i < spans.size(); ++i)
+            if (spans[i].first < spans[i - 1].second)
+                return fail(PRIME_ERR_ALIAS, "two of the tensors, norm and the workspace overlap");
+    } catch (...) {
+        return fail(PRIME_ERR_INVALID_ARG, "out of host memory for %d tensors", count);
+    }
+    return PRIME_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int prime_embedding(const void *ids, int ids64, int64_t n, const void *weight, int64_t ldw, int64_t V, int C,
+                    int dtype, float scale, void *out, void *stream) {
+    g_err[0] = 0;
+    int rc = embedding_checks("prime_embedding", ids, ids64, n, weight, ldw, V, C, dtype, out);
+    if (rc) return rc;
+    const int es = elem_size(dtype);
+    const size_t no = rows_span(n, C, C, es);
+    if (overlap(out, no, weight, rows_span(V, C, ldw, es)) || overlap(out, no, ids, static_cast<size_t>(n) * (ids64 ? 8 : 4)))
+        return fail(PRIME_ERR_ALIAS, "out overlaps weight or ids");
+    prime::EmbeddingArgs a{};
+    a.ids = ids; a.ids64 = ids64; a.n = n; a.V = V; a.C = C; a.dt = dtype; a.scale = scale; a.padding = -1;
+    a.weight = weight; a.ldw = ldw; a.out = out;
+    return check_hip(prime::launch_embedding(a, false, static_cast<hipStream_t>(stream)), "embedding launch");
+}
+
+size_t prime_embedding_backward_workspace_size(int64_t n, int64_t V, int C) {
+    if (n <= 0 || n > (1 << 30) || V <= 0 || V >= (int64_t{1} << 31) || C <= 0 || C > (1 << 20)) return 0;
+    return prime::embedding_workspace_bytes(n, V, C);
+}
+
+int prime_embedding_backward(const void *ids, int ids64, int64_t n, const void *dy, int64_t ldy, int64_t V, int C,
+                             int dtype, float scale, int64_t padding, void *dweight, void *workspace,
+                             size_t workspace_bytes, void *stream) {
+    g_err[0] = 0;
+    int rc = embedding_checks("prime_embedding_backward", ids, ids64, n, dy, ldy, V, C, dtype, dweight);
+    if (rc) return rc;
+    if (!prime::embedding_grid_fits(n, V, C, dtype))
+        return fail(PRIME_ERR_INVALID_ARG, "n=%lld V=%lld C=%d above the grid's limit", static_cast<long long>(n),
+                    static_cast<long long>(V), C);
+    const size_t need = prime_embedding_backward_workspace_size(n, V, C);
+    if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u))
+        return fail(PRIME_ERR_INVALID_ARG, "workspace of %zu bytes needed, 16-byte aligned", need);
+    const int es = elem_size(dtype);
+    const size_t nw = rows_span(V, C, C, es), ny = rows_span(n, C, ldy, es), ni = static_cast<size_t>(n) * (ids64 ? 8 : 4);
+    if (overlap(dweight, nw, dy, ny) || overlap(dweight, nw, ids, ni) || overlap(dweight, nw, workspace, need) ||
+        overlap(workspace, need, dy, ny) || overlap(workspace, need, ids, ni))
+        return fail(PRIME_ERR_ALIAS, "dweight or the workspace overlaps another buffer");
+    prime::EmbeddingArgs a{};
+    a.ids = ids; a.ids64 = ids64; a.n = n; a.V = V; a.C = C; a.dt = dtype; a.scale = scale; a.padding = padding;
+    a.dy = dy; a.ldy = ldy; a.dweight = dweight; a.workspace = workspace;
+    return check_hip(prime::launch_embedding(a, true, static_cast<hipStream_t>(stream)), "embedding backward launch");
+}
+
+}  // extern "C"
+
+namespace {
+
+int logprobs_checks(const char *who, const void *logits, int dtype, int n, int vocab, int64_t stride_n, const void *tokens) {
+    if (!logits || !tokens) return fail(PRIME_ERR_INVALID_ARG, "%s: null argument", who);
+    if (n <= 0 || vocab <= 0 || vocab > (1 << 24) || stride_n < 0 || stride_n > (int64_t{1} << 40))
+        return fail(PRIME_ERR_INVALID_ARG, "%s: bad sizes n=%d vocab=%d stride=%lld", who, n, vocab,
+                    static_cast<long long>(stride_n));
+    if (!valid_dtype(dtype)) return fail(PRIME_ERR_UNSUPPORTED_DTYPE, "unsupported logits dtype");
+    if (reinterpret_cast<uintptr_t>(logits) % elem_size(dtype) || (reinterpret_cast<uintptr_t>(tokens) & 7u))
+        return fail(PRIME_ERR_MISALIGNED, "logits or tokens misaligned");
+    return PRIME_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int prime_token_logprobs(const void *logits, int dtype, int n, int vocab, int64_t stride_n, const int64_t *tokens,
+                         int64_t ignore, float *logprobs, float *entropy, float *stats, int top, float *top_logprobs,
+                         int64_t *top_tokens, void *stream) {
+    g_err[0] = 0;
+    int rc = logprobs_checks("prime_token_logprobs", logits, dtype, n, vocab, stride_n, tokens);
+    if (rc) return rc;
+    if (!logprobs || (top > 0 && (!top_logprobs || !top_tokens)))
+        return fail(PRIME_ERR_INVALID_ARG, "prime_token_logprobs: null output");
+    if (top < 0 || top > prime::kLogprobsMaxTop || top > vocab)
+        return fail(PRIME_ERR_INVALID_ARG, "top=%d outside 0 .. min(%d, vocab)", top, prime::kLogprobsMaxTop);
+    if ((rc = check_floats(logprobs, "logprobs")) || (rc = check_floats(entropy, "entropy")) ||
+        (rc = check_floats(stats, "stats")) || (rc = check_floats(top_logprobs, "top_logprobs")))
+        return rc;
+    if (top && (reinterpret_cast<uintptr_t>(top_tokens) & 7u)) return fail(PRIME_ERR_MISALIGNED, "top_tokens misaligned");
+    const size_t N = static_cast<size_t>(n);
+    const void *out[5] = {logprobs, entropy, stats, top ? top_logprobs : nullptr, top ? top_tokens : nullptr};
+    const size_t no[5] = {N * 4, N * 4, N * 8, N * top * 4, N * top * 8};
+    const size_t nl = rows_span(n, vocab, stride_n, elem_size(dtype));
+    for (int i = 0; i < 5; ++i) {
+        if (!out[i]) continue;
+        if (overlap(out[i], no[i], logits, nl) || overlap(out[i], no[i], tokens, N * 8))
+            return fail(PRIME_ERR_ALIAS, "an output overlaps logits or tokens");
+        for (int j = 0; j < i; ++j)
+            if (out[j] && overlap(out[i], no[i], out[j], no[j])) return fail(PRIME_ERR_ALIAS, "two outputs overlap");
+    }
+    prime::LogprobsArgs a{};
+    a.logits = logits; a.stride_n = stride_n; a.n = n; a.vocab = vocab; a.dt = dtype; a.tokens = tokens; a.ignore = ignore;
+    a.logprobs = logprobs; a.entropy = entropy; a.stats = stats;
+    a.top = top; a.top_logprobs = top_logprobs; a.top_tokens = top_tokens;
+    return check_hip(prime::launch_logprobs(a, false, static_cast<hipStream_t>(stream)), "token logprobs launch");
+}
+
+int prime_token_logprobs_backward(const void *logits, int dtype, int n, int vocab, int64_t stride_n,
+                                  const int64_t *tokens, int64_t ignore, const float *stats, const float *entropy,
+                                  const float *dlogprobs, const float *dentropy, void *dlogits, int64_t stride_d,
+                                  void *stream) {
+    g_err[0] = 0;
+    int rc = logprobs_checks("prime_token_logprobs_backward", logits, dtype, n, vocab, stride_n, tokens);
+    if (rc) return rc;
+    if (!stats || !dlogits || (dentropy && !entropy))
+        return fail(PRIME_ERR_INVALID_ARG, "prime_token_logprobs_backward: null stats, entropy or dlogits");
+    if (n > 1 && (stride_d < vocab || stride_d > (int64_t{1} << 40)))
+        return fail(PRIME_ERR_INVALID_ARG, "dlogits' row stride %lld below vocab", static_cast<long long>(stride_d));
+    const int es = elem_size(dtype);
+    if (reinterpret_cast<uintptr_t>(dlogits) % es) return fail(PRIME_ERR_MISALIGNED, "dlogits misaligned");
+    if ((rc = check_floats(stats, "stats")) || (rc = check_floats(entropy, "entropy")) ||
+        (rc = check_floats(dlogprobs, "dlogprobs")) || (rc = check_floats(dentropy, "dentropy")))
+        return rc;
+    const size_t N = static_cast<size_t>(n), nd = rows_span(n, vocab, n > 1 ? stride_d : vocab, es);
+    const void *in[6] = {logits, tokens, stats, entropy, dlogprobs, dentropy};
+    const size_t ni[6] = {rows_span(n, vocab, stride_n, es), N * 8, N * 8, N * 4, N * 4, N * 4};
+    for (int i = 0; i < 6; ++i)
+        if (in[i] && overlap(dlogits, nd, in[i], ni[i])) return fail(PRIME_ERR_ALIAS, "dlogits overlaps an input");
+    prime::LogprobsArgs a{};
+    a.logits = logits; a.stride_n = stride_n; a.n = n; a.vocab = vocab; a.dt = dtype; a.tokens = tokens; a.ignore = ignore;
+    a.stats = const_cast<float *>(stats); a.entropy = const_cast<float *>(entropy);
+    a.dlogprobs = dlogprobs; a.dentropy = dentropy; a.dlogits = dlogits; a.stride_d = stride_d;
+    return check_hip(prime::launch_logprobs(a, true, static_cast<hipStream_t>(stream)), "token logprobs backward launch");
+}
+
+size_t prime_grad_norm_workspace_size(const int64_t *sizes, int count) {
+    if (!sizes || count <= 0) return 0;
+    size_t blocks = 0;
+    for (GradTables g{nullptr, sizes, nullptr, count}; g.next();) blocks += g.blocks;
+    return blocks * sizeof(double);
+}
+
+int prime_grad_norm(const void *const *tensors, const int64_t *sizes, const int32_t *dtypes, int count, float *norm,
+                    void *workspace, size_t workspace_bytes, void *stream) {
+    g_err[0] = 0;
+    int rc = grad_checks(tensors, sizes, dtypes, count, norm, workspace, workspace_bytes, false);
+    if (rc) return rc;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    double *parts = static_cast<double *>(workspace);
+    int blocks = 0;
+    for (GradTables g{tensors, sizes, dtypes, count}; g.next(); blocks += g.blocks)
+        if ((rc = check_hip(prime::launch_grad_squares(g.t, g.blocks, parts + blocks, s), "gradient norm launch"))) return rc;
+    return check_hip(prime::launch_grad_norm(parts, blocks, norm, s), "gradient norm launch");
+}
+
+int prime_grad_clip(void *const *tensors, const int64_t *sizes, const int32_t *dtypes, int count, double max_norm,
+                    float *norm, int given, void *workspace, size_t workspace_bytes, void *stream) {
+    g_err[0] = 0;
+    int rc = grad_checks(tensors, sizes, dtypes, count, norm, workspace, workspace_bytes, given);
+    if (rc) return rc;
+    if (!(max_norm >= 0.0)) return fail(PRIME_ERR_INVALID_ARG, "max_norm=%g below 0", max_norm);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    double *parts = static_cast<double *>(workspace);
+    int blocks = 0, tables = 0;
+    if (!given) {
+        for (GradTables g{tensors, sizes, dtypes, count}; g.next(); blocks += g.blocks, ++tables)
+            if ((rc = check_hip(prime::launch_grad_squares(g.t, g.blocks, parts + blocks, s), "gradient norm launch")))
+                return rc;
+        // one table: the scaling adds the parts itself
+        if (tables != 1 && (rc = check_hip(prime::launch_grad_norm(parts, blocks, norm, s), "gradient norm launch"))) return rc;
+    }
+    for (GradTables g{tensors, sizes, dtypes, count}; g.next();)
+        if ((rc = check_hip(prime::launch_grad_scale(g.t, g.blocks, tables == 1 ? parts : nullptr, blocks, norm, max_norm, s),
+                            "gradient scaling launch")))
+            return rc;
+    return PRIME_OK;
 }
 
 }  // extern "C"

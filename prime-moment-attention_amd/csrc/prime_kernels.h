@@ -473,6 +473,61 @@ struct SampleArgs {
 constexpr int kSampleMaxVocab = 1 << 20;
 hipError_t launch_sample(const SampleArgs &a, hipStream_t stream);
 
+// Embedding lookup and its gradient (embedding.hip).
+struct EmbeddingArgs {
+    const void *ids;                  // [n] int64 or int32
+    int ids64;
+    int64_t n, V;
+    int C, dt;
+    float scale;
+    int64_t padding;                  // an id without a gradient, or -1
+    const void *weight;               // forward: V rows, ldw elements apart
+    int64_t ldw;
+    void *out;                        // [n, C]
+    const void *dy;                   // backward: n rows, ldy elements apart
+    int64_t ldy;
+    void *dweight;                    // [V, C]
+    void *workspace;
+};
+size_t embedding_workspace_bytes(int64_t n, int64_t V, int C);
+bool embedding_grid_fits(int64_t n, int64_t V, int C, int dt);
+hipError_t launch_embedding(const EmbeddingArgs &a, bool backward, hipStream_t stream);
+
+// Log probabilities of given tokens (logprobs.hip).
+struct LogprobsArgs {
+    const void *logits;               // n rows of vocab, stride_n elements apart
+    int64_t stride_n;
+    int n, vocab, dt;
+    const int64_t *tokens;            // [n]
+    int64_t ignore;
+    float *logprobs, *entropy;        // [n]; entropy: forward or null, backward the forward's
+    float *stats;                     // [n, 2] or null: C (NaN: a row summed by differences) and L
+    int top;
+    float *top_logprobs;              // [n, top]
+    int64_t *top_tokens;
+    const float *dlogprobs, *dentropy;  // [n] or null
+    void *dlogits;                    // n rows, stride_d elements apart
+    int64_t stride_d;
+};
+constexpr int kLogprobsMaxTop = 64;
+hipError_t launch_logprobs(const LogprobsArgs &a, bool backward, hipStream_t stream);
+
+// The norm over many tensors and their scaling (grad_clip.hip).  A tensor in the table: its
+// address with the type in the two highest bits, its elements, and the slots of 8 elements
+// before it; a workgroup has `span` slots.  As large as a kernel's arguments may be.
+constexpr int kGradTable = 192;
+struct GradTable {
+    uint64_t data[kGradTable];
+    int64_t size[kGradTable];
+    uint32_t first[kGradTable + 1];
+    int32_t count;
+    uint32_t span;
+};
+hipError_t launch_grad_squares(const GradTable &t, int blocks, double *parts, hipStream_t stream);
+hipError_t launch_grad_norm(const double *parts, int count, float *norm, hipStream_t stream);
+hipError_t launch_grad_scale(const GradTable &t, int blocks, const double *parts, int count, float *norm,
+                             double max_norm, hipStream_t stream);
+
 // Launch timer (the C-ABI prime_timer_* calls).  timer_events(kernel) hands
 // out the event pair for one launch of `kernel` while that kernel is being
 // timed (both null otherwise); the launch passes them to hipExtLaunchKernelGGL,

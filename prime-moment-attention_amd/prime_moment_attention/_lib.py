@@ -6,6 +6,7 @@ calls raise.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import os
 from typing import Optional, Sequence, Tuple
@@ -37,7 +38,10 @@ EXPORTS = ("prime_abi_version", "prime_last_error", "prime_decode_step", "prime_
            "prime_delta_prefill_backward", "prime_delta_prefill_backward_workspace_size",
            "prime_delta_decode_step_backward", "prime_delta_gates",
            "prime_gated_scan", "prime_gated_scan_workspace_size", "prime_gated_scan_backward",
-           "prime_gated_scan_backward_workspace_size", "prime_dropout_add", "prime_sample")
+           "prime_gated_scan_backward_workspace_size", "prime_dropout_add", "prime_sample",
+           "prime_embedding", "prime_embedding_backward", "prime_embedding_backward_workspace_size",
+           "prime_token_logprobs", "prime_token_logprobs_backward",
+           "prime_grad_norm", "prime_grad_norm_workspace_size", "prime_grad_clip")
 
 # bytes of the fixed device scratch behind prime_accumulate_noalloc
 NOALLOC_SCRATCH_BYTES = 32 << 20
@@ -214,6 +218,20 @@ def load() -> ctypes.CDLL:
     L.prime_dropout_add.restype = ctypes.c_int
     L.prime_sample.argtypes = [fp, i32, i32, i32, i64, fp, f32, fp, i32, fp, f32, fp, f32, fp, fp, fp]
     L.prime_sample.restype = ctypes.c_int
+    f64, size = ctypes.c_double, ctypes.c_size_t
+    L.prime_embedding.argtypes = [fp, i32, i64, fp, i64, i64, i32, i32, f32, fp, fp]
+    L.prime_embedding_backward_workspace_size.argtypes = [i64, i64, i32]
+    L.prime_embedding_backward_workspace_size.restype = size
+    L.prime_embedding_backward.argtypes = [fp, i32, i64, fp, i64, i64, i32, i32, f32, i64, fp, fp, size, fp]
+    L.prime_token_logprobs.argtypes = [fp, i32, i32, i32, i64, fp, i64, fp, fp, fp, i32, fp, fp, fp]
+    L.prime_token_logprobs_backward.argtypes = [fp, i32, i32, i32, i64, fp, i64, fp, fp, fp, fp, fp, i64, fp]
+    L.prime_grad_norm_workspace_size.argtypes = [fp, i32]
+    L.prime_grad_norm_workspace_size.restype = size
+    L.prime_grad_norm.argtypes = [fp, fp, fp, i32, fp, fp, size, fp]
+    L.prime_grad_clip.argtypes = [fp, fp, fp, i32, f64, fp, i32, fp, size, fp]
+    for fn in (L.prime_embedding, L.prime_embedding_backward, L.prime_token_logprobs, L.prime_token_logprobs_backward,
+               L.prime_grad_norm, L.prime_grad_clip):
+        fn.restype = ctypes.c_int
     v = L.prime_abi_version()
     if v != ABI_VERSION:
         raise RuntimeError(f"libprime_mi355x ABI {v} != expected {ABI_VERSION}")
@@ -1277,6 +1295,126 @@ def sample(logits, uniforms, temperature, top_k, top_p, min_p, out) -> None:
         args.append(v.data_ptr())
     _launch(load().prime_sample, "prime_sample", logits.device, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab,
             logits.stride(0) if n > 1 else vocab, *args[1:], args[0])
+
+
+# ---------------------------------------------------------------- embedding, log probabilities, clipping
+def _check_table(ids, rows, C: int, what: str) -> None:
+    """ids (int64 or int32, contiguous) and rows [*, C] with contiguous columns."""
+    if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
+        raise ValueError(f"ids are {ids.dtype}: int64 or int32 is needed")
+    if rows.dtype not in _DTYPES:
+        raise RuntimeError(f"unsupported dtype {rows.dtype}")
+    if rows.dim() != 2 or rows.shape[1] != C or (rows.stride(1) != 1 and C > 1) or not ids.is_contiguous():
+        raise ValueError(f"{what} must be rows of {C} contiguous columns, ids contiguous")
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def embedding(ids, weight, scale: float, out) -> None:
+    """prime_embedding: contiguous ids of any shape, weight [V, C] with contiguous columns,
+    out [ids.numel(), C] contiguous."""
+    V, C = weight.shape
+    _check_table(ids, weight, C, "weight")
+    n = ids.numel()
+    if out.dtype is not weight.dtype or out.numel() != n * C or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {weight.dtype} tensor of {n} x {C}")
+    _same_device(weight, ids, out)
+    _launch(load().prime_embedding, "prime_embedding", weight.device, ids.data_ptr(), ids.dtype is torch.int64, n,
+            weight.data_ptr(), _row_stride(weight), V, C, _DTYPES[weight.dtype], scale, out.data_ptr())
+
+
+def embedding_backward(ids, dy, scale: float, padding: int, dweight) -> None:
+    """prime_embedding_backward: dy [ids.numel(), C] with contiguous columns, dweight [V, C]
+    contiguous; padding: an id without a gradient, or -1."""
+    V, C = dweight.shape
+    _check_table(ids, dy, C, "dy")
+    n = ids.numel()
+    if dy.shape[0] != n or dweight.dtype is not dy.dtype or not dweight.is_contiguous():
+        raise ValueError(f"dy must be [{n}, {C}], dweight contiguous and of its dtype")
+    _same_device(dy, ids, dweight)
+    L = load()
+    size = L.prime_embedding_backward_workspace_size(n, V, C)
+    ws = torch.empty(size, dtype=torch.uint8, device=dy.device)
+    _launch(L.prime_embedding_backward, "prime_embedding_backward", dy.device, ids.data_ptr(),
+            ids.dtype is torch.int64, n, dy.data_ptr(), _row_stride(dy), V, C, _DTYPES[dy.dtype], scale, padding,
+            dweight.data_ptr(), ws.data_ptr(), size)
+
+
+def _check_logits(logits, tokens) -> Tuple[int, int]:
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("logits must be [n, vocab] with a contiguous vocab dimension")
+    if logits.dtype not in _DTYPES:
+        raise RuntimeError(f"unsupported dtype {logits.dtype}")
+    n, vocab = logits.shape
+    if tokens.dtype is not torch.int64 or tokens.numel() != n or not tokens.is_contiguous():
+        raise ValueError(f"tokens must be a contiguous int64 tensor of {n} values")
+    return n, vocab
+
+
+def _f32_of(n: int, *ts) -> None:
+    for t in ts:
+        if t is not None and (t.dtype is not torch.float32 or t.numel() != n or not t.is_contiguous()):
+            raise ValueError(f"a contiguous fp32 tensor of {n} values is needed, not {tuple(t.shape)} {t.dtype}")
+
+
+def token_logprobs(logits, tokens, ignore: int, logprobs, entropy, stats, top: int, top_logprobs, top_tokens) -> None:
+    """prime_token_logprobs: logits [n, vocab], tokens int64 [n]; fp32 outputs of n (stats:
+    2 n) values, entropy and stats or None; top_logprobs fp32, top_tokens int64 of n * top, or
+    None."""
+    n, vocab = _check_logits(logits, tokens)
+    _f32_of(n, logprobs, entropy)
+    _f32_of(2 * n, stats)
+    if top:
+        _f32_of(n * top, top_logprobs)
+        if top_tokens.dtype is not torch.int64 or top_tokens.numel() != n * top or not top_tokens.is_contiguous():
+            raise ValueError(f"top_tokens must be a contiguous int64 tensor of {n * top} values")
+    _same_device(logits, tokens, logprobs, entropy, stats, top_logprobs, top_tokens)
+    _launch(load().prime_token_logprobs, "prime_token_logprobs", logits.device, logits.data_ptr(),
+            _DTYPES[logits.dtype], n, vocab, _row_stride(logits), tokens.data_ptr(), ignore, logprobs.data_ptr(),
+            _ptr(entropy), _ptr(stats), top, _ptr(top_logprobs), _ptr(top_tokens))
+
+
+def token_logprobs_backward(logits, tokens, ignore: int, stats, entropy, dlogprobs, dentropy, dlogits) -> None:
+    """prime_token_logprobs_backward: dlogits [n, vocab] of logits' dtype; dlogprobs and
+    dentropy fp32 [n] or None."""
+    n, vocab = _check_logits(logits, tokens)
+    _f32_of(2 * n, stats)
+    _f32_of(n, entropy, dlogprobs, dentropy)
+    if dlogits.shape != logits.shape or dlogits.dtype is not logits.dtype or (dlogits.stride(1) != 1 and vocab > 1):
+        raise ValueError("dlogits must have logits' shape and dtype and a contiguous vocab dimension")
+    _same_device(logits, tokens, stats, entropy, dlogprobs, dentropy, dlogits)
+    _launch(load().prime_token_logprobs_backward, "prime_token_logprobs_backward", logits.device, logits.data_ptr(),
+            _DTYPES[logits.dtype], n, vocab, _row_stride(logits), tokens.data_ptr(), ignore, stats.data_ptr(),
+            _ptr(entropy), _ptr(dlogprobs), _ptr(dentropy), dlogits.data_ptr(), _row_stride(dlogits))
+
+
+def grad_norm(tensors, norm, max_norm: Optional[float] = None, given: bool = False) -> None:
+    """prime_grad_norm of contiguous tensors (or dense ones: every element is theirs) into
+    norm (fp32, one value), or with max_norm prime_grad_clip of them; given: by the norm
+    that is there."""
+    dev = norm.device
+    _same_device(norm)
+    _f32_of(1, norm)
+    index = norm.get_device()
+    for t in tensors:
+        if t.get_device() != index:
+            _same_device(norm, t)
+        if t.dtype not in _DTYPES:
+            raise RuntimeError(f"unsupported dtype {t.dtype}")
+    L = load()
+    count = len(tensors)
+    data = array.array("Q", [t.data_ptr() for t in tensors])
+    sizes = array.array("q", [t.numel() for t in tensors])
+    dtypes = array.array("i", [_DTYPES[t.dtype] for t in tensors])
+    table = (data.buffer_info()[0], sizes.buffer_info()[0], dtypes.buffer_info()[0], count)
+    n = 0 if given else L.prime_grad_norm_workspace_size(table[1], count)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    if max_norm is None:
+        _launch(L.prime_grad_norm, "prime_grad_norm", dev, *table, norm.data_ptr(), _ptr(ws), n)
+    else:
+        _launch(L.prime_grad_clip, "prime_grad_clip", dev, *table, max_norm, norm.data_ptr(), given, _ptr(ws), n)
 
 
 def timer_enable(*kernels: int) -> None:
