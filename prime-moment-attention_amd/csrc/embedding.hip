@@ -9,7 +9,8 @@
 //           lie in the chunk is finished there; one that reaches over its end or its start
 //           leaves a part
 //   join    the parts of ids that reach over a chunk's end, in order
-// The rows of ids that do not occur are written as zeros by further workgroups of the sum.
+// The sort is short and leaves most of the card idle: further workgroups of its launches fill
+// the whole gradient with zeros meanwhile, which the rows with a token then replace.
 
 #include "prime_kernels.h"
 
@@ -18,11 +19,20 @@ namespace prime {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
 constexpr int kMaxBits = 9, kMaxBins = 1 << kMaxBits;
-constexpr int kSortItems = 1024;  // at least, of a workgroup
+constexpr int kFewTokens = 8192;
+constexpr int kSortItems = 4096;  // at least, of a workgroup
 constexpr int kSortBlocks = 512;  // at most
 constexpr int kChunk = 32;        // sorted rows
-constexpr int kZeroRows = 64;     // rows of the table that a workgroup looks at
+constexpr int kRows = 8;          // of a chunk, on their way at once
+
+// The part [from, to) of the gradient's 16-byte blocks that a launch's workgroups from `block`
+// on fill with zeros.
+struct Fill {
+    int block;
+    int64_t from, to;
+};
 
 struct __attribute__((packed, aligned(2))) Raw {  // 16 bytes of a row, wherever it starts
     u32x4 v;
@@ -115,128 +125,194 @@ __global__ __launch_bounds__(kThreads) void embedding_kernel(const EmbeddingArgs
     at.store(static_cast<char *>(a.out) + i * a.C * es, v);
 }
 
-// One counting pass: keys and positions in, their digits' counts out, or (SCATTER) both in the
-// digits' order.  FIRST: the keys are the ids', the positions the tokens' own.
-template <bool FIRST, bool SCATTER>
-__global__ __launch_bounds__(kThreads) void embedding_sort_kernel(const EmbeddingArgs a, const uint32_t *keys,
-                                                                  const uint32_t *index, uint32_t *keys_out,
-                                                                  uint32_t *index_out, uint32_t *hist, int shift,
-                                                                  int bits, int items) {
-    __shared__ uint32_t count[kWaves][kMaxBins];
-    __shared__ uint32_t wave_total[kWaves];
-    const int bins = 1 << bits, tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
-    for (int b = tid; b < kWaves * kMaxBins; b += kThreads) (&count[0][0])[b] = 0;
-    __syncthreads();
-    // a wave has `items` / kWaves tokens that lie one after the other
-    const int64_t begin = static_cast<int64_t>(blockIdx.x) * items + wave * (items / kWaves);
-    const int64_t end = begin + items / kWaves < a.n ? begin + items / kWaves : a.n;
-    auto key_of = [&](int64_t i) { return FIRST ? sort_key(a, i) : keys[i]; };
-    for (int64_t i = begin + lane; i < end; i += kWave) atomicAdd(&count[wave][key_of(i) >> shift & (bins - 1)], 1u);
-    __syncthreads();
-    if constexpr (!SCATTER) {
-        for (int b = tid; b < bins; b += kThreads) {
-            uint32_t sum = 0;
+// A workgroup's share of the gradient's zeros: 16-byte stores over [from, to) of the table's
+// 16-byte blocks, the elements before the first and behind the last by the share that has
+// them.
+__device__ __forceinline__ void fill_zeros(const EmbeddingArgs &a, const Fill &f) {
+    const int es = a.dt == PRIME_F32 ? 4 : 2;
+    char *dw = static_cast<char *>(a.dweight);
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(dw), end = begin + a.V * a.C * es;
+    const uintptr_t first = (begin + 15) & ~uintptr_t{15}, last = end & ~uintptr_t{15};
+    constexpr int U = 4;
+    u32x4 *p = reinterpret_cast<u32x4 *>(first);
+    const int64_t at = f.from + static_cast<int64_t>(blockIdx.x - f.block) * (kSortThreads * U) + threadIdx.x;
+    const int64_t blocks = first < last ? static_cast<int64_t>(last - first) / 16 : 0, to = f.to < blocks ? f.to : blocks;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) sum += count[w][b];
-            hist[static_cast<int64_t>(blockIdx.x) * bins + b] = sum;
-        }
-    } else {
-        // where each digit of this workgroup starts: behind the lower digits of all workgroups
-        // and behind its own of the workgroups before.  Thread t has the digits 2 t, 2 t + 1.
-        uint32_t total[2] = {}, before[2] = {};
-        const int blocks = gridDim.x;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int b = 2 * tid + k;
-            if (b >= bins) continue;
-#pragma unroll 8
-            for (int q = 0; q < blocks; ++q) {
-                const uint32_t h = hist[static_cast<int64_t>(q) * bins + b];
-                total[k] += h;
-                before[k] += q < static_cast<int>(blockIdx.x) ? h : 0;
-            }
-        }
-        uint32_t sum = total[0] + total[1], scan = sum;
-#pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            const uint32_t v = __shfl_up(scan, o, kWave);
-            scan += lane >= o ? v : 0;
-        }
-        if (lane == kWave - 1) wave_total[wave] = scan;
-        __syncthreads();
-        scan -= sum;
-        for (int w = 0; w < wave; ++w) scan += wave_total[w];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int b = 2 * tid + k;
-            if (b >= bins) continue;
-            uint32_t at = scan + before[k];
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                const uint32_t c = count[w][b];
-                count[w][b] = at;
-                at += c;
-            }
-            scan += total[k];
-        }
-        __syncthreads();
-        // 64 tokens at a time: those of one digit find each other by its bits
-        volatile uint32_t *next = count[wave];
-        for (int64_t i0 = begin; i0 < end; i0 += kWave) {
-            const int64_t i = i0 + lane;
-            const bool in = i < end;
-            const uint32_t key = in ? key_of(i) : 0, digit = key >> shift & (bins - 1);
-            uint64_t peers = __ballot(in);
-            for (int b = 0; b < bits; ++b) {
-                const uint64_t one = __ballot(digit >> b & 1);
-                peers &= digit >> b & 1 ? one : ~one;
-            }
-            const int below = __popcll(peers & ((1ull << lane) - 1));
-            uint32_t at = 0;
-            if (in) at = next[digit];
-            __builtin_amdgcn_wave_barrier();
-            if (in && below == 0) next[digit] = at + __popcll(peers);
-            __builtin_amdgcn_wave_barrier();
-            if (in) {
-                keys_out[at + below] = key;
-                index_out[at + below] = FIRST ? static_cast<uint32_t>(i) : index[i];
-            }
-        }
+    for (int u = 0; u < U; ++u)
+        if (at + u * kSortThreads < to) p[at + u * kSortThreads] = u32x4{0, 0, 0, 0};
+    if (f.from == 0 && blockIdx.x == f.block) {
+        const uintptr_t head = first < end ? first : end, tail = last > head ? last : head;
+        for (uintptr_t q = begin + threadIdx.x * 2; q < head; q += kSortThreads * 2) *reinterpret_cast<uint16_t *>(q) = 0;
+        for (uintptr_t q = tail + threadIdx.x * 2; q < end; q += kSortThreads * 2) *reinterpret_cast<uint16_t *>(q) = 0;
     }
 }
 
-// Workgroups below `sum_blocks`: chunks of sorted rows, 16 bytes of columns a thread.  The
-// others: the table's rows without a token.  part: [chunks][2][vecs VE], of the id that reaches
-// in from the chunk before (0) and of the one that begins here and reaches on (1).
+// The sum of v over the threads before this one.
+__device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t *wave_total) {
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    uint32_t scan = v;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+        const uint32_t u = __shfl_up(scan, o, kWave);
+        scan += lane >= o ? u : 0;
+    }
+    if (lane == kWave - 1) wave_total[wave] = scan;
+    __syncthreads();
+    uint32_t before = scan - v;
+    for (int w = 0; w < wave; ++w) before += wave_total[w];
+    return before;
+}
+
+// Items [begin, end) of a wave to the places that `next` counts up for their digits, 64 at a
+// time: those of one digit find each other by its bits.
+template <typename K, typename P>
+__device__ __forceinline__ void place_items(volatile uint32_t *next, int64_t begin, int64_t end, int shift, int bits, K key_of, P put) {
+    const int lane = threadIdx.x % kWave;
+    for (int64_t i0 = begin; i0 < end; i0 += kWave) {
+        const int64_t i = i0 + lane;
+        const bool in = i < end;
+        const uint32_t key = in ? key_of(i) : 0, digit = key >> shift & ((1u << bits) - 1);
+        uint64_t peers = __ballot(in);
+        for (int b = 0; b < bits; ++b) {
+            const uint64_t one = __ballot(digit >> b & 1);
+            peers &= digit >> b & 1 ? one : ~one;
+        }
+        const int below = __popcll(peers & ((1ull << lane) - 1));
+        uint32_t at = 0;
+        if (in) at = next[digit];
+        __builtin_amdgcn_wave_barrier();
+        if (in && below == 0) next[digit] = at + __popcll(peers);
+        __builtin_amdgcn_wave_barrier();
+        if (in) put(at + below, key, i);
+    }
+}
+
+// One counting pass: keys and positions in, their digits' counts out, or (SCATTER) both in the
+// digits' order.  FIRST: the keys are the ids', the positions the tokens' own.  Workgroups from
+// `fill.block` on write zeros meanwhile.
+template <bool FIRST, bool SCATTER>
+__global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(const EmbeddingArgs a, const uint32_t *keys,
+                                                                      const uint32_t *index, uint32_t *keys_out,
+                                                                      uint32_t *index_out, uint32_t *hist, int shift,
+                                                                      int bits, int items, const Fill fill) {
+    __shared__ uint32_t count[kSortWaves][kMaxBins];
+    __shared__ uint32_t total[kSortThreads], before[kSortThreads], wave_total[kSortWaves];
+    if (static_cast<int>(blockIdx.x) >= fill.block) {
+        fill_zeros(a, fill);
+        return;
+    }
+    const int bins = 1 << bits, tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave, blocks = fill.block;
+    if constexpr (SCATTER) {
+        // each digit's count in all workgroups and in those before this one, by threads that
+        // share the workgroups between them
+        const int bin = tid & (bins - 1), share = kSortThreads / bins;
+        uint32_t t = 0, b = 0;
+#pragma unroll 8
+        for (int q = tid / bins; q < blocks; q += share) {
+            const uint32_t h = hist[static_cast<int64_t>(q) * bins + bin];
+            t += h;
+            b += q < static_cast<int>(blockIdx.x) ? h : 0;
+        }
+        total[tid] = t, before[tid] = b;
+    }
+    for (int b = tid; b < kSortWaves * kMaxBins; b += kSortThreads) (&count[0][0])[b] = 0;
+    __syncthreads();
+    // a wave has `items` / kSortWaves tokens that lie one after the other
+    const int64_t begin = static_cast<int64_t>(blockIdx.x) * items + wave * (items / kSortWaves);
+    const int64_t end = begin + items / kSortWaves < a.n ? begin + items / kSortWaves : a.n;
+    auto key_of = [&](int64_t i) { return FIRST ? sort_key(a, i) : keys[i]; };
+#pragma unroll 4
+    for (int64_t i = begin + lane; i < end; i += kWave) atomicAdd(&count[wave][key_of(i) >> shift & (bins - 1)], 1u);
+    __syncthreads();
+    uint32_t here = 0, all = 0;
+    if (tid < bins) {
+        if constexpr (SCATTER) {
+            for (int q = tid; q < kSortThreads; q += bins) all += total[q], here += before[q];
+        } else {
+#pragma unroll
+            for (int w = 0; w < kSortWaves; ++w) all += count[w][tid];
+            hist[static_cast<int64_t>(blockIdx.x) * bins + tid] = all;
+        }
+    }
+    if constexpr (SCATTER) {
+        here += scan_before(all, wave_total);
+        if (tid < bins) {
+#pragma unroll
+            for (int w = 0; w < kSortWaves; ++w) {
+                const uint32_t c = count[w][tid];
+                count[w][tid] = here;
+                here += c;
+            }
+        }
+        __syncthreads();
+        place_items(count[wave], begin, end, shift, bits, key_of, [&](uint32_t at, uint32_t key, int64_t i) {
+            keys_out[at] = key;
+            index_out[at] = FIRST ? static_cast<uint32_t>(i) : index[i];
+        });
+    }
+}
+
+// All passes over at most kFewTokens tokens by one workgroup, in LDS; the others write zeros.
+__global__ __launch_bounds__(kSortThreads) void embedding_sort_few_kernel(const EmbeddingArgs a, uint32_t *keys_out,
+                                                                          uint32_t *index_out, int passes, int bits,
+                                                                          const Fill fill) {
+    __shared__ uint32_t count[kSortWaves][kMaxBins];
+    __shared__ uint32_t wave_total[kSortWaves];
+    __shared__ uint32_t keys[2][kFewTokens];
+    __shared__ uint16_t index[2][kFewTokens];
+    if (static_cast<int>(blockIdx.x) >= fill.block) {
+        fill_zeros(a, fill);
+        return;
+    }
+    const int bins = 1 << bits, tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave, n = static_cast<int>(a.n);
+    const int items = (n + kSortThreads - 1) / kSortThreads * kWave, begin = wave * items, end = min(begin + items, n);
+#pragma unroll 4
+    for (int i = tid; i < n; i += kSortThreads) keys[0][i] = sort_key(a, i), index[0][i] = static_cast<uint16_t>(i);
+    for (int p = 0; p < passes; ++p) {
+        const uint32_t *k = keys[p & 1];
+        const uint16_t *x = index[p & 1];
+        const int shift = p * bits;
+        for (int b = tid; b < kSortWaves * kMaxBins; b += kSortThreads) (&count[0][0])[b] = 0;
+        __syncthreads();
+        for (int i = begin + lane; i < end; i += kWave) atomicAdd(&count[wave][k[i] >> shift & (bins - 1)], 1u);
+        __syncthreads();
+        uint32_t all = 0;
+        if (tid < bins) {
+#pragma unroll
+            for (int w = 0; w < kSortWaves; ++w) all += count[w][tid];
+        }
+        uint32_t here = scan_before(all, wave_total);
+        if (tid < bins) {
+#pragma unroll
+            for (int w = 0; w < kSortWaves; ++w) {
+                const uint32_t c = count[w][tid];
+                count[w][tid] = here;
+                here += c;
+            }
+        }
+        __syncthreads();
+        const bool last = p + 1 == passes;
+        place_items(count[wave], begin, end, shift, bits, [&](int64_t i) { return k[i]; }, [&](uint32_t at, uint32_t key, int64_t i) {
+            if (last) {
+                keys_out[at] = key;
+                index_out[at] = x[i];
+            } else {
+                keys[~p & 1][at] = key;
+                index[~p & 1][at] = x[i];
+            }
+        });
+        __syncthreads();
+    }
+}
+
+// Chunks of sorted rows, 16 bytes of columns a thread.  part: [chunks][2][vecs VE], of the id
+// that reaches in from the chunk before (0) and of the one that begins here and reaches on (1).
 template <int DT>
 __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const EmbeddingArgs a, const uint32_t *keys,
-                                                                 const uint32_t *index, float *part, int vecs,
-                                                                 uint32_t sum_blocks) {
+                                                                 const uint32_t *index, float *part, int vecs) {
     constexpr int VE = kVec<DT>, es = Columns<DT>::es;
     const uint32_t V = static_cast<uint32_t>(a.V), n = static_cast<uint32_t>(a.n);
     char *dw = static_cast<char *>(a.dweight);
-    if (blockIdx.x >= sum_blocks) {
-        __shared__ uint32_t absent[kZeroRows];
-        const uint32_t first = (blockIdx.x - sum_blocks) * kZeroRows;
-        if (threadIdx.x < kZeroRows) {
-            const uint32_t v = first + threadIdx.x;
-            uint32_t lo = 0, hi = n;  // the first place with a key of at least v
-            while (lo < hi) {
-                const uint32_t mid = lo + (hi - lo) / 2;
-                if (keys[mid] < v) lo = mid + 1;
-                else hi = mid;
-            }
-            absent[threadIdx.x] = v < V && !(lo < n && keys[lo] == v);
-        }
-        __syncthreads();
-        const uint32_t items = static_cast<uint32_t>(vecs) * kZeroRows;
-        for (uint32_t q = threadIdx.x; q < items; q += kThreads) {
-            const uint32_t r = q / vecs;
-            if (absent[r])
-                Columns<DT>(q - r * vecs, a.C).store(dw + static_cast<int64_t>(first + r) * a.C * es, u32x4{0, 0, 0, 0});
-        }
-        return;
-    }
     const uint32_t item = blockIdx.x * kThreads + threadIdx.x, chunk = item / static_cast<uint32_t>(vecs);
     const uint32_t begin = chunk * kChunk;
     if (begin >= n) return;
@@ -260,22 +336,32 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const Embedding
             at.store(dw + static_cast<int64_t>(cur) * a.C * es, narrow<DT>(x));
         }
     };
-    constexpr int U = 8;
-    for (uint32_t i = begin; i < end; i += U) {
-        uint32_t key[U];
-        u32x4 v[U];
+    constexpr int U = kRows;
+    uint32_t key[U], row[U];
+    auto fetch = [&](uint32_t i) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            key[u] = i + u < end ? keys[i + u] : V;
-            v[u] = u32x4{0, 0, 0, 0};
-            if (key[u] < V) v[u] = at.load(static_cast<const char *>(a.dy) + static_cast<int64_t>(index[i + u]) * a.ldy * es);
+            const uint32_t q = i + u < end ? i + u : end - 1;
+            key[u] = keys[q], row[u] = index[q];
         }
+    };
+    fetch(begin);
+    for (uint32_t i = begin; i < end; i += U) {
+        u32x4 v[U];
+        uint32_t k[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            k[u] = key[u];
+            v[u] = u32x4{0, 0, 0, 0};
+            if (k[u] < V) v[u] = at.load(static_cast<const char *>(a.dy) + static_cast<int64_t>(row[u]) * a.ldy * es);
+        }
+        if (i + U < end) fetch(i + U);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (i + u >= end) break;
-            if (key[u] != cur) {
+            if (k[u] != cur) {
                 finish(false);
-                cur = key[u];
+                cur = k[u];
                 reaches_in = false;
 #pragma unroll
                 for (int j = 0; j < VE; ++j) acc[j] = 0.f;
@@ -289,31 +375,49 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const Embedding
     finish(cur == follows);
 }
 
-// The ids that begin in a chunk and reach over its end: their parts, in order.
+// The ids that begin in chunk blockIdx.x and reach over its end: their parts, wave w the w-th,
+// (w + 4)-th .. of them, then the waves' sums; four columns a lane.
 template <int DT>
 __global__ __launch_bounds__(kThreads) void embedding_join_kernel(const EmbeddingArgs a, const uint32_t *keys,
                                                                   const float *part, int vecs) {
-    constexpr int VE = kVec<DT>, es = Columns<DT>::es;
-    const uint32_t n = static_cast<uint32_t>(a.n);
-    const uint32_t item = blockIdx.x * kThreads + threadIdx.x, chunk = item / static_cast<uint32_t>(vecs);
-    const uint32_t begin = chunk * kChunk, end = begin + kChunk;
+    constexpr int VE = kVec<DT>;
+    __shared__ f32x4 sums[kWaves][kWave];
+    __shared__ uint32_t reach[kWaves];
+    const uint32_t n = static_cast<uint32_t>(a.n), chunk = blockIdx.x, begin = chunk * kChunk, end = begin + kChunk;
     if (end >= n) return;
     const uint32_t key = keys[end];
-    if (key >= static_cast<uint32_t>(a.V) || keys[end - 1] != key || (keys[begin] == key && begin > 0 && keys[begin - 1] == key))
-        return;
-    const int vec = item - chunk * vecs;
-    float acc[VE];
-    const float *p = part + ((static_cast<int64_t>(chunk) * 2 + 1) * vecs + vec) * VE;
-#pragma unroll
-    for (int j = 0; j < VE; ++j) acc[j] = p[j];
-    for (uint32_t c = chunk + 1; c * kChunk < n && keys[c * kChunk] == key; ++c) {
-        p = part + ((static_cast<int64_t>(c) * 2) * vecs + vec) * VE;
-#pragma unroll
-        for (int j = 0; j < VE; ++j) acc[j] += p[j];
+    if (key >= static_cast<uint32_t>(a.V) || keys[end - 1] != key || (begin > 0 && keys[begin - 1] == key)) return;
+    // the chunks behind that begin with the id: the keys are sorted, so they are the first ones
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    uint32_t count = 0;
+    for (;;) {
+        const uint64_t at = (static_cast<uint64_t>(chunk) + 1 + count + threadIdx.x) * kChunk;
+        const uint32_t here = __popcll(__ballot(at < n && keys[at] == key));
+        if (lane == 0) reach[wave] = here;
+        __syncthreads();
+        const uint32_t all = reach[0] + reach[1] + reach[2] + reach[3];
+        __syncthreads();
+        count += all;
+        if (all < kThreads) break;
     }
+    const int slot = (blockIdx.y * kWave + lane) * 4, width = vecs * VE;  // columns as the parts have them
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    if (slot < width) {
+        // part 0 is this chunk's, part c > 0 that of the c-th chunk behind
+        auto part_of = [&](uint32_t c) {
+            return *reinterpret_cast<const f32x4 *>(part + (static_cast<int64_t>(chunk + c) * 2 + (c == 0)) * width + slot);
+        };
+#pragma unroll 8
+        for (uint32_t c = wave; c <= count; c += kWaves) acc += part_of(c);
+    }
+    sums[wave][lane] = acc;
+    __syncthreads();
+    if (wave != 0 || slot >= width) return;
+    acc = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+    const int vec = slot / VE, first = a.C < VE ? 0 : vec * VE + VE <= a.C ? vec * VE : a.C - VE, col = first + slot % VE;
 #pragma unroll
-    for (int j = 0; j < VE; ++j) acc[j] *= a.scale;
-    Columns<DT>(vec, a.C).store(static_cast<char *>(a.dweight) + static_cast<int64_t>(key) * a.C * es, narrow<DT>(acc));
+    for (int j = 0; j < 4; ++j)
+        if (col + j < a.C) store_elem(a.dweight, static_cast<int64_t>(key) * a.C + col + j, DT, acc[j] * a.scale);
 }
 
 namespace {
@@ -329,7 +433,8 @@ Plan plan(int64_t n, int64_t V, int C) {
     while (bits < 32 && (static_cast<int64_t>(1) << bits) <= V) ++bits;  // keys 0 .. V
     p.passes = (bits + kMaxBits - 1) / kMaxBits;
     p.bits = (bits + p.passes - 1) / p.passes;
-    const int64_t per = (n + kSortBlocks - 1) / kSortBlocks, items = per < kSortItems ? kSortItems : (per + kThreads - 1) / kThreads * kThreads;
+    const int64_t per = (n + kSortBlocks - 1) / kSortBlocks;
+    const int64_t items = per < kSortItems ? kSortItems : (per + kSortThreads - 1) / kSortThreads * kSortThreads;
     p.items = static_cast<int>(items);
     p.blocks = static_cast<int>((n + items - 1) / items);
     p.chunks = (n + kChunk - 1) / kChunk;
@@ -362,23 +467,40 @@ void run_backward(const EmbeddingArgs &a, hipStream_t s) {
     uint32_t *hist = reinterpret_cast<uint32_t *>(w + 4 * p.keys_bytes);
     float *part = reinterpret_cast<float *>(w + 4 * p.keys_bytes + p.hist_bytes);
     const uint32_t *keys = nullptr, *index = nullptr;
-    const dim3 grid(p.blocks), block(kThreads);
-    for (int i = 0; i < p.passes; ++i) {
+    const dim3 sort(kSortThreads);
+    // the launches of the sort, each with its share of the zeros
+    const bool few = a.n <= kFewTokens;
+    const int launches = few ? 1 : 2 * p.passes;
+    const int64_t zeros = a.V * a.C * Columns<DT>::es / 16 + 1, share = (zeros + launches - 1) / launches;
+    int launch = 0;
+    auto next = [&](int blocks, Fill &f) {
+        f.block = blocks;
+        f.from = share * launch++;
+        f.to = f.from + share;
+        constexpr int per = kSortThreads * 4;
+        return dim3(static_cast<unsigned>(blocks + (share + per - 1) / per));
+    };
+    Fill f;
+    if (few) {
+        const dim3 grid = next(1, f);
+        hipLaunchKernelGGL(embedding_sort_few_kernel, grid, sort, 0, s, a, buf[0], buf[1], p.passes, p.bits, f);
+        keys = buf[0], index = buf[1];
+    }
+    for (int i = 0; i < p.passes && !few; ++i) {
         uint32_t *ko = buf[i % 2 * 2], *io = buf[i % 2 * 2 + 1];
         const int shift = i * p.bits;
-        if (i == 0) {
-            hipLaunchKernelGGL((embedding_sort_kernel<true, false>), grid, block, 0, s, a, keys, index, ko, io, hist, shift, p.bits, p.items);
-            hipLaunchKernelGGL((embedding_sort_kernel<true, true>), grid, block, 0, s, a, keys, index, ko, io, hist, shift, p.bits, p.items);
-        } else {
-            hipLaunchKernelGGL((embedding_sort_kernel<false, false>), grid, block, 0, s, a, keys, index, ko, io, hist, shift, p.bits, p.items);
-            hipLaunchKernelGGL((embedding_sort_kernel<false, true>), grid, block, 0, s, a, keys, index, ko, io, hist, shift, p.bits, p.items);
+        for (int scatter = 0; scatter < 2; ++scatter) {
+            const dim3 grid = next(p.blocks, f);
+            const auto kernel = i == 0 ? (scatter ? embedding_sort_kernel<true, true> : embedding_sort_kernel<true, false>)
+                                       : (scatter ? embedding_sort_kernel<false, true> : embedding_sort_kernel<false, false>);
+            hipLaunchKernelGGL(kernel, grid, sort, 0, s, a, keys, index, ko, io, hist, shift, p.bits, p.items, f);
         }
         keys = ko, index = io;
     }
-    const uint32_t sum_blocks = static_cast<uint32_t>((p.chunks * vecs + kThreads - 1) / kThreads);
-    const uint32_t zero_blocks = static_cast<uint32_t>((a.V + kZeroRows - 1) / kZeroRows);
-    hipLaunchKernelGGL(embedding_sum_kernel<DT>, dim3(sum_blocks + zero_blocks), block, 0, s, a, keys, index, part, vecs, sum_blocks);
-    hipLaunchKernelGGL(embedding_join_kernel<DT>, dim3(sum_blocks), block, 0, s, a, keys, part, vecs);
+    const dim3 grid(static_cast<unsigned>((p.chunks * vecs + kThreads - 1) / kThreads)), block(kThreads);
+    hipLaunchKernelGGL(embedding_sum_kernel<DT>, grid, block, 0, s, a, keys, index, part, vecs);
+    const dim3 join(static_cast<unsigned>(p.chunks), static_cast<unsigned>((vecs * kVec<DT> + 4 * kWave - 1) / (4 * kWave)));
+    if (p.chunks > 1) hipLaunchKernelGGL(embedding_join_kernel<DT>, join, block, 0, s, a, keys, part, vecs);
 }
 
 }  // namespace
@@ -390,8 +512,9 @@ size_t embedding_workspace_bytes(int64_t n, int64_t V, int C) {
 
 bool embedding_grid_fits(int64_t n, int64_t V, int C, int dt) {
     const Plan p = plan(n, V, C);
-    const int64_t vecs = (C + (dt == PRIME_F32 ? 3 : 7)) / (dt == PRIME_F32 ? 4 : 8);
-    return p.chunks * vecs + ((V + kZeroRows - 1) / kZeroRows + 1) * kThreads < (int64_t{1} << 32) - kThreads;
+    const int64_t vecs = (C + (dt == PRIME_F32 ? 3 : 7)) / (dt == PRIME_F32 ? 4 : 8), limit = (int64_t{1} << 32) - kSortThreads;
+    const int64_t fill = V * C * (dt == PRIME_F32 ? 4 : 2) / 64 + kSortThreads;  // threads, of one launch at most
+    return p.chunks * vecs < limit && p.chunks * kThreads < limit && fill + p.blocks * kSortThreads < limit;
 }
 
 hipError_t launch_embedding(const EmbeddingArgs &a, bool backward, hipStream_t stream) {
