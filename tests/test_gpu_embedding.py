@@ -46,7 +46,9 @@ def check(ids, weight, dy, scale=1.0, padding=None):
     (33, 3, 16, "ranked"), (64, 300, 64, "uniform"), (65, 511, 33, "sorted"), (255, 512, 24, "outside"),
     (1000, 513, 100, "ranked"), (1024, 40, 128, "same"), (1025, 50304, 40, "ranked"), (4097, 1000, 65, "same"),
     (2331, 32000, 501, "ranked"), (5000, 262143, 5, "uniform"), (5000, 262144, 5, "uniform"), (3000, 300000, 8, "outside"),
-    (70000, 50304, 64, "ranked"), (600000, 2000, 16, "ranked")])
+    (70000, 50304, 64, "ranked"), (600000, 2000, 16, "ranked"), (131072, 128, 8, "uniform"), (131073, 129, 8, "uniform"),
+    (140000, 3, 24, "outside"), (150000, 262145, 5, "outside"), (30000, 70000, 520, "ranked"), (17000, 65537, 1030, "ranked"),
+    (16384, 20, 700, "outside"), (16383, 20, 700, "outside")])
 def test_lookup_and_gradient(dtype, n, V, C, kind):
     g = gen(n * 7 + V)
     ids = make_ids(kind, (n,), V, g)
@@ -96,6 +98,28 @@ def test_gradient_is_the_lookup_turned_round():
     grad, = torch.autograd.grad(embedding_lookup(ids, w, 4.0), w, dy)
     step = embedding_lookup(ids, W + D, 4.0) - embedding_lookup(ids, W, 4.0)
     assert (dy.double() * step.double()).sum() == (grad.double() * D.double()).sum()
+
+
+@pytest.mark.parametrize("n", [40, 700, 16383, 16384, 40000, 140000])
+@pytest.mark.parametrize("ids64", [True, False])
+def test_runs_of_every_length(n, ids64):
+    """Ids that occur 1, 2, .. 100 times, in turn and at every place of a chunk, some of them
+    thousands of times, some outside the table: whole numbers, so that the sums are exact."""
+    g = gen(n)
+    lengths = [*range(1, 101), 3000, 1, 64, 31, 32, 33, 7, 8, 9, 5000, 15, 16, 17, 65, 96, 97]
+    runs = []
+    while sum(runs) < n:
+        runs += lengths[len(runs) % 7:]
+    keys = torch.repeat_interleave(torch.arange(len(runs), device="cuda"), torch.tensor(runs, device="cuda"))[:n]
+    V = int(keys.max()) + 1
+    mixed = torch.randperm(V + 9, generator=g, device="cuda")[keys]  # (some above the table)
+    ids = mixed[torch.randperm(n, generator=g, device="cuda")]
+    dy = torch.randint(-4, 5, (n, 70), generator=g, device="cuda").float()
+    w = torch.zeros(V, 70, device="cuda").requires_grad_()
+    for order in (ids, mixed):
+        grad, = torch.autograd.grad(embedding_lookup(order if ids64 else order.int(), w, 0.5), w, dy)
+        want, _ = R.lookup_grad(order, dy, V, 0.5)
+        assert torch.equal(grad.cpu().double(), want)
 
 
 def test_values_that_are_not_finite_stay_in_their_rows():
