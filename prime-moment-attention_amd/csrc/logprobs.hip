@@ -67,10 +67,20 @@ __device__ __forceinline__ uint32_t rank_key(float x) {
     const uint32_t b = __float_as_uint(x + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float key_logit(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
 
+// Largest over the lanes, in every lane, on the vector unit.
 __device__ __forceinline__ float wave_max(float x) {
-    for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, kWave));
-    return x;
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+    x = fmaxf(x, xor_lane<8>(x));
+    x = fmaxf(x, xor_lane<4>(x));
+    x = fmaxf(x, xor_lane<2>(x));
+    return fmaxf(x, xor_lane<1>(x));
 }
 
 // One row of a group of threads: WAVES waves of one workgroup, or (WAVES = 1) one wave of a
@@ -82,6 +92,7 @@ struct Group {
     __device__ __forceinline__ int thread() const { return threadIdx.x % kThreads; }
     __device__ __forceinline__ void sync() const {
         if constexpr (WAVES > 1) __syncthreads();
+        else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     __device__ float sum(float x) const {
         x = wave_sum(x);
@@ -155,18 +166,144 @@ __device__ __noinline__ Careful careful(const Group<WAVES> g, const char *row, i
 
 }  // namespace
 
+namespace {
+
+// What a group keeps in LDS.
+template <int WAVES>
+struct Shared {
+    static constexpr int kList = WAVES == 1 ? 512 : 1024;
+    __attribute__((aligned(16))) float red[4 * WAVES];
+    uint64_t list[kList];
+    uint32_t count;
+};
+
+// A value that at least `top` of the row's logits reach, and not many more: `best` is each
+// lane's largest.  The j-th largest lane of the wave in which that is smallest: with W waves and
+// j = top / W rounded up, W j lanes reach it.
+template <int WAVES>
+__device__ __forceinline__ float threshold(const Group<WAVES> &g, float best, int top) {
+    const int lane = threadIdx.x % kWave;
+    float mine;
+#pragma unroll 1
+    for (int j = 0; j < top; j += WAVES) {
+        mine = wave_max(best);
+        if (lane == __builtin_ctzll(__ballot(best == mine))) best = -kInf;
+    }
+    if constexpr (WAVES == 1) return mine;
+    g.sync();
+    if (lane == 0) g.red[threadIdx.x / kWave] = mine;
+    g.sync();
+    float least = g.red[0];
+    for (int w = 1; w < WAVES; ++w) least = fminf(least, g.red[w]);
+    return least;
+}
+
+// The `top` first tokens in the order of rank_key, equal ones by index: write(rank, token,
+// logit).  Those at the threshold or above are listed and ranked among each other; if they are
+// too many, those above it, and the first ones equal to it by index (a row with few tokens that
+// are not -infinity, or with equal logits); if these are too many, one after the other.
+// best: the lane's largest; tail: those of its vectors from `full` on.
+template <int DT, int WAVES, int U, typename W>
+__device__ __forceinline__ void likeliest(const Group<WAVES> &g, Shared<WAVES> &sh, const char *row, int vocab, int top,
+                                          float best, int full, const float (&tail)[U], W write) {
+    constexpr int VE = kVec<DT>, kThreads = WAVES * kWave, kList = Shared<WAVES>::kList;
+    const int tid = g.thread(), whole = vocab / VE;
+    const uint32_t bar = rank_key(threshold<WAVES>(g, best, top)), own = rank_key(best);
+    auto gather = [&](uint32_t least) {  // how many have a key of at least `least`; the first kList are listed
+        if (tid == 0) sh.count = 0;
+        g.sync();
+        auto take = [&](float x, int j) {
+            const uint32_t k = rank_key(x);
+            if (k < least) return;
+            const uint32_t at = atomicAdd(&sh.count, 1u);
+            if (at < kList) sh.list[at] = static_cast<uint64_t>(k) << 32 | static_cast<uint32_t>(~j);
+        };
+        auto take_vector = [&](const u32x4 &v, int i) {
+            float x[VE];
+            widen<DT>(v, x);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) take(x[e], i * VE + e);
+        };
+        if (own >= least) {
+            int i = tid;
+#pragma unroll 1
+            for (; i - tid < full; i += U * kThreads) {
+                u32x4 v[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) v[u] = reinterpret_cast<const Raw *>(row)[i + u * kThreads].v;
+#pragma unroll
+                for (int u = 0; u < U; ++u) take_vector(v[u], i + u * kThreads);
+            }
+            uint32_t reach = 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) reach |= (i + u * kThreads < whole && rank_key(tail[u]) >= least) << u;
+#pragma unroll 1
+            for (; reach; reach &= reach - 1) {
+                const int at = i + __builtin_ctz(reach) * kThreads;
+                take_vector(reinterpret_cast<const Raw *>(row)[at].v, at);
+            }
+            if (const int j = whole * VE + tid; j < vocab) take(load_elem(row, j, DT), j);
+        }
+        g.sync();
+        return sh.count;
+    };
+    uint32_t count = gather(bar);
+    int equal = 0;  // of the tokens at the threshold, how many are still wanted
+    if (count > kList) {
+        g.sync();
+        count = gather(bar + 1);
+        equal = count < static_cast<uint32_t>(top) ? top - count : 0;
+    }
+    auto give = [&](int rank, uint64_t key) { write(rank, static_cast<int>(~static_cast<uint32_t>(key)), key_logit(key >> 32)); };
+    if (count <= kList) {
+        for (uint32_t c = tid; c < count; c += kThreads) {
+            const uint64_t key = sh.list[c];
+            int rank = 0;
+#pragma unroll 4
+            for (uint32_t o = 0; o < count; ++o) rank += sh.list[o] > key;
+            if (rank < top) give(rank, key);
+        }
+        if (equal && tid < kWave) {  // one wave, in the order of the tokens
+            int rank = top - equal;
+            for (int j0 = 0; j0 < vocab && rank < top; j0 += kWave) {
+                const int j = j0 + tid;
+                const bool is = j < vocab && rank_key(load_elem(row, j, DT)) == bar;
+                const uint64_t all = __ballot(is);
+                const int at = rank + __popcll(all & ((1ull << tid) - 1));
+                if (is && at < top) write(at, j, key_logit(bar));
+                rank += __popcll(all);
+            }
+        }
+        return;
+    }
+    uint64_t last = ~0ull;
+#pragma unroll 1
+    for (int r = 0; r < top; ++r) {
+        uint64_t next = 0;
+        for (int j = tid; j < vocab; j += kThreads) {
+            const uint64_t key = static_cast<uint64_t>(rank_key(load_elem(row, j, DT))) << 32 | static_cast<uint32_t>(~j);
+            if (key < last) next = max_u64(next, key);
+        }
+        last = g.max(next);
+        if (tid == 0) give(r, last);
+    }
+}
+
+}  // namespace
+
 // WAVES > 1: one row a workgroup.  WAVES = 1: one row a wave, four a workgroup.
 template <int DT, int WAVES, bool ENTROPY>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void logprobs_kernel(const LogprobsArgs a) {
-    constexpr int VE = kVec<DT>, U = 4, es = DT == PRIME_F32 ? 4 : 2, kThreads = WAVES * kWave;
-    __shared__ __attribute__((aligned(8))) float red[4 * WAVES];
-    const Group<WAVES> g{red};
+    constexpr int VE = kVec<DT>, U = WAVES == 16 ? 8 : 4, es = DT == PRIME_F32 ? 4 : 2, kThreads = WAVES * kWave;
+    __shared__ Shared<WAVES> shared[WAVES == 1 ? 4 : 1];
+    Shared<WAVES> &sh = shared[WAVES == 1 ? threadIdx.x / kWave : 0];
+    const Group<WAVES> g{sh.red};
     const int row = WAVES == 1 ? blockIdx.x * 4 + threadIdx.x / kWave : blockIdx.x;
     if (WAVES == 1 && row >= a.n) return;
     const int tid = g.thread();
     const char *base = static_cast<const char *>(a.logits) + a.stride_n * es * row;
     const int64_t token = a.tokens[row];
-    const bool known = token != a.ignore;
+    const bool known = token != a.ignore, inside = token >= 0 && token < a.vocab;
     if (!ENTROPY && !a.top && !known) {  // nothing of this row is asked for
         if (tid == 0) {
             a.logprobs[row] = 0.f;
@@ -174,6 +311,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void logprobs_ker
         }
         return;
     }
+    const float at_token = inside ? load_elem(base, token, DT) : 0.f;
     float top = -kInf, m = kLowest, c = reference(kLowest), s = 0.f, t = 0.f;
     auto add = [&](auto count, const float *x) {
         constexpr int N = decltype(count)::value;
@@ -182,7 +320,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void logprobs_ker
         for (int j = 1; j < N; ++j) tm = fmaxf(tm, x[j]);
         top = fmaxf(top, tm);
         m = fmaxf(m, tm);
-        const float nc = reference(m), by = c - nc, f = exp2f(by);
+        const float nc = reference(m), by = c - nc, f = __builtin_amdgcn_exp2f(by);
         if constexpr (ENTROPY) t = f * fmaf(by, s, t);
         s *= f;
         c = nc;
@@ -192,10 +330,11 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void logprobs_ker
             s += e;
             if constexpr (ENTROPY) t = fmaf(e, fmaxf(d, kFloor), t);
         }
+        return tm;
     };
-    const int whole = a.vocab / VE;  // vectors
+    const int whole = a.vocab / VE, full = whole / (U * kThreads) * (U * kThreads);  // vectors
     int i = tid;
-    for (; i + (U - 1) * kThreads < whole; i += U * kThreads) {
+    for (; i - tid < full; i += U * kThreads) {
         u32x4 v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u] = reinterpret_cast<const Raw *>(base)[i + u * kThreads].v;
@@ -204,19 +343,47 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void logprobs_ker
         for (int u = 0; u < U; ++u) widen<DT>(v[u], x[u]);
         add(std::integral_constant<int, U * VE>{}, &x[0][0]);
     }
-    for (; i < whole; i += kThreads) {
-        float x[VE];
-        widen<DT>(reinterpret_cast<const Raw *>(base)[i].v, x);
-        add(std::integral_constant<int, VE>{}, x);
+    float tail[U];  // the largest of each of the last vectors
+#pragma unroll
+    for (int u = 0; u < U; ++u) tail[u] = -kInf;
+    if (i - tid < whole) {  // all on their way at once
+        u32x4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i - tid + u * kThreads < whole) v[u] = reinterpret_cast<const Raw *>(base)[min(i + u * kThreads, whole - 1)].v;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i - tid + u * kThreads >= whole) break;
+            if (i + u * kThreads >= whole) continue;
+            float x[VE];
+            widen<DT>(v[u], x);
+            tail[u] = add(std::integral_constant<int, VE>{}, x);
+        }
     }
     if (const int j = whole * VE + tid; j < a.vocab) {
         const float x = load_elem(base, j, DT);
         add(std::integral_constant<int, 1>{}, &x);
     }
-    const float all = g.max(top);
-    const float C = reference(fmaxf(all, kLowest)), by = c - C, f = exp2f(by);
-    if constexpr (ENTROPY) t = g.sum(f * fmaf(by, s, t));
-    s = g.sum(s * f);
+    // the wave's, then all waves'
+    float all = wave_max(top), C = reference(fmaxf(all, kLowest)), by = c - C, f = __builtin_amdgcn_exp2f(by);
+    if constexpr (ENTROPY) t = wave_sum(f * fmaf(by, s, t));
+    s = wave_sum(s * f);
+    if constexpr (WAVES > 1) {
+        if (threadIdx.x % kWave == 0) {
+            float *r = sh.red + threadIdx.x / kWave * 4;
+            r[0] = all, r[1] = s, r[2] = t;
+        }
+        g.sync();
+        for (int w = 0; w < WAVES; ++w) all = fmaxf(all, sh.red[4 * w]);
+        C = reference(fmaxf(all, kLowest)), s = 0.f, t = 0.f;
+#pragma unroll 4
+        for (int w = 0; w < WAVES; ++w) {
+            const f32x4 r = *reinterpret_cast<const f32x4 *>(sh.red + 4 * w);
+            by = reference(fmaxf(r[0], kLowest)) - C, f = __builtin_amdgcn_exp2f(by);
+            if constexpr (ENTROPY) t = fmaf(f, fmaf(by, r[1], r[2]), t);
+            s = fmaf(f, r[1], s);
+        }
+    }
     const bool fine = s > 0.f && s < kInf && all > kLowest && all < kHighest;  // (NaN: false)
     const float L = log2f(s);
     Careful k{};
@@ -227,27 +394,16 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void logprobs_ker
         return d > kLowest ? (d - L) * kLn2 : x - all;  // (in powers of 2 it may be beyond fp32)
     };
     if (tid == 0) {
-        float lp = 0.f;
-        if (known) lp = token >= 0 && token < a.vocab ? logprob(load_elem(base, token, DT)) : __builtin_nanf("");
-        a.logprobs[row] = lp;
+        a.logprobs[row] = !known ? 0.f : inside ? logprob(at_token) : __builtin_nanf("");
         if constexpr (ENTROPY) a.entropy[row] = fine ? (L - t / s) * kLn2 : k.entropy();
         if (a.stats) a.stats[2 * row] = fine ? C : __builtin_nanf(""), a.stats[2 * row + 1] = L;
     }
-    // the likeliest, one after the other: the largest key below the last one's
-    uint64_t last = ~0ull;
-    for (int r = 0; r < a.top; ++r) {
-        uint64_t best = 0;
-        for (int j = tid; j < a.vocab; j += kThreads) {
-            const uint64_t key = static_cast<uint64_t>(rank_key(load_elem(base, j, DT))) << 32 | static_cast<uint32_t>(~j);
-            if (key < last) best = max_u64(best, key);
-        }
-        last = g.max(best);
-        if (tid == 0) {
-            const int64_t id = static_cast<uint32_t>(~last);
-            a.top_tokens[static_cast<int64_t>(row) * a.top + r] = id;
-            a.top_logprobs[static_cast<int64_t>(row) * a.top + r] = logprob(load_elem(base, id, DT));
-        }
-    }
+    if (a.top)
+        likeliest<DT, WAVES>(g, sh, base, a.vocab, a.top, top, full, tail, [&](int rank, int id, float x) {
+            const int64_t at = static_cast<int64_t>(row) * a.top + rank;
+            a.top_tokens[at] = id;
+            a.top_logprobs[at] = logprob(x);
+        });
 }
 
 // The gradient of part blockIdx.x of row blockIdx.y's logits.
@@ -256,7 +412,7 @@ constexpr int kBackThreads = 256, kBackUnroll = 4;
 template <int DT>
 __global__ __launch_bounds__(kBackThreads) void logprobs_backward_kernel(const LogprobsArgs a) {
     constexpr int VE = kVec<DT>, U = kBackUnroll, es = DT == PRIME_F32 ? 4 : 2;
-    __shared__ __attribute__((aligned(8))) float red[4 * kBackThreads / kWave];
+    __shared__ __attribute__((aligned(16))) float red[4 * kBackThreads / kWave];
     const int64_t row = blockIdx.y;
     const char *base = static_cast<const char *>(a.logits) + a.stride_n * es * row;
     char *out = static_cast<char *>(a.dlogits) + a.stride_d * es * row;
@@ -336,7 +492,7 @@ void run(LogprobsArgs a, bool backward, hipStream_t s) {
             hipLaunchKernelGGL(logprobs_backward_kernel<DT>, dim3(parts, a.n), dim3(kBackThreads), 0, s, a);
         } else if (a.vocab <= 2048) {
             forward<DT, 1>(a, s);
-        } else if (n >= 512) {
+        } else if (n >= 512 || a.vocab <= 16384) {
             forward<DT, 4>(a, s);
         } else {
             forward<DT, 16>(a, s);

@@ -105,6 +105,45 @@ def test_rows_out_of_the_ordinary(dtype, V):
         check(x, tokens, 1, True, g)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [600, 2048, 3000, 16385, 50304])
+def test_alternatives_where_they_are_hard_to_tell(dtype, V):
+    """Sorted rows, neighbours that are the largest, coarse and equal logits, ties that reach over
+    the last place, few tokens that are not banned."""
+    g = gen(V)
+    rows = []
+    x = torch.randn(V, generator=g, device="cuda")
+    rows += [x.sort().values, x.sort(descending=True).values, torch.round(x), torch.round(4 * x), x.clamp(max=1.0)]
+    y = x.clone()
+    y[V // 3:V // 3 + 70] = 9.0 + torch.rand(70, generator=g, device="cuda")
+    rows.append(y)
+    y = x.clone()
+    y[::8] += 20.0  # one element of each vector
+    rows.append(y)
+    y = x.clone()
+    y[V - 300:] += 20.0
+    rows.append(y)
+    for count in (1, 3, 19, 63, 64, 200):
+        y = torch.full((V,), -INF, device="cuda")
+        at = torch.randperm(V, generator=g, device="cuda")[:count]
+        y[at] = x[at]
+        rows.append(y)
+    y = torch.zeros(V, device="cuda")
+    y[torch.randperm(V, generator=g, device="cuda")[:10]] = 1.0
+    rows += [y, -y, torch.full((V,), -0.0, device="cuda")]
+    for step in (7, 64, 1024):  # the largest all in the same lanes
+        y = x.clone()
+        y[5::step] = 30.0 + x[5::step]
+        rows.append(y)
+    x = torch.stack(rows).to(dtype)
+    tokens = torch.zeros(len(rows), dtype=torch.int64, device="cuda")
+    for top in (1, 5, 20, 64):
+        r = token_logprobs(x, tokens, top=top)
+        assert torch.equal(r.top_tokens, R.ranked(x, top)), top
+        many = x.repeat(30, 1)
+        assert torch.equal(token_logprobs(many, tokens.repeat(30), top=top).top_tokens, r.top_tokens.repeat(30, 1))
+
+
 def test_tokens_that_do_not_count():
     x = torch.randn(6, 3000, device="cuda")
     tokens = torch.tensor([3, -100, 2999, 3000, -1, -100], device="cuda")
