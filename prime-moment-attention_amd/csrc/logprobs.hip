@@ -175,6 +175,8 @@ struct Shared {
     __attribute__((aligned(16))) float red[4 * WAVES];
     uint64_t list[kList];
     uint32_t count;
+    static constexpr int kBatches = 8;
+    float batch[kBatches][WAVES * kWave];  // each lane's largest of its first batches of vectors
 };
 
 // A value that at least `top` of the row's logits reach, and not many more: `best` is each
@@ -227,7 +229,8 @@ __device__ __forceinline__ void likeliest(const Group<WAVES> &g, Shared<WAVES> &
         if (own >= least) {
             int i = tid;
 #pragma unroll 1
-            for (; i - tid < full; i += U * kThreads) {
+            for (int b = 0; i - tid < full; i += U * kThreads, ++b) {
+                if (b < Shared<WAVES>::kBatches && rank_key(sh.batch[b][tid]) < least) continue;
                 u32x4 v[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) v[u] = reinterpret_cast<const Raw *>(row)[i + u * kThreads].v;
@@ -334,14 +337,15 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void logprobs_ker
     };
     const int whole = a.vocab / VE, full = whole / (U * kThreads) * (U * kThreads);  // vectors
     int i = tid;
-    for (; i - tid < full; i += U * kThreads) {
+    for (int b = 0; i - tid < full; i += U * kThreads, ++b) {
         u32x4 v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u] = reinterpret_cast<const Raw *>(base)[i + u * kThreads].v;
         float x[U][VE];
 #pragma unroll
         for (int u = 0; u < U; ++u) widen<DT>(v[u], x[u]);
-        add(std::integral_constant<int, U * VE>{}, &x[0][0]);
+        const float most = add(std::integral_constant<int, U * VE>{}, &x[0][0]);
+        if (a.top && b < Shared<WAVES>::kBatches) sh.batch[b][tid] = most;
     }
     float tail[U];  // the largest of each of the last vectors
 #pragma unroll
@@ -408,6 +412,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void logprobs_ker
 
 // The gradient of part blockIdx.x of row blockIdx.y's logits.
 constexpr int kBackThreads = 256, kBackUnroll = 4;
+constexpr int kWaveRow = 8192;  // bytes of a row that one wave takes
 
 template <int DT>
 __global__ __launch_bounds__(kBackThreads) void logprobs_backward_kernel(const LogprobsArgs a) {
@@ -490,7 +495,7 @@ void run(LogprobsArgs a, bool backward, hipStream_t s) {
         a.n = n - row < most ? n - row : most;
         if (backward) {
             hipLaunchKernelGGL(logprobs_backward_kernel<DT>, dim3(parts, a.n), dim3(kBackThreads), 0, s, a);
-        } else if (a.vocab <= 2048) {
+        } else if (static_cast<int64_t>(a.vocab) * es <= kWaveRow) {
             forward<DT, 1>(a, s);
         } else if (n >= 512 || a.vocab <= 16384) {
             forward<DT, 4>(a, s);

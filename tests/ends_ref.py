@@ -115,7 +115,7 @@ def row_bounds(x):
     distance to the largest logit in powers of 2:
       2^d_j is off by |d_j| ln 2 (d's rounding and that of log2(e)) and 2 (the instruction);
       a sum of V terms by the additions that one term goes through: V / 256 + 32 in a lane (V / 64
-        for up to 2048), 16 for rescalings and joins;
+        for up to 4096), 16 for rescalings and joins;
       so L = log2 S by  e_L = 1.45 (sum p (2 |d| + 2) + adds) + 4 |L| + 2,
       entropy by        e_H = e_L + 1.45 (sum p |d| (3 |d| + 6 + 2 adds)) + 4 (|L| + sum p |d|) + 4."""
     logp, p = row_probs(x)
@@ -123,7 +123,7 @@ def row_bounds(x):
     V = x.shape[1]
     d = ((x - x.amax(1, keepdim=True)) * math.log2(math.e)).abs()
     d = torch.where(torch.isfinite(d), d, 0.0)
-    adds = (V / 64 if V <= 2048 else V / 256) + 48
+    adds = (V / 64 if V <= 4096 else V / 256) + 48
     mean, square = (p * d).nan_to_num().sum(1), (p * d * d).nan_to_num().sum(1)
     L = -(logp.amax(1) / math.log(2)).nan_to_num(neginf=0.0)
     e_l = 1.45 * (2 * mean + 2 + adds) + 4 * L.abs() + 2
