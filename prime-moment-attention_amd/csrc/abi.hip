@@ -1765,24 +1765,24 @@ struct GradTables {
     const int64_t *sizes;
     const int32_t *dtypes;
     int count, at = 0;
-    static constexpr uint32_t kMinSpan = 512, kMaxBlocks = 2048;
+    static constexpr uint64_t kMaxBlocks = 2048;  // workgroups
     prime::GradTable t;
     int blocks = 0;
 
     bool next() {
         t.count = 0;
-        uint64_t slots = 0;
+        uint64_t pieces = 0;
         for (; at < count && t.count < prime::kGradTable; ++at) {
             if (sizes[at] == 0) continue;
             if (tensors) t.data[t.count] = reinterpret_cast<uintptr_t>(tensors[at]) | static_cast<uint64_t>(dtypes[at]) << 62;
             t.size[t.count] = sizes[at];
-            t.first[t.count++] = static_cast<uint32_t>(slots);
-            slots += static_cast<uint64_t>(sizes[at] + 7) / 8;
+            t.first[t.count++] = static_cast<uint32_t>(pieces);
+            pieces += (static_cast<uint64_t>(sizes[at]) + prime::kGradBlock - 1) / prime::kGradBlock;
         }
-        t.first[t.count] = static_cast<uint32_t>(slots);
-        const uint64_t span = std::max<uint64_t>(kMinSpan, (slots + kMaxBlocks - 1) / kMaxBlocks);
+        t.first[t.count] = static_cast<uint32_t>(pieces);
+        const uint64_t span = std::max<uint64_t>(1, (pieces + 4 * kMaxBlocks - 1) / (4 * kMaxBlocks));
         t.span = static_cast<uint32_t>(span);
-        blocks = static_cast<int>((slots + span - 1) / span);
+        blocks = static_cast<int>((pieces + 4 * span - 1) / (4 * span));
         return t.count > 0;
     }
 };
@@ -1793,15 +1793,14 @@ int grad_checks(const void *const *tensors, const int64_t *sizes, const int32_t 
         return fail(PRIME_ERR_INVALID_ARG, "null tensors, sizes, dtypes or norm");
     int rc = check_floats(norm, "norm");
     if (rc) return rc;
-    int64_t slots = 0;
+    int64_t all = 0;
     for (int i = 0; i < count; ++i) {
         if (!valid_dtype(dtypes[i])) return fail(PRIME_ERR_UNSUPPORTED_DTYPE, "unsupported dtype of tensor %d", i);
         if (sizes[i] < 0 || sizes[i] >= (int64_t{1} << 35) || (sizes[i] && !tensors[i]))
             return fail(PRIME_ERR_INVALID_ARG, "tensor %d: null, or %lld elements", i, static_cast<long long>(sizes[i]));
         if (sizes[i] && reinterpret_cast<uintptr_t>(tensors[i]) % elem_size(dtypes[i]))
             return fail(PRIME_ERR_MISALIGNED, "tensor %d is misaligned", i);
-        slots += (sizes[i] + 7) / 8;
-        if (slots >= (int64_t{1} << 32)) return fail(PRIME_ERR_INVALID_ARG, "too many elements");
+        if ((all += sizes[i]) >= (int64_t{1} << 35)) return fail(PRIME_ERR_INVALID_ARG, "too many elements");
     }
     const size_t need = given ? 0 : prime_grad_norm_workspace_size(sizes, count);
     if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u)))

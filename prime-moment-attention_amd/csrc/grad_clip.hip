@@ -1,10 +1,12 @@
 // The norm over many tensors and their scaling by min(1, max_norm / (norm + 1e-6)).
 //
-// The tensors come as a table in the kernel's arguments, counted in slots of 8 elements (a
-// tensor's last one may be ragged); a workgroup has a span of slots that lie one after the
-// other over all tensors, so that spans are equal whatever the tensors' sizes.  Squares are
-// summed in 64 bits, where those of fp32 neither overflow nor vanish, and each span's sum is
-// stored; the scaling's workgroups each add these in the same order.
+// The tensors come as a table in the kernel's arguments, cut into blocks of kGradBlock elements
+// (a tensor's last one may be short): the loads of a block are on their way at once, so that a
+// small tensor costs as much time as one, and a wave has a span of blocks that lie one after
+// the other over all tensors.  Squares are summed in 64 bits, where those of fp32 neither
+// overflow nor vanish, and each workgroup's sum is stored; the scaling's workgroups each add
+// these in the same order.  The scaling goes through a span from its end: what the norm read
+// last is still in the last-level cache.
 
 #include "prime_kernels.h"
 
@@ -71,91 +73,91 @@ __device__ __forceinline__ double block_sum(double x, double *red) {
     return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// f(dtype, pointer, elements) over the tensors' pieces that the workgroup's span holds
-template <typename F>
-__device__ __forceinline__ void each_piece(const GradTable &t, F f) {
-    const uint32_t slots = t.first[t.count];
-    const uint64_t start = blockIdx.x * static_cast<uint64_t>(t.span), behind = start + t.span;
-    if (start >= slots) return;
-    const uint32_t begin = static_cast<uint32_t>(start), end = behind < slots ? static_cast<uint32_t>(behind) : slots;
-    int lo = 0, hi = t.count - 1;  // the last tensor that starts at `begin` or before
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (t.first[mid] <= begin) lo = mid;
-        else hi = mid - 1;
+// f(dtype, pointer, elements) over the blocks of the wave's span, from the last to the first
+// where BACK.
+template <bool BACK, typename F>
+__device__ __forceinline__ void each_block(const GradTable &t, F f) {
+    const uint32_t blocks = t.first[t.count];
+    const uint64_t start = (blockIdx.x * static_cast<uint64_t>(kThreads / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave)) * t.span;
+    if (start >= blocks) return;
+    const uint32_t begin = static_cast<uint32_t>(start), end = start + t.span < blocks ? static_cast<uint32_t>(start + t.span) : blocks;
+    uint32_t b = BACK ? end - 1 : begin;
+    // the tensor with block b: the last that starts there or before; each lane looks at three
+    int k = -1;
+#pragma unroll
+    for (int q = 0; q < kGradTable / kWave; ++q) {
+        const int i = q * kWave + threadIdx.x % kWave;
+        const uint32_t first = t.first[i];
+        k += __popcll(__ballot(i < t.count && first <= b));
     }
-    for (uint32_t at = begin; at < end; ++lo) {
-        const uint32_t stop = min(end, t.first[lo + 1]);
-        const uint64_t word = t.data[lo];
+    for (uint32_t left = end - begin; left;) {
+        // the span's blocks of tensor k
+        const uint32_t first = t.first[k], behind = t.first[k + 1], run = BACK ? min(left, b - first + 1) : min(left, behind - b);
+        const uint64_t word = t.data[k];
         const int dt = static_cast<int>(word >> 62);
-        const int64_t from = static_cast<int64_t>(at - t.first[lo]) * kSlot;
-        const int64_t size = t.size[lo] - from, most = static_cast<int64_t>(stop - at) * kSlot;
-        f(dt, reinterpret_cast<char *>(word & ((1ull << 62) - 1)) + from * (dt == PRIME_F32 ? 4 : 2), size < most ? size : most);
-        at = stop;
+        char *data = reinterpret_cast<char *>(word & ((1ull << 62) - 1));
+        const int64_t size = t.size[k];
+        for (uint32_t r = 0; r < run; ++r) {
+            const int64_t skip = static_cast<int64_t>((BACK ? b - r : b + r) - first) * kGradBlock;
+            f(dt, data + skip * (dt == PRIME_F32 ? 4 : 2), static_cast<int>(min(size - skip, static_cast<int64_t>(kGradBlock))));
+        }
+        left -= run;
+        BACK ? (b -= run, --k) : (b += run, ++k);
     }
 }
 
-template <int DT>
-__device__ __forceinline__ double square_sum(const char *p, int64_t size) {
-    constexpr int U = 4, es = DT == PRIME_F32 ? 4 : 2;
-    double acc[2] = {};
-    const int64_t whole = size / kSlot;
-    int64_t i = threadIdx.x;
-    for (; i + (U - 1) * kThreads < whole; i += U * kThreads) {
+// g(slot's address, values) over a block, all its loads before the first use; then the elements
+// behind the last whole slot: one(address).
+template <int DT, typename G, typename E>
+__device__ __forceinline__ void each_slot(char *p, int size, G g, E one) {
+    constexpr int es = DT == PRIME_F32 ? 4 : 2, bytes = kSlot * es, U = kGradBlock / (kSlot * kWave);
+    const int whole = size / kSlot, lane = threadIdx.x % kWave;
+    if (whole) {
         float x[U][kSlot];
 #pragma unroll
-        for (int u = 0; u < U; ++u) load_slot<DT>(p + (i + u * kThreads) * (kSlot * es), x[u]);
+        for (int u = 0; u < U; ++u) load_slot<DT>(p + min(lane + u * kWave, whole - 1) * bytes, x[u]);
 #pragma unroll
         for (int u = 0; u < U; ++u)
+            if (lane + u * kWave < whole) g(p + (lane + u * kWave) * bytes, x[u]);
+    }
+    if (const int j = whole * kSlot + lane; j < size) one(p + j * es);
+}
+
+template <int DT>
+__device__ __forceinline__ double square_sum(char *p, int size) {
+    double acc[2] = {};
+    each_slot<DT>(
+        p, size,
+        [&](char *, const float (&x)[kSlot]) {
 #pragma unroll
-            for (int j = 0; j < kSlot; ++j) acc[j & 1] = fma(static_cast<double>(x[u][j]), static_cast<double>(x[u][j]), acc[j & 1]);
-    }
-    for (; i < whole; i += kThreads) {
-        float x[kSlot];
-        load_slot<DT>(p + i * (kSlot * es), x);
-#pragma unroll
-        for (int j = 0; j < kSlot; ++j) acc[j & 1] = fma(static_cast<double>(x[j]), static_cast<double>(x[j]), acc[j & 1]);
-    }
-    if (const int64_t j = whole * kSlot + threadIdx.x; j < size) {
-        const double x = load_elem(p, j, DT);
-        acc[0] = fma(x, x, acc[0]);
-    }
+            for (int j = 0; j < kSlot; ++j) acc[j & 1] = fma(static_cast<double>(x[j]), static_cast<double>(x[j]), acc[j & 1]);
+        },
+        [&](char *q) {
+            const double x = load_elem(q, 0, DT);
+            acc[0] = fma(x, x, acc[0]);
+        });
     return acc[0] + acc[1];
 }
 
 template <int DT>
-__device__ __forceinline__ void scale_piece(char *p, int64_t size, float c) {
-    constexpr int U = 4, es = DT == PRIME_F32 ? 4 : 2;
-    const int64_t whole = size / kSlot;
-    int64_t i = threadIdx.x;
-    for (; i + (U - 1) * kThreads < whole; i += U * kThreads) {
-        float x[U][kSlot];
+__device__ __forceinline__ void scale_block(char *p, int size, float c) {
+    each_slot<DT>(
+        p, size,
+        [&](char *q, float (&x)[kSlot]) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) load_slot<DT>(p + (i + u * kThreads) * (kSlot * es), x[u]);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-#pragma unroll
-            for (int j = 0; j < kSlot; ++j) x[u][j] *= c;
-            store_slot<DT>(p + (i + u * kThreads) * (kSlot * es), x[u]);
-        }
-    }
-    for (; i < whole; i += kThreads) {
-        float x[kSlot];
-        load_slot<DT>(p + i * (kSlot * es), x);
-#pragma unroll
-        for (int j = 0; j < kSlot; ++j) x[j] *= c;
-        store_slot<DT>(p + i * (kSlot * es), x);
-    }
-    if (const int64_t j = whole * kSlot + threadIdx.x; j < size) store_elem(p, j, DT, load_elem(p, j, DT) * c);
+            for (int j = 0; j < kSlot; ++j) x[j] *= c;
+            store_slot<DT>(q, x);
+        },
+        [&](char *q) { store_elem(q, 0, DT, load_elem(q, 0, DT) * c); });
 }
 
 }  // namespace
 
-// parts[blockIdx.x]: the span's sum of squares
+// parts[blockIdx.x]: the sum of squares of the workgroup's four spans
 __global__ __launch_bounds__(kThreads) void grad_squares_kernel(const GradTable t, double *parts) {
     __shared__ double red[kThreads / kWave];
     double sum = 0.0;
-    each_piece(t, [&](int dt, char *p, int64_t size) {
+    each_block<false>(t, [&](int dt, char *p, int size) {
         if (dt == PRIME_BF16) sum += square_sum<PRIME_BF16>(p, size);
         else if (dt == PRIME_F16) sum += square_sum<PRIME_F16>(p, size);
         else sum += square_sum<PRIME_F32>(p, size);
@@ -165,9 +167,15 @@ __global__ __launch_bounds__(kThreads) void grad_squares_kernel(const GradTable 
 }
 
 __device__ __forceinline__ double parts_sum(const double *parts, int count, double *red) {
+    constexpr int U = 8;
     double sum = 0.0;
-#pragma unroll 8
-    for (int i = threadIdx.x; i < count; i += kThreads) sum += parts[i];
+    for (int i = threadIdx.x; i < count; i += U * kThreads) {
+        double x[U];  // all loads first
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = parts[min(i + u * kThreads, count - 1)];
+#pragma unroll
+        for (int u = 0; u < U; ++u) sum += i + u * kThreads < count ? x[u] : 0.0;
+    }
     return block_sum(sum, red);
 }
 
@@ -190,10 +198,10 @@ __global__ __launch_bounds__(kThreads) void grad_scale_kernel(const GradTable t,
     }
     const float c = static_cast<float>(max_norm / (total + 1e-6));
     if (c >= 1.f || max_norm == __builtin_inf()) return;  // (a NaN scales)
-    each_piece(t, [&](int dt, char *p, int64_t size) {
-        if (dt == PRIME_BF16) scale_piece<PRIME_BF16>(p, size, c);
-        else if (dt == PRIME_F16) scale_piece<PRIME_F16>(p, size, c);
-        else scale_piece<PRIME_F32>(p, size, c);
+    each_block<true>(t, [&](int dt, char *p, int size) {
+        if (dt == PRIME_BF16) scale_block<PRIME_BF16>(p, size, c);
+        else if (dt == PRIME_F16) scale_block<PRIME_F16>(p, size, c);
+        else scale_block<PRIME_F32>(p, size, c);
     });
 }
 

@@ -513,9 +513,9 @@ constexpr int kLogprobsMaxTop = 64;
 hipError_t launch_logprobs(const LogprobsArgs &a, bool backward, hipStream_t stream);
 
 // The norm over many tensors and their scaling (grad_clip.hip).  A tensor in the table: its
-// address with the type in the two highest bits, its elements, and the slots of 8 elements
-// before it; a workgroup has `span` slots.  As large as a kernel's arguments may be.
-constexpr int kGradTable = 192;
+// address with the type in the two highest bits, its elements, and the blocks before it; each of
+// a workgroup's four waves has `span` blocks.  As large as a kernel's arguments may be.
+constexpr int kGradTable = 192, kGradBlock = 2048;
 struct GradTable {
     uint64_t data[kGradTable];
     int64_t size[kGradTable];
