@@ -1765,7 +1765,7 @@ struct GradTables {
     const int64_t *sizes;
     const int32_t *dtypes;
     int count, at = 0;
-    static constexpr uint64_t kMaxBlocks = 2048;  // workgroups
+    static constexpr uint64_t kMaxBlocks = 4096;  // workgroups
     prime::GradTable t;
     int blocks = 0;
 

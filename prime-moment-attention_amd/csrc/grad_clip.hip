@@ -5,8 +5,7 @@
 // small tensor costs as much time as one, and a wave has a span of blocks that lie one after
 // the other over all tensors.  Squares are summed in 64 bits, where those of fp32 neither
 // overflow nor vanish, and each workgroup's sum is stored; the scaling's workgroups each add
-// these in the same order.  The scaling goes through a span from its end: what the norm read
-// last is still in the last-level cache.
+// these in the same order.
 
 #include "prime_kernels.h"
 
@@ -73,15 +72,14 @@ __device__ __forceinline__ double block_sum(double x, double *red) {
     return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// f(dtype, pointer, elements) over the blocks of the wave's span, from the last to the first
-// where BACK.
-template <bool BACK, typename F>
+// f(dtype, pointer, elements) over the blocks of the wave's span
+template <typename F>
 __device__ __forceinline__ void each_block(const GradTable &t, F f) {
     const uint32_t blocks = t.first[t.count];
     const uint64_t start = (blockIdx.x * static_cast<uint64_t>(kThreads / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave)) * t.span;
     if (start >= blocks) return;
     const uint32_t begin = static_cast<uint32_t>(start), end = start + t.span < blocks ? static_cast<uint32_t>(start + t.span) : blocks;
-    uint32_t b = BACK ? end - 1 : begin;
+    uint32_t b = begin;
     // the tensor with block b: the last that starts there or before; each lane looks at three
     int k = -1;
 #pragma unroll
@@ -90,19 +88,17 @@ __device__ __forceinline__ void each_block(const GradTable &t, F f) {
         const uint32_t first = t.first[i];
         k += __popcll(__ballot(i < t.count && first <= b));
     }
-    for (uint32_t left = end - begin; left;) {
+    for (; b < end; ++k) {
         // the span's blocks of tensor k
-        const uint32_t first = t.first[k], behind = t.first[k + 1], run = BACK ? min(left, b - first + 1) : min(left, behind - b);
+        const uint32_t first = t.first[k], stop = min(end, t.first[k + 1]);
         const uint64_t word = t.data[k];
         const int dt = static_cast<int>(word >> 62);
         char *data = reinterpret_cast<char *>(word & ((1ull << 62) - 1));
         const int64_t size = t.size[k];
-        for (uint32_t r = 0; r < run; ++r) {
-            const int64_t skip = static_cast<int64_t>((BACK ? b - r : b + r) - first) * kGradBlock;
+        for (; b < stop; ++b) {
+            const int64_t skip = static_cast<int64_t>(b - first) * kGradBlock;
             f(dt, data + skip * (dt == PRIME_F32 ? 4 : 2), static_cast<int>(min(size - skip, static_cast<int64_t>(kGradBlock))));
         }
-        left -= run;
-        BACK ? (b -= run, --k) : (b += run, ++k);
     }
 }
 
@@ -157,7 +153,7 @@ __device__ __forceinline__ void scale_block(char *p, int size, float c) {
 __global__ __launch_bounds__(kThreads) void grad_squares_kernel(const GradTable t, double *parts) {
     __shared__ double red[kThreads / kWave];
     double sum = 0.0;
-    each_block<false>(t, [&](int dt, char *p, int size) {
+    each_block(t, [&](int dt, char *p, int size) {
         if (dt == PRIME_BF16) sum += square_sum<PRIME_BF16>(p, size);
         else if (dt == PRIME_F16) sum += square_sum<PRIME_F16>(p, size);
         else sum += square_sum<PRIME_F32>(p, size);
@@ -198,7 +194,7 @@ __global__ __launch_bounds__(kThreads) void grad_scale_kernel(const GradTable t,
     }
     const float c = static_cast<float>(max_norm / (total + 1e-6));
     if (c >= 1.f || max_norm == __builtin_inf()) return;  // (a NaN scales)
-    each_block<true>(t, [&](int dt, char *p, int size) {
+    each_block(t, [&](int dt, char *p, int size) {
         if (dt == PRIME_BF16) scale_block<PRIME_BF16>(p, size, c);
         else if (dt == PRIME_F16) scale_block<PRIME_F16>(p, size, c);
         else scale_block<PRIME_F32>(p, size, c);
