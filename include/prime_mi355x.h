@@ -611,21 +611,25 @@ int prime_sample(const void *logits, int dtype, int n, int vocab, int64_t stride
  *   ids    : n <= 2^30 of int64 (ids64) or int32
  *   weight : V < 2^31 rows of C <= 2^20 contiguous elements, ldw >= C apart
  *   out    : [n, C], apart from weight and ids
+ *   order  : NULL, or prime_embedding_order_size bytes, 16-byte aligned, that receive the order
+ *            of the tokens by their ids for the backward.  Ids outside [0, V) and `padding` (-1:
+ *            none) have no gradient
  *
  * prime_embedding_backward: dweight[v] = scale * sum of the rows dy[i] with ids[i] = v, all
- * V rows written.  Ids outside [0, V) and `padding` (-1: none) have no gradient.  Sums are in
- * fp32 in a fixed order, rounded once.
+ * V rows written, for the order that the lookup made of the same n and V.  Sums are in fp32 in
+ * a fixed order, rounded once.
  *   dy        : n rows of C contiguous elements, ldy >= C apart
  *   dweight   : [V, C], apart from the inputs
  *   workspace : prime_embedding_backward_workspace_size bytes, 16-byte aligned, this call's
  *               own until it has run on `stream`
  */
 int prime_embedding(const void *ids, int ids64, int64_t n, const void *weight, int64_t ldw, int64_t V, int C,
-                    int dtype, float scale, void *out, void *stream);
-size_t prime_embedding_backward_workspace_size(int64_t n, int64_t V, int C);
-int prime_embedding_backward(const void *ids, int ids64, int64_t n, const void *dy, int64_t ldy, int64_t V, int C,
-                             int dtype, float scale, int64_t padding, void *dweight, void *workspace,
-                             size_t workspace_bytes, void *stream);
+                    int dtype, float scale, int64_t padding, void *out, void *order, size_t order_bytes, void *stream);
+size_t prime_embedding_order_size(int64_t n, int64_t V);
+size_t prime_embedding_backward_workspace_size(int64_t n, int C);
+int prime_embedding_backward(const void *order, size_t order_bytes, int64_t n, const void *dy, int64_t ldy, int64_t V,
+                             int C, int dtype, float scale, void *dweight, void *workspace, size_t workspace_bytes,
+                             void *stream);
 
 /*
  * Log probabilities of given tokens: per row of logits, in fp32, with p = softmax(logits),

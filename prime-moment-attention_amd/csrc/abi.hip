@@ -1743,18 +1743,19 @@ size_t rows_span(int64_t n, int64_t cols, int64_t ld, int es) {
     return n > 0 ? static_cast<size_t>(((n - 1) * ld + cols) * es) : 0;
 }
 
-int embedding_checks(const char *who, const void *ids, int ids64, int64_t n, const void *rows, int64_t ld, int64_t V,
-                     int C, int dtype, const void *out) {
-    if (!ids || !rows || !out) return fail(PRIME_ERR_INVALID_ARG, "%s: null argument", who);
+int embedding_checks(const char *who, int64_t n, const void *rows, int64_t ld, int64_t V, int C, int dtype, const void *out) {
+    if (!rows || !out) return fail(PRIME_ERR_INVALID_ARG, "%s: null argument", who);
     if (!valid_dtype(dtype)) return fail(PRIME_ERR_UNSUPPORTED_DTYPE, "unsupported dtype");
     if (n <= 0 || n > (1 << 30) || V <= 0 || V >= (int64_t{1} << 31) || C <= 0 || C > (1 << 20) || ld < C ||
         ld > (int64_t{1} << 40))
         return fail(PRIME_ERR_INVALID_ARG, "%s: bad sizes n=%lld V=%lld C=%d row stride=%lld", who,
                     static_cast<long long>(n), static_cast<long long>(V), C, static_cast<long long>(ld));
     const int es = elem_size(dtype);
-    if (reinterpret_cast<uintptr_t>(ids) % (ids64 ? 8 : 4) || reinterpret_cast<uintptr_t>(rows) % es ||
-        reinterpret_cast<uintptr_t>(out) % es)
+    if (reinterpret_cast<uintptr_t>(rows) % es || reinterpret_cast<uintptr_t>(out) % es)
         return fail(PRIME_ERR_MISALIGNED, "%s: misaligned argument", who);
+    if (!prime::embedding_grid_fits(n, V, C, dtype))
+        return fail(PRIME_ERR_INVALID_ARG, "n=%lld V=%lld C=%d above the grid's limit", static_cast<long long>(n),
+                    static_cast<long long>(V), C);
     return PRIME_OK;
 }
 
@@ -1829,46 +1830,56 @@ int grad_checks(const void *const *tensors, const int64_t *sizes, const int32_t 
 
 extern "C" {
 
+size_t prime_embedding_order_size(int64_t n, int64_t V) {
+    if (n <= 0 || n > (1 << 30) || V <= 0 || V >= (int64_t{1} << 31)) return 0;
+    return prime::embedding_order_bytes(n, V);
+}
+
+size_t prime_embedding_backward_workspace_size(int64_t n, int C) {
+    if (n <= 0 || n > (1 << 30) || C <= 0 || C > (1 << 20)) return 0;
+    return prime::embedding_workspace_bytes(n, C);
+}
+
 int prime_embedding(const void *ids, int ids64, int64_t n, const void *weight, int64_t ldw, int64_t V, int C,
-                    int dtype, float scale, void *out, void *stream) {
+                    int dtype, float scale, int64_t padding, void *out, void *order, size_t order_bytes, void *stream) {
     g_err[0] = 0;
-    int rc = embedding_checks("prime_embedding", ids, ids64, n, weight, ldw, V, C, dtype, out);
+    if (!ids) return fail(PRIME_ERR_INVALID_ARG, "prime_embedding: null argument");
+    int rc = embedding_checks("prime_embedding", n, weight, ldw, V, C, dtype, out);
     if (rc) return rc;
+    if (reinterpret_cast<uintptr_t>(ids) % (ids64 ? 8 : 4)) return fail(PRIME_ERR_MISALIGNED, "ids misaligned");
+    const size_t need = prime_embedding_order_size(n, V);
+    if (order && (order_bytes < need || (reinterpret_cast<uintptr_t>(order) & 15u)))
+        return fail(PRIME_ERR_INVALID_ARG, "order of %zu bytes needed, 16-byte aligned", need);
     const int es = elem_size(dtype);
-    const size_t no = rows_span(n, C, C, es);
-    if (overlap(out, no, weight, rows_span(V, C, ldw, es)) || overlap(out, no, ids, static_cast<size_t>(n) * (ids64 ? 8 : 4)))
-        return fail(PRIME_ERR_ALIAS, "out overlaps weight or ids");
+    const size_t no = rows_span(n, C, C, es), nw = rows_span(V, C, ldw, es), ni = static_cast<size_t>(n) * (ids64 ? 8 : 4);
+    if (overlap(out, no, weight, nw) || overlap(out, no, ids, ni) ||
+        (order && (overlap(order, need, weight, nw) || overlap(order, need, ids, ni) || overlap(order, need, out, no))))
+        return fail(PRIME_ERR_ALIAS, "out or order overlaps another buffer");
     prime::EmbeddingArgs a{};
-    a.ids = ids; a.ids64 = ids64; a.n = n; a.V = V; a.C = C; a.dt = dtype; a.scale = scale; a.padding = -1;
-    a.weight = weight; a.ldw = ldw; a.out = out;
+    a.ids = ids; a.ids64 = ids64; a.n = n; a.V = V; a.C = C; a.dt = dtype; a.scale = scale; a.padding = padding;
+    a.weight = weight; a.ldw = ldw; a.out = out; a.order = order;
     return check_hip(prime::launch_embedding(a, false, static_cast<hipStream_t>(stream)), "embedding launch");
 }
 
-size_t prime_embedding_backward_workspace_size(int64_t n, int64_t V, int C) {
-    if (n <= 0 || n > (1 << 30) || V <= 0 || V >= (int64_t{1} << 31) || C <= 0 || C > (1 << 20)) return 0;
-    return prime::embedding_workspace_bytes(n, V, C);
-}
-
-int prime_embedding_backward(const void *ids, int ids64, int64_t n, const void *dy, int64_t ldy, int64_t V, int C,
-                             int dtype, float scale, int64_t padding, void *dweight, void *workspace,
-                             size_t workspace_bytes, void *stream) {
+int prime_embedding_backward(const void *order, size_t order_bytes, int64_t n, const void *dy, int64_t ldy, int64_t V,
+                             int C, int dtype, float scale, void *dweight, void *workspace, size_t workspace_bytes,
+                             void *stream) {
     g_err[0] = 0;
-    int rc = embedding_checks("prime_embedding_backward", ids, ids64, n, dy, ldy, V, C, dtype, dweight);
+    int rc = embedding_checks("prime_embedding_backward", n, dy, ldy, V, C, dtype, dweight);
     if (rc) return rc;
-    if (!prime::embedding_grid_fits(n, V, C, dtype))
-        return fail(PRIME_ERR_INVALID_ARG, "n=%lld V=%lld C=%d above the grid's limit", static_cast<long long>(n),
-                    static_cast<long long>(V), C);
-    const size_t need = prime_embedding_backward_workspace_size(n, V, C);
+    const size_t norder = prime_embedding_order_size(n, V), need = prime_embedding_backward_workspace_size(n, C);
+    if (!order || order_bytes < norder || (reinterpret_cast<uintptr_t>(order) & 15u))
+        return fail(PRIME_ERR_INVALID_ARG, "order of %zu bytes needed, 16-byte aligned", norder);
     if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u))
         return fail(PRIME_ERR_INVALID_ARG, "workspace of %zu bytes needed, 16-byte aligned", need);
     const int es = elem_size(dtype);
-    const size_t nw = rows_span(V, C, C, es), ny = rows_span(n, C, ldy, es), ni = static_cast<size_t>(n) * (ids64 ? 8 : 4);
-    if (overlap(dweight, nw, dy, ny) || overlap(dweight, nw, ids, ni) || overlap(dweight, nw, workspace, need) ||
-        overlap(workspace, need, dy, ny) || overlap(workspace, need, ids, ni))
+    const size_t nw = rows_span(V, C, C, es), ny = rows_span(n, C, ldy, es);
+    if (overlap(dweight, nw, dy, ny) || overlap(dweight, nw, order, norder) || overlap(dweight, nw, workspace, need) ||
+        overlap(workspace, need, dy, ny) || overlap(workspace, need, order, norder))
         return fail(PRIME_ERR_ALIAS, "dweight or the workspace overlaps another buffer");
     prime::EmbeddingArgs a{};
-    a.ids = ids; a.ids64 = ids64; a.n = n; a.V = V; a.C = C; a.dt = dtype; a.scale = scale; a.padding = padding;
-    a.dy = dy; a.ldy = ldy; a.dweight = dweight; a.workspace = workspace;
+    a.n = n; a.V = V; a.C = C; a.dt = dtype; a.scale = scale;
+    a.dy = dy; a.ldy = ldy; a.dweight = dweight; a.order = const_cast<void *>(order); a.workspace = workspace;
     return check_hip(prime::launch_embedding(a, true, static_cast<hipStream_t>(stream)), "embedding backward launch");
 }
 

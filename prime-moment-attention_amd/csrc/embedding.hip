@@ -1,16 +1,18 @@
 // Embedding lookup y_i = scale W[id_i], and its gradient dW[v] = scale sum_{i: id_i = v} dy_i.
 //
-// The gradient puts the tokens of one id side by side, in their order, and sums over these rows
+// The gradient takes the tokens of one id side by side, in their order, and sums over these rows
 // in fp32, each row of dy read once: no atomics on floats, so the order of every sum is fixed.
-//   group   (token, id) pairs in the order of their ids' low bits, then of the others; a token
-//           without a gradient (padding, an id outside the table) gets the id V and comes
-//           last.  Up to kGroupTokens tokens in one launch, else by counting passes (sort)
-//   sum     a wave has 64 vectors of columns of a chunk of rows.  An id whose rows end before
+//   order   pairs (id, token) such that equal ids lie together, a token without a gradient
+//           (padding, an id outside the table) with the id V and behind all others; and which
+//           ids occur.  Made by the lookup, for which it is all but free: its few workgroups
+//           wait for memory while those that look up fill its bandwidth.  Up to kGroupTokens
+//           tokens in one launch, else by counting passes
+//   sum     a wave has 64 vectors of columns of a chunk of pairs.  An id whose rows end before
 //           the next chunk does is finished where it begins; a longer one leaves a part in
-//           each chunk
+//           each chunk.  Further workgroups write the zeros of the ids that do not occur
 //   join    the parts of the long ones, in a fixed order
-// Grouping leaves the memory system idle: further workgroups of its launches fill the whole
-// gradient with zeros meanwhile, which the rows with a token then replace.
+
+#include <type_traits>
 
 #include "prime_kernels.h"
 
@@ -18,22 +20,25 @@ namespace prime {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
 constexpr int kMaxBits = 9, kMaxBins = 1 << kMaxBits;
 constexpr int kGroups = 128;           // by the ids' low bits
 constexpr int kGroupList = 2048;       // tokens of a group that are sorted in LDS
+constexpr int kGroupRanked = 256;      // .. that are ranked by comparing each with each
 constexpr int kGroupTokens = 1 << 14;
 constexpr int kSortItems = 4096;       // at least, of a workgroup
 constexpr int kSortBlocks = 512;       // at most
 constexpr int kFewRows = 16384;        // tokens, below which chunks are short
+constexpr int kZeroRows = 64;
 constexpr int kRows = 8;               // of a chunk, on their way at once, twice
 
-// The part [from, to) of the gradient's 16-byte blocks that a launch's workgroups from `block`
-// on fill with zeros.
-struct Fill {
+// A launch's share of the lookup: rows [first, first + rows) by the workgroups from `block` on,
+// `vecs` vectors of 16 bytes each.
+struct Share {
     int block;
-    int64_t from, to;
+    int64_t first;
+    int rows, vecs;
 };
 
 struct __attribute__((packed, aligned(2))) Raw {  // 16 bytes of a row, wherever it starts
@@ -104,52 +109,54 @@ __device__ __forceinline__ uint32_t sort_key(const EmbeddingArgs &a, int64_t i) 
 
 }  // namespace
 
-// Rows [first, first + rows) of the output, 16 bytes a thread.
-template <int DT, bool SCALE, bool SHORT>
-__global__ __launch_bounds__(kThreads) void embedding_kernel(const EmbeddingArgs a, int64_t first, int rows, int vecs) {
-    constexpr int VE = kVec<DT>, es = Columns<DT, SHORT>::es;
-    const uint32_t item = blockIdx.x * kThreads + threadIdx.x, r = item / static_cast<uint32_t>(vecs);
-    if (r >= static_cast<uint32_t>(rows)) return;
-    const Columns<DT, SHORT> at(item - r * vecs, a.C);
-    const int64_t i = first + r, id = load_id(a, i);
-    u32x4 v = {0, 0, 0, 0};
-    if (id >= 0 && id < a.V) {
-        v = at.load(static_cast<const char *>(a.weight) + id * a.ldw * es);
-        if constexpr (SCALE) {
-            float x[VE];
-            widen<DT>(v, x);
-#pragma unroll
-            for (int j = 0; j < VE; ++j) x[j] *= a.scale;
-            v = narrow<DT>(x);
-        }
+// 16 bytes a thread of a row of the output; the last vector of a row ends with it, and where the
+// row is no multiple of 16 bytes shares some with the one before.  Without a scale bytes are
+// copied, whatever their type.
+__device__ __forceinline__ void look_up(const EmbeddingArgs &a, const Share &share, uint32_t item) {
+    const uint32_t r = item / static_cast<uint32_t>(share.vecs);
+    if (r >= static_cast<uint32_t>(share.rows)) return;
+    const int es = a.dt == PRIME_F32 ? 4 : 2, bytes = a.C * es, at = min(static_cast<int>(item - r * share.vecs) * 16, bytes - 16);
+    const int64_t i = share.first + r, id = load_id(a, i);
+    const bool inside = id >= 0 && id < a.V;
+    const char *from = static_cast<const char *>(a.weight) + (inside ? id : 0) * a.ldw * es;
+    char *to = static_cast<char *>(a.out) + i * bytes;
+    if (at < 0) {  // a row shorter than a vector
+        for (int j = 0; j < a.C; ++j) store_elem(to, j, a.dt, inside ? load_elem(from, j, a.dt) * a.scale : 0.f);
+        return;
     }
-    at.store(static_cast<char *>(a.out) + i * a.C * es, v);
+    u32x4 v = {0, 0, 0, 0};
+    if (inside) v = reinterpret_cast<const Raw *>(from + at)->v;
+    auto scaled = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        float x[kVec<DT>];
+        widen<DT>(v, x);
+#pragma unroll
+        for (int j = 0; j < kVec<DT>; ++j) x[j] *= a.scale;
+        v = narrow<DT>(x);
+    };
+    if (a.scale != 1.f && inside) {
+        if (a.dt == PRIME_BF16) scaled(std::integral_constant<int, PRIME_BF16>{});
+        else if (a.dt == PRIME_F16) scaled(std::integral_constant<int, PRIME_F16>{});
+        else scaled(std::integral_constant<int, PRIME_F32>{});
+    }
+    reinterpret_cast<Raw *>(to + at)->v = v;
+}
+// by the workgroups of a launch that makes the order
+__device__ __forceinline__ void look_up(const EmbeddingArgs &a, const Share &share) {
+    look_up(a, share, (blockIdx.x - share.block) * kSortThreads + threadIdx.x);
 }
 
-// A workgroup's share of the gradient's zeros: 16-byte stores over [from, to) of the table's
-// 16-byte blocks, the elements before the first and behind the last by the share that has
-// them.
-__device__ __forceinline__ void fill_zeros(const EmbeddingArgs &a, const Fill &f) {
-    const int es = a.dt == PRIME_F32 ? 4 : 2;
-    char *dw = static_cast<char *>(a.dweight);
-    const uintptr_t begin = reinterpret_cast<uintptr_t>(dw), end = begin + a.V * a.C * es;
-    const uintptr_t first = (begin + 15) & ~uintptr_t{15}, last = end & ~uintptr_t{15};
-    constexpr int U = 4;
-    u32x4 *p = reinterpret_cast<u32x4 *>(first);
-    const int64_t at = f.from + static_cast<int64_t>(blockIdx.x - f.block) * (kSortThreads * U) + threadIdx.x;
-    const int64_t blocks = first < last ? static_cast<int64_t>(last - first) / 16 : 0, to = f.to < blocks ? f.to : blocks;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-        if (at + u * kSortThreads < to) p[at + u * kSortThreads] = u32x4{0, 0, 0, 0};
-    if (f.from == 0 && blockIdx.x == f.block) {
-        const uintptr_t head = first < end ? first : end, tail = last > head ? last : head;
-        for (uintptr_t q = begin + threadIdx.x * 2; q < head; q += kSortThreads * 2) *reinterpret_cast<uint16_t *>(q) = 0;
-        for (uintptr_t q = tail + threadIdx.x * 2; q < end; q += kSortThreads * 2) *reinterpret_cast<uint16_t *>(q) = 0;
-    }
+__global__ __launch_bounds__(kThreads) void embedding_kernel(const EmbeddingArgs a, const Share share) {
+    look_up(a, share, blockIdx.x * kThreads + threadIdx.x);
+}
+
+// Where it is kept whether an id occurs: a group's ids lie together.
+__device__ __forceinline__ int64_t occurs_at(int64_t id, int64_t V) {
+    return id % kGroups * ((V + kGroups - 1) / kGroups) + id / kGroups;
 }
 
 // The sum of v over the threads before this one.
-__device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t *wave_total) {
+__device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t *wave_total) {  // a value a wave
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     uint32_t scan = v;
 #pragma unroll
@@ -229,15 +236,15 @@ __device__ __forceinline__ void sort_pass(uint32_t (*tally)[kMaxBins], uint32_t 
 // Workgroup g < kGroups: the tokens whose ids have the low bits g, in the order of the others.
 // Each reads all ids, so where its tokens go it knows by itself: behind those of lower groups.
 // Workgroup kGroups: the places behind all of them, for tokens without a gradient.  The
-// others write zeros.
+// others look up.
 __global__ __launch_bounds__(kSortThreads) void embedding_group_kernel(const EmbeddingArgs a, uint2 *pairs, uint2 *other,
-                                                                       int passes, int bits, const Fill fill) {
+                                                                       uint8_t *occurs, int passes, int bits, const Share share) {
     constexpr int kLow = __builtin_ctz(kGroups);
     __shared__ uint32_t tally[kSortWaves][kMaxBins];
     __shared__ uint32_t wave_total[kSortWaves], wave_lower[kSortWaves];
     __shared__ uint2 list[2][kGroupList];
-    if (static_cast<int>(blockIdx.x) >= fill.block) {
-        fill_zeros(a, fill);
+    if (static_cast<int>(blockIdx.x) >= share.block) {
+        look_up(a, share);
         return;
     }
     const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave, n = static_cast<int>(a.n);
@@ -262,6 +269,9 @@ __global__ __launch_bounds__(kSortThreads) void embedding_group_kernel(const Emb
             }
         }
     };
+    const int64_t ids = (a.V + kGroups - 1) / kGroups;  // of a group
+    if (group < kGroups)
+        for (int64_t i = tid; i < ids; i += kSortThreads) occurs[group * ids + i] = 0;
     uint32_t mine = 0, lower = 0;  // of the wave
     each([&](uint32_t id, bool valid, int) {
         const uint32_t low = id & (kGroups - 1);
@@ -288,10 +298,26 @@ __global__ __launch_bounds__(kSortThreads) void embedding_group_kernel(const Emb
     each([&](uint32_t id, bool valid, int i) {
         const bool in = valid && (id & (kGroups - 1)) == group;
         const uint64_t all = __ballot(in);
-        if (in) first[at + __popcll(all & ((1ull << lane) - 1))] = uint2{id, static_cast<uint32_t>(i)};
+        if (in) {
+            first[at + __popcll(all & ((1ull << lane) - 1))] = uint2{id, static_cast<uint32_t>(i)};
+            occurs[group * ids + (id >> kLow)] = 1;
+        }
         at += __popcll(all);
     });
     __syncthreads();
+    if (passes && count <= kGroupRanked) {  // each by its rank among the others
+        if (tid < static_cast<int>(count)) {
+            const uint2 item = list[0][tid];
+            uint32_t rank = 0;
+#pragma unroll 8
+            for (uint32_t o = 0; o < count; ++o) {
+                const uint32_t id = list[0][o].x;
+                rank += (id < item.x) | ((id == item.x) & (o < static_cast<uint32_t>(tid)));
+            }
+            pairs[base + rank] = item;
+        }
+        return;
+    }
     for (int p = 0; p < passes; ++p) {
         const int shift = kLow + p * bits;
         uint2 *to = (passes - p) & 1 ? pairs + base : other + base;
@@ -310,20 +336,25 @@ __global__ __launch_bounds__(kSortThreads) void embedding_group_kernel(const Emb
 
 // One counting pass over many tokens: their digits' counts, or (SCATTER) the pairs in the
 // digits' order.  FIRST: the pairs are the ids' and the tokens' own.  ONE: a workgroup has
-// kSortItems tokens, which its threads hold.  Workgroups from `fill.block` on write zeros
-// meanwhile.
+// kSortItems tokens, which its threads hold.  Workgroups from `share.block` on look up.  The
+// first launch clears `occurs`, the second sets it.
 template <bool FIRST, bool SCATTER, bool ONE>
 __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(const EmbeddingArgs a, const uint2 *pairs,
-                                                                      uint2 *pairs_out, uint32_t *hist, int shift,
-                                                                      int bits, int items, const Fill fill) {
+                                                                      uint2 *pairs_out, uint8_t *occurs,
+                                                                      uint32_t *hist, int shift, int bits, int items,
+                                                                      const Share share) {
     constexpr int R = kSortItems / kSortThreads;
     __shared__ uint32_t count[kSortWaves][kMaxBins];
     __shared__ uint32_t total[kSortThreads], before[kSortThreads], wave_total[kSortWaves];
-    if (static_cast<int>(blockIdx.x) >= fill.block) {
-        fill_zeros(a, fill);
+    if constexpr (FIRST && !SCATTER) {
+        const int64_t ids = (a.V + kGroups - 1) / kGroups * kGroups, step = static_cast<int64_t>(gridDim.x) * kSortThreads;
+        for (int64_t i = static_cast<int64_t>(blockIdx.x) * kSortThreads + threadIdx.x; i < ids; i += step) occurs[i] = 0;
+    }
+    if (static_cast<int>(blockIdx.x) >= share.block) {
+        look_up(a, share);
         return;
     }
-    const int bins = 1 << bits, tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave, blocks = fill.block;
+    const int bins = 1 << bits, tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave, blocks = share.block;
     if constexpr (ONE) items = kSortItems;
     // a wave has `items` / kSortWaves tokens that lie one after the other
     const int64_t begin = static_cast<int64_t>(blockIdx.x) * items + wave * (items / kSortWaves);
@@ -338,16 +369,16 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(const Embe
         // each digit's count in all workgroups and in those before this one, by threads that
         // share the workgroups between them
         constexpr int U = 8;
-        const int bin = tid & (bins - 1), share = kSortThreads / bins;
+        const int bin = tid & (bins - 1), parts = kSortThreads / bins;
         uint32_t t = 0, b = 0;
-        for (int q = tid / bins; q < blocks; q += U * share) {
+        for (int q = tid / bins; q < blocks; q += U * parts) {
             uint32_t h[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) h[u] = hist[static_cast<int64_t>(min(q + u * share, blocks - 1)) * bins + bin];
+            for (int u = 0; u < U; ++u) h[u] = hist[static_cast<int64_t>(min(q + u * parts, blocks - 1)) * bins + bin];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                t += q + u * share < blocks ? h[u] : 0;
-                b += q + u * share < static_cast<int>(blockIdx.x) ? h[u] : 0;
+                t += q + u * parts < blocks ? h[u] : 0;
+                b += q + u * parts < static_cast<int>(blockIdx.x) ? h[u] : 0;
             }
         }
         total[tid] = t, before[tid] = b;
@@ -384,7 +415,10 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(const Embe
             }
         }
         __syncthreads();
-        auto put = [&](uint32_t at, uint2 v) { pairs_out[at] = v; };
+        auto put = [&](uint32_t at, uint2 v) {
+            pairs_out[at] = v;
+            if (FIRST && v.x < static_cast<uint32_t>(a.V)) occurs[occurs_at(v.x, a.V)] = 1;
+        };
         if constexpr (ONE) {
 #pragma unroll
             for (int r = 0; r < R; ++r) place_64(count[wave], held[r], begin + r * kWave + lane < end, shift, bits, put);
@@ -394,21 +428,70 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(const Embe
     }
 }
 
+// The ids that reach over a chunk and the next: a section of kThreads chunks has its count, and
+// for each the chunk in which it begins, how many chunks behind it it reaches, and the id.
+struct LongIds {
+    uint32_t *count;  // [sections]
+    uint4 *list;      // [sections][kThreads]
+};
+
+template <int K>
+__device__ __forceinline__ void list_long(const EmbeddingArgs &a, const uint2 *pairs, const LongIds &longs, uint32_t chunks) {
+    __shared__ uint32_t listed;
+    if (threadIdx.x == 0) listed = 0;
+    __syncthreads();
+    const uint32_t n = static_cast<uint32_t>(a.n), chunk = blockIdx.x * kThreads + threadIdx.x;
+    const uint64_t begin = static_cast<uint64_t>(chunk) * K;
+    if (begin + 2 * K <= n) {
+        const uint32_t id = pairs[begin + K - 1].x, ahead = pairs[begin + 2 * K - 1].x, prior = begin > 0 ? pairs[begin - 1].x : ~id;
+        if (id < static_cast<uint32_t>(a.V) && ahead == id && prior != id) {
+            // the chunks behind that begin with the id are the first ones: by doubling, then halving
+            uint32_t in = chunk + 1, step = 1;  // `in` begins with it
+            while (in + step < chunks && pairs[static_cast<uint64_t>(in + step) * K].x == id) in += step, step *= 2;
+            for (; step; step /= 2)
+                if (in + step < chunks && pairs[static_cast<uint64_t>(in + step) * K].x == id) in += step;
+            longs.list[blockIdx.x * kThreads + atomicAdd(&listed, 1u)] = uint4{chunk, in - chunk, id, 0};
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) longs.count[blockIdx.x] = listed;
+}
+
 // A wave: 64 vectors of columns of the K rows of a chunk.  Lane l knows the pair l behind the
 // chunk's begin, K of this chunk and K of the next, so that all decisions are the wave's.  An id
 // is finished by the chunk in which it begins if it ends before the next one does; else it is
 // long, and each chunk leaves its part of it.  part: [chunks][2][vecs VE], of the long id that
-// reaches in from the chunk before (0) and of the one that begins here (1).
+// reaches in from the chunk before (0) and of the one that begins here (1).  The first list_blocks
+// workgroups list the long ids, those from sum_blocks on write zeros for kZeroRows rows each,
+// where their ids do not occur.
 template <int DT, bool SHORT, int K>
-__global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const EmbeddingArgs a, const uint2 *pairs, float *part,
-                                                                 int vecs, uint32_t chunks) {
+__global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const EmbeddingArgs a, const uint2 *pairs,
+                                                                 const uint8_t *occurs, const LongIds longs, float *part,
+                                                                 int vecs, uint32_t chunks, uint32_t list_blocks,
+                                                                 uint32_t sum_blocks) {
     constexpr int VE = kVec<DT>, es = Columns<DT, SHORT>::es, U = kRows;
     static_assert(2 * K <= kWave && K % U == 0, "");
     const uint32_t V = static_cast<uint32_t>(a.V), n = static_cast<uint32_t>(a.n);
-    const uint32_t chunk = blockIdx.x * (kThreads / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    if (blockIdx.x < list_blocks) {
+        list_long<K>(a, pairs, longs, chunks);
+        return;
+    }
+    if (blockIdx.x >= sum_blocks) {
+        constexpr int kRowsOfWave = kZeroRows / (kThreads / kWave);
+        const int64_t first = static_cast<int64_t>(blockIdx.x - sum_blocks) * kZeroRows + wave * kRowsOfWave, id = first + lane;
+        uint64_t absent = __ballot(lane < kRowsOfWave && id < a.V && !occurs[id < a.V ? occurs_at(id, a.V) : 0]);
+        for (; absent; absent &= absent - 1) {
+            char *row = static_cast<char *>(a.dweight) + (first + __builtin_ctzll(absent)) * a.C * es;
+            for (int q = lane; q < vecs; q += kWave) Columns<DT, SHORT>(q, a.C).store(row, u32x4{0, 0, 0, 0});
+        }
+        return;
+    }
+    const uint32_t groups = (chunks + kThreads / kWave - 1) / (kThreads / kWave), block = blockIdx.x - list_blocks, slab = block / groups;
+    const uint32_t chunk = (block - slab * groups) * (kThreads / kWave) + wave;
     if (chunk >= chunks) return;
     const uint32_t begin = chunk * K;
-    const int lane = threadIdx.x % kWave, vec = blockIdx.y * kWave + lane;
+    const int vec = slab * kWave + lane;
     const uint32_t place = begin + lane;
     const uint2 none = {~0u, 0};
     uint2 pair = place < n ? pairs[place] : none;
@@ -488,67 +571,57 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const Embedding
     }
 }
 
-// The long ids' parts: workgroup b looks for them at the chunks b, b + gridDim.x, ..; of an id's
-// parts wave w has the w-th, (w + 16)-th .., of four columns a lane, then the waves' sums.
-template <int DT, int K>
-__global__ __launch_bounds__(kSortThreads) void embedding_join_kernel(const EmbeddingArgs a, const uint2 *pairs,
-                                                                      const float *part, int vecs, uint32_t chunks) {
-    constexpr int VE = kVec<DT>;
-    __shared__ f32x4 sums[kSortWaves][kWave];
-    __shared__ uint32_t found[kSortThreads], reach[kSortWaves];
-    __shared__ int list;
-    const uint32_t n = static_cast<uint32_t>(a.n);
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const int slot = (blockIdx.y * kWave + lane) * 4, width = vecs * VE;  // columns as the parts have them
-    for (uint64_t c0 = blockIdx.x; c0 < chunks; c0 += static_cast<uint64_t>(gridDim.x) * kSortThreads) {
-        if (threadIdx.x == 0) list = 0;
-        __syncthreads();
-        const uint64_t c = c0 + static_cast<uint64_t>(threadIdx.x) * gridDim.x, begin = c * K;
-        if (begin + 2 * K <= n) {
-            const uint32_t id = pairs[begin + K - 1].x;
-            if (id < static_cast<uint32_t>(a.V) && pairs[begin + 2 * K - 1].x == id && !(begin > 0 && pairs[begin - 1].x == id))
-                found[atomicAdd(&list, 1)] = static_cast<uint32_t>(c);
-        }
-        __syncthreads();
-        for (int f = 0; f < list; ++f) {
-            const uint32_t chunk = found[f], id = pairs[static_cast<uint64_t>(chunk) * K + K - 1].x;
-            // the chunks behind that begin with the id are the first ones
-            uint32_t count = 0;
-            for (;;) {
-                const uint64_t at = (static_cast<uint64_t>(chunk) + 1 + count + threadIdx.x) * K;
-                const uint32_t here = __popcll(__ballot(at < n && pairs[at].x == id));
-                if (lane == 0) reach[wave] = here;
-                __syncthreads();
-                uint32_t all = 0;
-                for (int w = 0; w < kSortWaves; ++w) all += reach[w];
-                __syncthreads();
-                count += all;
-                if (all < kSortThreads) break;
-            }
+// The long ids' parts: of all sections' ids workgroup b has the b-th, (b + gridDim.x)-th ..; of an
+// id's parts the workgroup's r-th row of L lanes has the r-th, (r + rows)-th .., of four columns
+// a lane, then the rows' sums.  (One workgroup reads some 50 GB/s: narrow slabs bring more of
+// them to an id.)
+template <int DT, int L>
+__global__ __launch_bounds__(kThreads) void embedding_join_kernel(const EmbeddingArgs a, const LongIds longs,
+                                                                  const float *part, int vecs, uint32_t sections) {
+    constexpr int VE = kVec<DT>, kRowsOfLanes = kThreads / L;
+    __shared__ f32x4 sums[kWaves][L];
+    __shared__ uint32_t wave_total[kWaves];
+    __shared__ uint4 found;
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, col = threadIdx.x % L, row = threadIdx.x / L;
+    const int slot = (blockIdx.y * L + col) * 4, width = vecs * VE;  // columns as the parts have them
+    for (uint32_t s0 = 0; s0 < sections; s0 += kThreads) {
+        const uint32_t section = s0 + threadIdx.x, own = section < sections ? longs.count[section] : 0;
+        const uint32_t before = scan_before(own, wave_total);
+        uint32_t total = 0;
+        for (int w = 0; w < kWaves; ++w) total += wave_total[w];
+        for (uint32_t e = blockIdx.x; e < total; e += gridDim.x) {
+            if (before <= e && e < before + own) found = longs.list[section * kThreads + e - before];
+            __syncthreads();
+            const uint4 entry = found;
+            const uint32_t chunk = entry.x, reach = entry.y, id = entry.z;
             f32x4 acc = {0.f, 0.f, 0.f, 0.f};
             if (slot < width) {
                 // part 0 is this chunk's, part c > 0 that of the c-th chunk behind
                 constexpr int U = 8;
-                for (uint32_t q = wave; q <= count; q += U * kSortWaves) {
+                for (uint32_t q = row; q <= reach; q += U * kRowsOfLanes) {
                     f32x4 x[U];  // all loads first
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
-                        const uint32_t c = min(q + u * kSortWaves, count);
+                        const uint32_t c = min(q + u * kRowsOfLanes, reach);
                         x[u] = *reinterpret_cast<const f32x4 *>(part + (static_cast<int64_t>(chunk + c) * 2 + (c == 0)) * width + slot);
                     }
 #pragma unroll
                     for (int u = 0; u < U; ++u)
-                        if (q + u * kSortWaves <= count) acc += x[u];
+                        if (q + u * kRowsOfLanes <= reach) acc += x[u];
                 }
             }
-            sums[wave][lane] = acc;
+            if constexpr (L == 16) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j] = sum_lane32(sum_lane16(acc[j]));
+            }
+            if (lane < L) sums[wave][lane] = acc;
             __syncthreads();
-            if (wave == 0 && slot < width) {
-                for (int w = 1; w < kSortWaves; ++w) acc += sums[w][lane];
-                const int vec = slot / VE, first = a.C < VE ? 0 : vec * VE + VE <= a.C ? vec * VE : a.C - VE, col = first + slot % VE;
+            if (threadIdx.x < L && slot < width) {
+                for (int w = 1; w < kWaves; ++w) acc += sums[w][col];
+                const int vec = slot / VE, first = a.C < VE ? 0 : vec * VE + VE <= a.C ? vec * VE : a.C - VE, at = first + slot % VE;
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (col + j < a.C) store_elem(a.dweight, static_cast<int64_t>(id) * a.C + col + j, DT, acc[j] * a.scale);
+                    if (at + j < a.C) store_elem(a.dweight, static_cast<int64_t>(id) * a.C + at + j, DT, acc[j] * a.scale);
             }
             __syncthreads();
         }
@@ -558,15 +631,17 @@ __global__ __launch_bounds__(kSortThreads) void embedding_join_kernel(const Embe
 
 namespace {
 
+// The order of n tokens in a buffer of the caller's: the pairs, which ids occur, then what only
+// the making needs.
 struct Plan {
     bool grouped;        // in one launch
     int passes, bits;    // of the sort, or of a group
     int blocks, items;   // of the sort
-    int chunk;           // rows
+    int chunk;           // pairs
     int64_t chunks;
-    size_t pairs_bytes, hist_bytes, part_bytes;
+    size_t occurs, other, hist, bytes;  // where they begin, and the end
 };
-Plan plan(int64_t n, int64_t V, int C) {
+Plan plan(int64_t n, int64_t V) {
     Plan p{};
     p.grouped = n <= kGroupTokens;
     int bits = 0;  // of the ids; of the sort's keys 0 .. V
@@ -577,43 +652,19 @@ Plan plan(int64_t n, int64_t V, int C) {
     const int64_t per = (n + kSortBlocks - 1) / kSortBlocks;
     const int64_t items = per < kSortItems ? kSortItems : (per + kSortThreads - 1) / kSortThreads * kSortThreads;
     p.items = static_cast<int>(items);
-    p.blocks = static_cast<int>((n + items - 1) / items);
-    p.chunk = n < kFewRows ? 8 : 32;
+    p.blocks = p.grouped ? kGroups + 1 : static_cast<int>((n + items - 1) / items);
+    p.chunk = n >= 64 && n < kFewRows ? 8 : 32;  // (below 64 no id is long, and nothing to join)
     p.chunks = (n + p.chunk - 1) / p.chunk;
     auto round = [](size_t b) { return (b + 255) / 256 * 256; };
-    p.pairs_bytes = round(static_cast<size_t>(n) * 8);
-    p.hist_bytes = p.grouped ? 0 : round(static_cast<size_t>(p.blocks) * (size_t{1} << p.bits) * 4);
-    p.part_bytes = static_cast<size_t>(p.chunks) * 2 * ((static_cast<size_t>(C) + 7) / 8 * 8) * 4;
+    p.occurs = round(static_cast<size_t>(n) * 8);
+    p.other = p.occurs + round(static_cast<size_t>(V + kGroups - 1) / kGroups * kGroups);
+    p.hist = p.other + round(static_cast<size_t>(n) * 8);
+    p.bytes = p.hist + (p.grouped ? 0 : round(static_cast<size_t>(p.blocks) * (size_t{1} << p.bits) * 4));
     return p;
 }
 
-template <int DT>
-void run(const EmbeddingArgs &a, hipStream_t s) {
-    const int vecs = (a.C + kVec<DT> - 1) / kVec<DT>;
-    const int64_t most = (int64_t{1} << 30) / vecs;  // rows of a launch
-    const bool scales = a.scale != 1.f, is_short = a.C < kVec<DT>;
-    const auto kernel = is_short ? (scales ? embedding_kernel<DT, true, true> : embedding_kernel<DT, false, true>)
-                                 : (scales ? embedding_kernel<DT, true, false> : embedding_kernel<DT, false, false>);
-    for (int64_t first = 0; first < a.n; first += most) {
-        const int rows = static_cast<int>(a.n - first < most ? a.n - first : most);
-        const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(rows) * vecs + kThreads - 1) / kThreads));
-        hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, a, first, rows, vecs);
-    }
-}
-
-template <int DT, int K>
-void sum_and_join(const EmbeddingArgs &a, const Plan &p, const uint2 *pairs, float *part, hipStream_t s) {
-    const int vecs = (a.C + kVec<DT> - 1) / kVec<DT>, slabs = (vecs + kWave - 1) / kWave;
-    const uint32_t chunks = static_cast<uint32_t>(p.chunks);
-    const dim3 grid((chunks + kThreads / kWave - 1) / (kThreads / kWave), slabs);
-    const auto kernel = a.C < kVec<DT> ? embedding_sum_kernel<DT, true, K> : embedding_sum_kernel<DT, false, K>;
-    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, a, pairs, part, vecs, chunks);
-    if (a.n < 2 * K) return;  // (no long id)
-    const dim3 join(chunks < 256 ? chunks : 256, (vecs * kVec<DT> + 4 * kWave - 1) / (4 * kWave));
-    hipLaunchKernelGGL((embedding_join_kernel<DT, K>), join, dim3(kSortThreads), 0, s, a, pairs, part, vecs, chunks);
-}
-
-using SortKernel = void (*)(EmbeddingArgs, const uint2 *, uint2 *, uint32_t *, int, int, int, Fill);
+using SortKernel = void (*)(EmbeddingArgs, const uint2 *, uint2 *, uint8_t *, uint32_t *, int, int, int,
+                            Share);
 SortKernel sort_kernel(bool first, bool scatter, bool one) {
     if (one) {
         if (first) return scatter ? embedding_sort_kernel<true, true, true> : embedding_sort_kernel<true, false, true>;
@@ -623,62 +674,124 @@ SortKernel sort_kernel(bool first, bool scatter, bool one) {
     return scatter ? embedding_sort_kernel<false, true, false> : embedding_sort_kernel<false, false, false>;
 }
 
+void run(const EmbeddingArgs &a, hipStream_t s) {
+    const int es = a.dt == PRIME_F32 ? 4 : 2, vecs = (a.C * es + 15) / 16;
+    const int64_t most = (int64_t{1} << 30) / vecs;  // rows of a launch
+    Share share{0, 0, 0, vecs};
+    if (!a.order) {
+        for (; share.first < a.n; share.first += most) {
+            share.rows = static_cast<int>(a.n - share.first < most ? a.n - share.first : most);
+            const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(share.rows) * vecs + kThreads - 1) / kThreads));
+            hipLaunchKernelGGL(embedding_kernel, grid, dim3(kThreads), 0, s, a, share);
+        }
+        return;
+    }
+    const Plan p = plan(a.n, a.V);
+    char *w = static_cast<char *>(a.order);
+    uint2 *buf[2] = {reinterpret_cast<uint2 *>(w), reinterpret_cast<uint2 *>(w + p.other)};
+    uint8_t *occurs = reinterpret_cast<uint8_t *>(w + p.occurs);
+    uint32_t *hist = reinterpret_cast<uint32_t *>(w + p.hist);
+    const dim3 threads(kSortThreads);
+    share.block = p.blocks;
+    // the launches, each with its share of the rows
+    const int launches = p.grouped ? 1 : 2 * p.passes;
+    int64_t left = a.n;
+    auto next = [&](int launch) {
+        const int64_t fair = (left + launches - launch - 1) / (launches - launch);
+        share.first = a.n - left;
+        share.rows = static_cast<int>(fair < most ? fair : most);
+        left -= share.rows;
+        return dim3(static_cast<unsigned>(p.blocks + (static_cast<int64_t>(share.rows) * vecs + kSortThreads - 1) / kSortThreads));
+    };
+    if (p.grouped) {
+        const dim3 grid = next(0);
+        hipLaunchKernelGGL(embedding_group_kernel, grid, threads, 0, s, a, buf[0], buf[1], occurs, p.passes, p.bits, share);
+    }
+    const uint2 *pairs = nullptr;
+    for (int i = 0; i < p.passes && !p.grouped; ++i) {
+        uint2 *to = buf[(p.passes - 1 - i) & 1];
+        for (int scatter = 0; scatter < 2; ++scatter) {
+            const dim3 grid = next(2 * i + scatter);
+            hipLaunchKernelGGL(sort_kernel(i == 0, scatter, p.items == kSortItems), grid, threads, 0, s, a, pairs, to, occurs, hist,
+                               i * p.bits, p.bits, p.items, share);
+        }
+        pairs = to;
+    }
+    if (left) {  // more rows than the launches of the order take
+        EmbeddingArgs rest = a;
+        const int64_t done = a.n - left;
+        rest.order = nullptr;
+        rest.n = left;
+        rest.ids = static_cast<const char *>(a.ids) + done * (a.ids64 ? 8 : 4);
+        rest.out = static_cast<char *>(a.out) + done * a.C * es;
+        run(rest, s);
+    }
+}
+
+// The backward's workspace: the parts, the long ids.
+struct Parts {
+    size_t sections, counts, lists, bytes;
+};
+Parts parts(const Plan &p, int C) {
+    Parts w{};
+    w.sections = static_cast<size_t>(p.chunks + kThreads - 1) / kThreads;
+    w.lists = static_cast<size_t>(p.chunks) * 2 * ((static_cast<size_t>(C) + 7) / 8 * 8) * 4;
+    w.counts = w.lists + w.sections * kThreads * sizeof(uint4);
+    w.bytes = w.counts + w.sections * 4;
+    return w;
+}
+
+template <int DT, int K>
+void sum_and_join(const EmbeddingArgs &a, const Plan &p, hipStream_t s) {
+    const int vecs = (a.C + kVec<DT> - 1) / kVec<DT>, slabs = (vecs + kWave - 1) / kWave;
+    const bool joins = a.n >= 2 * K;  // (else no id is long)
+    const Parts space = parts(p, a.C);
+    const uint32_t chunks = static_cast<uint32_t>(p.chunks), waves = kThreads / kWave, sections = static_cast<uint32_t>(space.sections);
+    const uint32_t list_blocks = joins ? sections : 0, sum_blocks = list_blocks + (chunks + waves - 1) / waves * slabs;
+    const uint32_t zero_blocks = static_cast<uint32_t>((a.V + kZeroRows - 1) / kZeroRows);
+    const char *o = static_cast<const char *>(a.order);
+    const uint2 *pairs = reinterpret_cast<const uint2 *>(o);
+    const uint8_t *occurs = reinterpret_cast<const uint8_t *>(o + p.occurs);
+    char *w = static_cast<char *>(a.workspace);
+    float *part = reinterpret_cast<float *>(w);
+    const LongIds longs{reinterpret_cast<uint32_t *>(w + space.counts), reinterpret_cast<uint4 *>(w + space.lists)};
+    const auto kernel = a.C < kVec<DT> ? embedding_sum_kernel<DT, true, K> : embedding_sum_kernel<DT, false, K>;
+    hipLaunchKernelGGL(kernel, dim3(sum_blocks + zero_blocks), dim3(kThreads), 0, s, a, pairs, occurs, longs, part, vecs, chunks,
+                       list_blocks, sum_blocks);
+    if (!joins) return;
+    // some 1500 workgroups, each id a slab of its own
+    const uint32_t width = vecs * kVec<DT>, cols = width <= 1024 ? 64 : 256, y = (width + cols - 1) / cols;
+    const uint32_t x = y < 6 ? 256 : y < 96 ? 1536 / y : 16;
+    const auto join = cols == 64 ? embedding_join_kernel<DT, 16> : embedding_join_kernel<DT, 64>;
+    hipLaunchKernelGGL(join, dim3(x, y), dim3(kThreads), 0, s, a, longs, part, vecs, sections);
+}
+
 template <int DT>
 void run_backward(const EmbeddingArgs &a, hipStream_t s) {
-    const Plan p = plan(a.n, a.V, a.C);
-    char *w = static_cast<char *>(a.workspace);
-    uint2 *buf[2] = {reinterpret_cast<uint2 *>(w), reinterpret_cast<uint2 *>(w + p.pairs_bytes)};
-    uint32_t *hist = reinterpret_cast<uint32_t *>(w + 2 * p.pairs_bytes);
-    float *part = reinterpret_cast<float *>(w + 2 * p.pairs_bytes + p.hist_bytes);
-    const dim3 threads(kSortThreads);
-    // the launches, each with its share of the zeros
-    const int launches = p.grouped ? 1 : 2 * p.passes;
-    const int64_t zeros = a.V * a.C * (DT == PRIME_F32 ? 4 : 2) / 16 + 1, share = (zeros + launches - 1) / launches;
-    int launch = 0;
-    auto next = [&](int blocks, Fill &f) {
-        f.block = blocks;
-        f.from = share * launch++;
-        f.to = f.from + share;
-        constexpr int per = kSortThreads * 4;
-        return dim3(static_cast<unsigned>(blocks + (share + per - 1) / per));
-    };
-    Fill f;
-    const uint2 *pairs = buf[0];
-    if (p.grouped) {
-        const dim3 grid = next(kGroups + 1, f);
-        hipLaunchKernelGGL(embedding_group_kernel, grid, threads, 0, s, a, buf[0], buf[1], p.passes, p.bits, f);
-    } else {
-        for (int i = 0; i < p.passes; ++i) {
-            uint2 *to = buf[i & 1];
-            for (int scatter = 0; scatter < 2; ++scatter) {
-                const dim3 grid = next(p.blocks, f);
-                hipLaunchKernelGGL(sort_kernel(i == 0, scatter, p.items == kSortItems), grid, threads, 0, s, a, pairs, to, hist, i * p.bits, p.bits, p.items, f);
-            }
-            pairs = to;
-        }
-    }
-    if (p.chunk == 8) sum_and_join<DT, 8>(a, p, pairs, part, s);
-    else sum_and_join<DT, 32>(a, p, pairs, part, s);
+    const Plan p = plan(a.n, a.V);
+    if (p.chunk == 8) sum_and_join<DT, 8>(a, p, s);
+    else sum_and_join<DT, 32>(a, p, s);
 }
 
 }  // namespace
 
-size_t embedding_workspace_bytes(int64_t n, int64_t V, int C) {
-    const Plan p = plan(n, V, C);
-    return 2 * p.pairs_bytes + p.hist_bytes + p.part_bytes;
-}
+size_t embedding_order_bytes(int64_t n, int64_t V) { return plan(n, V).bytes; }
 
+size_t embedding_workspace_bytes(int64_t n, int C) { return parts(plan(n, 1), C).bytes; }
+
+// (threads of a launch are below 2^32)
 bool embedding_grid_fits(int64_t n, int64_t V, int C, int dt) {
-    const Plan p = plan(n, V, C);
-    const int64_t vecs = (C + (dt == PRIME_F32 ? 3 : 7)) / (dt == PRIME_F32 ? 4 : 8), limit = (int64_t{1} << 32) - kSortThreads;
-    const int64_t fill = V * C * (dt == PRIME_F32 ? 4 : 2) / 64 + kSortThreads;  // threads, of one launch at most
-    return (p.chunks + 3) * ((vecs + kWave - 1) / kWave) * kWave < limit && fill + (p.blocks + kGroups + 1) * kSortThreads < limit;
+    const int64_t vecs = (C + (dt == PRIME_F32 ? 3 : 7)) / (dt == PRIME_F32 ? 4 : 8), slabs = (vecs + kWave - 1) / kWave;
+    const int64_t chunks = plan(n, V).chunks, limit = (int64_t{1} << 32) - kSortThreads;
+    const int64_t sum = (chunks + 3) * slabs * kWave + ((V + kZeroRows - 1) / kZeroRows + 2 + chunks / kThreads) * kThreads;
+    return sum < limit;
 }
 
 hipError_t launch_embedding(const EmbeddingArgs &a, bool backward, hipStream_t stream) {
-    if (a.dt == PRIME_BF16) backward ? run_backward<PRIME_BF16>(a, stream) : run<PRIME_BF16>(a, stream);
-    else if (a.dt == PRIME_F16) backward ? run_backward<PRIME_F16>(a, stream) : run<PRIME_F16>(a, stream);
-    else backward ? run_backward<PRIME_F32>(a, stream) : run<PRIME_F32>(a, stream);
+    if (!backward) run(a, stream);
+    else if (a.dt == PRIME_BF16) run_backward<PRIME_BF16>(a, stream);
+    else if (a.dt == PRIME_F16) run_backward<PRIME_F16>(a, stream);
+    else run_backward<PRIME_F32>(a, stream);
     return hipGetLastError();
 }
 

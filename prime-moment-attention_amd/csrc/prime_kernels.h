@@ -487,9 +487,11 @@ struct EmbeddingArgs {
     const void *dy;                   // backward: n rows, ldy elements apart
     int64_t ldy;
     void *dweight;                    // [V, C]
-    void *workspace;
+    void *order;                      // forward: made, or null; backward: read
+    void *workspace;                  // backward: the parts of ids that reach over chunks
 };
-size_t embedding_workspace_bytes(int64_t n, int64_t V, int C);
+size_t embedding_order_bytes(int64_t n, int64_t V);
+size_t embedding_workspace_bytes(int64_t n, int C);
 bool embedding_grid_fits(int64_t n, int64_t V, int C, int dt);
 hipError_t launch_embedding(const EmbeddingArgs &a, bool backward, hipStream_t stream);
 

@@ -39,7 +39,8 @@ EXPORTS = ("prime_abi_version", "prime_last_error", "prime_decode_step", "prime_
            "prime_delta_decode_step_backward", "prime_delta_gates",
            "prime_gated_scan", "prime_gated_scan_workspace_size", "prime_gated_scan_backward",
            "prime_gated_scan_backward_workspace_size", "prime_dropout_add", "prime_sample",
-           "prime_embedding", "prime_embedding_backward", "prime_embedding_backward_workspace_size",
+           "prime_embedding", "prime_embedding_order_size", "prime_embedding_backward",
+           "prime_embedding_backward_workspace_size",
            "prime_token_logprobs", "prime_token_logprobs_backward",
            "prime_grad_norm", "prime_grad_norm_workspace_size", "prime_grad_clip")
 
@@ -219,10 +220,11 @@ def load() -> ctypes.CDLL:
     L.prime_sample.argtypes = [fp, i32, i32, i32, i64, fp, f32, fp, i32, fp, f32, fp, f32, fp, fp, fp]
     L.prime_sample.restype = ctypes.c_int
     f64, size = ctypes.c_double, ctypes.c_size_t
-    L.prime_embedding.argtypes = [fp, i32, i64, fp, i64, i64, i32, i32, f32, fp, fp]
-    L.prime_embedding_backward_workspace_size.argtypes = [i64, i64, i32]
-    L.prime_embedding_backward_workspace_size.restype = size
-    L.prime_embedding_backward.argtypes = [fp, i32, i64, fp, i64, i64, i32, i32, f32, i64, fp, fp, size, fp]
+    L.prime_embedding.argtypes = [fp, i32, i64, fp, i64, i64, i32, i32, f32, i64, fp, fp, size, fp]
+    L.prime_embedding_order_size.argtypes = [i64, i64]
+    L.prime_embedding_backward_workspace_size.argtypes = [i64, i32]
+    L.prime_embedding_order_size.restype = L.prime_embedding_backward_workspace_size.restype = size
+    L.prime_embedding_backward.argtypes = [fp, size, i64, fp, i64, i64, i32, i32, f32, fp, fp, size, fp]
     L.prime_token_logprobs.argtypes = [fp, i32, i32, i32, i64, fp, i64, fp, fp, fp, i32, fp, fp, fp]
     L.prime_token_logprobs_backward.argtypes = [fp, i32, i32, i32, i64, fp, i64, fp, fp, fp, fp, fp, i64, fp]
     L.prime_grad_norm_workspace_size.argtypes = [fp, i32]
@@ -1298,48 +1300,55 @@ def sample(logits, uniforms, temperature, top_k, top_p, min_p, out) -> None:
 
 
 # ---------------------------------------------------------------- embedding, log probabilities, clipping
-def _check_table(ids, rows, C: int, what: str) -> None:
-    """ids (int64 or int32, contiguous) and rows [*, C] with contiguous columns."""
-    if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
-        raise ValueError(f"ids are {ids.dtype}: int64 or int32 is needed")
-    if rows.dtype not in _DTYPES:
-        raise RuntimeError(f"unsupported dtype {rows.dtype}")
-    if rows.dim() != 2 or rows.shape[1] != C or (rows.stride(1) != 1 and C > 1) or not ids.is_contiguous():
-        raise ValueError(f"{what} must be rows of {C} contiguous columns, ids contiguous")
-
-
 def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def embedding(ids, weight, scale: float, out) -> None:
-    """prime_embedding: contiguous ids of any shape, weight [V, C] with contiguous columns,
-    out [ids.numel(), C] contiguous."""
+def _check_rows(rows, C: int, what: str) -> None:
+    if rows.dtype not in _DTYPES:
+        raise RuntimeError(f"unsupported dtype {rows.dtype}")
+    if rows.dim() != 2 or rows.shape[1] != C or (rows.stride(1) != 1 and C > 1):
+        raise ValueError(f"{what} must be rows of {C} contiguous columns")
+
+
+def embedding_order(n: int, V: int, device) -> torch.Tensor:
+    """A buffer for the order of n tokens of a table of V."""
+    return torch.empty(load().prime_embedding_order_size(n, V), dtype=torch.uint8, device=device)
+
+
+def embedding(ids, weight, scale: float, out, padding: int = -1, order=None) -> None:
+    """prime_embedding: contiguous ids of any shape (int64 or int32), weight [V, C] with
+    contiguous columns, out [ids.numel(), C] contiguous; order (embedding_order) receives the
+    tokens' order for embedding_backward, without those of the id `padding` (-1: none)."""
     V, C = weight.shape
-    _check_table(ids, weight, C, "weight")
+    if (ids.dtype is not torch.int64 and ids.dtype is not torch.int32) or not ids.is_contiguous():
+        raise ValueError(f"ids must be a contiguous int64 or int32 tensor, not {ids.dtype}")
+    _check_rows(weight, C, "weight")
     n = ids.numel()
     if out.dtype is not weight.dtype or out.numel() != n * C or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {weight.dtype} tensor of {n} x {C}")
-    _same_device(weight, ids, out)
+    _same_device(weight, ids, out, order)
     _launch(load().prime_embedding, "prime_embedding", weight.device, ids.data_ptr(), ids.dtype is torch.int64, n,
-            weight.data_ptr(), _row_stride(weight), V, C, _DTYPES[weight.dtype], scale, out.data_ptr())
+            weight.data_ptr(), _row_stride(weight), V, C, _DTYPES[weight.dtype], scale, padding, out.data_ptr(),
+            _ptr(order), 0 if order is None else order.numel())
 
 
-def embedding_backward(ids, dy, scale: float, padding: int, dweight) -> None:
-    """prime_embedding_backward: dy [ids.numel(), C] with contiguous columns, dweight [V, C]
-    contiguous; padding: an id without a gradient, or -1."""
+def embedding_backward(order, dy, scale: float, dweight) -> None:
+    """prime_embedding_backward: the order that embedding made of dy.shape[0] tokens and
+    dweight's V, dy [n, C] with contiguous columns, dweight [V, C] contiguous."""
     V, C = dweight.shape
-    _check_table(ids, dy, C, "dy")
-    n = ids.numel()
-    if dy.shape[0] != n or dweight.dtype is not dy.dtype or not dweight.is_contiguous():
-        raise ValueError(f"dy must be [{n}, {C}], dweight contiguous and of its dtype")
-    _same_device(dy, ids, dweight)
+    _check_rows(dy, C, "dy")
+    n = dy.shape[0]
+    if dweight.dtype is not dy.dtype or not dweight.is_contiguous():
+        raise ValueError("dweight must be contiguous and of dy's dtype")
+    if order.dtype is not torch.uint8 or not order.is_contiguous():
+        raise ValueError("order must be a buffer of embedding_order")
+    _same_device(dy, order, dweight)
     L = load()
-    size = L.prime_embedding_backward_workspace_size(n, V, C)
+    size = L.prime_embedding_backward_workspace_size(n, C)
     ws = torch.empty(size, dtype=torch.uint8, device=dy.device)
-    _launch(L.prime_embedding_backward, "prime_embedding_backward", dy.device, ids.data_ptr(),
-            ids.dtype is torch.int64, n, dy.data_ptr(), _row_stride(dy), V, C, _DTYPES[dy.dtype], scale, padding,
-            dweight.data_ptr(), ws.data_ptr(), size)
+    _launch(L.prime_embedding_backward, "prime_embedding_backward", dy.device, order.data_ptr(), order.numel(), n,
+            dy.data_ptr(), _row_stride(dy), V, C, _DTYPES[dy.dtype], scale, dweight.data_ptr(), ws.data_ptr(), size)
 
 
 def _check_logits(logits, tokens) -> Tuple[int, int]:

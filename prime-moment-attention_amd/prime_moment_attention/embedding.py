@@ -13,22 +13,27 @@ from .chunked_ssd import needs_grad, once
 from .dropout import _rows
 
 
-def _run(ids, weight, scale) -> torch.Tensor:
+def _run(ids, weight, scale, padding=-1, order=None) -> torch.Tensor:
     out = weight.new_empty((*ids.shape, weight.shape[1]))
     if out.numel() == 0:
         return out
     if weight.shape[0] == 0:
         return out.zero_()
-    _lib.embedding(ids, weight, scale, out)
+    _lib.embedding(ids, weight, scale, out, padding, order)
     return out
 
 
 class _EmbeddingFn(torch.autograd.Function):
+    """The lookup makes the tokens' order by their ids too, which is all that the gradient needs
+    of them."""
+
     @staticmethod
     def forward(ctx, weight, ids, scale, padding):
-        ctx.scale, ctx.padding, ctx.table = scale, padding, weight.shape
-        ctx.save_for_backward(ids)
-        return _run(ids, weight, scale)
+        ctx.scale, ctx.table = scale, weight.shape
+        ctx.order = None
+        if ids.numel() and weight.numel():
+            ctx.order = _lib.embedding_order(ids.numel(), weight.shape[0], weight.device)
+        return _run(ids, weight, scale, padding, ctx.order)
 
     @staticmethod
     def backward(ctx, dy):
@@ -36,12 +41,10 @@ class _EmbeddingFn(torch.autograd.Function):
 
     @staticmethod
     def _grads(ctx, dy):
-        ids, = ctx.saved_tensors
-        if dy.numel() == 0:
+        if ctx.order is None:
             return dy.new_zeros(ctx.table), None, None, None
         dweight = dy.new_empty(ctx.table)
-        if dweight.numel():
-            _lib.embedding_backward(ids, _rows(dy), ctx.scale, ctx.padding, dweight)
+        _lib.embedding_backward(ctx.order, _rows(dy), ctx.scale, dweight)
         return dweight, None, None, None
 
 

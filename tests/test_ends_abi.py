@@ -16,9 +16,11 @@ AT = [(i + 1) << 28 for i in range(12)]  # addresses far apart; never dereferenc
 
 
 def test_embedding_refuses_before_device_work():
-    def call(ids=AT[0], i64=1, n=8, w=AT[1], ld=64, V=100, C=64, dt=BF, out=AT[2]):
-        return _lib.load().prime_embedding(ids, i64, n, w, ld, V, C, dt, 1.0, out, None)
-    assert call(ids=None) == -1 and call(w=None) == -1 and call(out=None) == -1
+    need = _lib.load().prime_embedding_order_size(8, 100)
+
+    def call(ids=AT[0], i64=1, n=8, w=AT[1], ld=64, V=100, C=64, dt=BF, out=AT[2], order=AT[3], no=need):
+        return _lib.load().prime_embedding(ids, i64, n, w, ld, V, C, dt, 1.0, -1, out, order, no, None)
+    assert need > 0 and call(ids=None) == -1 and call(w=None) == -1 and call(out=None) == -1
     assert call(n=0) == -1 and call(V=0) == -1 and call(C=0) == -1 and call(n=(1 << 30) + 1) == -1
     assert call(V=1 << 31) == -1 and call(C=(1 << 20) + 1, ld=1 << 21) == -1
     assert call(ld=63) == -1 and "stride" in _lib.last_error()
@@ -26,22 +28,26 @@ def test_embedding_refuses_before_device_work():
     assert call(ids=AT[0] + 4) == -4 and call(ids=AT[0] + 2, i64=0) == -4
     assert call(w=AT[1] + 1) == -4 and call(out=AT[2] + 1) == -4 and call(out=AT[2] + 2, dt=F32) == -4
     assert call(out=AT[1] + 64) == -5 and call(out=AT[0]) == -5 and call(out=AT[1] + 2 * (99 * 64 + 63)) == -5
+    assert call(no=need - 1) == -1 and "order" in _lib.last_error() and call(order=AT[3] + 8) == -1
+    assert call(order=AT[0]) == -5 and call(order=AT[1] + 16) == -5 and call(order=AT[2] + 16) == -5
+    # more threads than a launch has
+    assert call(n=1 << 30, C=1 << 13, ld=1 << 13, order=None) == -1 and "grid" in _lib.last_error()
 
 
 def test_embedding_backward_refuses_before_device_work():
-    size = _lib.load().prime_embedding_backward_workspace_size
-    need = size(8, 100, 64)
+    L = _lib.load()
+    size, osize = L.prime_embedding_backward_workspace_size, L.prime_embedding_order_size
+    need, norder = size(8, 64), osize(8, 100)
 
-    def call(ids=AT[0], n=8, dy=AT[1], ld=64, V=100, C=64, dt=BF, dw=AT[2], ws=AT[3], nw=need):
-        return _lib.load().prime_embedding_backward(ids, 1, n, dy, ld, V, C, dt, 1.0, -1, dw, ws, nw, None)
-    assert need > 0 and size(0, 100, 64) == 0 and size(8, 0, 64) == 0 and size(8, 100, 0) == 0
-    assert call(ids=None) == -1 and call(dy=None) == -1 and call(dw=None) == -1 and call(ws=None) == -1
+    def call(order=AT[0], no=norder, n=8, dy=AT[1], ld=64, V=100, C=64, dt=BF, dw=AT[2], ws=AT[3], nw=need):
+        return L.prime_embedding_backward(order, no, n, dy, ld, V, C, dt, 1.0, dw, ws, nw, None)
+    assert need > 0 and size(0, 64) == 0 and size(8, 0) == 0 and osize(0, 100) == 0 and osize(8, 0) == 0
+    assert call(order=None) == -1 and call(dy=None) == -1 and call(dw=None) == -1 and call(ws=None) == -1
     assert call(nw=need - 1) == -1 and "workspace" in _lib.last_error() and call(ws=AT[3] + 8) == -1
+    assert call(no=norder - 1) == -1 and "order" in _lib.last_error() and call(order=AT[0] + 8) == -1
     assert call(ld=63) == -1 and call(dt=4) == -3 and call(dw=AT[2] + 1) == -4
     assert call(dw=AT[1] + 128) == -5 and call(dw=AT[0]) == -5 and call(ws=AT[2] + 16) == -5
     assert call(ws=AT[1]) == -5 and call(ws=AT[0]) == -5
-    big = size(1 << 30, 100, 1 << 12)  # more threads than a launch has
-    assert call(n=1 << 30, C=1 << 12, ld=1 << 12, nw=big) == -1 and "grid" in _lib.last_error()
 
 
 def test_logprobs_refuse_before_device_work():

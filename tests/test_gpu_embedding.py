@@ -156,9 +156,9 @@ def test_retained_graph_and_one_gradient_only():
         (again * again).sum().backward()
     ids = torch.tensor([1, 2], device="cuda")
     y = embedding_lookup(ids, w)
-    ids.add_(1)  # the gradient needs them as they were
-    with pytest.raises(RuntimeError, match="modified"):
-        y.sum().backward()
+    ids.add_(1)  # the gradient is that of the ids as they were
+    grad, = torch.autograd.grad(y.sum(), w)
+    assert (grad[[1, 2]] == 1).all() and grad.sum() == 8
 
 
 def test_streams_side_by_side():
@@ -231,10 +231,16 @@ def test_entry_point_leaves_what_is_not_its_own():
     buf = torch.full((n * C + 64,), 7.0, device="cuda")
     _lib.embedding(ids, w, 1.0, buf[32:-32].view(n, C))
     assert (buf[:32] == 7).all() and (buf[-32:] == 7).all() and torch.equal(buf[32:-32].view(n, C), w[ids])
+    size = _lib.embedding_order(n, V, "cuda").numel()
+    order = torch.full((size + 512,), 7, dtype=torch.uint8, device="cuda")
+    _lib.embedding(ids, w, 1.0, torch.empty(n, C, device="cuda"), -1, order[256:-256])
+    assert (order[:256] == 7).all() and (order[-256:] == 7).all()
     buf = torch.full((V * C + 64,), 7.0, device="cuda")
-    _lib.embedding_backward(ids, torch.randn(n, C, device="cuda"), 1.0, -1, buf[32:-32].view(V, C))
+    _lib.embedding_backward(order[256:-256], torch.randn(n, C, device="cuda"), 1.0, buf[32:-32].view(V, C))
     assert (buf[:32] == 7).all() and (buf[-32:] == 7).all()
     with pytest.raises(ValueError):
         _lib.embedding(ids, w, 1.0, buf[:5])
-    with pytest.raises(ValueError):
-        _lib.embedding_backward(ids, torch.randn(n - 1, C, device="cuda"), 1.0, -1, w)
+    with pytest.raises(RuntimeError, match="order"):
+        _lib.embedding_backward(order[:size - 1], torch.randn(n, C, device="cuda"), 1.0, w)
+    with pytest.raises(RuntimeError, match="order"):
+        _lib.embedding(ids, w, 1.0, torch.empty(n, C, device="cuda"), -1, order[1:])
