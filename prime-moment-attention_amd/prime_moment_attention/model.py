@@ -32,6 +32,13 @@ Additions for other layers and for training:
     layer's state is one fp32 tensor [B, heads * head_dim].
   * ``PrimeConfig.dropout``: in training each block's two branches are dropped
     out as they are added to the residual stream (dropout_add).
+  * ``PrimeConfig.embedding_scale``: the embeddings times a factor.
+  * ``PrimeConfig.fused_training``: the embedding by embedding_lookup (its gradient
+    without atomics: a step repeats bit for bit) and the loss by token_logprobs (no
+    fp32 copy of the logits, no softmax kept).
+  * ``clip_grad_norm_(max_norm)`` on the model; ``score(input_ids)`` for the log
+    probabilities of a text; ``SamplingDecoder(logprobs=k)`` for those of the tokens
+    that it chooses.
 """
 from __future__ import annotations
 
@@ -46,14 +53,18 @@ import torch.nn.functional as F
 from . import _lib
 from .attention import PrimeMomentAttention
 from .dropout import dropout_add, dropout_rng
+from .embedding import embedding_lookup
 from .gated_recurrence import GatedLinearRecurrence
+from .grad_clip import clip_grad_norm_
+from .logprobs import TokenLogprobs, token_logprobs
 from .sampling import _per_row, sample_tokens
 from .selective import PrimeSelectiveMomentAttention
 
 
 @dataclass
 class PrimeConfig:
-    """model.py:20-44, plus ``mlp_type``, ``dropout`` and ``gated_layers``."""
+    """model.py:20-44, plus ``mlp_type``, ``dropout``, ``gated_layers``, ``embedding_scale`` and
+    ``fused_training``."""
     vocab_size: int = 32000
     hidden_size: int = 512
     num_layers: int = 6
@@ -73,6 +84,8 @@ class PrimeConfig:
     mlp_type: str = "swiglu"
     dropout: float = 0.0
     gated_layers: Tuple[int, ...] = ()
+    embedding_scale: float = 1.0
+    fused_training: bool = False
 
     def __post_init__(self):
         if self.num_kv_heads is None:
@@ -198,6 +211,15 @@ class PrimeBlock(nn.Module):
         return dropout_add(h.to(dtype), residual.to(dtype), self.dropout, rng, call=2 * self.layer + branch)
 
 
+def _total(t: torch.Tensor) -> torch.Tensor:
+    """The sum, 1024 values at a time: torch's sum over several workgroups clears its counters by a
+    memset, which a captured training step would repeat wrongly."""
+    t = t.flatten()
+    while t.numel() > 1024:
+        t = F.pad(t, (0, -t.numel() % 1024)).view(-1, 1024).sum(1)
+    return t.sum()
+
+
 class PrimeForCausalLM(nn.Module):
     """model.py:121-242 on the HIP attention kernels."""
 
@@ -254,7 +276,8 @@ class PrimeForCausalLM(nn.Module):
             intermediate_size=get("intermediate_size"), decay=get("decay"), use_qk_norm=get("use_qk_norm"),
             rms_norm_eps=get("rms_norm_eps"), eps=get("eps"), tie_word_embeddings=get("tie_word_embeddings"),
             initializer_range=get("initializer_range"), use_selective=True, mlp_type=get("mlp_type", "swiglu"),
-            dropout=get("dropout", 0.0), gated_layers=get("gated_layers", ()), **tau_range)
+            dropout=get("dropout", 0.0), gated_layers=get("gated_layers", ()),
+            embedding_scale=get("embedding_scale", 1.0), fused_training=get("fused_training", False), **tau_range)
         model = cls(sel_config).to(device)
         sd = ckpt["model_state_dict"]
         missing_keys, unexpected_keys = model.load_state_dict(sd, strict=False)
@@ -284,6 +307,52 @@ class PrimeForCausalLM(nn.Module):
     def set_input_embeddings(self, value: nn.Embedding):
         self.embed_tokens = value
 
+    @property
+    def embedding_scale(self) -> float:
+        return getattr(self.config, "embedding_scale", 1.0)  # (a config of another class may lack it)
+
+    @property
+    def fused_training(self) -> bool:
+        return getattr(self.config, "fused_training", False)
+
+    def _embed(self, input_ids: torch.Tensor) -> torch.Tensor:
+        """The scaled embeddings of the tokens, a tensor of this call's own."""
+        e, scale = self.embed_tokens, self.embedding_scale
+        if not (self.fused_training or scale != 1.0):
+            return e(input_ids)
+        if (type(e) is nn.Embedding and e.max_norm is None and not e.scale_grad_by_freq and not e.sparse
+                and not (e._forward_hooks or e._forward_pre_hooks or e._backward_hooks)):
+            return embedding_lookup(input_ids, e.weight, scale, e.padding_idx)
+        x = e(input_ids)  # (a module of the user's own)
+        return x if scale == 1.0 else x * scale
+
+    def _loss(self, logits: torch.Tensor, labels: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+        """The mean cross entropy of the next tokens (model.py:190-198)."""
+        if labels is None:
+            return None
+        if self.fused_training:
+            # the logits as they lie: no token follows the last position's
+            target = F.pad(labels[..., 1:], (0, 1), value=-100)
+            return -_total(token_logprobs(logits, target, ignore_index=-100).logprobs) / _total(target != -100)
+        shift_logits = logits[..., :-1, :].contiguous().to(torch.float32)
+        return F.cross_entropy(shift_logits.view(-1, self.config.vocab_size),
+                               labels[..., 1:].contiguous().view(-1), ignore_index=-100)
+
+    def clip_grad_norm_(self, max_norm: float) -> torch.Tensor:
+        """clip_grad_norm_ over the model's parameters."""
+        return clip_grad_norm_(self.parameters(), max_norm)
+
+    @torch.no_grad()
+    def score(self, input_ids: torch.Tensor, top: int = 0, entropy: bool = False) -> TokenLogprobs:
+        """For every token of the texts input_ids [B, L] but the first, what token_logprobs says
+        of it after the tokens before it: [B, L - 1] each ([B, L - 1, top])."""
+        if self.drops_out:
+            raise ValueError("the model drops out while it trains: call its eval() before scoring")
+        logits = self.forward(input_ids)["logits"]
+        target = F.pad(input_ids[..., 1:], (0, 1), value=-100)  # (nothing of the last position is kept)
+        r = token_logprobs(logits, target, top=top, entropy=entropy)
+        return TokenLogprobs(*[None if t is None else t[:, :-1] for t in r])
+
     def forward(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None,
                 states: Optional[List[Tuple[torch.Tensor, ...]]] = None, return_states: bool = False,
                 logits_to_keep: int = 0) -> Dict[str, Any]:
@@ -298,17 +367,12 @@ class PrimeForCausalLM(nn.Module):
             else:
                 logits, ns = _fused_step(self, input_ids, states, consts, inplace=False)
             logits = logits.unsqueeze(1)
-            loss = None
-            if labels is not None:
-                shift_logits = logits[..., :-1, :].contiguous().to(torch.float32)
-                loss = F.cross_entropy(shift_logits.view(-1, self.config.vocab_size),
-                                       labels[..., 1:].contiguous().view(-1), ignore_index=-100)
-            return {"loss": loss, "logits": logits, "states": ns if return_states else None}
+            return {"loss": self._loss(logits, labels), "logits": logits, "states": ns if return_states else None}
         # x is this call's own residual stream, updated in place: each block's
         # output projection and its residual add are one GEMM with beta = 1
         # (x += y W^T, the sum rounded once), followed by the RMSNorm
         # (prime_add_rmsnorm without a delta).
-        x = self.embed_tokens(input_ids)
+        x = self._embed(input_ids)
         hidden = x.shape[-1]
         x2 = x.view(-1, hidden)
         next_states = [] if return_states else None
@@ -328,18 +392,13 @@ class PrimeForCausalLM(nn.Module):
         nf = torch.empty_like(x)
         _lib.add_rmsnorm(x.view(-1, hidden), None, self.norm.weight, nf.view(-1, hidden), self.norm.eps)
         logits = self.lm_head(nf)
-        loss = None
-        if labels is not None:
-            shift_logits = logits[..., :-1, :].contiguous().to(torch.float32)
-            loss = F.cross_entropy(shift_logits.view(-1, self.config.vocab_size),
-                                   labels[..., 1:].contiguous().view(-1), ignore_index=-100)
-        return {"loss": loss, "logits": logits, "states": next_states}
+        return {"loss": self._loss(logits, labels), "logits": logits, "states": next_states}
 
     def _forward_graph(self, input_ids, labels, states, return_states, logits_to_keep):
         """The reference's composition (model.py:175-200) for autograd: each
         block's residual adds and RMSNorms as torch ops, the attention through
         the differentiable prefill."""
-        x = self.embed_tokens(input_ids)
+        x = self._embed(input_ids)
         next_states = [] if return_states else None
         # without dropout a block needs no more than (hidden_states, state, return_state)
         drop = {"rng": dropout_rng(x.device)} if self.drops_out else {}
@@ -350,12 +409,7 @@ class PrimeForCausalLM(nn.Module):
         if logits_to_keep:
             x = x[:, -logits_to_keep:]
         logits = self.lm_head(self.norm(x))
-        loss = None
-        if labels is not None:
-            shift_logits = logits[..., :-1, :].contiguous().to(torch.float32)
-            loss = F.cross_entropy(shift_logits.view(-1, self.config.vocab_size),
-                                   labels[..., 1:].contiguous().view(-1), ignore_index=-100)
-        return {"loss": loss, "logits": logits, "states": next_states}
+        return {"loss": self._loss(logits, labels), "logits": logits, "states": next_states}
 
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int = 50, temperature: float = 1.0,
@@ -586,7 +640,7 @@ def _fused_step(model: "PrimeForCausalLM", tokens: torch.Tensor, states, consts:
     module was built with inplace_state and the given tensors are its own
     layout)."""
     cfg = model.config
-    x = model.embed_tokens(tokens).reshape(-1, cfg.hidden_size)  # the residual stream, updated in place
+    x = model._embed(tokens).reshape(-1, cfg.hidden_size)  # the residual stream, updated in place
     B = x.shape[0]
     dev = x.device
     # folded form: RMSNorm -> projection and projection -> residual add /
@@ -667,7 +721,8 @@ def _frag_step(model: "PrimeForCausalLM", tokens: torch.Tensor, states, consts: 
     model.py:160, the greedy choice of model.py:230-231).  The residual stream
     x, the attention output y and the MLP's hidden layer stay in the fragment
     layout from the embedding gather to the lm_head:
-      x  <- embed_tokens[tokens]                      (prime_pack_frag)
+      x  <- embed_tokens[tokens]                      (prime_pack_frag; scaled: after
+                                                       prime_embedding)
       per layer:
         qkv <- RMS(x) . Wqkv'^T (+ step bias)         (prime_linear_frag, row-major)
         y   <- decode step (QK-norm, 1/sqrt(D) inside; selective gate from qkv)
@@ -687,7 +742,10 @@ def _frag_step(model: "PrimeForCausalLM", tokens: torch.Tensor, states, consts: 
     B = tok.numel()
     dev = tok.device
     Mp = _lib.frag_rows(B)
-    x = _lib.pack_frag(model.embed_tokens.weight, rows=tok)
+    if model.embedding_scale == 1.0:
+        x = _lib.pack_frag(model.embed_tokens.weight, rows=tok)
+    else:
+        x = _lib.pack_frag(model._embed(tok))
     at0 = model.layers[0].self_attn
     y = torch.empty(Mp * at0.num_heads * at0.head_dim, device=dev, dtype=x.dtype)
     t = torch.empty(Mp * consts[0].frag.inter, device=dev, dtype=x.dtype)
@@ -824,13 +882,20 @@ class SamplingDecoder(GreedyDecoder):
     nothing; temperature 0 is greedy), and one uniform number per token from
     ``generator`` (on the model's device; None: torch's own).  The numbers are drawn
     before each step into a fixed buffer, so that replays of the captured step sample
-    anew and a seeded generator gives the same tokens with and without a graph."""
+    anew and a seeded generator gives the same tokens with and without a graph.
+
+    logprobs: how many alternatives (0 to 64) come with each token's own log probability in
+    ``decoder.logprobs``, a TokenLogprobs of [B] and [B, logprobs] of the model's distribution
+    (before temperature and cuts); the next step writes over it.  None: not computed."""
 
     def __init__(self, model: PrimeForCausalLM, temperature=1.0, top_k=50, top_p=1.0, min_p=0.0,
-                 generator: Optional[torch.Generator] = None, use_graph: bool = True):
+                 generator: Optional[torch.Generator] = None, use_graph: bool = True,
+                 logprobs: Optional[int] = None):
         super().__init__(model, use_graph)
         self.cuts = (temperature, top_k, top_p, min_p)
         self.generator = generator
+        self.alternatives = logprobs
+        self.logprobs: Optional[TokenLogprobs] = None
 
     @torch.no_grad()
     def prefill(self, input_ids: torch.Tensor) -> torch.Tensor:
@@ -843,6 +908,8 @@ class SamplingDecoder(GreedyDecoder):
 
     def _choose(self, logits: torch.Tensor) -> None:
         sample_tokens(logits, self.uniforms, *self.params, out=self.token.view(-1))
+        if self.alternatives is not None:
+            self.logprobs = token_logprobs(logits, self.token.view(-1), top=self.alternatives)
 
     @torch.no_grad()
     def _step_eager(self) -> torch.Tensor:
