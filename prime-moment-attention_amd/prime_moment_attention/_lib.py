@@ -1130,7 +1130,7 @@ def _launch(fn, what: str, dev: torch.device, *args) -> None:
     """The entry point fn on the current stream of the tensors' device, which need not be
     the current device."""
     index = dev.index
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
@@ -1316,39 +1316,46 @@ def embedding_order(n: int, V: int, device) -> torch.Tensor:
     return torch.empty(load().prime_embedding_order_size(n, V), dtype=torch.uint8, device=device)
 
 
-def embedding(ids, weight, scale: float, out, padding: int = -1, order=None) -> None:
+def embedding(ids, weight, scale: float, out, padding: int = -1, order=None, checked: bool = False) -> None:
     """prime_embedding: contiguous ids of any shape (int64 or int32), weight [V, C] with
     contiguous columns, out [ids.numel(), C] contiguous; order (embedding_order) receives the
-    tokens' order for embedding_backward, without those of the id `padding` (-1: none)."""
+    tokens' order for embedding_backward, without those of the id `padding` (-1: none).
+    checked: the caller knows the operands to be so."""
     V, C = weight.shape
-    if (ids.dtype is not torch.int64 and ids.dtype is not torch.int32) or not ids.is_contiguous():
-        raise ValueError(f"ids must be a contiguous int64 or int32 tensor, not {ids.dtype}")
-    _check_rows(weight, C, "weight")
     n = ids.numel()
-    if out.dtype is not weight.dtype or out.numel() != n * C or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous {weight.dtype} tensor of {n} x {C}")
-    _same_device(weight, ids, out, order)
+    if not checked:
+        if (ids.dtype is not torch.int64 and ids.dtype is not torch.int32) or not ids.is_contiguous():
+            raise ValueError(f"ids must be a contiguous int64 or int32 tensor, not {ids.dtype}")
+        _check_rows(weight, C, "weight")
+        if out.dtype is not weight.dtype or out.numel() != n * C or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {weight.dtype} tensor of {n} x {C}")
+        _same_device(weight, ids, out, order)
     _launch(load().prime_embedding, "prime_embedding", weight.device, ids.data_ptr(), ids.dtype is torch.int64, n,
-            weight.data_ptr(), _row_stride(weight), V, C, _DTYPES[weight.dtype], scale, padding, out.data_ptr(),
-            _ptr(order), 0 if order is None else order.numel())
+            weight.data_ptr(), weight.stride(0) if V > 1 else C, V, C, _DTYPES[weight.dtype], scale, padding,
+            out.data_ptr(), *((None, 0) if order is None else (order.data_ptr(), order.numel())))
 
 
-def embedding_backward(order, dy, scale: float, dweight) -> None:
-    """prime_embedding_backward: the order that embedding made of dy.shape[0] tokens and
-    dweight's V, dy [n, C] with contiguous columns, dweight [V, C] contiguous."""
+def embedding_backward(order, dy, scale: float, dweight, checked: bool = False) -> None:
+    """prime_embedding_backward: the order that embedding made of the n tokens and dweight's
+    V, dy [n, C] with contiguous columns (or contiguous, of any shape), dweight [V, C]
+    contiguous.  checked: the caller knows the operands to be so."""
     V, C = dweight.shape
-    _check_rows(dy, C, "dy")
-    n = dy.shape[0]
-    if dweight.dtype is not dy.dtype or not dweight.is_contiguous():
-        raise ValueError("dweight must be contiguous and of dy's dtype")
-    if order.dtype is not torch.uint8 or not order.is_contiguous():
-        raise ValueError("order must be a buffer of embedding_order")
-    _same_device(dy, order, dweight)
+    if dy.dim() == 2:
+        n, pitch = dy.shape[0], dy.stride(0)
+    else:
+        n, pitch = dy.numel() // C, C
+    if not checked:
+        _check_rows(dy if dy.dim() == 2 else dy.view(-1, C), C, "dy")
+        if dweight.dtype is not dy.dtype or not dweight.is_contiguous():
+            raise ValueError("dweight must be contiguous and of dy's dtype")
+        if order.dtype is not torch.uint8 or not order.is_contiguous():
+            raise ValueError("order must be a buffer of embedding_order")
+        _same_device(dy, order, dweight)
     L = load()
     size = L.prime_embedding_backward_workspace_size(n, C)
     ws = torch.empty(size, dtype=torch.uint8, device=dy.device)
     _launch(L.prime_embedding_backward, "prime_embedding_backward", dy.device, order.data_ptr(), order.numel(), n,
-            dy.data_ptr(), _row_stride(dy), V, C, _DTYPES[dy.dtype], scale, dweight.data_ptr(), ws.data_ptr(), size)
+            dy.data_ptr(), pitch if n > 1 else C, V, C, _DTYPES[dy.dtype], scale, dweight.data_ptr(), ws.data_ptr(), size)
 
 
 def _check_logits(logits, tokens) -> Tuple[int, int]:
@@ -1368,35 +1375,43 @@ def _f32_of(n: int, *ts) -> None:
             raise ValueError(f"a contiguous fp32 tensor of {n} values is needed, not {tuple(t.shape)} {t.dtype}")
 
 
-def token_logprobs(logits, tokens, ignore: int, logprobs, entropy, stats, top: int, top_logprobs, top_tokens) -> None:
+def token_logprobs(logits, tokens, ignore: int, logprobs, entropy, stats, top: int, top_logprobs, top_tokens,
+                   checked: bool = False) -> None:
     """prime_token_logprobs: logits [n, vocab], tokens int64 [n]; fp32 outputs of n (stats:
     2 n) values, entropy and stats or None; top_logprobs fp32, top_tokens int64 of n * top, or
-    None."""
-    n, vocab = _check_logits(logits, tokens)
-    _f32_of(n, logprobs, entropy)
-    _f32_of(2 * n, stats)
-    if top:
-        _f32_of(n * top, top_logprobs)
-        if top_tokens.dtype is not torch.int64 or top_tokens.numel() != n * top or not top_tokens.is_contiguous():
-            raise ValueError(f"top_tokens must be a contiguous int64 tensor of {n * top} values")
-    _same_device(logits, tokens, logprobs, entropy, stats, top_logprobs, top_tokens)
+    None.  checked: the caller knows the operands to be so."""
+    if not checked:
+        n, vocab = _check_logits(logits, tokens)
+        _f32_of(n, logprobs, entropy)
+        _f32_of(2 * n, stats)
+        if top:
+            _f32_of(n * top, top_logprobs)
+            if top_tokens.dtype is not torch.int64 or top_tokens.numel() != n * top or not top_tokens.is_contiguous():
+                raise ValueError(f"top_tokens must be a contiguous int64 tensor of {n * top} values")
+        _same_device(logits, tokens, logprobs, entropy, stats, top_logprobs, top_tokens)
+    n, vocab = logits.shape
     _launch(load().prime_token_logprobs, "prime_token_logprobs", logits.device, logits.data_ptr(),
-            _DTYPES[logits.dtype], n, vocab, _row_stride(logits), tokens.data_ptr(), ignore, logprobs.data_ptr(),
-            _ptr(entropy), _ptr(stats), top, _ptr(top_logprobs), _ptr(top_tokens))
+            _DTYPES[logits.dtype], n, vocab, logits.stride(0) if n > 1 else vocab, tokens.data_ptr(), ignore,
+            logprobs.data_ptr(), _ptr(entropy), _ptr(stats), top, _ptr(top_logprobs), _ptr(top_tokens))
 
 
-def token_logprobs_backward(logits, tokens, ignore: int, stats, entropy, dlogprobs, dentropy, dlogits) -> None:
+def token_logprobs_backward(logits, tokens, ignore: int, stats, entropy, dlogprobs, dentropy, dlogits,
+                            checked: bool = False) -> None:
     """prime_token_logprobs_backward: dlogits [n, vocab] of logits' dtype; dlogprobs and
-    dentropy fp32 [n] or None."""
-    n, vocab = _check_logits(logits, tokens)
-    _f32_of(2 * n, stats)
-    _f32_of(n, entropy, dlogprobs, dentropy)
-    if dlogits.shape != logits.shape or dlogits.dtype is not logits.dtype or (dlogits.stride(1) != 1 and vocab > 1):
-        raise ValueError("dlogits must have logits' shape and dtype and a contiguous vocab dimension")
-    _same_device(logits, tokens, stats, entropy, dlogprobs, dentropy, dlogits)
+    dentropy fp32 [n] or None.  checked: the caller knows the operands to be so, and dlogits to
+    be contiguous."""
+    if not checked:
+        n, vocab = _check_logits(logits, tokens)
+        _f32_of(2 * n, stats)
+        _f32_of(n, entropy, dlogprobs, dentropy)
+        if dlogits.shape != logits.shape or dlogits.dtype is not logits.dtype or (dlogits.stride(1) != 1 and vocab > 1):
+            raise ValueError("dlogits must have logits' shape and dtype and a contiguous vocab dimension")
+        _same_device(logits, tokens, stats, entropy, dlogprobs, dentropy, dlogits)
+    n, vocab = logits.shape
     _launch(load().prime_token_logprobs_backward, "prime_token_logprobs_backward", logits.device, logits.data_ptr(),
-            _DTYPES[logits.dtype], n, vocab, _row_stride(logits), tokens.data_ptr(), ignore, stats.data_ptr(),
-            _ptr(entropy), _ptr(dlogprobs), _ptr(dentropy), dlogits.data_ptr(), _row_stride(dlogits))
+            _DTYPES[logits.dtype], n, vocab, logits.stride(0) if n > 1 else vocab, tokens.data_ptr(), ignore,
+            stats.data_ptr(), _ptr(entropy), _ptr(dlogprobs), _ptr(dentropy), dlogits.data_ptr(),
+            vocab if checked else _row_stride(dlogits))
 
 
 def grad_norm(tensors, norm, max_norm: Optional[float] = None, given: bool = False) -> None:

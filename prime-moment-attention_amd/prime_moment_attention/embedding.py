@@ -19,7 +19,7 @@ def _run(ids, weight, scale, padding=-1, order=None) -> torch.Tensor:
         return out
     if weight.shape[0] == 0:
         return out.zero_()
-    _lib.embedding(ids, weight, scale, out, padding, order)
+    _lib.embedding(ids, weight, scale, out, padding, order, checked=True)
     return out
 
 
@@ -29,10 +29,10 @@ class _EmbeddingFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, weight, ids, scale, padding):
-        ctx.scale, ctx.table = scale, weight.shape
-        ctx.order = None
-        if ids.numel() and weight.numel():
-            ctx.order = _lib.embedding_order(ids.numel(), weight.shape[0], weight.device)
+        table = weight.shape
+        n = ids.numel()
+        ctx.order = _lib.embedding_order(n, table[0], weight.device) if n and weight.numel() else None
+        ctx.scale, ctx.table = scale, table
         return _run(ids, weight, scale, padding, ctx.order)
 
     @staticmethod
@@ -44,7 +44,7 @@ class _EmbeddingFn(torch.autograd.Function):
         if ctx.order is None:
             return dy.new_zeros(ctx.table), None, None, None
         dweight = dy.new_empty(ctx.table)
-        _lib.embedding_backward(ctx.order, _rows(dy), ctx.scale, dweight)
+        _lib.embedding_backward(ctx.order, dy if dy.is_contiguous() else _rows(dy), ctx.scale, dweight, checked=True)
         return dweight, None, None, None
 
 

@@ -29,22 +29,23 @@ def _rows(logits: torch.Tensor) -> torch.Tensor:
 
 
 def _run(logits, tokens, top, entropy, ignore, stats):
-    lead, f32 = tokens.shape, torch.float32
-    new = lambda shape, dtype=f32: torch.empty(shape, device=logits.device, dtype=dtype)
-    out = (new(lead), new(lead) if entropy else None, new((*lead, top)) if top else None,
-           new((*lead, top), torch.int64) if top else None)
-    if tokens.numel():
-        _lib.token_logprobs(_rows(logits), tokens, ignore, out[0], out[1], stats, top, out[2], out[3])
-    return out
+    lead, dev, f32 = tokens.shape, logits.device, torch.float32
+    lp = torch.empty(lead, device=dev, dtype=f32)
+    ent = torch.empty(lead, device=dev, dtype=f32) if entropy else None
+    top_lp = torch.empty((*lead, top), device=dev, dtype=f32) if top else None
+    top_tokens = torch.empty((*lead, top), device=dev, dtype=torch.int64) if top else None
+    if lp.numel():
+        _lib.token_logprobs(_rows(logits), tokens, ignore, lp, ent, stats, top, top_lp, top_tokens, checked=True)
+    return lp, ent, top_lp, top_tokens
 
 
 class _TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top, entropy, ignore):
-        stats = torch.empty((*tokens.shape, 2), device=logits.device, dtype=torch.float32)
-        out = _run(logits, tokens, top, entropy, ignore, stats)
+        ctx.stats = torch.empty((*tokens.shape, 2), device=logits.device, dtype=torch.float32)
+        out = _run(logits, tokens, top, entropy, ignore, ctx.stats)
         ctx.ignore = ignore
-        ctx.save_for_backward(logits, tokens, stats, out[1])
+        ctx.save_for_backward(logits, tokens, out[1])
         if top:
             ctx.mark_non_differentiable(out[2], out[3])
         ctx.set_materialize_grads(False)
@@ -58,12 +59,15 @@ class _TokenLogprobsFn(torch.autograd.Function):
     def _grads(ctx, dlogprobs, dentropy):
         if dlogprobs is None and dentropy is None:
             return None, None, None, None, None
-        logits, tokens, stats, entropy = ctx.saved_tensors
-        d = [None if t is None else t.contiguous() for t in (dlogprobs, dentropy)]
+        logits, tokens, entropy = ctx.saved_tensors
+        if dlogprobs is not None and not dlogprobs.is_contiguous():
+            dlogprobs = dlogprobs.contiguous()
+        if dentropy is not None and not dentropy.is_contiguous():
+            dentropy = dentropy.contiguous()
         dlogits = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
         if tokens.numel():
-            _lib.token_logprobs_backward(_rows(logits), tokens, ctx.ignore, stats, entropy, *d,
-                                         dlogits.view(-1, logits.shape[-1]))
+            _lib.token_logprobs_backward(_rows(logits), tokens, ctx.ignore, ctx.stats, entropy, dlogprobs, dentropy,
+                                         dlogits, checked=True)
         return dlogits, None, None, None, None
 
 
