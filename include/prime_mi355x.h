@@ -663,7 +663,8 @@ int prime_token_logprobs_backward(const void *logits, int dtype, int n, int voca
 /*
  * The norm over many tensors, and clipping by it.  tensors, sizes, dtypes: host arrays of
  * `count` device addresses, numbers of elements (0: skipped, below 2^35 in all) and types
- * (F32 / BF16 / F16, mixed as they come), contiguous tensors that do not overlap.
+ * (F32 / BF16 / F16, mixed as they come) of contiguous tensors, which do not overlap where they
+ * are clipped.
  *   prime_grad_norm : norm (fp32, on the device) = sqrt(sum of all squares), in 64 bits
  *   prime_grad_clip : the same, and every element times min(1, max_norm / (norm + 1e-6)),
  *                     in fp32, rounded once; nothing is written where that is 1.  given: norm

@@ -1789,7 +1789,7 @@ struct GradTables {
 };
 
 int grad_checks(const void *const *tensors, const int64_t *sizes, const int32_t *dtypes, int count, const float *norm,
-                const void *workspace, size_t workspace_bytes, bool given) {
+                const void *workspace, size_t workspace_bytes, bool given, bool writes) {
     if (count < 0 || (count && (!tensors || !sizes || !dtypes)) || !norm)
         return fail(PRIME_ERR_INVALID_ARG, "null tensors, sizes, dtypes or norm");
     int rc = check_floats(norm, "norm");
@@ -1803,10 +1803,17 @@ int grad_checks(const void *const *tensors, const int64_t *sizes, const int32_t 
             return fail(PRIME_ERR_MISALIGNED, "tensor %d is misaligned", i);
         if ((all += sizes[i]) >= (int64_t{1} << 35)) return fail(PRIME_ERR_INVALID_ARG, "too many elements");
     }
-    const size_t need = given ? 0 : prime_grad_norm_workspace_size(sizes, count);
+    size_t need = 0;
+    if (!given) need = prime_grad_norm_workspace_size(sizes, count);
     if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
         return fail(PRIME_ERR_INVALID_ARG, "workspace of %zu bytes needed, 16-byte aligned", need);
-    // no two of the tensors, norm and the workspace overlap
+    // norm and the workspace overlap nothing, nor do tensors that are written each other
+    for (int i = 0; i < count && !writes; ++i) {
+        const size_t bytes = static_cast<size_t>(sizes[i]) * elem_size(dtypes[i]);
+        if (bytes && (overlap(norm, sizeof(float), tensors[i], bytes) || (need && overlap(workspace, need, tensors[i], bytes))))
+            return fail(PRIME_ERR_ALIAS, "norm or the workspace overlaps tensor %d", i);
+    }
+    if (!writes) return need && overlap(norm, sizeof(float), workspace, need) ? fail(PRIME_ERR_ALIAS, "norm and the workspace overlap") : PRIME_OK;
     try {
         std::vector<std::pair<uintptr_t, uintptr_t>> spans;
         spans.reserve(static_cast<size_t>(count) + 2);
@@ -1972,7 +1979,7 @@ size_t prime_grad_norm_workspace_size(const int64_t *sizes, int count) {
 int prime_grad_norm(const void *const *tensors, const int64_t *sizes, const int32_t *dtypes, int count, float *norm,
                     void *workspace, size_t workspace_bytes, void *stream) {
     g_err[0] = 0;
-    int rc = grad_checks(tensors, sizes, dtypes, count, norm, workspace, workspace_bytes, false);
+    int rc = grad_checks(tensors, sizes, dtypes, count, norm, workspace, workspace_bytes, false, false);
     if (rc) return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     double *parts = static_cast<double *>(workspace);
@@ -1985,7 +1992,7 @@ int prime_grad_norm(const void *const *tensors, const int64_t *sizes, const int3
 int prime_grad_clip(void *const *tensors, const int64_t *sizes, const int32_t *dtypes, int count, double max_norm,
                     float *norm, int given, void *workspace, size_t workspace_bytes, void *stream) {
     g_err[0] = 0;
-    int rc = grad_checks(tensors, sizes, dtypes, count, norm, workspace, workspace_bytes, given);
+    int rc = grad_checks(tensors, sizes, dtypes, count, norm, workspace, workspace_bytes, given, true);
     if (rc) return rc;
     if (!(max_norm >= 0.0)) return fail(PRIME_ERR_INVALID_ARG, "max_norm=%g below 0", max_norm);
     const hipStream_t s = static_cast<hipStream_t>(stream);

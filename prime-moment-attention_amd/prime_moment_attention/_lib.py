@@ -1414,6 +1414,11 @@ def token_logprobs_backward(logits, tokens, ignore: int, stats, entropy, dlogpro
             vocab if checked else _row_stride(dlogits))
 
 
+_T = torch._C.TensorBase
+_dtype_of, _data_ptr, _numel, _get_device = _T.dtype.__get__, _T.data_ptr, _T.numel, _T.get_device
+GRAD_TABLE, GRAD_PARTS = 192, 4096 * 8  # tensors of a launch, and the workspace that they take at most
+
+
 def grad_norm(tensors, norm, max_norm: Optional[float] = None, given: bool = False) -> None:
     """prime_grad_norm of contiguous tensors (or dense ones: every element is theirs) into
     norm (fp32, one value), or with max_norm prime_grad_clip of them; given: by the norm
@@ -1422,18 +1427,17 @@ def grad_norm(tensors, norm, max_norm: Optional[float] = None, given: bool = Fal
     _same_device(norm)
     _f32_of(1, norm)
     index = norm.get_device()
-    for t in tensors:
-        if t.get_device() != index:
-            _same_device(norm, t)
-        if t.dtype not in _DTYPES:
-            raise RuntimeError(f"unsupported dtype {t.dtype}")
+    if set(map(_get_device, tensors)) - {index}:
+        _same_device(norm, *tensors)
+    try:
+        dtypes = array.array("i", map(_DTYPES.__getitem__, map(_dtype_of, tensors)))
+    except KeyError as e:
+        raise RuntimeError(f"unsupported dtype {e.args[0]}") from None
     L = load()
     count = len(tensors)
-    data = array.array("Q", [t.data_ptr() for t in tensors])
-    sizes = array.array("q", [t.numel() for t in tensors])
-    dtypes = array.array("i", [_DTYPES[t.dtype] for t in tensors])
+    data, sizes = array.array("Q", map(_data_ptr, tensors)), array.array("q", map(_numel, tensors))
     table = (data.buffer_info()[0], sizes.buffer_info()[0], dtypes.buffer_info()[0], count)
-    n = 0 if given else L.prime_grad_norm_workspace_size(table[1], count)
+    n = 0 if given else -(-count // GRAD_TABLE) * GRAD_PARTS
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     if max_norm is None:
         _launch(L.prime_grad_norm, "prime_grad_norm", dev, *table, norm.data_ptr(), _ptr(ws), n)

@@ -9,36 +9,39 @@ import torch
 from . import _lib
 
 Parameters = Union[torch.Tensor, Iterable[torch.Tensor]]
+_grad_of, _is_contiguous = torch._C.TensorBase.grad.__get__, torch._C.TensorBase.is_contiguous
 
 
 def _grads(parameters: Parameters) -> List[torch.Tensor]:
     if isinstance(parameters, torch.Tensor):
         parameters = (parameters,)
-    return [g for g in [p.grad for p in parameters] if g is not None]
+    return [g for g in map(_grad_of, parameters) if g is not None]
 
 
-def _dense(g: torch.Tensor) -> bool:
-    """Whether g's elements fill a range of memory; ValueError where some share one."""
-    span = 1
+def _dense(g: torch.Tensor, written: bool) -> bool:
+    """Whether g's elements fill a range of memory; ValueError where some share one and are to be
+    written."""
+    span, apart = 1, True
     for stride, size in sorted((st, sz) for sz, st in zip(g.shape, g.stride()) if sz != 1):
-        if stride < span:
-            raise ValueError(f"a gradient of shape {tuple(g.shape)} and strides {g.stride()} overlaps itself")
+        apart = apart and stride >= span
         span += stride * (size - 1)
-    return span == g.numel()
+    if written and not apart:
+        raise ValueError(f"a gradient of shape {tuple(g.shape)} and strides {g.stride()} overlaps itself")
+    return apart and span == g.numel()
 
 
-def _flat(grads: List[torch.Tensor]) -> Tuple[List[torch.Tensor], list]:
+def _flat(grads: List[torch.Tensor], written: bool) -> Tuple[List[torch.Tensor], list]:
     """The gradients as ranges of memory, copies in place of those that are none, and
     (gradient, copy) of these."""
-    if all([g.is_contiguous() for g in grads]):
+    if all(map(_is_contiguous, grads)):
         return grads, []
     copies = []
     for i, g in enumerate(grads):
         if g.layout is not torch.strided:
             raise ValueError(f"a gradient of layout {g.layout}: dense ones are needed")
-        if not g.is_contiguous() and g.numel() and not _dense(g):
-            grads[i] = g.contiguous()
-            copies.append((g, grads[i]))
+        if not g.is_contiguous() and g.numel() and not _dense(g, written):
+            grads[i] = g.detach().contiguous()
+            copies.append((g.detach(), grads[i]))
     return grads, copies
 
 
@@ -46,7 +49,6 @@ def _norm_of(grads: List[torch.Tensor]) -> torch.Tensor:
     return torch.empty((), device=grads[0].device, dtype=torch.float32)
 
 
-@torch.no_grad()
 def grad_norm(parameters: Parameters) -> torch.Tensor:
     """The 2-norm over all gradients of the parameters (those without one are passed over) as
     one vector: an fp32 scalar on their device, its squares summed in 64 bits in a fixed order.
@@ -54,13 +56,12 @@ def grad_norm(parameters: Parameters) -> torch.Tensor:
     grads = _grads(parameters)
     if not grads:
         return torch.zeros(())
-    grads, _ = _flat(grads)
+    grads, _ = _flat(grads, False)
     norm = _norm_of(grads)
     _lib.grad_norm(grads, norm)
     return norm
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters: Parameters, max_norm: float) -> torch.Tensor:
     """grad_norm, and every gradient times min(1, max_norm / (norm + 1e-6)) in place, in fp32,
     rounded once.  Returns the norm before clipping; the device is not waited for.
@@ -75,7 +76,7 @@ def clip_grad_norm_(parameters: Parameters, max_norm: float) -> torch.Tensor:
     if not grads:
         return torch.zeros(())
     written = list(grads)
-    grads, copies = _flat(grads)
+    grads, copies = _flat(grads, True)
     norm = _norm_of(grads)
     _lib.grad_norm(grads, norm, max_norm)
     for g, copy in copies:
@@ -84,7 +85,6 @@ def clip_grad_norm_(parameters: Parameters, max_norm: float) -> torch.Tensor:
     return norm
 
 
-@torch.no_grad()
 def clip_grads_with_norm_(parameters: Parameters, max_norm: float, norm: torch.Tensor) -> None:
     """clip_grad_norm_ by a given norm (fp32 scalar on the gradients' device), as where it is
     taken over several processes' gradients: the root of the sum of their grad_norm squared."""
@@ -95,7 +95,7 @@ def clip_grads_with_norm_(parameters: Parameters, max_norm: float, norm: torch.T
     if not grads:
         return
     written = list(grads)
-    grads, copies = _flat(grads)
+    grads, copies = _flat(grads, True)
     _lib.grad_norm(grads, norm, max_norm, given=True)
     for g, copy in copies:
         g.copy_(copy)

@@ -74,21 +74,22 @@ def test_logprobs_backward_refuses_before_device_work():
 def test_clipping_refuses_before_device_work():
     L = _lib.load()
 
-    def call(data=(AT[0], AT[1]), sizes=(100, 50), dts=(BF, F32), norm=AT[4], ws=AT[5], n=1 << 20, max_norm=1.0, given=0):
+    def call(data=(AT[0], AT[1]), sizes=(100, 50), dts=(BF, F32), norm=AT[4], ws=AT[5], n=1 << 20, max_norm=1.0, given=0, both=True):
         a = [array.array(t, v) for t, v in (("Q", data), ("q", sizes), ("i", dts))]
         p = [x.buffer_info()[0] for x in a]
-        rc = L.prime_grad_clip(*p, len(data), max_norm, norm, given, ws, n, None)
-        if max_norm == 1.0 and not given:
-            assert L.prime_grad_norm(*p, len(data), norm, ws, n, None) == rc
-        return rc
+        if both:
+            assert L.prime_grad_norm(*p, len(data), norm, ws, n, None) == L.prime_grad_clip(*p, len(data), max_norm, norm, given, ws, n, None)
+        return L.prime_grad_clip(*p, len(data), max_norm, norm, given, ws, n, None)
     assert call(norm=None) == -1 and call(ws=None) == -1 and call(n=7) == -1 and "workspace" in _lib.last_error()
     assert call(sizes=(100, -1)) == -1 and call(data=(AT[0], 0)) == -1 and call(sizes=(1 << 35, 1)) == -1
     assert call(sizes=((1 << 35) - 8, (1 << 35) - 8)) == -1
     assert call(dts=(BF, 7)) == -3
     assert call(data=(AT[0] + 1, AT[1])) == -4 and call(data=(AT[0], AT[1] + 2)) == -4 and call(norm=AT[4] + 2) == -4
-    assert call(data=(AT[0], AT[0] + 196)) == -5 and call(data=(AT[1] + 4, AT[1])) == -5 and "overlap" in _lib.last_error()
-    assert call(data=(AT[0], AT[0])) == -5 and call(norm=AT[0] + 8) == -5 and call(ws=AT[1]) == -5
-    assert call(max_norm=-1.0) == -1 and call(max_norm=math.nan) == -1
+    assert call(norm=AT[0] + 8) == -5 and call(ws=AT[1]) == -5 and call(norm=AT[5] + 4) == -5
+    # tensors that overlap each other have a norm, but are not clipped
+    assert call(data=(AT[0], AT[0] + 196), both=False) == -5 and "overlap" in _lib.last_error()
+    assert call(data=(AT[1] + 4, AT[1]), both=False) == -5 and call(data=(AT[0], AT[0]), both=False) == -5
+    assert call(max_norm=-1.0, both=False) == -1 and call(max_norm=math.nan, both=False) == -1
     assert L.prime_grad_norm_workspace_size(None, 3) == 0
 
 

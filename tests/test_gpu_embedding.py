@@ -48,7 +48,8 @@ def check(ids, weight, dy, scale=1.0, padding=None):
     (2331, 32000, 501, "ranked"), (5000, 262143, 5, "uniform"), (5000, 262144, 5, "uniform"), (3000, 300000, 8, "outside"),
     (70000, 50304, 64, "ranked"), (600000, 2000, 16, "ranked"), (131072, 128, 8, "uniform"), (131073, 129, 8, "uniform"),
     (140000, 3, 24, "outside"), (150000, 262145, 5, "outside"), (30000, 70000, 520, "ranked"), (17000, 65537, 1030, "ranked"),
-    (16384, 20, 700, "outside"), (16383, 20, 700, "outside")])
+    (16384, 20, 700, "outside"), (16383, 20, 700, "outside"), (9000, 100000, 16, "same"), (9000, 100000, 16, "ranked"),
+    (16000, 100000, 20, "uniform"), (2200000, 70000, 3, "ranked")])
 def test_lookup_and_gradient(dtype, n, V, C, kind):
     g = gen(n * 7 + V)
     ids = make_ids(kind, (n,), V, g)
@@ -221,6 +222,20 @@ def test_tables_and_gradients_beyond_32_bits():
     want, bound = R.lookup_grad(torch.tensor([0, 0, 1]), w.detach()[[1, V - 2, V - 1]], 2)
     R.assert_within(grad[[3, 15]], want, bound(torch.bfloat16))
     assert grad.abs().amax(1).count_nonzero() == 2
+
+
+@pytest.mark.parametrize("n", [5000, 50000])
+def test_a_table_of_very_many_rows(n):
+    """More rows than two digits tell apart; whole numbers, so that the sums are exact."""
+    V = (1 << 25) + 1001
+    g = gen(n)
+    w = torch.zeros(V, 1, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    ids = torch.cat([torch.randint(0, V, (n // 2,), generator=g, device="cuda"), torch.full((n - n // 2,), V - 1, device="cuda")])
+    ids = ids[torch.randperm(n, generator=g, device="cuda")]
+    dy = torch.randint(-2, 3, (n, 1), generator=g, device="cuda").bfloat16()
+    grad, = torch.autograd.grad(embedding_lookup(ids, w), w, dy)
+    want = torch.zeros(V, 1, device="cuda").index_add_(0, ids, dy.float())
+    assert torch.equal(grad, want.bfloat16())
 
 
 def test_entry_point_leaves_what_is_not_its_own():

@@ -142,10 +142,14 @@ def test_refusals_on_the_device():
     p = params([a, a])
     with pytest.raises(RuntimeError, match="overlap"):
         clip_grad_norm_(p, 1.0)
+    twice = math.sqrt(2) * float(a.double().norm())  # which has a norm all the same
+    assert abs(float(grad_norm(p)) - twice) <= 2 * R.U32 * twice
     p = params([a[:1].expand(4, 1)])
     p[0].grad = a[:1].expand(4)[:, None]
     with pytest.raises(ValueError, match="overlaps itself"):
         clip_grad_norm_(p, 1.0)
+    twice = 2 * abs(float(a[0]))
+    assert abs(float(grad_norm(p)) - twice) <= 2 * R.U32 * twice
     with pytest.raises(RuntimeError, match="dtype"):
         clip_grad_norm_(params([a.double()]), 1.0)
     with pytest.raises(ValueError, match="fp32"):
