@@ -29,9 +29,9 @@ constexpr int kGroupRanked = 256;      // .. that are ranked by comparing each w
 constexpr int kGroupTokens = 1 << 14;
 constexpr int kSortItems = 4096;       // at least, of a workgroup
 constexpr int kSortBlocks = 512;       // at most
-constexpr int kFewRows = 16384;        // tokens, below which chunks are short
-constexpr int kZeroRows = 64;
+constexpr int kChunk = 32;             // pairs
 constexpr int kRows = 8;               // of a chunk, on their way at once, twice
+constexpr int kZeroRows = 64;          // of the table, that a workgroup writes where their ids do not occur
 
 // A launch's share of the lookup: rows [first, first + rows) by the workgroups from `block` on,
 // `vecs` vectors of 16 bytes each.
@@ -435,11 +435,11 @@ struct LongIds {
     uint4 *list;      // [sections][kThreads]
 };
 
-template <int K>
 __device__ __forceinline__ void list_long(const EmbeddingArgs &a, const uint2 *pairs, const LongIds &longs, uint32_t chunks) {
     __shared__ uint32_t listed;
     if (threadIdx.x == 0) listed = 0;
     __syncthreads();
+    constexpr int K = kChunk;
     const uint32_t n = static_cast<uint32_t>(a.n), chunk = blockIdx.x * kThreads + threadIdx.x;
     const uint64_t begin = static_cast<uint64_t>(chunk) * K;
     if (begin + 2 * K <= n) {
@@ -457,24 +457,24 @@ __device__ __forceinline__ void list_long(const EmbeddingArgs &a, const uint2 *p
     if (threadIdx.x == 0) longs.count[blockIdx.x] = listed;
 }
 
-// A wave: 64 vectors of columns of the K rows of a chunk.  Lane l knows the pair l behind the
-// chunk's begin, K of this chunk and K of the next, so that all decisions are the wave's.  An id
+// A wave: 64 vectors of columns of the rows of a chunk.  Lane l knows the pair l behind the
+// chunk's begin, those of this chunk and of the next, so that all decisions are the wave's.  An id
 // is finished by the chunk in which it begins if it ends before the next one does; else it is
 // long, and each chunk leaves its part of it.  part: [chunks][2][vecs VE], of the long id that
 // reaches in from the chunk before (0) and of the one that begins here (1).  The first list_blocks
 // workgroups list the long ids, those from sum_blocks on write zeros for kZeroRows rows each,
-// where their ids do not occur.
-template <int DT, bool SHORT, int K>
+// where their ids do not occur.  ONCE: dy is read past the caches.
+template <int DT, bool SHORT, bool ONCE>
 __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const EmbeddingArgs a, const uint2 *pairs,
                                                                  const uint8_t *occurs, const LongIds longs, float *part,
                                                                  int vecs, uint32_t chunks, uint32_t list_blocks,
                                                                  uint32_t sum_blocks) {
-    constexpr int VE = kVec<DT>, es = Columns<DT, SHORT>::es, U = kRows;
-    static_assert(2 * K <= kWave && K % U == 0, "");
+    constexpr int VE = kVec<DT>, es = Columns<DT, SHORT>::es, U = kRows, K = kChunk;
+    static_assert(2 * K == kWave && K % U == 0, "");
     const uint32_t V = static_cast<uint32_t>(a.V), n = static_cast<uint32_t>(a.n);
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if (blockIdx.x < list_blocks) {
-        list_long<K>(a, pairs, longs, chunks);
+        list_long(a, pairs, longs, chunks);
         return;
     }
     if (blockIdx.x >= sum_blocks) {
@@ -501,8 +501,8 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const Embedding
     // where ids begin
     uint32_t before = __shfl_up(pair.x, 1, kWave);
     if (lane == 0) before = prior;
-    constexpr uint64_t kHere = (1ull << K) - 1, kWindow = K == 32 ? ~0ull : (1ull << (2 * K)) - 1;
-    const uint64_t starts = __ballot(pair.x != before) & kWindow, own = starts & kHere;
+    constexpr uint64_t kHere = (1ull << K) - 1;
+    const uint64_t starts = __ballot(pair.x != before), own = starts & kHere;
     // the id that reaches in: long if it fills this chunk or the one before
     const bool reaches_in = !(starts & 1), lead = reaches_in && (own == 0 || older == first);
     int from = 0, to = K;
@@ -531,6 +531,7 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const Embedding
             const uint32_t row = __builtin_amdgcn_readlane(pair.y, q);
             const char *p = dy + row * pitch;
             if constexpr (SHORT) w[u] = at.load(p);
+            else if constexpr (ONCE) w[u] = __builtin_nontemporal_load(&reinterpret_cast<const Raw *>(p)->v);
             else w[u] = reinterpret_cast<const Raw *>(p)->v;
         }
     };
@@ -637,7 +638,6 @@ struct Plan {
     bool grouped;        // in one launch
     int passes, bits;    // of the sort, or of a group
     int blocks, items;   // of the sort
-    int chunk;           // pairs
     int64_t chunks;
     size_t occurs, other, hist, bytes;  // where they begin, and the end
 };
@@ -653,8 +653,7 @@ Plan plan(int64_t n, int64_t V) {
     const int64_t items = per < kSortItems ? kSortItems : (per + kSortThreads - 1) / kSortThreads * kSortThreads;
     p.items = static_cast<int>(items);
     p.blocks = p.grouped ? kGroups + 1 : static_cast<int>((n + items - 1) / items);
-    p.chunk = n >= 64 && n < kFewRows ? 8 : 32;  // (below 64 no id is long, and nothing to join)
-    p.chunks = (n + p.chunk - 1) / p.chunk;
+    p.chunks = (n + kChunk - 1) / kChunk;
     auto round = [](size_t b) { return (b + 255) / 256 * 256; };
     p.occurs = round(static_cast<size_t>(n) * 8);
     p.other = p.occurs + round(static_cast<size_t>(V + kGroups - 1) / kGroups * kGroups);
@@ -741,10 +740,11 @@ Parts parts(const Plan &p, int C) {
     return w;
 }
 
-template <int DT, int K>
-void sum_and_join(const EmbeddingArgs &a, const Plan &p, hipStream_t s) {
+template <int DT>
+void run_backward(const EmbeddingArgs &a, hipStream_t s) {
+    const Plan p = plan(a.n, a.V);
     const int vecs = (a.C + kVec<DT> - 1) / kVec<DT>, slabs = (vecs + kWave - 1) / kWave;
-    const bool joins = a.n >= 2 * K;  // (else no id is long)
+    const bool joins = a.n >= 2 * kChunk;  // (else no id is long)
     const Parts space = parts(p, a.C);
     const uint32_t chunks = static_cast<uint32_t>(p.chunks), waves = kThreads / kWave, sections = static_cast<uint32_t>(space.sections);
     const uint32_t list_blocks = joins ? sections : 0, sum_blocks = list_blocks + (chunks + waves - 1) / waves * slabs;
@@ -755,7 +755,9 @@ void sum_and_join(const EmbeddingArgs &a, const Plan &p, hipStream_t s) {
     char *w = static_cast<char *>(a.workspace);
     float *part = reinterpret_cast<float *>(w);
     const LongIds longs{reinterpret_cast<uint32_t *>(w + space.counts), reinterpret_cast<uint4 *>(w + space.lists)};
-    const auto kernel = a.C < kVec<DT> ? embedding_sum_kernel<DT, true, K> : embedding_sum_kernel<DT, false, K>;
+    // a dy that the caches do not hold: past them (100 MB: 37 us for 43; 4.7 MB that was read before: 22 for 15)
+    const bool once = a.n * a.C * (DT == PRIME_F32 ? 4 : 2) >= int64_t{1} << 26;
+    const auto kernel = a.C < kVec<DT> ? embedding_sum_kernel<DT, true, false> : once ? embedding_sum_kernel<DT, false, true> : embedding_sum_kernel<DT, false, false>;
     hipLaunchKernelGGL(kernel, dim3(sum_blocks + zero_blocks), dim3(kThreads), 0, s, a, pairs, occurs, longs, part, vecs, chunks,
                        list_blocks, sum_blocks);
     if (!joins) return;
@@ -764,13 +766,6 @@ void sum_and_join(const EmbeddingArgs &a, const Plan &p, hipStream_t s) {
     const uint32_t x = y < 6 ? 256 : y < 96 ? 1536 / y : 16;
     const auto join = cols == 64 ? embedding_join_kernel<DT, 16> : embedding_join_kernel<DT, 64>;
     hipLaunchKernelGGL(join, dim3(x, y), dim3(kThreads), 0, s, a, longs, part, vecs, sections);
-}
-
-template <int DT>
-void run_backward(const EmbeddingArgs &a, hipStream_t s) {
-    const Plan p = plan(a.n, a.V);
-    if (p.chunk == 8) sum_and_join<DT, 8>(a, p, s);
-    else sum_and_join<DT, 32>(a, p, s);
 }
 
 }  // namespace
