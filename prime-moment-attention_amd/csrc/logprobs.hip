@@ -174,30 +174,36 @@ struct Shared {
     static constexpr int kList = WAVES == 1 ? 512 : 1024;
     __attribute__((aligned(16))) float red[4 * WAVES];
     uint64_t list[kList];
+    float best[kWave];
     uint32_t count;
     static constexpr int kBatches = 8;
     float batch[kBatches][WAVES * kWave];  // each lane's largest of its first batches of vectors
 };
 
 // A value that at least `top` of the row's logits reach, and not many more: `best` is each
-// lane's largest.  The j-th largest lane of the wave in which that is smallest: with W waves and
-// j = top / W rounded up, W j lanes reach it.
+// lane's largest.  The `top`-th largest of the j largest lanes of every wave: with W waves and
+// j = top / W rounded up.
 template <int WAVES>
-__device__ __forceinline__ float threshold(const Group<WAVES> &g, float best, int top) {
+__device__ __forceinline__ float threshold(const Group<WAVES> &g, Shared<WAVES> &sh, float best, int top) {
     const int lane = threadIdx.x % kWave;
     float mine;
+    int count = 0;
 #pragma unroll 1
-    for (int j = 0; j < top; j += WAVES) {
+    for (; count < top; count += WAVES) {
         mine = wave_max(best);
         if (lane == __builtin_ctzll(__ballot(best == mine))) best = -kInf;
+        if (WAVES > 1 && lane == 0) sh.best[count + threadIdx.x / kWave] = mine;
     }
     if constexpr (WAVES == 1) return mine;
     g.sync();
-    if (lane == 0) g.red[threadIdx.x / kWave] = mine;
-    g.sync();
-    float least = g.red[0];
-    for (int w = 1; w < WAVES; ++w) least = fminf(least, g.red[w]);
-    return least;
+    const float x = lane < count ? sh.best[lane] : -kInf;
+    int rank = 0;
+#pragma unroll 4
+    for (int o = 0; o < count; ++o) {
+        const float y = sh.best[o];
+        rank += y > x || (y == x && o < lane);
+    }
+    return sh.best[__builtin_ctzll(__ballot(lane < count && rank == top - 1))];
 }
 
 // The `top` first tokens in the order of rank_key, equal ones by index: write(rank, token,
@@ -210,7 +216,7 @@ __device__ __forceinline__ void likeliest(const Group<WAVES> &g, Shared<WAVES> &
                                           float best, int full, const float (&tail)[U], W write) {
     constexpr int VE = kVec<DT>, kThreads = WAVES * kWave, kList = Shared<WAVES>::kList;
     const int tid = g.thread(), whole = vocab / VE;
-    const uint32_t bar = rank_key(threshold<WAVES>(g, best, top)), own = rank_key(best);
+    const uint32_t bar = rank_key(threshold<WAVES>(g, sh, best, top)), own = rank_key(best);
     auto gather = [&](uint32_t least) {  // how many have a key of at least `least`; the first kList are listed
         if (tid == 0) sh.count = 0;
         g.sync();
@@ -314,7 +320,6 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void logprobs_ker
         }
         return;
     }
-    const float at_token = inside ? load_elem(base, token, DT) : 0.f;
     float top = -kInf, m = kLowest, c = reference(kLowest), s = 0.f, t = 0.f;
     auto add = [&](auto count, const float *x) {
         constexpr int N = decltype(count)::value;
@@ -368,6 +373,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void logprobs_ker
         const float x = load_elem(base, j, DT);
         add(std::integral_constant<int, 1>{}, &x);
     }
+    const float at_token = inside ? load_elem(base, token, DT) : 0.f;
     // the wave's, then all waves'
     float all = wave_max(top), C = reference(fmaxf(all, kLowest)), by = c - C, f = __builtin_amdgcn_exp2f(by);
     if constexpr (ENTROPY) t = wave_sum(f * fmaf(by, s, t));
