@@ -1766,7 +1766,9 @@ struct GradTables {
     const int64_t *sizes;
     const int32_t *dtypes;
     int count, at = 0;
-    static constexpr uint64_t kMaxBlocks = 4096;  // workgroups
+    // Workgroups.  Sums and scaling of 124 M fp32: 2048 137 + 178 us, 4096 134 + 168, 8192 135 + 170; each
+    // adds all workgroups' sums, which is most of a scaling that scales nothing: 4.7 us, 12 with 8192.
+    static constexpr uint64_t kMaxBlocks = 4096;
     prime::GradTable t;
     int blocks = 0;
 

@@ -11,6 +11,12 @@
 //           the next chunk does is finished where it begins; a longer one leaves a part in
 //           each chunk.  Further workgroups write the zeros of the ids that do not occur
 //   join    the parts of the long ones, in a fixed order
+//
+// All three are bound by memory.  65536 tokens x 768 bf16 of a table of 50304, ids of a language's
+// frequencies (us on the device): the lookup alone 23-25 (100 MB written, the table's rows in
+// the caches: 4.1 TB/s of writes); with the order, four launches of 10-12, 44; the sums 36.8
+// (100 MB of dy read, 77 MB of gradient written: 4.8 TB/s, a copy's rate); the join 7.4.  2331 x
+// 501 fp32 of 10000: 8.7, 15 and 4.  One token's lookup takes 1.8.
 
 #include <type_traits>
 
@@ -23,14 +29,22 @@ namespace {
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
 constexpr int kMaxBits = 9, kMaxBins = 1 << kMaxBits;
+// (128 groups and the one behind them, each reading all ids, are half of the workgroups that fit.
+// A group of 2048 pairs, twice, and its counts are 66 KB of LDS)
 constexpr int kGroups = 128;           // by the ids' low bits
 constexpr int kGroupList = 2048;       // tokens of a group that are sorted in LDS
+// Ranked / sorted in two passes, us: 2331 tokens 7.6 / 9.7, 8000 10.2 / 10.9; 16000 of ranked ids 18.8 / 17.0.
 constexpr int kGroupRanked = 256;      // .. that are ranked by comparing each with each
+// One launch against two passes of two launches (us, with the lookup of 768 bf16): 16000 tokens of
+// ranked ids 18.7 / 30, of one id, which one workgroup then has, 40 / 34; 32000 tokens 25 / 35
+// and 74 / 40; 65536 of one id 136.
 constexpr int kGroupTokens = 1 << 14;
 constexpr int kSortItems = 4096;       // at least, of a workgroup
 constexpr int kSortBlocks = 512;       // at most
+// Two chunks are one pair a lane.  Chunks of 8 pairs at 12000 tokens: sums and join 20.9 us for 24
+// with ranked ids, 44 for 23 with one id.
 constexpr int kChunk = 32;             // pairs
-constexpr int kRows = 8;               // of a chunk, on their way at once, twice
+constexpr int kRows = 8;               // of a chunk, on their way at once, twice (4: 35.4 us for 36.5; 16: 46 for 43)
 constexpr int kZeroRows = 64;          // of the table, that a workgroup writes where their ids do not occur
 
 // A launch's share of the lookup: rows [first, first + rows) by the workgroups from `block` on,
@@ -233,6 +247,8 @@ __device__ __forceinline__ void sort_pass(uint32_t (*tally)[kMaxBins], uint32_t 
     __syncthreads();
 }
 
+// Bound by latency: three reads of the ids, which the caches hold, and a sort in LDS: 8.7 us at 2331
+// tokens, the lookup among them.
 // Workgroup g < kGroups: the tokens whose ids have the low bits g, in the order of the others.
 // Each reads all ids, so where its tokens go it knows by itself: behind those of lower groups.
 // Workgroup kGroups: the places behind all of them, for tokens without a gradient.  The
@@ -337,7 +353,9 @@ __global__ __launch_bounds__(kSortThreads) void embedding_group_kernel(const Emb
 // One counting pass over many tokens: their digits' counts, or (SCATTER) the pairs in the
 // digits' order.  FIRST: the pairs are the ids' and the tokens' own.  ONE: a workgroup has
 // kSortItems tokens, which its threads hold.  Workgroups from `share.block` on look up.  The
-// first launch clears `occurs`, the second sets it.
+// first launch clears `occurs`, the second sets it.  At 65536 tokens the 16 workgroups that sort
+// take 5-8 us of the 10-12 of a launch, which the lookup's share fills (all shares being equal;
+// 1 : 2 or 2 : 3 for counting and placing is within a microsecond of that).
 template <bool FIRST, bool SCATTER, bool ONE>
 __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(const EmbeddingArgs a, const uint2 *pairs,
                                                                       uint2 *pairs_out, uint8_t *occurs,
@@ -464,6 +482,7 @@ __device__ __forceinline__ void list_long(const EmbeddingArgs &a, const uint2 *p
 // reaches in from the chunk before (0) and of the one that begins here (1).  The first list_blocks
 // workgroups list the long ids, those from sum_blocks on write zeros for kZeroRows rows each,
 // where their ids do not occur.  ONCE: dy is read past the caches.
+// Reads are random rows of dy, each once, two batches of kRows rows of 1 KB on their way in a wave.
 template <int DT, bool SHORT, bool ONCE>
 __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const EmbeddingArgs a, const uint2 *pairs,
                                                                  const uint8_t *occurs, const LongIds longs, float *part,
@@ -574,8 +593,9 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const Embedding
 
 // The long ids' parts: of all sections' ids workgroup b has the b-th, (b + gridDim.x)-th ..; of an
 // id's parts the workgroup's r-th row of L lanes has the r-th, (r + rows)-th .., of four columns
-// a lane, then the rows' sums.  (One workgroup reads some 50 GB/s: narrow slabs bring more of
-// them to an id.)
+// a lane, then the rows' sums.  One workgroup reads some 50 GB/s, so narrow slabs bring more of
+// them to an id: 65536 tokens of one id x 768, 6 MB of parts, take 15 us.  The slabs of an id begin at
+// different places of x, so on different XCDs (all at the same: 37).
 template <int DT, int L>
 __global__ __launch_bounds__(kThreads) void embedding_join_kernel(const EmbeddingArgs a, const LongIds longs,
                                                                   const float *part, int vecs, uint32_t sections) {
@@ -590,7 +610,7 @@ __global__ __launch_bounds__(kThreads) void embedding_join_kernel(const Embeddin
         const uint32_t before = scan_before(own, wave_total);
         uint32_t total = 0;
         for (int w = 0; w < kWaves; ++w) total += wave_total[w];
-        for (uint32_t e = blockIdx.x; e < total; e += gridDim.x) {
+        for (uint32_t e = (blockIdx.x + blockIdx.y) % gridDim.x; e < total; e += gridDim.x) {
             if (before <= e && e < before + own) found = longs.list[section * kThreads + e - before];
             __syncthreads();
             const uint4 entry = found;
@@ -755,14 +775,18 @@ void run_backward(const EmbeddingArgs &a, hipStream_t s) {
     char *w = static_cast<char *>(a.workspace);
     float *part = reinterpret_cast<float *>(w);
     const LongIds longs{reinterpret_cast<uint32_t *>(w + space.counts), reinterpret_cast<uint4 *>(w + space.lists)};
-    // a dy that the caches do not hold: past them (100 MB: 37 us for 43; 4.7 MB that was read before: 22 for 15)
+    // a dy larger than the L2 caches (32 MB) together: past them.  (Past / through them, x 768 bf16, us:
+    // last touched long ago, 131072 tokens 55 / 75, 65536 36 / 40-43, 32768 27 / 22; just
+    // written, 59 / 51, 39.6 / 37, 22.5 / 21.)
     const bool once = a.n * a.C * (DT == PRIME_F32 ? 4 : 2) >= int64_t{1} << 26;
     const auto kernel = a.C < kVec<DT> ? embedding_sum_kernel<DT, true, false> : once ? embedding_sum_kernel<DT, false, true> : embedding_sum_kernel<DT, false, false>;
     hipLaunchKernelGGL(kernel, dim3(sum_blocks + zero_blocks), dim3(kThreads), 0, s, a, pairs, occurs, longs, part, vecs, chunks,
                        list_blocks, sum_blocks);
     if (!joins) return;
-    // some 1500 workgroups, each id a slab of its own
-    const uint32_t width = vecs * kVec<DT>, cols = width <= 1024 ? 64 : 256, y = (width + cols - 1) / cols;
+    // some 1500 workgroups, an id's columns over y of them: slabs of 64 columns, or of 256 for wide rows
+    // (64 / 256, us: 65536 tokens of one id x 1024 15 / 46, x 2048 19 / 54; 16384 x 4096 of ranked ids
+    // 6.7 / 5.2, of one 6.6 / 14.4; x 8192 11.5 / 6.7 and 19 / 16.6)
+    const uint32_t width = vecs * kVec<DT>, cols = width <= 4096 ? 64 : 256, y = (width + cols - 1) / cols;
     const uint32_t x = y < 6 ? 256 : y < 96 ? 1536 / y : 16;
     const auto join = cols == 64 ? embedding_join_kernel<DT, 16> : embedding_join_kernel<DT, 64>;
     hipLaunchKernelGGL(join, dim3(x, y), dim3(kThreads), 0, s, a, longs, part, vecs, sections);
