@@ -14,7 +14,7 @@
 // A forward reads a row once, the likeliest tokens' vectors again; a backward reads it and writes
 // its gradient.  8192 x 50304 bf16 (us on the device): 139 forward (824 MB, 5.9 TB/s, a read's
 // rate; 164 while the caches write back the last gradient), 167 with 5 alternatives and the
-// entropy, 255 backward (1.65 GB, 6.5 TB/s).  Few rows are bound by latency, a workgroup reading at
+// entropy, 250 backward behind it (1.65 GB, 6.6 TB/s).  Few rows are bound by latency, a workgroup reading at
 // what one compute unit does: 1 x 50304 5.7, with 5 alternatives 9; 256 x 50304 with both 13.5.
 
 #include <type_traits>
@@ -428,7 +428,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void logprobs_ker
 }
 
 // The gradient of part blockIdx.x of row blockIdx.y's logits.  (At 8192 x 50304 bf16 2, 4 and 8
-// vectors a thread take 279, 259 and 289 us.)
+// vectors a thread take 281, 275 and 310 us, one call after the other.)
 constexpr int kBackThreads = 256, kBackUnroll = 4;
 
 template <int DT>
@@ -450,20 +450,16 @@ __global__ __launch_bounds__(kBackThreads) void logprobs_backward_kernel(const L
     if (!none && !fine) k = careful<DT>(Group<kBackThreads / kWave>{red}, base, a.vocab);
     // p (a0 + a1 log2 p), and g at the token
     const float a0 = -(gl + h * H), a1 = -h * kLn2;
-    auto grad = [&](float x, int j) {
-        float r = 0.f;
-        if (fine) {
-            const float d = fmaxf(fmaf(x, kLog2e, -C) - L, kFloor);
-            r = __builtin_amdgcn_exp2f(d) * fmaf(a1, d, a0);
-        } else if (k.nan) {
-            return __builtin_nanf("");
-        } else if (k.top == -kInf) {
-            return 0.f;
-        } else {
-            const float d = k.diff(x) - k.log_sum;
-            r = __expf(d) * (a0 - h * fmaxf(d, kFloor));
-        }
-        return j == token ? gl + r : r;
+    const int at = token >= 0 && token < a.vocab && (fine || k.top != -kInf) ? static_cast<int>(token) : -1;
+    auto grad = [&](float x) {
+        const float d = fmaxf(fmaf(x, kLog2e, -C) - L, kFloor);
+        return __builtin_amdgcn_exp2f(d) * fmaf(a1, d, a0);
+    };
+    auto careful_grad = [&](float x) {
+        if (k.nan) return __builtin_nanf("");
+        if (k.top == -kInf) return 0.f;
+        const float d = k.diff(x) - k.log_sum;
+        return __expf(d) * (a0 - h * fmaxf(d, kFloor));
     };
     u32x4 v[U];
     if (!none) {
@@ -481,14 +477,27 @@ __global__ __launch_bounds__(kBackThreads) void logprobs_backward_kernel(const L
             if (none) {
 #pragma unroll
                 for (int j = 0; j < VE; ++j) x[j] = 0.f;
-            } else {
-                widen<DT>(v[u], x);
+            } else if (widen<DT>(v[u], x); fine) {
 #pragma unroll
-                for (int j = 0; j < VE; ++j) x[j] = grad(x[j], e + j);
+                for (int j = 0; j < VE; ++j) x[j] = grad(x[j]);
+            } else {
+#pragma unroll 1
+                for (int j = 0; j < VE; ++j) x[j] = careful_grad(x[j]);
+            }
+            if (!none && at >= e && at < e + VE) {
+#pragma unroll
+                for (int j = 0; j < VE; ++j) x[j] = e + j == at ? gl + x[j] : x[j];
             }
             reinterpret_cast<Raw *>(out + static_cast<int64_t>(e) * es)->v = narrow<DT>(x);
         } else {
-            for (int j = e; j < a.vocab; ++j) store_elem(out, j, DT, none ? 0.f : grad(load_elem(base, j, DT), j));
+            for (int j = e; j < a.vocab; ++j) {
+                float x = 0.f;
+                if (!none) {
+                    x = load_elem(base, j, DT);
+                    x = (fine ? grad(x) : careful_grad(x)) + (j == at ? gl : 0.f);
+                }
+                store_elem(out, j, DT, x);
+            }
         }
     }
 }
