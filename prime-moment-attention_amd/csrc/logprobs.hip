@@ -14,8 +14,11 @@
 // A forward reads a row once, the likeliest tokens' vectors again; a backward reads it and writes
 // its gradient.  8192 x 50304 bf16 (us on the device): 139 forward (824 MB, 5.9 TB/s, a read's
 // rate; 164 while the caches write back the last gradient), 167 with 5 alternatives and the
-// entropy, 250 backward behind it (1.65 GB, 6.6 TB/s).  Few rows are bound by latency, a workgroup reading at
-// what one compute unit does: 1 x 50304 5.7, with 5 alternatives 9; 256 x 50304 with both 13.5.
+// entropy, 250 backward behind it (1.65 GB, 6.6 TB/s).  A row has one compute unit, whose vector unit
+// bounds few rows (2.6 us of exponentials and sums for 50304 logits, 11000 cycles of a
+// workgroup's first 22000 with what it waits for), and each meeting of its waves costs
+// some 0.3 us: 1 x 50304 5.8, with 5 alternatives 8.8, with 20 10.5; 256 x 50304 with 5 and the
+// entropy 13.
 
 #include <type_traits>
 
@@ -187,21 +190,20 @@ struct Shared {
 };
 
 // A value that at least `top` of the row's logits reach, and not many more: `best` is each
-// lane's largest.  The `top`-th largest of the j largest lanes of every wave: with W waves and
-// j = top / W rounded up.
+// lane's largest, `mine` the wave's, which is in sh.best.  The `top`-th largest of the j largest
+// lanes of every wave: with W waves and j = top / W rounded up.
 template <int WAVES>
-__device__ __forceinline__ float threshold(const Group<WAVES> &g, Shared<WAVES> &sh, float best, int top) {
+__device__ __forceinline__ float threshold(const Group<WAVES> &g, Shared<WAVES> &sh, float best, float mine, int top) {
     const int lane = threadIdx.x % kWave;
-    float mine;
-    int count = 0;
+    int count = WAVES;
 #pragma unroll 1
     for (; count < top; count += WAVES) {
-        mine = wave_max(best);
         if (lane == __builtin_ctzll(__ballot(best == mine))) best = -kInf;
+        mine = wave_max(best);
         if (WAVES > 1 && lane == 0) sh.best[count + threadIdx.x / kWave] = mine;
     }
     if constexpr (WAVES == 1) return mine;
-    g.sync();
+    if (count > WAVES) g.sync();
     const float x = lane < count ? sh.best[lane] : -kInf;
     int rank = 0;
 #pragma unroll 4
@@ -217,15 +219,15 @@ __device__ __forceinline__ float threshold(const Group<WAVES> &g, Shared<WAVES> 
 // too many, those above it, and the first ones equal to it by index (a row with few tokens that
 // are not -infinity, or with equal logits); if these are too many, one after the other.
 // A lane whose largest is below the threshold reads nothing again, another one only the batches
-// and vectors whose largest is not.  (The last vectors kept in registers instead: 15.8 us for 9.1
-// at 1 x 50304 with 5, 208 for 168 at 8192 rows.)
-// best: the lane's largest; tail: those of its vectors from `full` on.
+// and vectors whose largest is not.  (The last vectors kept in registers instead: 11.1 us for 8.8
+// at 1 x 50304 with 5, 201 for 165 at 8192 rows with the entropy.)
+// best, mine: the lane's and the wave's largest; tail: those of its vectors from `full` on.
 template <int DT, int WAVES, int U, typename W>
 __device__ __forceinline__ void likeliest(const Group<WAVES> &g, Shared<WAVES> &sh, const char *row, int vocab, int top,
-                                          float best, int full, const float (&tail)[U], W write) {
+                                          float best, float mine, int full, const float (&tail)[U], W write) {
     constexpr int VE = kVec<DT>, kThreads = WAVES * kWave, kList = Shared<WAVES>::kList;
     const int tid = g.thread(), whole = vocab / VE;
-    const uint32_t bar = rank_key(threshold<WAVES>(g, sh, best, top)), own = rank_key(best);
+    const uint32_t bar = rank_key(threshold<WAVES>(g, sh, best, mine, top)), own = rank_key(best);
     auto gather = [&](uint32_t least) {  // how many have a key of at least `least`; the first kList are listed
         if (tid == 0) sh.count = 0;
         g.sync();
@@ -386,13 +388,15 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void logprobs_ker
     }
     const float at_token = inside ? load_elem(base, token, DT) : 0.f;
     // the wave's, then all waves'
-    float all = wave_max(top), C = reference(fmaxf(all, kLowest)), by = c - C, f = __builtin_amdgcn_exp2f(by);
+    const float mine = wave_max(top);
+    float all = mine, C = reference(fmaxf(all, kLowest)), by = c - C, f = __builtin_amdgcn_exp2f(by);
     if constexpr (ENTROPY) t = wave_sum(f * fmaf(by, s, t));
     s = wave_sum(s * f);
     if constexpr (WAVES > 1) {
         if (threadIdx.x % kWave == 0) {
             float *r = sh.red + threadIdx.x / kWave * 4;
             r[0] = all, r[1] = s, r[2] = t;
+            sh.best[threadIdx.x / kWave] = mine;
         }
         g.sync();
         for (int w = 0; w < WAVES; ++w) all = fmaxf(all, sh.red[4 * w]);
@@ -420,7 +424,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void logprobs_ker
         if (a.stats) a.stats[2 * row] = fine ? C : __builtin_nanf(""), a.stats[2 * row + 1] = L;
     }
     if (a.top)
-        likeliest<DT, WAVES>(g, sh, base, a.vocab, a.top, top, full, tail, [&](int rank, int id, float x) {
+        likeliest<DT, WAVES>(g, sh, base, a.vocab, a.top, top, mine, full, tail, [&](int rank, int id, float x) {
             const int64_t at = static_cast<int64_t>(row) * a.top + rank;
             a.top_tokens[at] = id;
             a.top_logprobs[at] = logprob(x);
