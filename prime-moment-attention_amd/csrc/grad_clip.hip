@@ -10,8 +10,8 @@
 // Bound by memory, but for small models, where two launches are (us on the device, sums and
 // scaling): 124 M elements fp32 133 + 168, 4.9 TB/s, a copy's rate; bf16 69 + 76; the sums alone
 // 84 and 45 (5.9 and 5.5 TB/s), where no scaling's writes are still on their way out of the
-// caches.  28 small fp32 tensors 4.1 + 5.1; 37 tensors of 34 MB whose norm clips nothing
-// 15 + 4.9.  (Sums in fp32 are no faster; nor is scaling from the end, what the sums read last.)
+// caches.  28 small fp32 tensors 4.1 + 5.1; 80 tensors, 34 M elements, mostly
+// bf16, whose norm clips nothing 15 + 4.9.  (Sums in fp32 are no faster; nor is scaling from the end, what the sums read last.)
 
 #include "prime_kernels.h"
 
