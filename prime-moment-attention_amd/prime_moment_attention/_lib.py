@@ -1335,27 +1335,43 @@ def embedding(ids, weight, scale: float, out, padding: int = -1, order=None, che
             out.data_ptr(), *((None, 0) if order is None else (order.data_ptr(), order.numel())))
 
 
-def embedding_backward(order, dy, scale: float, dweight, checked: bool = False) -> None:
+def embedding_backward(order, dy, scale: float, dweight) -> None:
     """prime_embedding_backward: the order that embedding made of the n tokens and dweight's
     V, dy [n, C] with contiguous columns (or contiguous, of any shape), dweight [V, C]
-    contiguous.  checked: the caller knows the operands to be so."""
+    contiguous."""
     V, C = dweight.shape
     if dy.dim() == 2:
         n, pitch = dy.shape[0], dy.stride(0)
     else:
         n, pitch = dy.numel() // C, C
-    if not checked:
-        _check_rows(dy if dy.dim() == 2 else dy.view(-1, C), C, "dy")
-        if dweight.dtype is not dy.dtype or not dweight.is_contiguous():
-            raise ValueError("dweight must be contiguous and of dy's dtype")
-        if order.dtype is not torch.uint8 or not order.is_contiguous():
-            raise ValueError("order must be a buffer of embedding_order")
-        _same_device(dy, order, dweight)
+    _check_rows(dy if dy.dim() == 2 else dy.view(-1, C), C, "dy")
+    if dweight.dtype is not dy.dtype or not dweight.is_contiguous():
+        raise ValueError("dweight must be contiguous and of dy's dtype")
+    if order.dtype is not torch.uint8 or not order.is_contiguous():
+        raise ValueError("order must be a buffer of embedding_order")
+    _same_device(dy, order, dweight)
+    embedding_gradient(order, n, V, C, dy.dtype, scale)(dy, pitch if n > 1 else C, dweight)
+
+
+def embedding_gradient(order, n: int, V: int, C: int, dtype, scale: float):
+    """embedding_backward of operands that are known to be so, as f(dy, pitch, dweight): all that
+    does not depend on dy is looked up here.  (Each step takes autograd's thread about three
+    times as long as the thread of the forward: a small training call 81 us for 85, of log
+    probabilities 88 for 93.)"""
     L = load()
-    size = L.prime_embedding_backward_workspace_size(n, C)
-    ws = torch.empty(size, dtype=torch.uint8, device=dy.device)
-    _launch(L.prime_embedding_backward, "prime_embedding_backward", dy.device, order.data_ptr(), order.numel(), n,
-            dy.data_ptr(), pitch if n > 1 else C, V, C, _DTYPES[dy.dtype], scale, dweight.data_ptr(), ws.data_ptr(), size)
+    fn, size = L.prime_embedding_backward, L.prime_embedding_backward_workspace_size(n, C)
+    dev, dt = order.device, _DTYPES[dtype]
+    index, at, held = dev.index, order.data_ptr(), order.numel()
+
+    def run(dy, pitch: int, dweight) -> None:
+        ws = order.new_empty(size)
+        args = (at, held, n, dy.data_ptr(), pitch, V, C, dt, scale, dweight.data_ptr(), ws.data_ptr(), size)
+        if index != torch._C._cuda_getDevice():
+            _launch(fn, "prime_embedding_backward", dev, *args)
+        elif rc := fn(*args, torch._C._cuda_getCurrentRawStream(index)):
+            _check(rc, "prime_embedding_backward")
+
+    return run
 
 
 def _check_logits(logits, tokens) -> Tuple[int, int]:
@@ -1395,28 +1411,44 @@ def token_logprobs(logits, tokens, ignore: int, logprobs, entropy, stats, top: i
             logprobs.data_ptr(), _ptr(entropy), _ptr(stats), top, _ptr(top_logprobs), _ptr(top_tokens))
 
 
-def token_logprobs_backward(logits, tokens, ignore: int, stats, entropy, dlogprobs, dentropy, dlogits,
-                            checked: bool = False) -> None:
+def token_logprobs_backward(logits, tokens, ignore: int, stats, entropy, dlogprobs, dentropy, dlogits) -> None:
     """prime_token_logprobs_backward: dlogits [n, vocab] of logits' dtype; dlogprobs and
-    dentropy fp32 [n] or None.  checked: the caller knows the operands to be so, and dlogits to
-    be contiguous."""
-    if not checked:
-        n, vocab = _check_logits(logits, tokens)
-        _f32_of(2 * n, stats)
-        _f32_of(n, entropy, dlogprobs, dentropy)
-        if dlogits.shape != logits.shape or dlogits.dtype is not logits.dtype or (dlogits.stride(1) != 1 and vocab > 1):
-            raise ValueError("dlogits must have logits' shape and dtype and a contiguous vocab dimension")
-        _same_device(logits, tokens, stats, entropy, dlogprobs, dentropy, dlogits)
-    n, vocab = logits.shape
-    _launch(load().prime_token_logprobs_backward, "prime_token_logprobs_backward", logits.device, logits.data_ptr(),
-            _DTYPES[logits.dtype], n, vocab, logits.stride(0) if n > 1 else vocab, tokens.data_ptr(), ignore,
-            stats.data_ptr(), _ptr(entropy), _ptr(dlogprobs), _ptr(dentropy), dlogits.data_ptr(),
-            vocab if checked else _row_stride(dlogits))
+    dentropy fp32 [n] or None."""
+    n, vocab = _check_logits(logits, tokens)
+    _f32_of(2 * n, stats)
+    _f32_of(n, entropy, dlogprobs, dentropy)
+    if dlogits.shape != logits.shape or dlogits.dtype is not logits.dtype or (dlogits.stride(1) != 1 and vocab > 1):
+        raise ValueError("dlogits must have logits' shape and dtype and a contiguous vocab dimension")
+    _same_device(logits, tokens, stats, entropy, dlogprobs, dentropy, dlogits)
+    token_logprobs_gradient(stats, n, vocab, logits.dtype, ignore)(logits, tokens, entropy, dlogprobs, dentropy, dlogits,
+                                                                   _row_stride(dlogits))
 
 
 _T = torch._C.TensorBase
 _dtype_of, _data_ptr, _numel, _get_device = _T.dtype.__get__, _T.data_ptr, _T.numel, _T.get_device
 GRAD_TABLE, GRAD_PARTS = 192, 4096 * 8  # tensors of a launch, and the workspace that they take at most
+
+
+def token_logprobs_gradient(stats, n: int, vocab: int, dtype, ignore: int):
+    """token_logprobs_backward of operands that are known to be so, as f(logits, tokens, entropy,
+    dlogprobs, dentropy, dlogits): all that does not depend on them is looked up here, as in
+    embedding_gradient.  logits: [n, vocab] with a contiguous vocabulary, or contiguous; dlogits'
+    rows `out_pitch` apart."""
+    fn, dt = load().prime_token_logprobs_backward, _DTYPES[dtype]
+    dev = stats.device
+    index = dev.index
+
+    def run(logits, tokens, entropy, dlogprobs, dentropy, dlogits, out_pitch: int = vocab) -> None:
+        pitch = logits.stride(0) if n > 1 and logits.dim() == 2 else vocab
+        args = (logits.data_ptr(), dt, n, vocab, pitch, tokens.data_ptr(), ignore, stats.data_ptr(),
+                None if entropy is None else entropy.data_ptr(), None if dlogprobs is None else dlogprobs.data_ptr(),
+                None if dentropy is None else dentropy.data_ptr(), dlogits.data_ptr(), out_pitch)
+        if index != torch._C._cuda_getDevice():
+            _launch(fn, "prime_token_logprobs_backward", dev, *args)
+        elif rc := fn(*args, torch._C._cuda_getCurrentRawStream(index)):
+            _check(rc, "prime_token_logprobs_backward")
+
+    return run
 
 
 def grad_norm(tensors, norm, max_norm: Optional[float] = None, given: bool = False) -> None:

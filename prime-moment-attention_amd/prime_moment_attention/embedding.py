@@ -29,11 +29,13 @@ class _EmbeddingFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, weight, ids, scale, padding):
-        table = weight.shape
+        V, C = ctx.table = weight.shape
         n = ids.numel()
-        ctx.order = _lib.embedding_order(n, table[0], weight.device) if n and weight.numel() else None
-        ctx.scale, ctx.table = scale, table
-        return _run(ids, weight, scale, padding, ctx.order)
+        order = ctx.gradient = None
+        if n and V and C:
+            order = _lib.embedding_order(n, V, weight.device)
+            ctx.gradient = _lib.embedding_gradient(order, n, V, C, weight.dtype, scale)
+        return _run(ids, weight, scale, padding, order)
 
     @staticmethod
     def backward(ctx, dy):
@@ -41,10 +43,13 @@ class _EmbeddingFn(torch.autograd.Function):
 
     @staticmethod
     def _grads(ctx, dy):
-        if ctx.order is None:
+        if ctx.gradient is None:
             return dy.new_zeros(ctx.table), None, None, None
-        dweight = dy.new_empty(ctx.table)
-        _lib.embedding_backward(ctx.order, dy if dy.is_contiguous() else _rows(dy), ctx.scale, dweight, checked=True)
+        dweight, pitch = dy.new_empty(ctx.table), ctx.table[1]
+        if not dy.is_contiguous():
+            dy = _rows(dy)
+            pitch = dy.stride(0) if dy.shape[0] > 1 else pitch
+        ctx.gradient(dy, pitch, dweight)
         return dweight, None, None, None
 
 

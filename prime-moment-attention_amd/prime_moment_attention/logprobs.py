@@ -42,9 +42,9 @@ def _run(logits, tokens, top, entropy, ignore, stats):
 class _TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top, entropy, ignore):
-        ctx.stats = torch.empty((*tokens.shape, 2), device=logits.device, dtype=torch.float32)
-        out = _run(logits, tokens, top, entropy, ignore, ctx.stats)
-        ctx.ignore = ignore
+        stats = torch.empty((*tokens.shape, 2), device=logits.device, dtype=torch.float32)
+        out = _run(logits, tokens, top, entropy, ignore, stats)
+        ctx.gradient = _lib.token_logprobs_gradient(stats, tokens.numel(), logits.shape[-1], logits.dtype, ignore)
         ctx.save_for_backward(logits, tokens, out[1])
         if top:
             ctx.mark_non_differentiable(out[2], out[3])
@@ -64,10 +64,9 @@ class _TokenLogprobsFn(torch.autograd.Function):
             dlogprobs = dlogprobs.contiguous()
         if dentropy is not None and not dentropy.is_contiguous():
             dentropy = dentropy.contiguous()
-        dlogits = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-        if tokens.numel():
-            _lib.token_logprobs_backward(_rows(logits), tokens, ctx.ignore, ctx.stats, entropy, dlogprobs, dentropy,
-                                         dlogits, checked=True)
+        dlogits = logits.new_empty(logits.shape)
+        if dlogits.numel():
+            ctx.gradient(logits if logits.is_contiguous() else _rows(logits), tokens, entropy, dlogprobs, dentropy, dlogits)
         return dlogits, None, None, None, None
 
 
