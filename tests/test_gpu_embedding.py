@@ -162,6 +162,19 @@ def test_retained_graph_and_one_gradient_only():
     assert (grad[[1, 2]] == 1).all() and grad.sum() == 8
 
 
+def test_order_outlives_the_forward():
+    w = torch.randn(500, 33, device="cuda", requires_grad=True)
+    for n in (40, 3000, 20000):
+        ids, dy = torch.randint(0, 500, (n,), device="cuda"), torch.randn(n, 33, device="cuda")
+        want, = torch.autograd.grad(embedding_lookup(ids, w), w, dy)
+        y = embedding_lookup(ids, w)
+        size = _lib.load().prime_embedding_order_size(n, 500)
+        full = [torch.full((size,), 255, dtype=torch.uint8, device="cuda") for _ in range(8)]
+        del full
+        got, = torch.autograd.grad(y, w, dy)
+        assert torch.equal(got, want)
+
+
 def test_streams_side_by_side():
     g = gen(8)
     streams = [torch.cuda.Stream() for _ in range(3)]

@@ -1,5 +1,6 @@
 """Log probabilities of tokens, entropy, alternatives and gradients, against their plain forms
 in 64 bits."""
+import contextlib
 import math
 
 import pytest
@@ -270,6 +271,26 @@ def test_saved_and_once():
         x.add_(1.0)
     with pytest.raises(RuntimeError, match="modified"):
         r.logprobs.sum().backward()
+
+
+def test_saved_on_the_host_and_memory_used_in_between():
+    """What the backward needs outlives the forward: saved tensors that come back as others (in
+    rows without the view's gaps), and everything free in memory written over."""
+    buf, t = torch.randn(37, 1010, device="cuda"), torch.randint(0, 1003, (37,), device="cuda")
+    g = torch.randn(37, device="cuda")
+
+    def grad(hooks, dirty):
+        x = buf[:, 4:1007].detach().requires_grad_()
+        with hooks:
+            r = token_logprobs(x, t, entropy=True)
+        if dirty:
+            full = [torch.full((size,), NAN, device="cuda") for size in (37, 74, 37 * 1003) for _ in range(8)]
+            del full
+        return torch.autograd.grad([r.logprobs, r.entropy], x, [g, g])[0]
+
+    want = grad(contextlib.nullcontext(), False)
+    assert torch.equal(grad(contextlib.nullcontext(), True), want)
+    assert torch.equal(grad(torch.autograd.graph.save_on_cpu(), True), want)
 
 
 def test_streams_side_by_side():
