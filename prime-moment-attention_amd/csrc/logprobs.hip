@@ -420,6 +420,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void logprobs_ker
     };
     if (tid == 0) {
         a.logprobs[row] = !known ? 0.f : inside ? logprob(at_token) : __builtin_nanf("");
+        // (where one token has all the probability this may round to -3e-8; the gradient cancels that
+        // against the same in log p, so that it is left as it is)
         if constexpr (ENTROPY) a.entropy[row] = fine ? (L - t / s) * kLn2 : k.entropy();
         if (a.stats) a.stats[2 * row] = fine ? C : __builtin_nanf(""), a.stats[2 * row + 1] = L;
     }
