@@ -17,8 +17,8 @@
 // entropy, 250 backward behind it (1.65 GB, 6.6 TB/s).  A row has one compute unit, whose vector unit
 // bounds few rows (2.6 us of exponentials and sums for 50304 logits, 11000 cycles of a
 // workgroup's first 22000 with what it waits for), and each meeting of its waves costs
-// some 0.3 us: 1 x 50304 5.8, with 5 alternatives 8.8, with 20 10.5; 256 x 50304 with 5 and the
-// entropy 13.
+// some 0.3 us: 1 x 50304 5.8, with 5 alternatives 8.4, with 20 10.4; 256 x 50304 with 5 and the
+// entropy 12.9.
 
 #include <type_traits>
 
@@ -229,8 +229,6 @@ __device__ __forceinline__ void likeliest(const Group<WAVES> &g, Shared<WAVES> &
     const int tid = g.thread(), whole = vocab / VE;
     const uint32_t bar = rank_key(threshold<WAVES>(g, sh, best, mine, top)), own = rank_key(best);
     auto gather = [&](uint32_t least) {  // how many have a key of at least `least`; the first kList are listed
-        if (tid == 0) sh.count = 0;
-        g.sync();
         auto take = [&](float x, int j) {
             const uint32_t k = rank_key(x);
             if (k < least) return;
@@ -270,6 +268,8 @@ __device__ __forceinline__ void likeliest(const Group<WAVES> &g, Shared<WAVES> &
     uint32_t count = gather(bar);
     int equal = 0;  // of the tokens at the threshold, how many are still wanted
     if (count > kList) {
+        g.sync();
+        if (tid == 0) sh.count = 0;
         g.sync();
         count = gather(bar + 1);
         equal = count < static_cast<uint32_t>(top) ? top - count : 0;
@@ -323,6 +323,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void logprobs_ker
     const int row = WAVES == 1 ? blockIdx.x * 4 + threadIdx.x / kWave : blockIdx.x;
     if (WAVES == 1 && row >= a.n) return;
     const int tid = g.thread();
+    if (a.top && tid == 0) sh.count = 0;  // (read behind the meeting below)
     const char *base = static_cast<const char *>(a.logits) + a.stride_n * es * row;
     const int64_t token = a.tokens[row];
     const bool known = token != a.ignore, inside = token >= 0 && token < a.vocab;
