@@ -1,0 +1,95 @@
+"""Log probabilities, entropy and gradients over the whole range of finite logits: masks of any
+size, largest logits of any size, and both in the places where a lane, a wave or a batch of
+vectors has nothing else."""
+import pytest
+import torch
+
+from prime_moment_attention import token_logprobs
+from test_gpu_logprobs import check, gen
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def magnitudes(dtype, g):
+    """Powers of two, whose product with log2(e) leaves no residual in fp32, masks in use, and
+    sizes at random from 2^20 to 2^127."""
+    out = [2.0 ** k for k in (*range(20, 121, 4), *range(121, 128))]
+    out += [8e6, 1e7, 1.2e7, 1e8, 1e9, 1660944384.0, 1888815488.0, 2.5e9, 1e10, 1e30, 1e38, 1.7e38, 3e38]
+    out += torch.exp2(20 + 107 * torch.rand(24, generator=g, device="cuda").double()).tolist()
+    out += torch.exp2(29 + 5 * torch.rand(24, generator=g, device="cuda").double()).tolist()
+    if dtype is F16:
+        out = [2.0 ** k for k in range(8, 16)] + [1e4, 65504.0]
+    return out
+
+
+def rows_with(a, base, lane, wave):
+    """Rows like `base` with a as a mask and as the largest logit; lane, wave: the places that one
+    lane and one wave read."""
+    V = base.numel()
+    first = torch.arange(V, device="cuda") < V // 2
+    keep = torch.zeros(V, dtype=torch.bool, device="cuda")
+    keep[-1] = True
+    masks = [first, ~first, lane, wave, ~keep]
+    rows = [torch.where(m, -a, base) for m in masks]
+    rows += [base.clone(), base.clone(), torch.full_like(base, -a), torch.full_like(base, a), base.clone()]
+    rows[5][V // 2] = a
+    rows[6][V // 3] = rows[6][V // 2] = a  # two share the probability
+    rows[9][:] = -a
+    rows[9][V // 2] = a
+    return rows
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("V, threads", [(100, 64), (2048, 64), (9001, 256), (20001, 1024), (70001, 1024)])
+def test_masks_and_largest_logits_of_any_size(dtype, V, threads):
+    g = gen(V)
+    base = (2 * torch.randn(V, generator=g, device="cuda")).to(dtype).float()
+    owner = torch.arange(V, device="cuda") // (4 if dtype is F32 else 8) % threads
+    lane, wave = owner == 3, owner // 64 == (1 if threads > 64 else 0)
+    if threads == 64:
+        wave = owner < 32
+    x = torch.cat([torch.stack(rows_with(a, base, lane, wave)) for a in magnitudes(dtype, g)]).to(dtype)
+    for part in x.split(300):
+        n = part.shape[0]
+        tokens = torch.randint(0, V, (n,), generator=g, device="cuda")
+        tokens[::2] = part[::2].float().argmax(1)
+        a, b = torch.randn(2, n, generator=g, device="cuda")
+        check(part, tokens, 2, True, a, b)
+        check(part, tokens, 0, True, None, b)
+
+
+def test_masks_in_many_rows():
+    """The form for many rows of a large vocabulary."""
+    g = gen(3)
+    n, V = 600, 17001
+    x = 2 * torch.randn(n, V, generator=g, device="cuda")
+    a = torch.exp2(20 + 107 * torch.rand(n, 1, generator=g, device="cuda"))
+    a[::3] = torch.exp2(29 + 5 * torch.rand(n // 3, 1, generator=g, device="cuda"))
+    x = torch.where(torch.arange(V, device="cuda") < V // 2, -a, x)
+    tokens = torch.randint(0, V, (n,), generator=g, device="cuda")
+    d = torch.randn(2, n, generator=g, device="cuda")
+    check(x, tokens, 3, True, d[0], d[1])
+
+
+@pytest.mark.parametrize("V", [100, 9001, 50304])
+def test_a_finite_mask_is_as_good_as_minus_infinity(V):
+    """Masked tokens have no probability, whatever the mask: the same bits as of -infinity."""
+    g = gen(V)
+    base = 3 * torch.randn(8, V, generator=g, device="cuda")
+    banned = torch.rand(8, V, generator=g, device="cuda") < 0.7
+    banned[:4, : V // 2] = True
+    banned[:, -1] = False
+    tokens = torch.full((8,), V - 1, device="cuda")
+    d = torch.randn(2, 8, generator=g, device="cuda")
+
+    def results(mask, dtype):
+        x = torch.where(banned, mask, base).to(dtype).requires_grad_()
+        r = token_logprobs(x, tokens, entropy=True)
+        return r.logprobs.detach(), r.entropy.detach(), torch.autograd.grad([r.logprobs, r.entropy], x, [d[0], d[1]])[0]
+
+    for dtype in (F32, BF16):
+        want = results(-float("inf"), dtype)
+        for mask in (-1e9, -1e10, -2.5e9, -1660944384.0, -1e30, -1e38, -2.0 ** 126, torch.finfo(dtype).min):
+            for a, b in zip(results(mask, dtype), want):
+                assert torch.equal(a, b), (dtype, mask)
