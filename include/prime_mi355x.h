@@ -647,9 +647,10 @@ int prime_embedding_backward(const void *order, size_t order_bytes, int64_t n, c
  *   tokens : int64 [n]
  *
  * prime_token_logprobs_backward: with g = dlogprobs (0 where the token is `ignore`) and
- * h = dentropy (fp32 [n], either may be NULL),
+ * h = dentropy (fp32 [n], either may be NULL, which takes its term away),
  *   dlogits_j = g (delta_j,token - p_j) - h p_j (log p_j + entropy)
- * in logits' dtype, rounded once; stats, and with h entropy, are the forward's.  dlogits:
+ * in logits' dtype, rounded once (NaN with dlogprobs for a token that has a NaN for its log
+ * probability); stats, and with h entropy, are the forward's.  dlogits:
  * rows stride_d >= vocab apart, apart from logits.
  */
 int prime_token_logprobs(const void *logits, int dtype, int n, int vocab, int64_t stride_n, const int64_t *tokens,

@@ -4,6 +4,7 @@ vectors has nothing else."""
 import pytest
 import torch
 
+import ends_ref as R
 from prime_moment_attention import token_logprobs
 from test_gpu_logprobs import check, gen
 
@@ -93,3 +94,16 @@ def test_a_finite_mask_is_as_good_as_minus_infinity(V):
         for mask in (-1e9, -1e10, -2.5e9, -1660944384.0, -1e30, -1e38, -2.0 ** 126, torch.finfo(dtype).min):
             for a, b in zip(results(mask, dtype), want):
                 assert torch.equal(a, b), (dtype, mask)
+
+def test_a_token_outside_the_vocabulary_has_an_entropy_all_the_same():
+    """Its log probability is NaN; of the entropy alone the gradient is that of any other row."""
+    for V in (70, 3000, 20000):
+        x = torch.randn(4, V, generator=gen(V), device="cuda")
+        tokens = torch.tensor([3, V, -1, -100], device="cuda")
+        h = torch.randn(4, device="cuda")
+        leaf = x.clone().requires_grad_()
+        r = token_logprobs(leaf, tokens, entropy=True)
+        dx, = torch.autograd.grad(r.entropy, leaf, h)
+        want = R.logprobs_grad(x, tokens, None, h)
+        assert want.isfinite().all()
+        R.assert_within(dx, want, R.grad_bound(x, tokens, None, h, want), "gradient")
