@@ -1304,7 +1304,22 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+# what the entry points take; a C int would hold the low 32 bits of more
+EMBEDDING_COLUMNS, LOGPROBS_ROWS, LOGPROBS_VOCAB = 1 << 20, (1 << 31) - 1, 1 << 24
+
+
+def check_columns(C: int) -> None:
+    if C > EMBEDDING_COLUMNS:
+        raise ValueError(f"{C} columns: at most {EMBEDDING_COLUMNS} are supported")
+
+
+def check_logits_size(n: int, vocab: int) -> None:
+    if n > LOGPROBS_ROWS or vocab > LOGPROBS_VOCAB:
+        raise ValueError(f"{n} rows of {vocab}: at most {LOGPROBS_ROWS} of {LOGPROBS_VOCAB} are supported")
+
+
 def _check_rows(rows, C: int, what: str) -> None:
+    check_columns(C)
     if rows.dtype not in _DTYPES:
         raise RuntimeError(f"unsupported dtype {rows.dtype}")
     if rows.dim() != 2 or rows.shape[1] != C or (rows.stride(1) != 1 and C > 1):
@@ -1375,11 +1390,14 @@ def embedding_gradient(order, n: int, V: int, C: int, dtype, scale: float):
 
 
 def _check_logits(logits, tokens) -> Tuple[int, int]:
-    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
-        raise ValueError("logits must be [n, vocab] with a contiguous vocab dimension")
+    if logits.dim() != 2:
+        raise ValueError("logits must be [n, vocab]")
+    n, vocab = logits.shape
+    check_logits_size(n, vocab)
+    if logits.stride(1) != 1 and vocab > 1:
+        raise ValueError("logits must have a contiguous vocab dimension")
     if logits.dtype not in _DTYPES:
         raise RuntimeError(f"unsupported dtype {logits.dtype}")
-    n, vocab = logits.shape
     if tokens.dtype is not torch.int64 or tokens.numel() != n or not tokens.is_contiguous():
         raise ValueError(f"tokens must be a contiguous int64 tensor of {n} values")
     return n, vocab

@@ -58,8 +58,8 @@ def embedding_lookup(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0
     """scale * weight[ids]: [*ids.shape, C] of weight's dtype, the product in fp32 and rounded
     once (a copy where scale is 1).
 
-    ids: int64 or int32, any shape; weight: [V, C] fp32, bf16 or fp16 on the same device.  An
-    id outside [0, V) gives a row of zeros and takes no gradient; padding_idx (from -V to
+    ids: int64 or int32, any shape; weight: [V, C <= 2^20] fp32, bf16 or fp16 on the same
+    device.  An id outside [0, V) gives a row of zeros and takes no gradient; padding_idx (from -V to
     V - 1) is looked up but takes none.
 
     Differentiable once in weight: a dense gradient [V, C], each row the sum over its tokens
@@ -70,6 +70,7 @@ def embedding_lookup(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0
     if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
         raise ValueError(f"ids are {ids.dtype}: int64 or int32 is needed")
     V, C = weight.shape
+    _lib.check_columns(C)
     padding = -1
     if padding_idx is not None:
         if not -V <= padding_idx < V:

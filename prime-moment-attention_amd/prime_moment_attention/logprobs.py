@@ -80,9 +80,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, ent
       top_tokens [..., top]     the ``top`` (at most 64) largest logits' tokens, equal ones by
       top_logprobs [..., top]   index, NaN last, and their log probabilities (None for top 0)
 
-    logits: [..., vocab] fp32, bf16 or fp16; tokens: [...] int64 or int32.  A logit of -infinity
-    has probability 0 (a row of nothing else: log probabilities -infinity, entropy 0, no
-    gradient); +infinity shares the probability with its equals; a NaN makes its row's results
+    logits: [..., vocab] fp32, bf16 or fp16, fewer than 2^31 rows of at most 2^24; tokens: [...]
+    int64 or int32.  A logit of -infinity has probability 0 (a row of nothing else: log
+    probabilities -infinity, entropy 0, no gradient); +infinity shares the probability with its equals; a NaN makes its row's results
     NaN.  The mean of -logprobs over the tokens that count is the cross entropy.
 
     Differentiable once in logits through logprobs and entropy, not through the top ones.
@@ -97,6 +97,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, ent
         raise RuntimeError(f"unsupported dtype {logits.dtype}")
     if logits.shape[-1] == 0:
         raise ValueError("the vocabulary is empty")
+    _lib.check_logits_size(tokens.numel(), logits.shape[-1])
     if not 0 <= top <= min(MAX_TOP, logits.shape[-1]):
         raise ValueError(f"top={top} outside 0 .. min({MAX_TOP}, vocab)")
     if not -(1 << 63) <= ignore_index < 1 << 63:
