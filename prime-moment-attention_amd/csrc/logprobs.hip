@@ -531,8 +531,8 @@ void run(LogprobsArgs a, bool backward, hipStream_t s) {
     const int part = kBackThreads * kBackUnroll * kVec<DT>, parts = (a.vocab + part - 1) / part, n = a.n;
     // a launch has below 2^32 threads and 2^16 rows in a grid's second dimension
     const int most = backward ? 65535 : 1 << 21;
-    for (int row = 0; row < n; row += most) {
-        a.n = n - row < most ? n - row : most;
+    for (int64_t row = 0; row < n; row += most) {  // (the last sum may pass 2^31)
+        a.n = n - row < most ? static_cast<int>(n - row) : most;
         if (backward) {
             hipLaunchKernelGGL(logprobs_backward_kernel<DT>, dim3(parts, a.n), dim3(kBackThreads), 0, s, a);
         } else if (static_cast<int64_t>(a.vocab) * es <= kWaveRow) {

@@ -82,8 +82,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, ent
 
     logits: [..., vocab] fp32, bf16 or fp16, fewer than 2^31 rows of at most 2^24; tokens: [...]
     int64 or int32.  A logit of -infinity has probability 0 (a row of nothing else: log
-    probabilities -infinity, entropy 0, no gradient); +infinity shares the probability with its equals; a NaN makes its row's results
-    NaN.  The mean of -logprobs over the tokens that count is the cross entropy.
+    probabilities -infinity, entropy 0, no gradient); +infinity shares the probability with its
+    equals; a NaN makes its row's results NaN.  The mean of -logprobs over the tokens that count is
+    the cross entropy.
 
     Differentiable once in logits through logprobs and entropy, not through the top ones.
     Forward and backward can be captured into a graph."""

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import ends_ref as R
-from prime_moment_attention import token_logprobs
+from prime_moment_attention import _lib, token_logprobs
 from test_gpu_logprobs import check, gen
 
 pytestmark = pytest.mark.gpu
@@ -107,3 +107,20 @@ def test_a_token_outside_the_vocabulary_has_an_entropy_all_the_same():
         want = R.logprobs_grad(x, tokens, None, h)
         assert want.isfinite().all()
         R.assert_within(dx, want, R.grad_bound(x, tokens, None, h, want), "gradient")
+
+
+def test_as_many_rows_as_a_call_takes():
+    """2^31 - 1 rows of one token each, whose probability is 1: 4 GB of logits, 17 GB of tokens."""
+    n = (1 << 31) - 1
+    x = torch.randn(n, 1, device="cuda", dtype=BF16)
+    tokens = torch.zeros(n, dtype=torch.int64, device="cuda")
+    tokens[-1] = tokens[(1 << 30) + 3] = -100
+    tokens[5] = 1
+    guard = torch.full((n + 8,), 7.0, device="cuda")
+    lp = guard[:n]
+    _lib.token_logprobs(x, tokens, -100, lp, None, None, 0, None, None)
+    assert lp[5].isnan() and (guard[n:] == 7).all()
+    lp[5] = 0.0
+    # d - log2 S with S = 2^d (1 + e): |e| <= 2 u of the exponential, so that e / ln 2, log2's rounding
+    # (2 u of |log2 S| < 1) and the difference's come to less than 6 u; times ln 2
+    assert lp.abs().max() <= 6 * R.U32
