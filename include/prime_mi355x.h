@@ -612,8 +612,8 @@ int prime_sample(const void *logits, int dtype, int n, int vocab, int64_t stride
  *   weight : V < 2^31 rows of C <= 2^20 contiguous elements, ldw >= C apart
  *   out    : [n, C], apart from weight and ids
  *   order  : NULL, or prime_embedding_order_size bytes, 16-byte aligned, that receive the order
- *            of the tokens by their ids for the backward.  Ids outside [0, V) and `padding` (-1:
- *            none) have no gradient
+ *            of the tokens by their ids for the backward.  Ids outside [0, V) and `padding` (in
+ *            [0, V), or -1: none) have no gradient
  *
  * prime_embedding_backward: dweight[v] = scale * sum of the rows dy[i] with ids[i] = v, all
  * V rows written, for the order that the lookup made of the same n and V.  Sums are in fp32 in

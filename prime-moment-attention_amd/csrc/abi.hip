@@ -1855,6 +1855,9 @@ int prime_embedding(const void *ids, int ids64, int64_t n, const void *weight, i
     if (!ids) return fail(PRIME_ERR_INVALID_ARG, "prime_embedding: null argument");
     int rc = embedding_checks("prime_embedding", n, weight, ldw, V, C, dtype, out);
     if (rc) return rc;
+    if (padding < -1 || padding >= V)
+        return fail(PRIME_ERR_INVALID_ARG, "padding=%lld is neither an id below %lld nor -1", static_cast<long long>(padding),
+                    static_cast<long long>(V));
     if (reinterpret_cast<uintptr_t>(ids) % (ids64 ? 8 : 4)) return fail(PRIME_ERR_MISALIGNED, "ids misaligned");
     const size_t need = prime_embedding_order_size(n, V);
     if (order && (order_bytes < need || (reinterpret_cast<uintptr_t>(order) & 15u)))

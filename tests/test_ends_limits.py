@@ -30,3 +30,18 @@ def test_sizes_beyond_the_entry_points_are_refused():
         token_logprobs(one.expand(1, 1 << 24), ids[:1])
     with pytest.raises(RuntimeError, match="HIP device"):
         embedding_lookup(ids, one.expand(2, 1 << 20))
+
+
+def test_embedding_refuses_a_padding_that_is_no_id():
+    """-1 is none; 2^32 + 5 was id 5 to few tokens and none to many."""
+    L, at = _lib.load(), [(i + 1) << 28 for i in range(4)]
+
+    def call(padding, order=at[3], n=8, V=100, out=at[2]):
+        return L.prime_embedding(at[0], 1, n, at[1], 64, V, 64, _lib.PRIME_BF16, 1.0, padding, out, order,
+                                 L.prime_embedding_order_size(n, V), None)
+    for n in (8, 40000):
+        for padding in (-2, -100, 100, 1 << 31, (1 << 32) + 5, -(1 << 32) + 5):
+            assert call(padding, n=n) == -1 and "padding" in _lib.last_error()
+            assert call(padding, order=None, n=n) == -1
+        for padding in (-1, 0, 99):  # these go on to the next check
+            assert call(padding, n=n, out=at[1]) == -5
