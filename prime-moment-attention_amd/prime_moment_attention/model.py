@@ -211,6 +211,21 @@ class PrimeBlock(nn.Module):
         return dropout_add(h.to(dtype), residual.to(dtype), self.dropout, rng, call=2 * self.layer + branch)
 
 
+_EMBEDDING_FORWARD = nn.Embedding.forward
+
+
+def _plain_embedding(m: nn.Module) -> bool:
+    """Whether m(ids) is weight[ids] with a dense gradient and nothing else: an nn.Embedding without
+    hooks of its own or of all modules, forward or backward, whose ``forward`` nobody has replaced, on
+    the instance (offloading and adapter wrappers do) or on the class."""
+    g = torch.nn.modules.module
+    return (type(m) is nn.Embedding and m.max_norm is None and not m.scale_grad_by_freq and not m.sparse
+            and "forward" not in m.__dict__ and nn.Embedding.forward is _EMBEDDING_FORWARD
+            and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
+                     or g._global_forward_hooks or g._global_forward_pre_hooks
+                     or g._global_backward_hooks or g._global_backward_pre_hooks))
+
+
 def _total(t: torch.Tensor) -> torch.Tensor:
     """The sum, 1024 values at a time: torch's sum over several workgroups clears its counters by a
     memset, which a captured training step would repeat wrongly."""
@@ -320,8 +335,7 @@ class PrimeForCausalLM(nn.Module):
         e, scale = self.embed_tokens, self.embedding_scale
         if not (self.fused_training or scale != 1.0):
             return e(input_ids)
-        if (type(e) is nn.Embedding and e.max_norm is None and not e.scale_grad_by_freq and not e.sparse
-                and not (e._forward_hooks or e._forward_pre_hooks or e._backward_hooks)):
+        if _plain_embedding(e):
             return embedding_lookup(input_ids, e.weight, scale, e.padding_idx)
         x = e(input_ids)  # (a module of the user's own)
         return x if scale == 1.0 else x * scale

@@ -3,7 +3,7 @@ the model leaves to modules of the user's own."""
 import pytest
 import torch
 
-from prime_moment_attention import _lib, embedding_lookup, token_logprobs
+from prime_moment_attention import PrimeConfig, PrimeForCausalLM, _lib, embedding_lookup, token_logprobs
 
 BIG = (1 << 32) + 5  # 5 in the 32 bits of a C int
 
@@ -45,3 +45,48 @@ def test_embedding_refuses_a_padding_that_is_no_id():
             assert call(padding, order=None, n=n) == -1
         for padding in (-1, 0, 99):  # these go on to the next check
             assert call(padding, n=n, out=at[1]) == -5
+
+
+def _watch(module, name, calls):
+    """Registers what the module's call is watched by under `name`; returns what takes it away."""
+    seen = lambda *a: calls.append(name)
+    if name.startswith("global"):
+        return getattr(torch.nn.modules.module, "register_module_" + name[7:])(seen)
+    if name == "forward":
+        plain = module.forward
+        module.forward = lambda ids: (seen(), plain(ids))[1]
+        return None
+    return getattr(module, "register_" + name)(seen)
+
+
+@pytest.mark.parametrize("name", ["forward", "forward_hook", "forward_pre_hook", "full_backward_hook", "full_backward_pre_hook",
+                                  "global forward_hook", "global forward_pre_hook", "global full_backward_hook",
+                                  "global full_backward_pre_hook"])
+@pytest.mark.parametrize("how", [dict(fused_training=True), dict(embedding_scale=2.0)])
+def test_a_watched_embedding_is_called(name, how):
+    model = PrimeForCausalLM(PrimeConfig(vocab_size=11, hidden_size=8, num_layers=1, num_heads=1, head_dim=8, **how))
+    ids, calls = torch.tensor([[1, 10, 1]]), []
+    handle = _watch(model.embed_tokens, name, calls)
+    try:
+        x = model._embed(ids)
+        assert torch.equal(x, model.embed_tokens.weight[ids] * model.embedding_scale)
+        x.sum().backward()
+    finally:
+        if handle is not None:
+            handle.remove()
+    assert name in calls
+
+
+def test_a_replaced_class_forward_of_embeddings_is_called(monkeypatch):
+    model = PrimeForCausalLM(PrimeConfig(vocab_size=11, hidden_size=8, num_layers=1, num_heads=1, head_dim=8,
+                                         fused_training=True))
+    monkeypatch.setattr(torch.nn.Embedding, "forward", lambda self, ids: 3 * self.weight[ids])
+    ids = torch.tensor([[1, 10, 1]])
+    assert torch.equal(model._embed(ids), 3 * model.embed_tokens.weight[ids])
+
+
+def test_an_embedding_as_it_is_goes_to_the_kernel():
+    model = PrimeForCausalLM(PrimeConfig(vocab_size=11, hidden_size=8, num_layers=1, num_heads=1, head_dim=8,
+                                         fused_training=True))
+    with pytest.raises(RuntimeError, match="HIP device"):
+        model._embed(torch.tensor([[1, 10, 1]]))
