@@ -670,7 +670,9 @@ int prime_token_logprobs_backward(const void *logits, int dtype, int n, int voca
  *   prime_grad_clip : the same, and every element times min(1, max_norm / (norm + 1e-6)),
  *                     in fp32, rounded once; nothing is written where that is 1.  given: norm
  *                     is read instead (one that other processes share in) and no workspace
- *                     needed.  An infinite norm scales by 0, a NaN one by NaN; an infinite max_norm clips nothing.
+ *                     needed.  Without, the factor is that of the norm in 64 bits, also where the
+ *                     one that is written is infinite.  An infinite norm scales by 0, a NaN one by
+ *                     NaN; an infinite max_norm clips nothing.
  * workspace: prime_grad_norm_workspace_size bytes, 16-byte aligned, this call's own until it
  * has run on `stream`.
  */

@@ -2007,11 +2007,12 @@ int prime_grad_clip(void *const *tensors, const int64_t *sizes, const int32_t *d
         for (GradTables g{tensors, sizes, dtypes, count}; g.next(); blocks += g.blocks, ++tables)
             if ((rc = check_hip(prime::launch_grad_squares(g.t, g.blocks, parts + blocks, s), "gradient norm launch")))
                 return rc;
-        // one table: the scaling adds the parts itself
+        // one table: the scaling adds the parts itself; more: it finds their sum in the first
         if (tables != 1 && (rc = check_hip(prime::launch_grad_norm(parts, blocks, norm, s), "gradient norm launch"))) return rc;
+        if (tables != 1) blocks = 1;
     }
     for (GradTables g{tensors, sizes, dtypes, count}; g.next();)
-        if ((rc = check_hip(prime::launch_grad_scale(g.t, g.blocks, tables == 1 ? parts : nullptr, blocks, norm, max_norm, s),
+        if ((rc = check_hip(prime::launch_grad_scale(g.t, g.blocks, given ? nullptr : parts, blocks, norm, max_norm, s),
                             "gradient scaling launch")))
             return rc;
     return PRIME_OK;

@@ -181,10 +181,13 @@ __device__ __forceinline__ double parts_sum(const double *parts, int count, doub
     return block_sum(sum, red);
 }
 
-__global__ __launch_bounds__(kThreads) void grad_norm_kernel(const double *parts, int count, float *norm) {
+// One workgroup: the norm, and the whole sum in parts[0] for the scaling of several tables.
+__global__ __launch_bounds__(kThreads) void grad_norm_kernel(double *parts, int count, float *norm) {
     __shared__ double red[kThreads / kWave];
-    const double sum = parts_sum(parts, count, red);
-    if (threadIdx.x == 0) *norm = static_cast<float>(sqrt(sum));
+    const double sum = parts_sum(parts, count, red);  // (behind its barriers all parts are read)
+    if (threadIdx.x != 0) return;
+    *norm = static_cast<float>(sqrt(sum));
+    if (count) parts[0] = sum;
 }
 
 // parts: the sums of squares, whose root is written to `norm`; or null, `norm` being given.
@@ -211,7 +214,7 @@ hipError_t launch_grad_squares(const GradTable &t, int blocks, double *parts, hi
     hipLaunchKernelGGL(grad_squares_kernel, dim3(blocks), dim3(kThreads), 0, stream, t, parts);
     return hipGetLastError();
 }
-hipError_t launch_grad_norm(const double *parts, int count, float *norm, hipStream_t stream) {
+hipError_t launch_grad_norm(double *parts, int count, float *norm, hipStream_t stream) {
     hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(kThreads), 0, stream, parts, count, norm);
     return hipGetLastError();
 }

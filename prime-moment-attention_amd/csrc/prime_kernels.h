@@ -526,7 +526,7 @@ struct GradTable {
     uint32_t span;
 };
 hipError_t launch_grad_squares(const GradTable &t, int blocks, double *parts, hipStream_t stream);
-hipError_t launch_grad_norm(const double *parts, int count, float *norm, hipStream_t stream);
+hipError_t launch_grad_norm(double *parts, int count, float *norm, hipStream_t stream);
 hipError_t launch_grad_scale(const GradTable &t, int blocks, const double *parts, int count, float *norm,
                              double max_norm, hipStream_t stream);
 

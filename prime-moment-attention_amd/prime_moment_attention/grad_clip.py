@@ -66,9 +66,10 @@ def clip_grad_norm_(parameters: Parameters, max_norm: float) -> torch.Tensor:
     """grad_norm, and every gradient times min(1, max_norm / (norm + 1e-6)) in place, in fp32,
     rounded once.  Returns the norm before clipping; the device is not waited for.
 
-    Nothing is written where that factor is 1.  An infinite norm gives 0 (and NaN for the
-    infinite elements), a NaN one NaN, as torch.nn.utils.clip_grad_norm_; an infinite max_norm
-    clips nothing.  Gradients must not overlap each other."""
+    Nothing is written where that factor is 1.  The factor is taken from the norm in 64 bits, so
+    that finite gradients are clipped to max_norm also where the norm is beyond fp32 and returned
+    as infinity.  An infinite element gives 0 (and NaN in its own place), a NaN NaN, as
+    torch.nn.utils.clip_grad_norm_; an infinite max_norm clips nothing.  Gradients must not overlap each other."""
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm={max_norm} below 0")
@@ -87,7 +88,8 @@ def clip_grad_norm_(parameters: Parameters, max_norm: float) -> torch.Tensor:
 
 def clip_grads_with_norm_(parameters: Parameters, max_norm: float, norm: torch.Tensor) -> None:
     """clip_grad_norm_ by a given norm (fp32 scalar on the gradients' device), as where it is
-    taken over several processes' gradients: the root of the sum of their grad_norm squared."""
+    taken over several processes' gradients: the root of the sum of their grad_norm squared.  An
+    infinite norm gives 0."""
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm={max_norm} below 0")
