@@ -142,15 +142,15 @@ __device__ __forceinline__ double square_sum(char *p, int size) {
 }
 
 template <int DT>
-__device__ __forceinline__ void scale_block(char *p, int size, float c) {
+__device__ __forceinline__ void scale_block(char *p, int size, float c, float power) {
     each_slot<DT>(
         p, size,
         [&](char *q, float (&x)[kSlot]) {
 #pragma unroll
-            for (int j = 0; j < kSlot; ++j) x[j] *= c;
+            for (int j = 0; j < kSlot; ++j) x[j] = x[j] * c * power;
             store_slot<DT>(q, x);
         },
-        [&](char *q) { store_elem(q, 0, DT, load_elem(q, 0, DT) * c); });
+        [&](char *q) { store_elem(q, 0, DT, load_elem(q, 0, DT) * c * power); });
 }
 
 }  // namespace
@@ -201,12 +201,15 @@ __global__ __launch_bounds__(kThreads) void grad_scale_kernel(const GradTable t,
     } else {
         total = *norm;
     }
-    const float c = static_cast<float>(max_norm / (total + 1e-6));
-    if (c >= 1.f || max_norm == __builtin_inf()) return;  // (a NaN scales)
+    // One fp32 number would lose bits of a factor near fp32's least or below it: then 2^100 times
+    // the factor, and the power of two, which rounds nothing more, behind the product.
+    const double factor = max_norm / (total + 1e-6);
+    if (static_cast<float>(factor) >= 1.f || max_norm == __builtin_inf()) return;  // (a NaN scales)
+    const float power = factor < 0x1p-100 ? 0x1p-100f : 1.f, c = static_cast<float>(factor / power);
     each_block(t, [&](int dt, char *p, int size) {
-        if (dt == PRIME_BF16) scale_block<PRIME_BF16>(p, size, c);
-        else if (dt == PRIME_F16) scale_block<PRIME_F16>(p, size, c);
-        else scale_block<PRIME_F32>(p, size, c);
+        if (dt == PRIME_BF16) scale_block<PRIME_BF16>(p, size, c, power);
+        else if (dt == PRIME_F16) scale_block<PRIME_F16>(p, size, c, power);
+        else scale_block<PRIME_F32>(p, size, c, power);
     });
 }
 

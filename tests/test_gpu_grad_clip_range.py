@@ -28,6 +28,21 @@ def test_the_factor_does_not_depend_on_the_number_of_tensors(count):
         R.assert_within(torch.cat(grads), want[0], bounds[0], f"{size}")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_factors_below_fp32s_normal_numbers(dtype):
+    """A norm above 2^126 times the limit: as a single fp32 number the factor would have lost bits."""
+    for count, size, max_norm in ((9000, 3e38, 1.0), (9000, 3e38, 1e-3), (10, 3e38, 1e-4), (9000, 1e38, 1e-6), (4099, 2e38, 30.0),
+                                  (9000, 1e-3, 1e-33), (300, 3e38, 1e9)):
+        g = (size * (0.5 + 0.5 * torch.rand(count, device="cuda"))).to(dtype)
+        g[::7] = 0.0
+        g[1::7] = 1.0
+        for parts in (1, 250):
+            mine = g.clone()
+            norm, want, bounds = R.clipped([g], max_norm)
+            clip_grad_norm_(params(list(mine.split(-(-count // parts)))), max_norm)
+            R.assert_within(mine, want[0], bounds[0], f"{count} of {size}")
+
+
 def test_not_finite_in_many_tensors():
     for bad in (math.inf, math.nan):
         grads = [torch.ones(3, device="cuda") for _ in range(200)]
