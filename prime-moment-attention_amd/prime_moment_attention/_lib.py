@@ -1365,21 +1365,28 @@ def embedding_backward(order, dy, scale: float, dweight) -> None:
     if order.dtype is not torch.uint8 or not order.is_contiguous():
         raise ValueError("order must be a buffer of embedding_order")
     _same_device(dy, order, dweight)
-    embedding_gradient(order, n, V, C, dy.dtype, scale)(dy, pitch if n > 1 else C, dweight)
+    embedding_gradient(n, V, C, dy.dtype, dy.device, scale)(order, dy, pitch if n > 1 else C, dweight)
 
 
-def embedding_gradient(order, n: int, V: int, C: int, dtype, scale: float):
-    """embedding_backward of operands that are known to be so, as f(dy, pitch, dweight): all that
-    does not depend on dy is looked up here.  (Each step takes autograd's thread about three
-    times as long as the thread of the forward: a small training call 81 us for 85, of log
-    probabilities 88 for 93.)"""
+def _came_back(t, what: str, like, index: int, n: int) -> int:
+    """The address of a saved tensor of n contiguous values, which hooks of the user's may have had
+    elsewhere."""
+    if t.dtype is not like or t.get_device() != index or t.numel() != n or not t.is_contiguous():
+        raise RuntimeError(f"{what} came back as {tuple(t.shape)} {t.dtype} on {t.device}: {n} contiguous values of {like} "
+                           f"on device {index} were kept")
+    return t.data_ptr()
+
+
+def embedding_gradient(n: int, V: int, C: int, dtype, dev, scale: float):
+    """embedding_backward of operands that are known to be so but for the order, as f(order, dy,
+    pitch, dweight): all that does not depend on them is looked up here.  (Each step takes
+    autograd's thread about three times as long as the thread of the forward.)"""
     L = load()
     fn, size = L.prime_embedding_backward, L.prime_embedding_backward_workspace_size(n, C)
-    dev, dt = order.device, _DTYPES[dtype]
-    index, at, held = dev.index, order.data_ptr(), order.numel()
+    index, dt, held = dev.index, _DTYPES[dtype], L.prime_embedding_order_size(n, V)
 
-    def run(dy, pitch: int, dweight) -> None:
-        ws = order.new_empty(size)
+    def run(order, dy, pitch: int, dweight) -> None:
+        at, ws = _came_back(order, "the order", torch.uint8, index, held), order.new_empty(size)
         args = (at, held, n, dy.data_ptr(), pitch, V, C, dt, scale, dweight.data_ptr(), ws.data_ptr(), size)
         if index != torch._C._cuda_getDevice():
             _launch(fn, "prime_embedding_backward", dev, *args)
@@ -1438,8 +1445,8 @@ def token_logprobs_backward(logits, tokens, ignore: int, stats, entropy, dlogpro
     if dlogits.shape != logits.shape or dlogits.dtype is not logits.dtype or (dlogits.stride(1) != 1 and vocab > 1):
         raise ValueError("dlogits must have logits' shape and dtype and a contiguous vocab dimension")
     _same_device(logits, tokens, stats, entropy, dlogprobs, dentropy, dlogits)
-    token_logprobs_gradient(stats, n, vocab, logits.dtype, ignore)(logits, tokens, entropy, dlogprobs, dentropy, dlogits,
-                                                                   _row_stride(dlogits))
+    token_logprobs_gradient(n, vocab, logits.dtype, logits.device, ignore)(logits, tokens, stats, entropy, dlogprobs,
+                                                                           dentropy, dlogits, _row_stride(dlogits))
 
 
 _T = torch._C.TensorBase
@@ -1447,20 +1454,24 @@ _dtype_of, _data_ptr, _numel, _get_device = _T.dtype.__get__, _T.data_ptr, _T.nu
 GRAD_TABLE, GRAD_PARTS = 192, 4096 * 8  # tensors of a launch, and the workspace that they take at most
 
 
-def token_logprobs_gradient(stats, n: int, vocab: int, dtype, ignore: int):
-    """token_logprobs_backward of operands that are known to be so, as f(logits, tokens, entropy,
-    dlogprobs, dentropy, dlogits): all that does not depend on them is looked up here, as in
+def token_logprobs_gradient(n: int, vocab: int, dtype, dev, ignore: int):
+    """token_logprobs_backward of gradients that are known to be so, as f(logits, tokens, stats,
+    entropy, dlogprobs, dentropy, dlogits): all that does not depend on them is looked up here, as in
     embedding_gradient.  logits: [n, vocab] with a contiguous vocabulary, or contiguous; dlogits'
     rows `out_pitch` apart."""
     fn, dt = load().prime_token_logprobs_backward, _DTYPES[dtype]
-    dev = stats.device
-    index = dev.index
+    index, f32, i64 = dev.index, torch.float32, torch.int64
 
-    def run(logits, tokens, entropy, dlogprobs, dentropy, dlogits, out_pitch: int = vocab) -> None:
+    def run(logits, tokens, stats, entropy, dlogprobs, dentropy, dlogits, out_pitch: int = vocab) -> None:
+        if logits.dtype is not dtype or logits.get_device() != index or logits.numel() != n * vocab:
+            raise RuntimeError(f"logits came back as {tuple(logits.shape)} {logits.dtype} on {logits.device}: {n} x {vocab} "
+                               f"of {dtype} on device {index} were kept")
         pitch = logits.stride(0) if n > 1 and logits.dim() == 2 else vocab
-        args = (logits.data_ptr(), dt, n, vocab, pitch, tokens.data_ptr(), ignore, stats.data_ptr(),
-                None if entropy is None else entropy.data_ptr(), None if dlogprobs is None else dlogprobs.data_ptr(),
-                None if dentropy is None else dentropy.data_ptr(), dlogits.data_ptr(), out_pitch)
+        args = (logits.data_ptr(), dt, n, vocab, pitch, _came_back(tokens, "tokens", i64, index, n), ignore,
+                _came_back(stats, "stats", f32, index, 2 * n),
+                None if entropy is None else _came_back(entropy, "entropy", f32, index, n),
+                None if dlogprobs is None else dlogprobs.data_ptr(), None if dentropy is None else dentropy.data_ptr(),
+                dlogits.data_ptr(), out_pitch)
         if index != torch._C._cuda_getDevice():
             _launch(fn, "prime_token_logprobs_backward", dev, *args)
         elif rc := fn(*args, torch._C._cuda_getCurrentRawStream(index)):

@@ -34,7 +34,8 @@ class _EmbeddingFn(torch.autograd.Function):
         order = ctx.gradient = None
         if n and V and C:
             order = _lib.embedding_order(n, V, weight.device)
-            ctx.gradient = _lib.embedding_gradient(order, n, V, C, weight.dtype, scale)
+            ctx.gradient = _lib.embedding_gradient(n, V, C, weight.dtype, weight.device, scale)
+        ctx.save_for_backward(order)
         return _run(ids, weight, scale, padding, order)
 
     @staticmethod
@@ -43,13 +44,14 @@ class _EmbeddingFn(torch.autograd.Function):
 
     @staticmethod
     def _grads(ctx, dy):
+        order, = ctx.saved_tensors
         if ctx.gradient is None:
             return dy.new_zeros(ctx.table), None, None, None
         dweight, pitch = dy.new_empty(ctx.table), ctx.table[1]
         if not dy.is_contiguous():
             dy = _rows(dy)
             pitch = dy.stride(0) if dy.shape[0] > 1 else pitch
-        ctx.gradient(dy, pitch, dweight)
+        ctx.gradient(order, dy, pitch, dweight)
         return dweight, None, None, None
 
 

@@ -44,8 +44,8 @@ class _TokenLogprobsFn(torch.autograd.Function):
     def forward(ctx, logits, tokens, top, entropy, ignore):
         stats = torch.empty((*tokens.shape, 2), device=logits.device, dtype=torch.float32)
         out = _run(logits, tokens, top, entropy, ignore, stats)
-        ctx.gradient = _lib.token_logprobs_gradient(stats, tokens.numel(), logits.shape[-1], logits.dtype, ignore)
-        ctx.save_for_backward(logits, tokens, out[1])
+        ctx.gradient = _lib.token_logprobs_gradient(tokens.numel(), logits.shape[-1], logits.dtype, logits.device, ignore)
+        ctx.save_for_backward(logits, tokens, stats, out[1])
         if top:
             ctx.mark_non_differentiable(out[2], out[3])
         ctx.set_materialize_grads(False)
@@ -59,14 +59,14 @@ class _TokenLogprobsFn(torch.autograd.Function):
     def _grads(ctx, dlogprobs, dentropy):
         if dlogprobs is None and dentropy is None:
             return None, None, None, None, None
-        logits, tokens, entropy = ctx.saved_tensors
+        logits, tokens, stats, entropy = ctx.saved_tensors
         if dlogprobs is not None and not dlogprobs.is_contiguous():
             dlogprobs = dlogprobs.contiguous()
         if dentropy is not None and not dentropy.is_contiguous():
             dentropy = dentropy.contiguous()
         dlogits = logits.new_empty(logits.shape)
         if dlogits.numel():
-            ctx.gradient(logits if logits.is_contiguous() else _rows(logits), tokens, entropy, dlogprobs, dentropy, dlogits)
+            ctx.gradient(logits if logits.is_contiguous() else _rows(logits), tokens, stats, entropy, dlogprobs, dentropy, dlogits)
         return dlogits, None, None, None, None
 
 
