@@ -14,6 +14,7 @@
 // bf16, whose norm clips nothing 15 + 4.9.  (Sums in fp32 are no faster; nor is scaling from the end, what the sums read last.)
 
 #include "prime_kernels.h"
+#include "row_vec.h"
 
 namespace prime {
 
@@ -21,43 +22,20 @@ namespace {
 
 constexpr int kThreads = 256, kSlot = 8;
 
-struct __attribute__((packed, aligned(2))) Raw {  // 16 bytes, wherever they start
-    u32x4 v;
-};
-
 template <int DT>
 __device__ __forceinline__ void load_slot(const char *p, float (&x)[kSlot]) {
-    if constexpr (DT == PRIME_F32) {
-        const u32x4 a = reinterpret_cast<const Raw *>(p)[0].v, b = reinterpret_cast<const Raw *>(p)[1].v;
+    constexpr int V = kVec<DT>;
+    u32x4 v[kSlot / V];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(a[j]), x[j + 4] = __uint_as_float(b[j]);
-    } else {
-        const u32x4 v = reinterpret_cast<const Raw *>(p)->v;
+    for (int i = 0; i < kSlot / V; ++i) v[i] = reinterpret_cast<const Raw *>(p)[i].v;
 #pragma unroll
-        for (int j = 0; j < kSlot; ++j) {
-            const uint32_t u = v[j / 2];
-            if constexpr (DT == PRIME_BF16) x[j] = __uint_as_float(j & 1 ? u & 0xFFFF0000u : u << 16);
-            else x[j] = h16_bits_to_f32(static_cast<uint16_t>(j & 1 ? u >> 16 : u));
-        }
-    }
+    for (int i = 0; i < kSlot / V; ++i) widen<DT>(v[i], reinterpret_cast<float(&)[V]>(x[i * V]));
 }
 template <int DT>
 __device__ __forceinline__ void store_slot(char *p, const float (&x)[kSlot]) {
-    if constexpr (DT == PRIME_F32) {
-        u32x4 a, b;
+    constexpr int V = kVec<DT>;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) a[j] = __float_as_uint(x[j]), b[j] = __float_as_uint(x[j + 4]);
-        reinterpret_cast<Raw *>(p)[0].v = a;
-        reinterpret_cast<Raw *>(p)[1].v = b;
-    } else {
-        u32x4 v;
-#pragma unroll
-        for (int j = 0; j < kSlot; j += 2) {
-            if constexpr (DT == PRIME_BF16) v[j / 2] = f32_to_bf16_bits(x[j]) | static_cast<uint32_t>(f32_to_bf16_bits(x[j + 1])) << 16;
-            else v[j / 2] = f32_to_h16_bits(x[j]) | static_cast<uint32_t>(f32_to_h16_bits(x[j + 1])) << 16;
-        }
-        reinterpret_cast<Raw *>(p)->v = v;
-    }
+    for (int i = 0; i < kSlot / V; ++i) reinterpret_cast<Raw *>(p)[i].v = narrow<DT>(reinterpret_cast<const float(&)[V]>(x[i * V]));
 }
 
 __device__ __forceinline__ double wave_sum_f64(double x) {

@@ -25,6 +25,7 @@
 #include <type_traits>
 
 #include "prime_kernels.h"
+#include "row_vec.h"
 
 namespace prime {
 
@@ -35,35 +36,6 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -1e7f, kHighest = 1e7f;  // times log2(e) below 2^24
 constexpr float kFar = -2e38f;                     // an exponent that may be the end of fp32
 constexpr float kFloor = -1e4f;                    // 2^kFloor = 0: for 0 times an exponent of -infinity
-
-struct __attribute__((packed, aligned(2))) Raw {  // 16 bytes of a row, wherever it starts
-    u32x4 v;
-};
-
-template <int DT>
-constexpr int kVec = DT == PRIME_F32 ? 4 : 8;  // elements of 16 bytes
-
-template <int DT>
-__device__ __forceinline__ void widen(const u32x4 &v, float (&x)[kVec<DT>]) {
-#pragma unroll
-    for (int j = 0; j < kVec<DT>; ++j) {
-        if constexpr (DT == PRIME_F32) x[j] = __uint_as_float(v[j]);
-        else if constexpr (DT == PRIME_BF16) x[j] = __uint_as_float(j & 1 ? v[j / 2] & 0xFFFF0000u : v[j / 2] << 16);
-        else x[j] = h16_bits_to_f32(static_cast<uint16_t>(j & 1 ? v[j / 2] >> 16 : v[j / 2]));
-    }
-}
-
-template <int DT>
-__device__ __forceinline__ u32x4 narrow(const float (&x)[kVec<DT>]) {
-    u32x4 v;
-#pragma unroll
-    for (int j = 0; j < kVec<DT>; j += DT == PRIME_F32 ? 1 : 2) {
-        if constexpr (DT == PRIME_F32) v[j] = __float_as_uint(x[j]);
-        else if constexpr (DT == PRIME_BF16) v[j / 2] = f32_to_bf16_bits(x[j]) | static_cast<uint32_t>(f32_to_bf16_bits(x[j + 1])) << 16;
-        else v[j / 2] = f32_to_h16_bits(x[j]) | static_cast<uint32_t>(f32_to_h16_bits(x[j + 1])) << 16;
-    }
-    return v;
-}
 
 // The reference C of a largest logit m, the same number wherever it is used: contracted into a
 // difference it would be another one.

@@ -32,6 +32,7 @@
 #include <type_traits>
 
 #include "prime_kernels.h"
+#include "row_vec.h"
 
 namespace prime {
 
@@ -176,9 +177,6 @@ __device__ __forceinline__ uint64_t block_scan(SampleShared<WAVES> &sh, uint64_t
 // A row: wave w has the chunks [w per, (w + 1) per) of 64 lanes with VE elements each.  A
 // chunk past the vocabulary's end becomes the last VE elements, those that an earlier chunk
 // has as -infinity.  STAGED > 0: per is at most that, and after the first pass the row is in LDS.
-struct __attribute__((packed, aligned(2))) Raw {  // 16 bytes of a row, wherever it starts
-    u32x4 v;
-};
 template <int DT, int STAGED>
 struct SampleRow {
     static constexpr int VE = DT == PRIME_F32 ? 4 : 8, es = DT == PRIME_F32 ? 4 : 2;
