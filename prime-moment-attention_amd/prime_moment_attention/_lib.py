@@ -1365,6 +1365,7 @@ def embedding_backward(order, dy, scale: float, dweight) -> None:
     if order.dtype is not torch.uint8 or not order.is_contiguous():
         raise ValueError("order must be a buffer of embedding_order")
     _same_device(dy, order, dweight)
+    order = order.view(-1)[:load().prime_embedding_order_size(n, V)]  # (a buffer may have room for more tokens)
     embedding_gradient(n, V, C, dy.dtype, dy.device, scale)(order, dy, pitch if n > 1 else C, dweight)
 
 

@@ -2,8 +2,9 @@
 that hooks see, that are freed by the backward, and that come back as they were or are refused."""
 import pytest
 import torch
+import torch.utils.checkpoint
 
-from prime_moment_attention import embedding_lookup, token_logprobs
+from prime_moment_attention import _lib, embedding_lookup, token_logprobs
 
 pytestmark = pytest.mark.gpu
 
@@ -96,3 +97,26 @@ def test_what_comes_back_otherwise_is_refused(make, count, kind):
             continue
         with pytest.raises(RuntimeError, match="came back"):
             backward(out)
+
+
+@pytest.mark.parametrize("reentrant", [True, False])
+@pytest.mark.parametrize("make", STEPS)
+def test_recomputed_by_a_checkpoint(make, reentrant):
+    leaf, forward, backward = make()
+    total = lambda out: out.square().sum() if torch.is_tensor(out) else out.logprobs.square().sum() + out.entropy.square().sum()
+    want, = torch.autograd.grad(total(forward()), leaf)
+    torch.utils.checkpoint.checkpoint(lambda _: total(forward()), leaf, use_reentrant=reentrant).backward()
+    assert torch.equal(leaf.grad, want)
+
+
+def test_an_order_with_room_for_more_tokens():
+    """A buffer that is kept for the largest batch serves smaller ones."""
+    V, C = 300, 20
+    room = _lib.embedding_order(30000, V, "cuda")
+    w = torch.randn(V, C, device="cuda", requires_grad=True)
+    for n in (7, 3000, 30000):
+        ids, dy = torch.randint(0, V, (n,), device="cuda"), torch.randn(n, C, device="cuda")
+        _lib.embedding(ids, w.detach(), 1.0, torch.empty(n, C, device="cuda"), -1, room)
+        got = torch.empty(V, C, device="cuda")
+        _lib.embedding_backward(room, dy, 1.0, got)
+        assert torch.equal(got, torch.autograd.grad(embedding_lookup(ids, w), w, dy)[0])
