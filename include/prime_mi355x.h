@@ -636,8 +636,8 @@ int prime_embedding_backward(const void *order, size_t order_bytes, int64_t n, c
  *   logprobs = log p[token]     0 where token is `ignore`, NaN for another one outside the
  *                               vocabulary
  *   entropy  = -sum p log p     (or NULL)
- *   top_tokens, top_logprobs    the `top` <= 64 largest logits, equal ones by index, NaN last
- *                               ([n, top]; NULL where top is 0)
+ *   top_tokens, top_logprobs    the `top` <= 64 largest logits, equal ones by index, NaN as
+ *                               -infinity ([n, top]; NULL where top is 0)
  *   stats                       [n, 2] for the backward, or NULL
  * A logit of -infinity has probability 0; a row with nothing else has log probabilities of
  * -infinity, entropy 0 and no gradient.  Logits of +infinity share the probability among

@@ -1,7 +1,8 @@
 // Embedding lookup y_i = scale W[id_i], and its gradient dW[v] = scale sum_{i: id_i = v} dy_i.
 //
 // The gradient takes the tokens of one id side by side, in their order, and sums over these rows
-// in fp32, each row of dy read once: no atomics on floats, so the order of every sum is fixed.
+// (those of many tokens by parts) in fp32, each row of dy read once: no atomics on floats, so the
+// order of every sum is fixed.
 //   order   pairs (id, token) such that equal ids lie together, a token without a gradient
 //           (padding, an id outside the table) with the id V and behind all others; and which
 //           ids occur.  Made by the lookup, for which it is all but free: its few workgroups
@@ -749,7 +750,7 @@ void run_backward(const EmbeddingArgs &a, hipStream_t s) {
     char *w = static_cast<char *>(a.workspace);
     float *part = reinterpret_cast<float *>(w);
     const LongIds longs{reinterpret_cast<uint32_t *>(w + space.counts), reinterpret_cast<uint4 *>(w + space.lists)};
-    // a dy larger than the L2 caches (32 MB) together: past them.  (Past / through them, x 768 bf16, us:
+    // a dy of 64 MB or more, twice what the L2 caches hold together: past them.  (Past / through them, x 768 bf16, us:
     // last touched long ago, 131072 tokens 55 / 75, 65536 36 / 40-43, 32768 27 / 22; just
     // written, 59 / 51, 39.6 / 37, 22.5 / 21.)
     const bool once = a.n * a.C * (DT == PRIME_F32 ? 4 : 2) >= int64_t{1} << 26;

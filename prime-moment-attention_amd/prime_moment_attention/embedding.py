@@ -1,5 +1,5 @@
 """Embedding lookup with a scale, and its gradient by sorted tokens: rows of equal ids are
-summed in their order in fp32, without atomics, so that a training step repeats bit for bit.
+summed in a fixed order in fp32, without atomics, so that a training step repeats bit for bit.
 """
 from __future__ import annotations
 
@@ -65,7 +65,7 @@ def embedding_lookup(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0
     V - 1) is looked up but takes none.
 
     Differentiable once in weight: a dense gradient [V, C], each row the sum over its tokens
-    in their order, in fp32, rounded once.  Forward and backward can be captured into a graph
+    in a fixed order, in fp32, rounded once.  Forward and backward can be captured into a graph
     (the ids may change between replays)."""
     if weight.dim() != 2:
         raise ValueError(f"weight has shape {tuple(weight.shape)}, expected [V, C]")

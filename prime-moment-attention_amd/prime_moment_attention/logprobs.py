@@ -78,7 +78,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, ent
                                 token outside the vocabulary
       entropy [...]             -sum p log p (None without ``entropy``)
       top_tokens [..., top]     the ``top`` (at most 64) largest logits' tokens, equal ones by
-      top_logprobs [..., top]   index, NaN last, and their log probabilities (None for top 0)
+      top_logprobs [..., top]   index, NaN as -infinity, and their log probabilities
+                                (None for top 0)
 
     logits: [..., vocab] fp32, bf16 or fp16, fewer than 2^31 rows of at most 2^24; tokens: [...]
     int64 or int32.  A logit of -infinity has probability 0 (a row of nothing else: log

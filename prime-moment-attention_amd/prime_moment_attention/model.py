@@ -35,7 +35,8 @@ Additions for other layers and for training:
   * ``PrimeConfig.embedding_scale``: the embeddings times a factor.
   * ``PrimeConfig.fused_training``: the embedding by embedding_lookup (its gradient
     without atomics: a step repeats bit for bit) and the loss by token_logprobs (no
-    fp32 copy of the logits, no softmax kept).
+    fp32 copy of the logits, no softmax kept).  A step of a few tokens and a small table
+    is faster without: a call of either costs the host 80 us, whatever its size.
   * ``clip_grad_norm_(max_norm)`` on the model; ``score(input_ids)`` for the log
     probabilities of a text; ``SamplingDecoder(logprobs=k)`` for those of the tokens
     that it chooses.
