@@ -10,8 +10,9 @@
 // product C is then below 2^24, so that rounding it moves all d_j by 1/2 at most, and 2^d, S, T and
 // what rescales them stay finite.  References begin at kLowest, so that in such a row a mask, whatever
 // its size, comes to 0.  Other rows (a largest logit beyond, infinities that are the largest, nothing
-// but masks, NaN) are summed again by differences (Careful), which takes 3 to 9 times as long (512 x
-// 50304 bf16 of such rows alone: 157 us for 17.5); the backward knows them by a NaN in the row's C.
+// but masks, NaN) are summed again by differences (Careful), two more passes over the row (512 x
+// 50304 bf16 of such rows alone, with 5 alternatives and the entropy: 80 us, the ties of equal masks among
+// them, for 17.5); the backward finds their largest and sum in place of C and L.
 //
 // A forward reads a row once, the likeliest tokens' vectors again; a backward reads it and writes
 // its gradient.  8192 x 50304 bf16 (us on the device): 139 forward (824 MB, 5.9 TB/s, a read's
@@ -131,18 +132,28 @@ template <int DT, int WAVES>
 __device__ __noinline__ Careful careful(const Group<WAVES> g, const char *row, int vocab) {
     Careful c;
     float top = -kInf, bad = 0.f, s = 0.f, t = 0.f;
-    for (int j = g.thread(); j < vocab; j += g.kThreads) {
-        const float x = load_elem(row, j, DT);
+    auto each = [&](auto f) {
+        constexpr int U = 8;
+        for (int j = g.thread(); j < vocab; j += U * g.kThreads) {
+            float x[U];  // all loads first
+#pragma unroll
+            for (int u = 0; u < U; ++u) x[u] = load_elem(row, min(j + u * g.kThreads, vocab - 1), DT);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (j + u * g.kThreads < vocab) f(x[u]);
+        }
+    };
+    each([&](float x) {
         top = fmaxf(top, x);
         bad += x != x ? 1.f : 0.f;
-    }
+    });
     c.top = g.max(top);
     c.nan = g.sum(bad) > 0.f;
-    for (int j = g.thread(); j < vocab; j += g.kThreads) {
-        const float d = c.diff(load_elem(row, j, DT)), e = __expf(d);
+    each([&](float x) {
+        const float d = c.diff(x), e = __expf(d);
         s += e;
         t += e > 0.f ? e * d : 0.f;
-    }
+    });
     s = g.sum(s), t = g.sum(t);
     c.log_sum = logf(s), c.mean = t / s;
     return c;
@@ -399,7 +410,10 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void logprobs_ker
         // (where one token has all the probability this may round to -3e-8; the gradient cancels that
         // against the same in log p, so that it is left as it is)
         if constexpr (ENTROPY) a.entropy[row] = fine ? (L - t / s) * kLn2 : k.entropy();
-        if (a.stats) a.stats[2 * row] = fine ? C : __builtin_nanf(""), a.stats[2 * row + 1] = L;
+        if (a.stats) {  // (an ordinary row's L is above -1: its largest d is -1/2 at least)
+            a.stats[2 * row] = fine ? C : k.nan ? __builtin_nanf("") : k.top;
+            a.stats[2 * row + 1] = fine ? L : -1.f - k.log_sum;
+        }
     }
     if (a.top)
         likeliest<DT, WAVES>(g, sh, base, a.vocab, a.top, top, mine, full, tail, [&](int rank, int id, float x) {
@@ -416,7 +430,6 @@ constexpr int kBackThreads = 256, kBackUnroll = 4;
 template <int DT>
 __global__ __launch_bounds__(kBackThreads) void logprobs_backward_kernel(const LogprobsArgs a) {
     constexpr int VE = kVec<DT>, U = kBackUnroll, es = DT == PRIME_F32 ? 4 : 2;
-    __shared__ __attribute__((aligned(16))) float red[4 * kBackThreads / kWave];
     const int64_t row = blockIdx.y;
     const char *base = static_cast<const char *>(a.logits) + a.stride_n * es * row;
     char *out = static_cast<char *>(a.dlogits) + a.stride_d * es * row;
@@ -426,10 +439,9 @@ __global__ __launch_bounds__(kBackThreads) void logprobs_backward_kernel(const L
     if (a.dlogprobs && token != a.ignore && (token < 0 || token >= a.vocab)) gl = __builtin_nanf("");
     const int first = blockIdx.x * (kBackThreads * U * VE) + threadIdx.x * VE;
     const float C = a.stats[2 * row], L = a.stats[2 * row + 1];
-    const bool none = gl == 0.f && h == 0.f, fine = C == C;
+    const bool none = gl == 0.f && h == 0.f, fine = L > -1.f;
     const float H = a.dentropy && !none ? a.entropy[row] : 0.f;
-    Careful k{};
-    if (!none && !fine) k = careful<DT>(Group<kBackThreads / kWave>{red}, base, a.vocab);
+    const Careful k{C, -1.f - L, 0.f, C != C};  // as the forward left it
     // p (a0 + a1 log2 p), and g at the token
     const float a0 = -(gl + h * H), a1 = -h * kLn2;
     const int at = token >= 0 && token < a.vocab && (fine || k.top != -kInf) ? static_cast<int>(token) : -1;

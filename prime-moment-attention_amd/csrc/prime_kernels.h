@@ -503,7 +503,8 @@ struct LogprobsArgs {
     const int64_t *tokens;            // [n]
     int64_t ignore;
     float *logprobs, *entropy;        // [n]; entropy: forward or null, backward the forward's
-    float *stats;                     // [n, 2] or null: C (NaN: a row summed by differences) and L
+    float *stats;                     // [n, 2] or null: C and L, or of a row summed by differences its
+                                      // largest (NaN: one is in the row) and -1 - log S
     int top;
     float *top_logprobs;              // [n, top]
     int64_t *top_tokens;
